@@ -38,7 +38,8 @@ extern "C" {
  * mh3_quantize_rows, test_flags in mh3_attn_args (was reserved0) and
  * mh3_gemm_args; 5: mh3_absmax_seg, mh3_quantize_seg; 6: mh3_peer_alloc,
  * mh3_peer_free, mh3_peer_handle, mh3_peer_open, mh3_peer_close;
- * 7: mh3_key_bias. */
+ * 7: mh3_key_bias.  Added since without changing what was there (look them up
+ * by name): mh3_rotary, mh3_block_norm_*, mh3_*_fp4, mh3_fp4_*. */
 #define MH3_ABI_VERSION 7
 
 #define MH3_OK 0
@@ -390,6 +391,157 @@ MH3_API int mh3_copy_rows(void* dst, int64_t dst_pitch, const void* src, int64_t
 MH3_API uint64_t mh3_step_diff_workspace_bytes(void);
 MH3_API int mh3_step_diff(const void* h1, void* prev, int32_t dtype, int64_t n, int32_t copy, double* sums,
                           void* workspace, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Rotary positions with several axes                                        */
+/* ------------------------------------------------------------------------ */
+/*
+ * q [B,Hq,S,D] and k [B,Hk,S,D] (either may have 0 heads) under element
+ * strides, channels contiguous, bf16, f16 or f32.  Channels [0, R) are
+ * rotated, R = sum of axes_dim (each even), the others copied.  Pair p is
+ * channels (2p, 2p+1) with ``interleaved``, else (p, p + R/2); the pairs go to
+ * the axes in order, axes_dim[a]/2 each, and the j-th of axis a turns by
+ * pos[a] * theta[a]^(-2j/axes_dim[a]) (its negative with ``inverse``, the
+ * gradient).  positions: [.., n_axes] int32, int64 or f32 (pos_kind 0, 1, 2)
+ * with strides for batch (0: shared) and token.  An output may be its own input
+ * (the same pointer and strides), not otherwise overlap one.  head_dim <= 256,
+ * n_axes <= 4.  No reference counterpart (the model applies it outside the
+ * reference's kernels).
+ */
+typedef struct mh3_rotary_args {
+  int32_t batch, seqlen, heads_q, heads_k, head_dim;
+  int32_t dtype, pos_kind, n_axes, interleaved, inverse;
+  int32_t axes_dim[4];
+  double theta[4];
+  const void* q;
+  int64_t q_stride_b, q_stride_h, q_stride_s;
+  const void* k;
+  int64_t k_stride_b, k_stride_h, k_stride_s;
+  void* q_out;
+  int64_t qo_stride_b, qo_stride_h, qo_stride_s;
+  void* k_out;
+  int64_t ko_stride_b, ko_stride_h, ko_stride_s;
+  const void* positions;
+  int64_t pos_stride_b, pos_stride_s;
+} mh3_rotary_args;
+
+MH3_API int mh3_rotary(const mh3_rotary_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Norms before and after a block, with gate, residual and modulation        */
+/* ------------------------------------------------------------------------ */
+/*
+ * Per row of [rows, channels] (bf16, f16 or f32; channels <= 8192):
+ *   z = ynorm(y) * y_weight          (y_norm 0: z = y)
+ *   r = residual_scale * x + gate * z (no y: r = x, and no r is written)
+ *   h = (norm(r) * weight + bias) * (1 + scale) + shift
+ * norm / y_norm: 1 = RMS, 2 = layer norm (y_norm 0 = none), both with ``eps``.
+ * A null gate, weight or y_weight is 1; a null bias, scale or shift 0.
+ * gate, scale, shift: element (group, row, c) at group * stride_group +
+ * row * stride_row + c; groups are ``group_rows`` rows each, or the packed
+ * sequences of cu_seqlens (int32 [groups+1] on the device, non-decreasing,
+ * entries clamped to [0, rows]; rows outside every sequence give zeros).
+ * With ``per_row`` the modulation's gradients have a row for each row of x
+ * (else one for each group).  weight, bias, y_weight: [channels].
+ * stats (float4 per row; optional in the forward pass) holds the rows' means
+ * and reciprocal deviations for the backward pass.
+ *
+ * mh3_block_norm_bwd reads dr and dh (either may be null), x, y, stats and the
+ * modulation, and writes every gradient whose pointer is given: dx, dy
+ * [rows, channels] in dtype; dgate, dscale, dshift [groups or rows, channels]
+ * and dweight, dbias, dy_weight [channels], each in its tensor's type, all
+ * contiguous.  Column sums are added in a fixed order.  workspace:
+ * mh3_block_norm_workspace_bytes() bytes, 16-byte aligned.
+ * No reference counterpart (the model's blocks are outside the reference).
+ */
+typedef struct mh3_norm_mod {
+  const void* ptr;
+  int64_t stride_group, stride_row;
+  int32_t dtype, reserved;
+} mh3_norm_mod;
+
+typedef struct mh3_block_norm_args {
+  int64_t rows, group_rows;
+  int32_t channels, groups, dtype, norm, y_norm, per_row;
+  float eps, residual_scale;
+  const int32_t* cu_seqlens;
+  const void* x;
+  int64_t x_stride;
+  const void* y;
+  int64_t y_stride;
+  mh3_norm_mod gate, scale, shift;
+  mh3_norm_mod weight, bias, y_weight; /* strides unused */
+  void* r; /* outputs of the forward pass: [rows, channels] contiguous, or null */
+  void* h;
+  void* stats;
+  const void* dr; /* inputs and outputs of the backward pass */
+  int64_t dr_stride;
+  const void* dh;
+  int64_t dh_stride;
+  void *dx, *dy, *dgate, *dscale, *dshift, *dweight, *dbias, *dy_weight;
+  void* workspace;
+} mh3_block_norm_args;
+
+MH3_API uint64_t mh3_block_norm_workspace_bytes(int64_t rows, int32_t channels, int32_t groups);
+MH3_API int mh3_block_norm_fwd(const mh3_block_norm_args* args, void* stream);
+MH3_API int mh3_block_norm_bwd(const mh3_block_norm_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Microscaled 4-bit rows and their product                                   */
+/* ------------------------------------------------------------------------ */
+/*
+ * A 4-bit matrix [M, K] (K a multiple of 32) is three buffers:
+ *   x4     [M, K/2] bytes: element 2j in the low four bits of byte j, 2j+1 in
+ *          the high ones; e2m1 codes (sign, then 0 .5 1 1.5 2 3 4 6);
+ *   blocks e4m3 scales of 16 elements, in blocks of 128 rows x 4 scales:
+ *          scale (m, b) at byte ((m/128) * ceil(K/64) + b/4) * 512
+ *          + (m%32) * 16 + (m%128)/32 * 4 + b%4
+ *          (mh3_fp4_block_bytes() bytes; the layout tensor memory takes);
+ *   scale  f32 [M]: a power of two per row.
+ * The element is code * blocks * scale.
+ *
+ * mh3_quantize_fp4: scale = 2^max(-100, ceil(log2(absmax(row) / 2688))),
+ * 2688 = 448 * 6; blocks = e4m3(absmax(16) / (6 scale)); code = e2m1(x /
+ * (blocks scale)), both rounded to nearest even from correctly rounded
+ * quotients; a block whose scale rounds to 0 has codes 0.  A row with an
+ * infinity or NaN gets scale NaN and zeros elsewhere.  Scales past K and past M
+ * in the last blocks are 0.
+ * mh3_dequantize_fp4: the values, bf16 or f32 (both exact), [M, K] contiguous.
+ *
+ * mh3_fp4_gemm: out[m,n] = bf16((sum_k a[m,k] b[n,k] + sum_r a2[m,r] b2[n,r])
+ *   * a_scale[m] * b_scale[n] + bias[n]), a [M,K] and b [N,K] such matrices
+ * (their products and sums take the block scales), a2 [M,R], b2 [N,R] optional
+ * bf16 low-rank operands.  N, R and the strides of out, a2 and b2 multiples of
+ * 8; x4 buffers contiguous, all pointers 16-byte aligned.
+ */
+MH3_API uint64_t mh3_fp4_block_bytes(int64_t M, int64_t K);
+MH3_API int mh3_quantize_fp4(const void* x, int64_t x_stride, int32_t in_dtype, int64_t M, int64_t K, void* x4,
+                             void* blocks, float* scale, void* stream);
+MH3_API int mh3_dequantize_fp4(const void* x4, const void* blocks, const float* scale, int64_t M, int64_t K,
+                               int32_t out_dtype, void* out, void* stream);
+
+typedef struct mh3_fp4_gemm_args {
+  int64_t M, N, K, R;
+  const void* a;
+  const void* a_blocks;
+  const float* a_scale;
+  const void* b;
+  const void* b_blocks;
+  const float* b_scale;
+  const void* bias; /* bf16 [N] or NULL */
+  const void* a2;
+  int64_t lda2;
+  const void* b2;
+  int64_t ldb2;
+  void* out; /* bf16 [M, N], row stride ldo */
+  int64_t ldo;
+  int* err;
+  uint64_t timeout_ns;
+  int32_t test_flags; /* 0; MH3_TEST_* bits */
+  int32_t reserved1;
+} mh3_fp4_gemm_args;
+
+MH3_API int mh3_fp4_gemm(const mh3_fp4_gemm_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -84,6 +84,56 @@ class GemmArgs(ctypes.Structure):
     ]
 
 
+class RotaryArgs(ctypes.Structure):
+    """``mh3_rotary_args`` (include/mh3_b200.h)."""
+
+    _fields_ = [
+        ("batch", c_i32), ("seqlen", c_i32), ("heads_q", c_i32), ("heads_k", c_i32), ("head_dim", c_i32),
+        ("dtype", c_i32), ("pos_kind", c_i32), ("n_axes", c_i32), ("interleaved", c_i32), ("inverse", c_i32),
+        ("axes_dim", c_i32 * 4), ("theta", ctypes.c_double * 4),
+        ("q", c_ptr), ("q_stride_b", c_i64), ("q_stride_h", c_i64), ("q_stride_s", c_i64),
+        ("k", c_ptr), ("k_stride_b", c_i64), ("k_stride_h", c_i64), ("k_stride_s", c_i64),
+        ("q_out", c_ptr), ("qo_stride_b", c_i64), ("qo_stride_h", c_i64), ("qo_stride_s", c_i64),
+        ("k_out", c_ptr), ("ko_stride_b", c_i64), ("ko_stride_h", c_i64), ("ko_stride_s", c_i64),
+        ("positions", c_ptr), ("pos_stride_b", c_i64), ("pos_stride_s", c_i64),
+    ]
+
+
+class NormMod(ctypes.Structure):
+    """``mh3_norm_mod`` (include/mh3_b200.h)."""
+
+    _fields_ = [("ptr", c_ptr), ("stride_group", c_i64), ("stride_row", c_i64), ("dtype", c_i32), ("reserved", c_i32)]
+
+
+class BlockNormArgs(ctypes.Structure):
+    """``mh3_block_norm_args`` (include/mh3_b200.h)."""
+
+    _fields_ = [
+        ("rows", c_i64), ("group_rows", c_i64),
+        ("channels", c_i32), ("groups", c_i32), ("dtype", c_i32), ("norm", c_i32), ("y_norm", c_i32), ("per_row", c_i32),
+        ("eps", c_f32), ("residual_scale", c_f32), ("cu_seqlens", c_ptr),
+        ("x", c_ptr), ("x_stride", c_i64), ("y", c_ptr), ("y_stride", c_i64),
+        ("gate", NormMod), ("scale", NormMod), ("shift", NormMod),
+        ("weight", NormMod), ("bias", NormMod), ("y_weight", NormMod),
+        ("r", c_ptr), ("h", c_ptr), ("stats", c_ptr),
+        ("dr", c_ptr), ("dr_stride", c_i64), ("dh", c_ptr), ("dh_stride", c_i64),
+        ("dx", c_ptr), ("dy", c_ptr), ("dgate", c_ptr), ("dscale", c_ptr), ("dshift", c_ptr),
+        ("dweight", c_ptr), ("dbias", c_ptr), ("dy_weight", c_ptr), ("workspace", c_ptr),
+    ]
+
+
+class Fp4GemmArgs(ctypes.Structure):
+    """``mh3_fp4_gemm_args`` (include/mh3_b200.h)."""
+
+    _fields_ = [
+        ("M", c_i64), ("N", c_i64), ("K", c_i64), ("R", c_i64),
+        ("a", c_ptr), ("a_blocks", c_ptr), ("a_scale", c_ptr), ("b", c_ptr), ("b_blocks", c_ptr), ("b_scale", c_ptr),
+        ("bias", c_ptr), ("a2", c_ptr), ("lda2", c_i64), ("b2", c_ptr), ("ldb2", c_i64),
+        ("out", c_ptr), ("ldo", c_i64), ("err", c_ptr), ("timeout_ns", c_u64),
+        ("test_flags", c_i32), ("reserved1", c_i32),
+    ]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "mh3_abi_version": (c_i32, []),
@@ -111,6 +161,14 @@ _SIGNATURES = {
     "mh3_peer_handle": (c_i32, [c_ptr, c_ptr]),
     "mh3_peer_open": (c_i32, [c_ptr, c_ptr]),
     "mh3_peer_close": (c_i32, [c_ptr]),
+    "mh3_rotary": (c_i32, [ctypes.POINTER(RotaryArgs), c_ptr]),
+    "mh3_block_norm_workspace_bytes": (c_u64, [c_i64, c_i32, c_i32]),
+    "mh3_block_norm_fwd": (c_i32, [ctypes.POINTER(BlockNormArgs), c_ptr]),
+    "mh3_block_norm_bwd": (c_i32, [ctypes.POINTER(BlockNormArgs), c_ptr]),
+    "mh3_fp4_block_bytes": (c_u64, [c_i64, c_i64]),
+    "mh3_quantize_fp4": (c_i32, [c_ptr, c_i64, c_i32, c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_ptr]),
+    "mh3_dequantize_fp4": (c_i32, [c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i32, c_ptr, c_ptr]),
+    "mh3_fp4_gemm": (c_i32, [ctypes.POINTER(Fp4GemmArgs), c_ptr]),
     "mh3_step_diff_workspace_bytes": (c_u64, []),
     "mh3_step_diff": (c_i32, [c_ptr, c_ptr, c_i32, c_i64, c_i32, c_ptr, c_ptr, c_ptr]),
 }

@@ -1,0 +1,779 @@
+// The norms before and after a transformer block, with the block's gate, the
+// residual scale and the next norm's modulation in the same pass.
+//
+//   z    = ynorm(y) * wy                  (ynorm: none, RMS or layer norm; wy only with a norm)
+//   r    = alpha * x + gate * z           (no y: r = x)
+//   xhat = (r - mean) * rstd              (layer)  or  r * rstd  (RMS, mean = 0)
+//   h    = (xhat * w + b) * (1 + scale) + shift
+//
+// gate, scale and shift belong to a group of rows (a batch item or a packed
+// sequence) or to each row.  Every quantity between the inputs and r, h is fp32;
+// the variance is summed around the mean (a second pass over registers), so a
+// stream whose mean is far from zero loses nothing; r and h are rounded once.
+//
+// Backward, with dn = dh w (1 + scale), d = dr + rstd (dn - mean(dn) - xhat mean(dn xhat)):
+//   dx = alpha d,  dz = d gate,  dy = dz or the norm's gradient of dz wy,
+//   dscale = sum dh (xhat w + b), dshift = sum dh, dgate = sum d z,
+//   dw = sum dh (1 + scale) xhat, db = sum dh (1 + scale), dwy = sum d gate yhat.
+// It recomputes xhat and yhat from x, y and the rows' saved (mean, rstd).
+//
+// Bound: HBM (4 bytes a bf16 element for norm_modulate, 8 for the gated form;
+// backward 6 and 12).  One CTA holds a row, eight channels a thread, and walks a
+// contiguous range of rows, so the modulation is read and combined once per
+// group (kept in the thread's own slots of shared memory) and the next row's
+// vectors are loaded before the current row is reduced.  Column sums stay in
+// registers over the range; each (CTA, group) writes one partial row and a second
+// kernel adds the partials in a fixed order: no atomics, the same bits every time.
+#include <algorithm>
+
+#include "mh3_b200.h"
+#include "mh3_internal.h"
+#include "ptx.cuh"
+
+namespace mh3 {
+namespace bnorm {
+
+constexpr int kMaxC = 8192;  // 1024 threads x 8 channels
+constexpr int kSMs = 148;    // fixed: the order of the column sums depends on the sizes only
+
+// A modulation tensor: element (group, row, c) at group * sg + row * sr + c.
+struct Mod {
+  const void* p;
+  long long sg, sr;
+  int dt;
+};
+struct Chan {
+  const void* p;  // [C]
+  int dt;
+};
+
+struct Params {
+  const void *x, *y, *dr, *dh;
+  void *r, *h, *dx, *dy;
+  long long x_s, y_s, dr_s, dh_s;  // row strides, elements (outputs are [rows, C])
+  float4* stats;  // per row: mean and rstd of y, mean and rstd of r
+  Mod gate, scale, shift;
+  Chan w, b, wy;
+  void *dgate, *dscale, *dshift, *dw, *db, *dwy;  // gradients, in their tensors' types, contiguous
+  float* part;       // [ctas + G][3][C]
+  float* gsum;       // [G][3][C]
+  long long rows, S; // S: rows of a group (dense)
+  const int* cu;     // packed: [G + 1]
+  int C, G, ynorm, norm, ctas;
+  float eps, alpha;
+};
+
+enum { kNone = 0, kRms = 1, kLayer = 2 };
+
+__device__ __forceinline__ float get1(const void* p, int dt, long long i) {
+  if (dt == MH3_DTYPE_F32) return static_cast<const float*>(p)[i];
+  if (dt == MH3_DTYPE_F16) return __half2float(static_cast<const __half*>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void put1(void* p, int dt, long long i, float v) {
+  if (dt == MH3_DTYPE_F32) static_cast<float*>(p)[i] = v;
+  else if (dt == MH3_DTYPE_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// Eight channels of a row as loaded: converted only where they are used, so a
+// row that waits its turn holds four registers of 16-bit data.
+template <typename T>
+struct Raw {
+  uint4 u[sizeof(T) == 4 ? 2 : 1];
+};
+
+template <typename T, bool VEC>
+__device__ __forceinline__ Raw<T> load8(const T* p, int n) {
+  Raw<T> r;
+  if constexpr (VEC) {
+    r.u[0] = *reinterpret_cast<const uint4*>(p);
+    if constexpr (sizeof(T) == 4) r.u[1] = *reinterpret_cast<const uint4*>(p + 4);
+  } else {
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = i < n ? p[i] : T(0.0f);
+    memcpy(&r, e, sizeof(r));
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void unpack(const Raw<T>& r, float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    memcpy(v, &r, sizeof(r));
+  } else {
+    const uint32_t w[4] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float2 f;
+      if constexpr (std::is_same<T, __half>::value) f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      else f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
+  if constexpr (VEC) {
+    if constexpr (sizeof(T) == 4) {
+      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __half>::value) {
+          const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
+      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) {
+        if constexpr (std::is_same<T, float>::value) p[i] = v[i];
+        else if constexpr (std::is_same<T, __half>::value) p[i] = __float2half_rn(v[i]);
+        else p[i] = __float2bfloat16_rn(v[i]);
+      }
+  }
+}
+
+// Eight modulation values (any of the three types), ``dflt`` where there is none.
+template <bool VEC>
+__device__ __forceinline__ void mod8(const void* p, int dt, long long at, int n, float dflt, float (&v)[8]) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = dflt;
+  } else if (dt == MH3_DTYPE_F32) {
+    unpack(load8<float, VEC>(static_cast<const float*>(p) + at, n), v);
+  } else if (dt == MH3_DTYPE_F16) {
+    unpack(load8<__half, VEC>(static_cast<const __half*>(p) + at, n), v);
+  } else {
+    unpack(load8<__nv_bfloat16, VEC>(static_cast<const __nv_bfloat16*>(p) + at, n), v);
+  }
+}
+
+// A thread's eight values in shared memory, as two float4 a stride of the CTA apart.
+__device__ __forceinline__ void slot_put(float4* s, const float (&v)[8]) {
+  s[threadIdx.x] = make_float4(v[0], v[1], v[2], v[3]);
+  s[blockDim.x + threadIdx.x] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void slot_get(const float4* s, float (&v)[8]) {
+  const float4 a = s[threadIdx.x], b = s[blockDim.x + threadIdx.x];
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+
+// Sums over the CTA of N values per thread.  Consecutive calls use the two halves
+// of ``buf`` in turn, so one barrier per call is enough: a warp can reach the
+// second-next call only when every warp has left this one.
+template <int N>
+__device__ __forceinline__ void block_sum(float (&v)[N], float (*buf)[2][32], int& turn) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  const int nw = blockDim.x >> 5;
+  if (nw == 1) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (lane == 0)
+#pragma unroll
+    for (int k = 0; k < N; ++k) buf[turn][k][warp] = v[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = lane < nw ? buf[turn][k][lane] : 0.0f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  turn ^= 1;
+}
+
+// (mean, rstd) of the row held as v (n valid channels in this thread).
+__device__ __forceinline__ float2 row_stats(const float (&v)[8], int n, int C, int kind, float eps, float (*buf)[2][32],
+                                            int& turn) {
+  float mean = 0.0f, s[1];
+  if (kind == kLayer) {
+    s[0] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[0] += v[i];  // channels past n are 0
+    block_sum(s, buf, turn);
+    mean = s[0] / (float)C;
+  }
+  s[0] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float d = i < n ? v[i] - mean : 0.0f;
+    s[0] = fmaf(d, d, s[0]);
+  }
+  block_sum(s, buf, turn);
+  return make_float2(mean, rsqrtf(s[0] / (float)C + eps));
+}
+
+// The group of a row that lies at or after the rows of group ``g``, with the
+// first row past it in ``end``; G when the row is outside every packed sequence.
+__device__ __forceinline__ long long bound(const Params& p, int i) {
+  return min(max((long long)p.cu[i], 0ll), p.rows);
+}
+__device__ __forceinline__ int group_of(const Params& p, long long row, int g, long long& end) {
+  if (p.cu == nullptr) {
+    g = (int)(row / p.S);
+    end = (g + 1) * p.S;
+    return g;
+  }
+  if (g < 0) {  // first lookup: the number of sequences that end at or before the row
+    int lo = 0, hi = p.G;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (bound(p, mid + 1) <= row) lo = mid + 1;
+      else hi = mid;
+    }
+    g = lo;
+  }
+  while (g < p.G && bound(p, g + 1) <= row) ++g;
+  if (g >= p.G) {
+    end = p.rows;
+    return p.G;
+  }
+  const long long first = bound(p, g);
+  if (row < first) {  // before the first sequence
+    end = first;
+    return p.G;
+  }
+  end = bound(p, g + 1);
+  return g;
+}
+
+// PT: the modulation has a row for each row of x.
+template <typename T, bool VEC, bool PT>
+__global__ void __launch_bounds__(1024) fwd_kernel(const __grid_constant__ Params p) {
+  extern __shared__ float4 slots[];
+  __shared__ float red[2][2][32];
+  float4* sA = slots;                    // w (1 + scale)        (PT: w)
+  float4* sB = slots + 2 * blockDim.x;   // b (1 + scale) + shift (PT: b)
+  float4* sG = slots + 4 * blockDim.x;   // gate wy              (PT: wy); only with y
+  const int c = threadIdx.x * 8;
+  const int n = max(0, min(8, p.C - c));
+  const bool live = n > 0;
+  const long long lo = p.rows * blockIdx.x / p.ctas, hi = p.rows * (blockIdx.x + 1) / p.ctas;
+  const bool has_y = p.y != nullptr;
+  int turn = 0, g = -1;
+  long long end = lo;
+  Raw<T> nx = {}, ny = {};
+  auto fetch = [&](long long row) {
+    if (live && row < hi) {
+      nx = load8<T, VEC>(static_cast<const T*>(p.x) + row * p.x_s + c, n);
+      if (has_y) ny = load8<T, VEC>(static_cast<const T*>(p.y) + row * p.y_s + c, n);
+    }
+  };
+  fetch(lo);
+  for (long long row = lo; row < hi; ++row) {
+    const Raw<T> rx = nx, ry = ny;
+    fetch(row + 1);
+    if (row >= end) {
+      g = group_of(p, row, g == p.G ? -1 : g, end);
+      if (live && g < p.G) {
+        float w[8], b[8], t[8];
+        mod8<VEC>(p.w.p, p.w.dt, c, n, 1.0f, w);
+        mod8<VEC>(p.b.p, p.b.dt, c, n, 0.0f, b);
+        if constexpr (!PT) {
+          mod8<VEC>(p.scale.p, p.scale.dt, g * p.scale.sg + c, n, 0.0f, t);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            w[i] *= 1.0f + t[i];
+            b[i] *= 1.0f + t[i];
+          }
+          mod8<VEC>(p.shift.p, p.shift.dt, g * p.shift.sg + c, n, 0.0f, t);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) b[i] += t[i];
+        }
+        slot_put(sA, w);
+        slot_put(sB, b);
+        if (has_y) {
+          mod8<VEC>(p.wy.p, p.wy.dt, c, n, 1.0f, w);
+          if constexpr (!PT) {
+            mod8<VEC>(p.gate.p, p.gate.dt, g * p.gate.sg + c, n, 1.0f, t);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] *= t[i];
+          }
+          slot_put(sG, w);
+        }
+      }
+    }
+    float v[8] = {};
+    if (g >= p.G) {  // outside every packed sequence: zeros
+      if (live) {
+        if (p.r) store8<T, VEC>(static_cast<T*>(p.r) + row * p.C + c, n, v);
+        if (p.h) store8<T, VEC>(static_cast<T*>(p.h) + row * p.C + c, n, v);
+      }
+      if (threadIdx.x == 0 && p.stats) p.stats[row] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      continue;
+    }
+    float a[8], t[8];
+    if (live) unpack(rx, v);
+    float2 sy = make_float2(0.0f, 1.0f);
+    if (has_y) {
+      float y[8] = {};
+      if (live) unpack(ry, y);
+      if (p.ynorm != kNone) {
+        sy = row_stats(y, n, p.C, p.ynorm, p.eps, red, turn);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = (y[i] - sy.x) * sy.y;
+      }
+      if (live) {
+        slot_get(sG, a);
+        if constexpr (PT) {
+          mod8<VEC>(p.gate.p, p.gate.dt, g * p.gate.sg + row * p.gate.sr + c, n, 1.0f, t);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) a[i] *= t[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? fmaf(a[i], y[i], p.alpha * v[i]) : 0.0f;
+        if (p.r) store8<T, VEC>(static_cast<T*>(p.r) + row * p.C + c, n, v);
+      }
+    }
+    float2 sr = make_float2(0.0f, 1.0f);
+    if (p.h != nullptr) {
+      sr = row_stats(v, n, p.C, p.norm, p.eps, red, turn);
+      if (live) {
+        float b[8];
+        slot_get(sA, a);
+        slot_get(sB, b);
+        if constexpr (PT) {
+          mod8<VEC>(p.scale.p, p.scale.dt, g * p.scale.sg + row * p.scale.sr + c, n, 0.0f, t);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            a[i] *= 1.0f + t[i];
+            b[i] *= 1.0f + t[i];
+          }
+          mod8<VEC>(p.shift.p, p.shift.dt, g * p.shift.sg + row * p.shift.sr + c, n, 0.0f, t);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) b[i] += t[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = fmaf((v[i] - sr.x) * sr.y, a[i], b[i]);
+        store8<T, VEC>(static_cast<T*>(p.h) + row * p.C + c, n, v);
+      }
+    }
+    if (threadIdx.x == 0 && p.stats) p.stats[row] = make_float4(sy.x, sy.y, sr.x, sr.y);
+  }
+}
+
+template <typename T, bool VEC, bool PT>
+__global__ void __launch_bounds__(1024) bwd_kernel(const __grid_constant__ Params p) {
+  extern __shared__ float4 slots[];
+  __shared__ float red[2][2][32];
+  float4* sA = slots;                   // w (1 + scale)  (PT: w)
+  float4* sG = slots + 2 * blockDim.x;  // gate wy        (PT: wy); only with y
+  const int c = threadIdx.x * 8;
+  const int n = max(0, min(8, p.C - c));
+  const bool live = n > 0;
+  const long long lo = p.rows * blockIdx.x / p.ctas, hi = p.rows * (blockIdx.x + 1) / p.ctas;
+  const bool has_y = p.y != nullptr, has_dr = p.dr != nullptr, has_dh = p.dh != nullptr;
+  int turn = 0, g = -1;
+  long long end = lo;
+  // column sums of dh xhat, dh and d yhat (PT: with the row's factors 1 + scale and gate)
+  float a1[8] = {}, a2[8] = {}, a3[8] = {};
+  auto flush = [&](int grp) {
+    if (!live) return;
+    float* o = p.part + (long long)(blockIdx.x + (PT ? 0 : grp)) * 3 * p.C + c;
+    store8<float, VEC>(o, n, a1);
+    store8<float, VEC>(o + p.C, n, a2);
+    store8<float, VEC>(o + 2 * p.C, n, a3);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a1[i] = a2[i] = a3[i] = 0.0f;
+  };
+  for (long long row = lo; row < hi; ++row) {
+    if (row >= end) {
+      const int was = g;
+      g = group_of(p, row, g == p.G ? -1 : g, end);
+      if (!PT && was >= 0 && was < p.G) flush(was);
+      if (live && g < p.G) {
+        float w[8], t[8];
+        mod8<VEC>(p.w.p, p.w.dt, c, n, 1.0f, w);
+        if constexpr (!PT) {
+          mod8<VEC>(p.scale.p, p.scale.dt, g * p.scale.sg + c, n, 0.0f, t);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] *= 1.0f + t[i];
+        }
+        slot_put(sA, w);
+        if (has_y) {
+          mod8<VEC>(p.wy.p, p.wy.dt, c, n, 1.0f, w);
+          if constexpr (!PT) {
+            mod8<VEC>(p.gate.p, p.gate.dt, g * p.gate.sg + c, n, 1.0f, t);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] *= t[i];
+          }
+          slot_put(sG, w);
+        }
+      }
+    }
+    float d[8] = {}, t[8];
+    if (g >= p.G) {  // outside every packed sequence: no gradient
+      if (live) {
+        if (p.dx) store8<T, VEC>(static_cast<T*>(p.dx) + row * p.C + c, n, d);
+        if (p.dy) store8<T, VEC>(static_cast<T*>(p.dy) + row * p.C + c, n, d);
+        if constexpr (PT) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i < n) {
+              if (p.dscale) put1(p.dscale, p.scale.dt, row * p.C + c + i, 0.0f);
+              if (p.dshift) put1(p.dshift, p.shift.dt, row * p.C + c + i, 0.0f);
+              if (p.dgate) put1(p.dgate, p.gate.dt, row * p.C + c + i, 0.0f);
+            }
+        }
+      }
+      continue;
+    }
+    const float4 st = p.stats[row];
+    float xh[8] = {}, yh[8] = {}, gt[8] = {};
+    if (live) {
+      const Raw<T> rx = load8<T, VEC>(static_cast<const T*>(p.x) + row * p.x_s + c, n);
+      Raw<T> ry = {}, rd = {}, rh = {};
+      if (has_y) ry = load8<T, VEC>(static_cast<const T*>(p.y) + row * p.y_s + c, n);
+      if (has_dr) rd = load8<T, VEC>(static_cast<const T*>(p.dr) + row * p.dr_s + c, n);
+      if (has_dh) rh = load8<T, VEC>(static_cast<const T*>(p.dh) + row * p.dh_s + c, n);
+      unpack(rx, xh);
+      if (has_y) {
+        unpack(ry, yh);
+        slot_get(sG, gt);
+        if constexpr (PT) {
+          mod8<VEC>(p.gate.p, p.gate.dt, g * p.gate.sg + row * p.gate.sr + c, n, 1.0f, t);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) gt[i] *= t[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          yh[i] = (yh[i] - st.x) * st.y;
+          xh[i] = fmaf(gt[i], yh[i], p.alpha * xh[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) xh[i] = i < n ? (xh[i] - st.z) * st.w : 0.0f;
+      if (has_dr) unpack(rd, d);
+      if (has_dh) unpack(rh, t);
+    }
+    if (has_dh) {
+      float dn[8] = {}, s[2] = {0.0f, 0.0f};
+      if (live) {
+        slot_get(sA, dn);
+        if constexpr (PT) {
+          float sc[8];
+          mod8<VEC>(p.scale.p, p.scale.dt, g * p.scale.sg + row * p.scale.sr + c, n, 0.0f, sc);
+          if (p.dscale) {
+            float w[8], b[8], o[8];
+            mod8<VEC>(p.b.p, p.b.dt, c, n, 0.0f, b);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = dn[i];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = t[i] * fmaf(xh[i], w[i], b[i]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (i < n) put1(p.dscale, p.scale.dt, row * p.C + c + i, o[i]);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i < n && p.dshift) put1(p.dshift, p.shift.dt, row * p.C + c + i, t[i]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float m = t[i] * (1.0f + sc[i]);
+            a1[i] = fmaf(m, xh[i], a1[i]);
+            a2[i] += m;
+            dn[i] = dn[i] * m;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            a1[i] = fmaf(t[i], xh[i], a1[i]);
+            a2[i] += t[i];
+            dn[i] *= t[i];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          s[0] += dn[i];
+          s[1] = fmaf(dn[i], xh[i], s[1]);
+        }
+      }
+      block_sum(s, red, turn);
+      const float m0 = p.norm == kLayer ? s[0] / (float)p.C : 0.0f, m1 = s[1] / (float)p.C;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) d[i] = fmaf(st.w, dn[i] - m0 - xh[i] * m1, d[i]);
+    }
+    if (live && p.dx) {
+      const float k = has_y ? p.alpha : 1.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = k * d[i];
+      store8<T, VEC>(static_cast<T*>(p.dx) + row * p.C + c, n, t);
+    }
+    if (has_y) {
+      if (live) {
+        if constexpr (PT) {
+          float gv[8], wy[8];
+          mod8<VEC>(p.gate.p, p.gate.dt, g * p.gate.sg + row * p.gate.sr + c, n, 1.0f, gv);
+          slot_get(sG, wy);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (i < n && p.dgate) put1(p.dgate, p.gate.dt, row * p.C + c + i, d[i] * yh[i] * wy[i]);
+            a3[i] = fmaf(d[i] * gv[i], yh[i], a3[i]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) a3[i] = fmaf(d[i], yh[i], a3[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] = i < n ? d[i] * gt[i] : 0.0f;
+      }
+      if (p.ynorm != kNone && p.dy) {
+        float s[2] = {0.0f, 0.0f};
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            s[0] += d[i];
+            s[1] = fmaf(d[i], yh[i], s[1]);
+          }
+        }
+        block_sum(s, red, turn);
+        const float m0 = p.ynorm == kLayer ? s[0] / (float)p.C : 0.0f, m1 = s[1] / (float)p.C;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] = st.y * (d[i] - m0 - yh[i] * m1);
+      }
+      if (live && p.dy) store8<T, VEC>(static_cast<T*>(p.dy) + row * p.C + c, n, d);
+    }
+  }
+  if (PT) flush(0);
+  else if (g >= 0 && g < p.G) flush(g);
+}
+
+// Column sums of group blockIdx.y..: 32 channels x 8 partials at a time.  PT: one
+// "group" holds every CTA's partial.
+template <bool PT>
+__global__ void __launch_bounds__(256) group_sum_kernel(const __grid_constant__ Params p) {
+  __shared__ float sh[3][8][32];
+  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
+  const int groups = PT ? 1 : p.G;
+  for (int g = blockIdx.y; g < groups; g += gridDim.y) {
+    int i0 = 0, i1 = p.ctas;  // the CTAs whose rows meet the group's
+    if (!PT) {
+      long long r0, r1;
+      if (p.cu == nullptr) {
+        r0 = g * p.S;
+        r1 = r0 + p.S;
+      } else {
+        r0 = bound(p, g);
+        r1 = bound(p, g + 1);
+      }
+      // CTA i holds rows [rows i / ctas, rows (i + 1) / ctas): row r is in CTA ((r + 1) ctas - 1) / rows
+      i0 = r0 < r1 ? (int)(((r0 + 1) * p.ctas - 1) / p.rows) : 0;
+      i1 = r0 < r1 ? (int)((r1 * p.ctas - 1) / p.rows) + 1 : 0;
+    }
+    float s[3] = {0.0f, 0.0f, 0.0f};
+    if (c < p.C) {
+#pragma unroll 4
+      for (int i = i0 + part; i < i1; i += 8) {
+        const float* q = p.part + (long long)(i + (PT ? 0 : g)) * 3 * p.C + c;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) s[k] += q[(long long)k * p.C];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) sh[k][part][lane] = s[k];
+    __syncthreads();
+    if (part == 0 && c < p.C) {
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        s[k] = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s[k] += sh[k][q][lane];
+        p.gsum[((long long)g * 3 + k) * p.C + c] = s[k];
+      }
+      if (!PT) {
+        const float w = p.w.p ? get1(p.w.p, p.w.dt, c) : 1.0f, b = p.b.p ? get1(p.b.p, p.b.dt, c) : 0.0f;
+        const float wy = p.wy.p ? get1(p.wy.p, p.wy.dt, c) : 1.0f;
+        const long long at = (long long)g * p.C + c;
+        if (p.dscale) put1(p.dscale, p.scale.dt, at, fmaf(w, s[0], b * s[1]));
+        if (p.dshift) put1(p.dshift, p.shift.dt, at, s[1]);
+        if (p.dgate) put1(p.dgate, p.gate.dt, at, wy * s[2]);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Gradients of the channel vectors from the groups' column sums.
+template <bool PT>
+__global__ void __launch_bounds__(128) chan_kernel(const __grid_constant__ Params p) {
+  const int c = blockIdx.x * 128 + threadIdx.x;
+  if (c >= p.C) return;
+  float sw = 0.0f, sb = 0.0f, sy = 0.0f;
+  for (int g = 0; g < (PT ? 1 : p.G); ++g) {
+    const float* s = p.gsum + (long long)g * 3 * p.C + c;
+    const float m = !PT && p.scale.p ? 1.0f + get1(p.scale.p, p.scale.dt, g * p.scale.sg + c) : 1.0f;
+    const float gt = !PT && p.gate.p ? get1(p.gate.p, p.gate.dt, g * p.gate.sg + c) : 1.0f;
+    sw = fmaf(m, s[0], sw);
+    sb = fmaf(m, s[p.C], sb);
+    sy = fmaf(gt, s[2 * (long long)p.C], sy);
+  }
+  if (p.dw) put1(p.dw, p.w.dt, c, sw);
+  if (p.db) put1(p.db, p.b.dt, c, sb);
+  if (p.dwy) put1(p.dwy, p.wy.dt, c, sy);
+}
+
+static int threads_of(int C) { return ((C + 7) / 8 + 31) / 32 * 32; }
+
+// CTAs: two of a 5120-channel row's 640 threads fill an SM's registers; narrow
+// rows get as many warps.
+static int ctas_of(long long rows, int C) {
+  const int per = std::max(1, std::min(32, 1536 / threads_of(C)));
+  return (int)std::min<long long>(rows, (long long)kSMs * per);
+}
+
+template <typename T, bool VEC, bool PT>
+static cudaError_t launch_fwd(const Params& p, cudaStream_t st) {
+  const int nt = threads_of(p.C);
+  const size_t smem = (size_t)nt * 8 * sizeof(float) * (p.y ? 3 : 2);
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(fwd_kernel<T, VEC, PT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 98304);
+    if (e != cudaSuccess) return e;
+  }
+  fwd_kernel<T, VEC, PT><<<p.ctas, nt, smem, st>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename T, bool VEC, bool PT>
+static cudaError_t launch_bwd(const Params& p, cudaStream_t st) {
+  const int nt = threads_of(p.C);
+  const size_t smem = (size_t)nt * 8 * sizeof(float) * (p.y ? 2 : 1);
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(bwd_kernel<T, VEC, PT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536);
+    if (e != cudaSuccess) return e;
+  }
+  if (p.rows > 0) bwd_kernel<T, VEC, PT><<<p.ctas, nt, smem, st>>>(p);
+  const bool chan = p.dw || p.db || p.dwy;
+  if (chan || (!PT && (p.dscale || p.dshift || p.dgate))) {
+    const dim3 grid((unsigned)((p.C + 31) / 32), (unsigned)std::min(PT ? 1 : p.G, 65535));
+    group_sum_kernel<PT><<<grid, 256, 0, st>>>(p);
+    if (chan) chan_kernel<PT><<<(p.C + 127) / 128, 128, 0, st>>>(p);
+  }
+  return cudaGetLastError();
+}
+
+template <typename T>
+static cudaError_t launch(const Params& p, bool bwd, bool vec, bool pt, cudaStream_t st) {
+#define MH3_BN(F)                                                              \
+  return vec ? (pt ? F<T, true, true>(p, st) : F<T, true, false>(p, st))       \
+             : (pt ? F<T, false, true>(p, st) : F<T, false, false>(p, st))
+  if (bwd) MH3_BN(launch_bwd);
+  MH3_BN(launch_fwd);
+#undef MH3_BN
+}
+
+static bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+static int size_of(int dt) { return dt == MH3_DTYPE_F32 ? 4 : 2; }
+static bool float_type(int dt) { return dt == MH3_DTYPE_BF16 || dt == MH3_DTYPE_F16 || dt == MH3_DTYPE_F32; }
+
+static int run(const mh3_block_norm_args* a, bool bwd, void* stream) {
+  if (a == nullptr) return fail(MH3_ERR_INVALID, "mh3_block_norm: null args");
+  if (a->rows < 0 || a->channels <= 0 || a->groups <= 0) return fail(MH3_ERR_INVALID, "mh3_block_norm: bad sizes");
+  if (a->channels > kMaxC) return fail(MH3_ERR_TOO_LARGE, "mh3_block_norm: at most 8192 channels");
+  if (a->rows > (1ll << 40)) return fail(MH3_ERR_TOO_LARGE, "mh3_block_norm: too many rows");
+  if (!float_type(a->dtype)) return fail(MH3_ERR_INVALID, "mh3_block_norm: dtype must be bf16, f16 or f32");
+  if (a->norm != kRms && a->norm != kLayer) return fail(MH3_ERR_INVALID, "mh3_block_norm: norm must be 1 (rms) or 2 (layer)");
+  if (a->y_norm < kNone || a->y_norm > kLayer) return fail(MH3_ERR_INVALID, "mh3_block_norm: y_norm must be 0, 1 or 2");
+  if (a->cu_seqlens == nullptr && a->rows != a->groups * a->group_rows)
+    return fail(MH3_ERR_INVALID, "mh3_block_norm: rows must be groups * group_rows");
+  if (a->y == nullptr && (a->gate.ptr || a->y_weight.ptr || a->y_norm != kNone))
+    return fail(MH3_ERR_INVALID, "mh3_block_norm: gate, y_norm and y_weight need y");
+  if (a->y_norm == kNone && a->y_weight.ptr) return fail(MH3_ERR_INVALID, "mh3_block_norm: y_weight needs y_norm");
+  if (a->rows > 0) {
+    if (!a->x) return fail(MH3_ERR_INVALID, "mh3_block_norm: null x");
+    if (!bwd && !a->h && !a->r) return fail(MH3_ERR_INVALID, "mh3_block_norm: no output");
+    if (!bwd && a->r && !a->y) return fail(MH3_ERR_INVALID, "mh3_block_norm: r needs y");
+    if (bwd && !a->stats) return fail(MH3_ERR_INVALID, "mh3_block_norm: the backward pass needs stats");
+  }
+  if (bwd && !a->dr && !a->dh && a->rows > 0) return fail(MH3_ERR_INVALID, "mh3_block_norm: no gradient given");
+  if (bwd && (!a->workspace || !al16(a->workspace)))
+    return fail(MH3_ERR_INVALID, "mh3_block_norm: the backward pass needs a 16-byte aligned workspace");
+  if (!al16(a->stats)) return fail(MH3_ERR_INVALID, "mh3_block_norm: stats must be 16-byte aligned");
+  Params p;
+  memset(&p, 0, sizeof(p));
+  const int es = size_of(a->dtype);
+  bool vec = a->channels % 8 == 0;
+  auto rows_fit = [&](const void* q, long long stride) { vec = vec && (q == nullptr || (al16(q) && stride * es % 16 == 0)); };
+  rows_fit(a->x, a->x_stride);
+  rows_fit(a->y, a->y_stride);
+  rows_fit(a->dr, a->dr_stride);
+  rows_fit(a->dh, a->dh_stride);
+  for (const void* q : {(const void*)a->r, (const void*)a->h, (const void*)a->dx, (const void*)a->dy}) rows_fit(q, 0);
+  Mod* mods[3] = {&p.gate, &p.scale, &p.shift};
+  const mh3_norm_mod* given[3] = {&a->gate, &a->scale, &a->shift};
+  for (int i = 0; i < 3; ++i) {
+    if (given[i]->ptr && !float_type(given[i]->dtype))
+      return fail(MH3_ERR_INVALID, "mh3_block_norm: modulations must be bf16, f16 or f32");
+    *mods[i] = Mod{given[i]->ptr, given[i]->stride_group, given[i]->stride_row, given[i]->dtype};
+    if (given[i]->ptr) {
+      const int ms = size_of(given[i]->dtype);
+      vec = vec && al16(given[i]->ptr) && given[i]->stride_group * ms % 16 == 0 && given[i]->stride_row * ms % 16 == 0;
+    }
+  }
+  Chan* chans[3] = {&p.w, &p.b, &p.wy};
+  const mh3_norm_mod* vecs[3] = {&a->weight, &a->bias, &a->y_weight};
+  for (int i = 0; i < 3; ++i) {
+    if (vecs[i]->ptr && !float_type(vecs[i]->dtype))
+      return fail(MH3_ERR_INVALID, "mh3_block_norm: weights must be bf16, f16 or f32");
+    *chans[i] = Chan{vecs[i]->ptr, vecs[i]->dtype};
+    vec = vec && (vecs[i]->ptr == nullptr || al16(vecs[i]->ptr));
+  }
+  p.x = a->x; p.y = a->y; p.dr = a->dr; p.dh = a->dh;
+  p.r = a->r; p.h = a->h; p.dx = a->dx; p.dy = a->dy;
+  p.x_s = a->x_stride; p.y_s = a->y_stride; p.dr_s = a->dr_stride; p.dh_s = a->dh_stride;
+  p.stats = static_cast<float4*>(a->stats);
+  p.dgate = a->dgate; p.dscale = a->dscale; p.dshift = a->dshift;
+  p.dw = a->dweight; p.db = a->dbias; p.dwy = a->dy_weight;
+  p.rows = a->rows;
+  p.S = a->group_rows;
+  p.cu = a->cu_seqlens;
+  p.C = a->channels;
+  p.G = a->groups;
+  p.norm = a->norm;
+  p.ynorm = a->y_norm;
+  p.eps = a->eps;
+  p.alpha = a->residual_scale;
+  p.ctas = ctas_of(a->rows, a->channels);
+  p.part = static_cast<float*>(a->workspace);
+  if (bwd) p.gsum = p.part + ((long long)p.ctas + p.G) * 3 * p.C;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (a->rows == 0 && !bwd) return MH3_OK;
+  const bool pt = a->per_row != 0;
+  const cudaError_t e = a->dtype == MH3_DTYPE_BF16  ? launch<__nv_bfloat16>(p, bwd, vec, pt, st)
+                        : a->dtype == MH3_DTYPE_F16 ? launch<__half>(p, bwd, vec, pt, st)
+                                                    : launch<float>(p, bwd, vec, pt, st);
+  return e == cudaSuccess ? MH3_OK : fail_cuda(e, "mh3_block_norm launch");
+}
+
+}  // namespace bnorm
+}  // namespace mh3
+
+using namespace mh3;
+
+extern "C" uint64_t mh3_block_norm_workspace_bytes(int64_t rows, int32_t channels, int32_t groups) {
+  if (rows < 0 || channels <= 0 || channels > bnorm::kMaxC || groups <= 0) return 0;
+  return ((uint64_t)bnorm::ctas_of(rows, channels) + 2ull * (uint64_t)groups) * 3 * (uint64_t)channels * sizeof(float);
+}
+
+extern "C" int mh3_block_norm_fwd(const mh3_block_norm_args* a, void* stream) {
+  const mh3::NvtxRange nvtx_range("mh3_block_norm_fwd");
+  return bnorm::run(a, false, stream);
+}
+
+extern "C" int mh3_block_norm_bwd(const mh3_block_norm_args* a, void* stream) {
+  const mh3::NvtxRange nvtx_range("mh3_block_norm_bwd");
+  return bnorm::run(a, true, stream);
+}

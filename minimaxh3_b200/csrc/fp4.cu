@@ -1,0 +1,304 @@
+// Microscaled 4-bit rows: rounding to e2m1 with an e4m3 scale for 16 elements and
+// a power of two for the row, and back.
+//
+// Why two levels: an e4m3 scale follows the blocks inside a row over 2^15, but a
+// token's activations or a channel's weights may lie anywhere, so the row's
+// largest block is put at e4m3's upper end.  The row scale is a power of two: x /
+// scale and the row factors of a product are then exact, and it costs at most
+// one of e4m3's 18 binades.
+//
+//   scale  = 2^max(-100, ceil(log2(absmax_row / 2688)))       2688 = 448 * 6
+//   block  = e4m3(absmax_16 / (6 scale)),  code = e2m1(x / (block scale))
+//
+// Both quotients are correctly rounded (Markstein's step, see quant.cu's
+// div_rn_by) and then rounded to nearest even: for bf16 and f16 input a quotient
+// lies on a border exactly when the true one does, so the bytes are those of the
+// definition.  With M in [1, 2) and absmax = M 2^E, absmax / 2688 = (M / 1.3125)
+// 2^(E-11): the exponent is E - 11, one more if M > 1.3125 - integer compares.
+//
+// Bound: HBM, 2 bytes in and 0.5625 out per 16-bit element.  A thread owns the 16
+// elements of a block (32 contiguous bytes, kept in registers between the row's
+// reduction and the rounding), so the input is read once and the block's maximum
+// needs no exchange; rows longer than 1024 threads' blocks are read twice.
+#include <algorithm>
+#include <string>
+
+#include "mh3_b200.h"
+#include "mh3_internal.h"
+#include "ptx.cuh"
+
+namespace mh3 {
+namespace fp4 {
+
+constexpr int kMaxThreads = 1024;
+
+// x / s rounded to nearest even, r = 1/s rounded to nearest (quant.cu's div_rn_by).
+__device__ __forceinline__ float div_by(float x, float s, float r) {
+  const float q = x * r;
+  return fmaf(fmaf(-s, q, x), r, q);
+}
+
+template <typename T>
+__device__ __forceinline__ void load16(const T* p, float (&v)[16], bool vec) {
+  constexpr int NV = 16 * sizeof(T) / 16;
+  T e[16];
+  if (vec) {
+    uint4 u[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
+    memcpy(e, u, sizeof(e));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) e[i] = p[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if constexpr (std::is_same<T, float>::value) v[i] = e[i];
+    else if constexpr (std::is_same<T, __half>::value) v[i] = __half2float(e[i]);
+    else v[i] = __bfloat162float(e[i]);
+  }
+}
+
+// Largest magnitude as the integer of its bits: an infinity or NaN orders above
+// every finite value, so none is lost.
+__device__ __forceinline__ uint32_t absmax16(const float (&v)[16]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  return m;
+}
+
+__device__ __forceinline__ uint32_t e2m1x8(const float* q) {
+  uint32_t d;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(d)
+      : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
+  return d;
+}
+
+__device__ __forceinline__ float e4m3_value(uint32_t byte) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)byte));
+  return __half2float(__ushort_as_half((unsigned short)(h & 0xffffu)));
+}
+
+// Exponent of the row scale from the bits of a finite absmax.
+__device__ __forceinline__ int row_exponent(uint32_t bits) {
+  if (bits < 0x00800000u) return -100;  // 0 or subnormal: below 2^-126
+  const int e = (int)(bits >> 23) - 127 - 11 + ((bits & 0x7fffffu) > 0x280000u ? 1 : 0);  // 0.3125 * 2^23
+  return max(e, -100);
+}
+
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+__device__ __forceinline__ long long block_offset(long long row, int b, int nk64) {
+  return ((row >> 7) * nk64 + (b >> 2)) * 512 + (row & 31) * 16 + ((row & 127) >> 5) * 4 + (b & 3);
+}
+
+// Blocks of 32 x warps threads per row, rows side by side in y.  ONE: a row has at
+// most blockDim.x blocks, which stay in registers.  Rows M.. of the last block of
+// 128 get zero scales, so the buffer is the same whatever the memory held.
+template <typename T, bool ONE>
+__global__ void __launch_bounds__(kMaxThreads) quantize_kernel(const T* __restrict__ x, long long stride, long long M, int K,
+                                                              uint8_t* __restrict__ x4, uint8_t* __restrict__ blocks,
+                                                              float* __restrict__ scale, int vec) {
+  __shared__ uint32_t red[32];
+  const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+  const int nb = K / 16, nk64 = (K + 63) / 64;
+  const int warps = blockDim.x >> 5;
+  const T* xp = x + row * stride;
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+  uint32_t top = 0, mine = 0;
+  if (row < M) {
+    if constexpr (ONE) {
+      if ((int)threadIdx.x < nb) load16(xp + threadIdx.x * 16, v, vec != 0);
+      top = mine = absmax16(v);
+    } else {
+      for (int b = threadIdx.x; b < nb; b += blockDim.x) {
+        load16(xp + (long long)b * 16, v, vec != 0);
+        top = max(top, absmax16(v));
+      }
+    }
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (warps > 1) {
+    const int w0 = threadIdx.y * warps;  // this row's partial maxima
+    if ((threadIdx.x & 31) == 0) red[w0 + (threadIdx.x >> 5)] = top;
+    __syncthreads();
+    top = 0;
+    for (int w = 0; w < warps; ++w) top = max(top, red[w0 + w]);
+  }
+  if (row >= (M + 127) / 128 * 128) return;  // whole warps: blockDim.x is a multiple of 32
+  const bool live = row < M;
+  const bool finite = top < 0x7f800000u;
+  const int e = row_exponent(top);
+  const float inv = pow2f(-e);  // e in [-100, 117]
+  if (live && threadIdx.x == 0) scale[row] = finite ? pow2f(e) : __uint_as_float(0x7fffffffu);
+  for (int b = threadIdx.x; b < nk64 * 4; b += blockDim.x) {  // nk64 * 4: past K the scales are 0
+    uint32_t s8 = 0;
+    uint2 code = make_uint2(0, 0);
+    if (b < nb && live && finite) {
+      if constexpr (!ONE) {
+        load16(xp + (long long)b * 16, v, vec != 0);
+        mine = absmax16(v);
+      }
+      // e4m3 of absmax / (6 scale): the division by 6 is the only rounding before it
+      const float raw = div_by(__uint_as_float(mine) * inv, 6.0f, 1.0f / 6.0f);
+      s8 = cvt_e4m3x2_f32(0.0f, raw) & 0xffu;
+      if (s8 != 0) {
+        const float s = e4m3_value(s8), r = __frcp_rn(s);
+        float q[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) q[i] = div_by(v[i] * inv, s, r);
+        code = make_uint2(e2m1x8(q), e2m1x8(q + 8));
+      }
+    }
+    if (b < nb && live) *reinterpret_cast<uint2*>(x4 + row * (K / 2) + (long long)b * 8) = code;
+    // four neighbouring lanes hold the four scales of one word
+    uint32_t word = s8 << (8 * (b & 3));
+    const uint32_t lanes = 0xfu << (threadIdx.x & 28);
+    word |= __shfl_xor_sync(lanes, word, 1);
+    word |= __shfl_xor_sync(lanes, word, 2);
+    if ((b & 3) == 0) *reinterpret_cast<uint32_t*>(blocks + block_offset(row, b, nk64)) = word;
+  }
+}
+
+// Two e2m1 codes of a byte as two f16 (exact).
+__device__ __forceinline__ void e2m1x8_halves(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
+
+// One 16-element block per thread.
+template <typename T>
+__global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ x4, const uint8_t* __restrict__ blocks,
+                                                         const float* __restrict__ scale, int nb, long long M, T* __restrict__ out) {
+  const int b = blockIdx.x * blockDim.x + threadIdx.x;
+  const int nk64 = (nb + 3) / 4;
+  if (b >= nb) return;
+  for (long long row = (long long)blockIdx.y * blockDim.y + threadIdx.y; row < M; row += (long long)gridDim.y * blockDim.y) {
+    const uint2 code = *reinterpret_cast<const uint2*>(x4 + (row * nb + b) * 8);
+    const float s = e4m3_value(blocks[block_offset(row, b, nk64)]) * scale[row];
+    uint32_t h[8];
+    {
+      uint32_t t[4];
+      e2m1x8_halves(code.x, t);
+      for (int i = 0; i < 4; ++i) h[i] = t[i];
+      e2m1x8_halves(code.y, t);
+      for (int i = 0; i < 4; ++i) h[4 + i] = t[i];
+    }
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+      v[2 * i] = f.x * s;
+      v[2 * i + 1] = f.y * s;
+    }
+    T* o = out + (row * nb + b) * 16;
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(o)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&p);
+      }
+      reinterpret_cast<uint4*>(o)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+      reinterpret_cast<uint4*>(o)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+  }
+}
+
+template <typename T>
+static cudaError_t launch_quantize(const void* x, long long stride, long long M, int K, void* x4, void* blocks, float* scale,
+                                   cudaStream_t st) {
+  const int nb4 = (K + 63) / 64 * 4;  // scales of a row, the last word filled up
+  const int tx = std::min(kMaxThreads, (nb4 + 31) / 32 * 32);
+  const dim3 block((unsigned)tx, (unsigned)std::max(1, 256 / tx));
+  const long long padded = (M + 127) / 128 * 128;
+  const unsigned grid = (unsigned)((padded + block.y - 1) / block.y);
+  const int vec = ((uintptr_t)x & 15u) == 0 && stride * (long long)sizeof(T) % 16 == 0;
+  const T* xp = static_cast<const T*>(x);
+  uint8_t *c = static_cast<uint8_t*>(x4), *b = static_cast<uint8_t*>(blocks);
+  if (nb4 <= tx) quantize_kernel<T, true><<<grid, block, 0, st>>>(xp, stride, M, K, c, b, scale, vec);
+  else quantize_kernel<T, false><<<grid, block, 0, st>>>(xp, stride, M, K, c, b, scale, vec);
+  return cudaGetLastError();
+}
+
+}  // namespace fp4
+}  // namespace mh3
+
+using namespace mh3;
+
+extern "C" uint64_t mh3_fp4_block_bytes(int64_t M, int64_t K) {
+  if (M <= 0 || K <= 0) return 0;
+  return (uint64_t)((M + 127) / 128) * (uint64_t)((K + 63) / 64) * 512;
+}
+
+static int check_fp4(const char* what, int64_t M, int64_t K, const void* x4, const void* blocks, const float* scale) {
+  static thread_local std::string msg;
+  auto bad = [&](int code, const char* why) {
+    msg = std::string(what) + ": " + why;
+    return fail(code, msg.c_str());
+  };
+  if (M < 0 || K <= 0 || K % 32) return bad(MH3_ERR_INVALID, "K must be a positive multiple of 32");
+  if (M > 0x7fffff00LL || K > (1ll << 30)) return bad(MH3_ERR_TOO_LARGE, "dimension too large");
+  if (M > 0 && (!x4 || !blocks || !scale)) return bad(MH3_ERR_INVALID, "null pointer");
+  if (((uintptr_t)x4 & 15u) || ((uintptr_t)blocks & 15u))
+    return bad(MH3_ERR_INVALID, "the 4-bit buffers must be 16-byte aligned");
+  return MH3_OK;
+}
+
+extern "C" int mh3_quantize_fp4(const void* x, int64_t x_stride, int32_t in_dtype, int64_t M, int64_t K, void* x4,
+                                void* blocks, float* scale, void* stream) {
+  const mh3::NvtxRange nvtx_range("mh3_quantize_fp4");
+  const int rc = check_fp4("mh3_quantize_fp4", M, K, x4, blocks, scale);
+  if (rc) return rc;
+  if (in_dtype != MH3_DTYPE_BF16 && in_dtype != MH3_DTYPE_F16 && in_dtype != MH3_DTYPE_F32)
+    return fail(MH3_ERR_INVALID, "mh3_quantize_fp4: in_dtype must be bf16, f16 or f32");
+  if (M == 0) return MH3_OK;
+  if (!x) return fail(MH3_ERR_INVALID, "mh3_quantize_fp4: null x");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const cudaError_t e = in_dtype == MH3_DTYPE_BF16 ? fp4::launch_quantize<__nv_bfloat16>(x, x_stride, M, (int)K, x4, blocks, scale, st)
+                        : in_dtype == MH3_DTYPE_F16 ? fp4::launch_quantize<__half>(x, x_stride, M, (int)K, x4, blocks, scale, st)
+                                                    : fp4::launch_quantize<float>(x, x_stride, M, (int)K, x4, blocks, scale, st);
+  return e == cudaSuccess ? MH3_OK : fail_cuda(e, "mh3_quantize_fp4 launch");
+}
+
+extern "C" int mh3_dequantize_fp4(const void* x4, const void* blocks, const float* scale, int64_t M, int64_t K,
+                                  int32_t out_dtype, void* out, void* stream) {
+  const mh3::NvtxRange nvtx_range("mh3_dequantize_fp4");
+  const int rc = check_fp4("mh3_dequantize_fp4", M, K, x4, blocks, scale);
+  if (rc) return rc;
+  if (out_dtype != MH3_DTYPE_BF16 && out_dtype != MH3_DTYPE_F32)
+    return fail(MH3_ERR_INVALID, "mh3_dequantize_fp4: out_dtype must be bf16 or f32");
+  if (M == 0) return MH3_OK;
+  if (!out || ((uintptr_t)out & 15u)) return fail(MH3_ERR_INVALID, "mh3_dequantize_fp4: out must be 16-byte aligned and not null");
+  const int nb = (int)(K / 16);
+  const int tx = std::min(256, (nb + 31) / 32 * 32);
+  const dim3 block((unsigned)tx, (unsigned)std::max(1, 256 / tx));
+  const dim3 grid((unsigned)((nb + tx - 1) / tx), (unsigned)std::min<int64_t>((M + block.y - 1) / block.y, 65535));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const uint8_t *c = static_cast<const uint8_t*>(x4), *b = static_cast<const uint8_t*>(blocks);
+  if (out_dtype == MH3_DTYPE_F32)
+    fp4::dequantize_kernel<float><<<grid, block, 0, st>>>(c, b, scale, nb, M, static_cast<float*>(out));
+  else
+    fp4::dequantize_kernel<__nv_bfloat16><<<grid, block, 0, st>>>(c, b, scale, nb, M, static_cast<__nv_bfloat16*>(out));
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? MH3_OK : fail_cuda(e, "mh3_dequantize_fp4 launch");
+}

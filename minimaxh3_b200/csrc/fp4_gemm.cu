@@ -1,0 +1,605 @@
+// Product of two microscaled 4-bit matrices (mh3_fp4_gemm) for sm_100a.
+//
+//   out[m,n] = bf16((sum_k a[m,k] b[n,k] + sum_r a2[m,r] b2[n,r]) * as[m] * bs[n] + bias[n])
+//
+// a and b are e2m1 codes with an e4m3 scale for 16 of them; as and bs are the
+// rows' powers of two, so they factor out of the sum exactly.  Two kernels:
+//
+// * pair_kernel (M > kSmallM): persistent, a cluster of two CTAs per 256x256 tile,
+//   tcgen05.mma.cta_group::2 kind::mxf4nvf4 with the block scales in tensor memory.
+//   A stage is 256 elements of K: per CTA 128 rows of A and of B (128 bytes each),
+//   2 KB of A's scales and 4 KB of B's (every CTA needs the scales of all 256
+//   columns).  Bound: the tensor cores' 4-bit rate and the power limit.
+//   Tensor memory (512 columns): the block scales take 2 x 48 columns, so two whole
+//   256-column accumulators do not fit; they overlap in 96 columns.  The epilogue
+//   takes those 96 into registers first and hands them over, then drains the other
+//   160 while the next tile's MMAs run.  A scale buffer is rewritten only after the
+//   MMAs that read it two stages earlier have completed.
+// * small_kernel (M <= kSmallM): bound by reading b once.  A CTA takes 16 rows of b,
+//   its warps split K; codes are widened to f16 with their block scale (6
+//   significant bits: exact) and multiplied by mma.sync.m16n8k16 with f32 sums.
+//   The weights are the 16-row operand, up to 32 tokens the narrow one, and both
+//   sides use the same permutation of k, so a lane loads 32 consecutive codes.
+#include <algorithm>
+#include <mutex>
+
+#include "mh3_b200.h"
+#include "mh3_internal.h"
+#include "ptx.cuh"
+
+namespace mh3 {
+namespace fp4gemm {
+
+constexpr int NUM_THREADS = 192;
+constexpr int STAGES = 5;
+constexpr int STAGE_K = 256;                  // elements of K per stage (128 bytes)
+constexpr int BM = 256, BN = 256, HALF = 128;  // tile; rows of A and B per CTA
+constexpr int TILE_BYTES = HALF * 128;
+constexpr int SF_BLOCK = 512;                  // scales of 128 rows x 64 elements
+constexpr int EPI_BOX = 32 * 32 * 2;
+constexpr int kGroupM = 8;                     // 256-row blocks per raster group
+constexpr int ACC1 = 160;                      // first column of the second accumulator
+constexpr int OVERLAP = 3;                     // shared 32-column chunks
+constexpr int SF_COL = 416, SF_COLS = 48;      // scale buffers: 4 x 4 columns of A, 4 x 8 of B
+constexpr int kSmallM = 32;
+
+struct Params {
+  CUtensorMap tma_a, tma_b;    // bytes (K/2, rows), box (128, 128), 128B swizzle
+  CUtensorMap tma_sa, tma_sb;  // words (128, K/64, rows/128), box (128, 4, 1)
+  CUtensorMap tma_a2, tma_b2;  // bf16 (R, rows), box (64, 128), 128B swizzle
+  CUtensorMap tma_out;         // bf16 (N, M), box (32, 32), 64B swizzle
+  int M, N, K, R;
+  const float *rs, *cs;
+  const __nv_bfloat16* bias;
+  int* err;
+  unsigned long long timeout_ns;
+  int test_flags;
+};
+
+struct __align__(1024) Smem {
+  uint8_t a[STAGES][TILE_BYTES];
+  uint8_t b[STAGES][TILE_BYTES];
+  uint8_t sa[STAGES][4 * SF_BLOCK];
+  uint8_t sb[STAGES][2][4 * SF_BLOCK];
+  uint8_t epi[4][2][EPI_BOX];
+  float col_scale[2][BN];
+  float col_bias[2][BN];
+  uint64_t full[STAGES];  // used in the leader
+  uint64_t empty[STAGES];
+  uint64_t acc_full[2];
+  uint64_t acc_part;      // used in the leader: the overlapping columns are drained (4 warps x 2 CTAs)
+  uint64_t mma_done;
+  uint64_t bar_never;     // nothing arrives on it (test hook)
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+__global__ void __launch_bounds__(NUM_THREADS, 1) pair_kernel(const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t crank = cluster_ctarank();
+  const int pair = blockIdx.x >> 1;
+  const int npairs = gridDim.x >> 1;
+  const int num_m = (p.M + BM - 1) / BM;
+  const int num_n = (p.N + BN - 1) / BN;
+  const int num_tiles = num_m * num_n;
+  const int nk64 = (p.K + 63) / 64;
+  const int kst_main = (p.K + STAGE_K - 1) / STAGE_K;
+  const int kst = kst_main + (p.R + 63) / 64;  // then the low-rank stages, 64 bf16 each
+
+  auto coords = [&](int t, int& mb, int& nb) {
+    const int per_group = kGroupM * num_n;
+    const int g = t / per_group;
+    const int r = t - g * per_group;
+    const int gm = min(kGroupM, num_m - g * kGroupM);
+    nb = r / gm;
+    mb = g * kGroupM + (r - nb * gm);
+  };
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(smem_u32(&sm.full[i]), 1);
+      mbar_init(smem_u32(&sm.empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&sm.acc_full[i]), 1);
+    mbar_init(smem_u32(&sm.acc_part), 8);
+    mbar_init(smem_u32(&sm.mma_done), 1);
+    mbar_init(smem_u32(&sm.bar_never), 1);
+    sm.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(&sm.tmem_base), 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();  // both CTAs' barriers are initialised before any copy or arrive crosses
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+  const WaitGuard g{&sm.abort_flag, p.err, p.timeout_ns};
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- producer (both CTAs)
+    if (elect_one_sync()) {
+      tma_prefetch_desc(&p.tma_a);
+      tma_prefetch_desc(&p.tma_b);
+      tma_prefetch_desc(&p.tma_sa);
+      tma_prefetch_desc(&p.tma_sb);
+    }
+    __syncwarp();
+    int it = 0, last_issued = -1;
+    bool ok = true;
+    if (p.test_flags & MH3_TEST_STALL_PRODUCER) {  // a wait that nothing ends runs out first
+      bool w = true;
+      if (lane == 0) w = mbar_wait(smem_u32(&sm.bar_never), 0, g);
+      ok = __shfl_sync(0xffffffffu, w ? 1 : 0, 0) != 0;
+    }
+    for (int t = pair; t < num_tiles && ok; t += npairs) {
+      int mb, nb;
+      coords(t, mb, nb);
+      const int row_a = mb * BM + (int)crank * HALF;
+      const int row_b = nb * BN + (int)crank * HALF;
+      for (int s = 0; s < kst; ++s, ++it) {
+        const int st = it % STAGES;
+        bool w = true;
+        if (lane == 0) w = mbar_wait(smem_u32(&sm.empty[st]), ((uint32_t)(it / STAGES) & 1u) ^ 1u, g);
+        if (!__shfl_sync(0xffffffffu, w ? 1 : 0, 0)) {
+          ok = false;
+          break;
+        }
+        last_issued = it;
+        if (elect_one_sync()) {
+          const bool main = s < kst_main;
+          // the leader counts both CTAs' copies (clipped boxes are filled and counted whole)
+          if (crank == 0)
+            mbar_arrive_expect_tx(smem_u32(&sm.full[st]), 2u * (2u * TILE_BYTES + (main ? 12u * SF_BLOCK : 0u)));
+          const uint32_t fb = mapa_shared(smem_u32(&sm.full[st]), 0);
+          if (main) {
+            tma_load_2d_pair(smem_u32(sm.a[st]), &p.tma_a, fb, s * 128, row_a);
+            tma_load_2d_pair(smem_u32(sm.b[st]), &p.tma_b, fb, s * 128, row_b);
+            tma_load_3d_pair(smem_u32(sm.sa[st]), &p.tma_sa, fb, 0, s * 4, row_a / HALF);
+            tma_load_3d_pair(smem_u32(sm.sb[st][0]), &p.tma_sb, fb, 0, s * 4, nb * 2);
+            tma_load_3d_pair(smem_u32(sm.sb[st][1]), &p.tma_sb, fb, 0, s * 4, nb * 2 + 1);
+          } else {
+            tma_load_2d_pair(smem_u32(sm.a[st]), &p.tma_a2, fb, (s - kst_main) * 64, row_a);
+            tma_load_2d_pair(smem_u32(sm.b[st]), &p.tma_b2, fb, (s - kst_main) * 64, row_b);
+          }
+        }
+        __syncwarp();
+      }
+    }
+    // Teardown (leader): the last copies counted on each stage must land.
+    if (crank == 0 && lane == 0)
+      for (int i = max(0, last_issued - STAGES + 1); i <= last_issued; ++i)
+        mbar_wait_teardown(smem_u32(&sm.full[i % STAGES]), (uint32_t)(i / STAGES) & 1u);
+  } else if (warp == 1) {
+    if (crank == 0) {
+      // -------------------------------------------------------------- MMA issuer (leader)
+      constexpr uint32_t kIdF4 = idesc_nvf4(BM, BN);
+      constexpr uint32_t kIdBF = idesc_bf16(BM, BN, false, false);
+      int it = 0, tcount = 0, nsf = 0;
+      int used[2] = {-STAGES, -STAGES};  // the stage whose MMAs last read each scale buffer
+      for (int t = pair; t < num_tiles; t += npairs, ++tcount) {
+        const int acc = tcount & 1;
+        const uint32_t d_tmem = tmem + (uint32_t)(acc * ACC1);
+        // The previous tile's epilogue has read the shared columns, and with them
+        // the whole of the tile before it.
+        if (tcount > 0) mbar_wait_cluster(smem_u32(&sm.acc_part), (uint32_t)(tcount - 1) & 1u, g);
+        tc_fence_after();
+        for (int s = 0; s < kst; ++s, ++it) {
+          const int st = it % STAGES;
+          mbar_wait(smem_u32(&sm.full[st]), (uint32_t)(it / STAGES) & 1u, g);
+          const bool main = s < kst_main;
+          if (main) {
+            // A stage number that has come round again was filled only after its
+            // MMAs were done; a younger one is waited for here.
+            const int u = used[nsf & 1];
+            if (u >= 0 && it < u + STAGES) mbar_wait(smem_u32(&sm.empty[u % STAGES]), (uint32_t)(u / STAGES) & 1u, g);
+            used[nsf & 1] = it;
+          }
+          tc_fence_after();
+          __syncwarp();
+          if (elect_one_sync()) {
+            if (main) {
+              const int nmma = min(4, nk64 - s * 4);  // 64 elements each
+              const uint32_t sfa = tmem + SF_COL + (uint32_t)(nsf & 1) * SF_COLS, sfb = sfa + 16;
+              for (int kk = 0; kk < nmma; ++kk) {
+                tmem_cp_scales_pair(sfa + kk * 4, smem_desc(smem_u32(sm.sa[st]) + kk * SF_BLOCK, 0, 128, kLayoutNone));
+                tmem_cp_scales_pair(sfb + kk * 8, smem_desc(smem_u32(sm.sb[st][0]) + kk * SF_BLOCK, 0, 128, kLayoutNone));
+                tmem_cp_scales_pair(sfb + kk * 8 + 4, smem_desc(smem_u32(sm.sb[st][1]) + kk * SF_BLOCK, 0, 128, kLayoutNone));
+              }
+              for (int kk = 0; kk < nmma; ++kk)
+                mma_nvf4_ss_pair(d_tmem, smem_desc(smem_u32(sm.a[st]) + kk * 32, 16, 1024, kLayoutSW128),
+                                 smem_desc(smem_u32(sm.b[st]) + kk * 32, 16, 1024, kLayoutSW128), kIdF4, sfa + kk * 4,
+                                 sfb + kk * 8, (s > 0 || kk > 0) ? 1u : 0u);
+            } else {
+              for (int kk = 0; kk < 4; ++kk)  // 16 bf16 each
+                mma_f16_ss_pair(d_tmem, smem_desc(smem_u32(sm.a[st]) + kk * 32, 16, 1024, kLayoutSW128),
+                                smem_desc(smem_u32(sm.b[st]) + kk * 32, 16, 1024, kLayoutSW128), kIdBF, 1u);
+            }
+            mma_commit_pair(smem_u32(&sm.empty[st]), 0x3);
+          }
+          if (main) ++nsf;
+          __syncwarp();
+        }
+        if (elect_one_sync()) mma_commit_pair(smem_u32(&sm.acc_full[acc]), 0x3);
+        __syncwarp();
+      }
+      if (elect_one_sync()) mma_commit_pair(smem_u32(&sm.mma_done), 0x3);
+      __syncwarp();
+    }
+    // Both CTAs: every pair MMA (they write both CTAs' TMEM) must be
+    // finished before TMEM is freed, also on the abort path.
+    if (lane == 0) mbar_wait_teardown(smem_u32(&sm.mma_done), 0);
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ epilogue (both CTAs)
+    const int q = warp & 3;           // TMEM lane quarter of this warp
+    const int et = threadIdx.x - 64;  // 0..127 over the 4 epilogue warps
+    const uint32_t lane_off = (uint32_t)(q * 32) << 16;
+    int tcount = 0, buf = 0;
+    for (int t = pair; t < num_tiles; t += npairs, ++tcount) {
+      int mb, nb;
+      coords(t, mb, nb);
+      const int acc = tcount & 1;
+      const int n0 = nb * BN;
+      for (int j = et; j < BN; j += 128) {
+        const int n = n0 + j;
+        const bool in = n < p.N;
+        sm.col_scale[acc][j] = in ? __ldg(p.cs + n) : 0.0f;
+        sm.col_bias[acc][j] = (p.bias != nullptr && in) ? __bfloat162float(p.bias[n]) : 0.0f;
+      }
+      named_barrier_sync(1, 128);
+      const int m0 = mb * BM + (int)crank * HALF + q * 32;  // first row of this warp's box
+      const int m = m0 + lane;
+      const float rsv = m < p.M ? __ldg(p.rs + m) : 0.0f;
+      mbar_wait(smem_u32(&sm.acc_full[acc]), (uint32_t)(tcount >> 1) & 1u, g);
+      tc_fence_after();
+      const uint32_t base = tmem + (uint32_t)(acc * ACC1) + lane_off;
+      // One 32-column chunk of the tile to its output box.
+      auto put = [&](int c, const uint32_t (&v)[32]) {
+        if (n0 + c * 32 >= p.N || m0 >= p.M) return;  // warp-uniform: box wholly outside
+        const float* cs = &sm.col_scale[acc][c * 32];
+        const float* bs = &sm.col_bias[acc][c * 32];
+        uint32_t packed[16];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 c4 = *reinterpret_cast<const float4*>(cs + 4 * i);
+          const float4 b4 = *reinterpret_cast<const float4*>(bs + 4 * i);
+          const __nv_bfloat162 h0 = __floats2bfloat162_rn(fmaf(__uint_as_float(v[4 * i + 0]) * rsv, c4.x, b4.x),
+                                                          fmaf(__uint_as_float(v[4 * i + 1]) * rsv, c4.y, b4.y));
+          const __nv_bfloat162 h1 = __floats2bfloat162_rn(fmaf(__uint_as_float(v[4 * i + 2]) * rsv, c4.z, b4.z),
+                                                          fmaf(__uint_as_float(v[4 * i + 3]) * rsv, c4.w, b4.w));
+          packed[2 * i] = *reinterpret_cast<const uint32_t*>(&h0);
+          packed[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+        }
+        if (lane == 0) bulk_wait_group_read<1>();  // the store that last read this box is done
+        __syncwarp();
+        uint8_t* box = sm.epi[q][buf];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)  // 64B swizzle: 16-byte piece j of row ``lane``
+          *reinterpret_cast<uint4*>(box + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) =
+              make_uint4(packed[4 * j], packed[4 * j + 1], packed[4 * j + 2], packed[4 * j + 3]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&p.tma_out, smem_u32(box), n0 + c * 32, m0);
+          bulk_commit_group();
+        }
+        buf ^= 1;
+      };
+      // the chunks that the next tile's accumulator shares: the last three of the
+      // first accumulator, the first three of the second
+      const int c0 = acc == 0 ? BN / 32 - OVERLAP : 0;
+      {
+        uint32_t v[OVERLAP][32];
+#pragma unroll
+        for (int i = 0; i < OVERLAP; ++i) tmem_ld32(base + (uint32_t)(c0 + i) * 32, v[i]);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&sm.acc_part), 0));
+#pragma unroll
+        for (int i = 0; i < OVERLAP; ++i) put(c0 + i, v[i]);
+      }
+      const int c1 = acc == 0 ? 0 : OVERLAP;
+#pragma unroll 1
+      for (int c = c1; c < c1 + BN / 32 - OVERLAP; ++c) {
+        uint32_t v[32];
+        tmem_ld32(base + (uint32_t)c * 32, v);
+        tmem_wait_ld();
+        put(c, v);
+      }
+      tc_fence_before();
+    }
+    if (lane == 0) bulk_wait_group<0>();  // stores complete before the CTA's shared memory goes
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // no CTA leaves while its peer may still arrive on or copy into it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Few rows
+// ---------------------------------------------------------------------------
+constexpr int kWarps = 8;
+
+struct SmallParams {
+  const uint8_t *a, *sa, *b, *sb;
+  const float *rs, *cs;
+  const __nv_bfloat16 *bias, *a2, *b2;
+  long long lda2, ldb2, ldo;
+  __nv_bfloat16* out;
+  int M, N, K, R;
+};
+
+// 32 codes and their two scales (little endian in ``sf``) as 16 pairs of f16: code * scale, exact.
+__device__ __forceinline__ void widen32(const uint4& code, uint32_t sf, uint32_t (&h)[16]) {
+  uint32_t s;  // two f16
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(s) : "h"((uint16_t)sf));
+  const __half2 s2 = *reinterpret_cast<const __half2*>(&s);
+  const __half2 lo = __low2half2(s2), hi = __high2half2(s2);
+  const uint32_t w[4] = {code.x, code.y, code.z, code.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t t[4];
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+        : "=r"(t[0]), "=r"(t[1]), "=r"(t[2]), "=r"(t[3])
+        : "r"(w[i]));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&t[j]), i < 2 ? lo : hi);
+      h[4 * i + j] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+  }
+}
+
+__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                            uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// NT: groups of 8 rows of a.
+template <int NT>
+__global__ void __launch_bounds__(kWarps * 32) small_kernel(const __grid_constant__ SmallParams p) {
+  __shared__ float red[kWarps][16][NT * 8 + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n0 = blockIdx.x * 16;
+  const int gr = lane >> 2, q = lane & 3;
+  const int units = p.K / 32, nk64 = (p.K + 63) / 64;
+  const long long kb = p.K / 2;
+  // scale word of 32 codes: two bytes of the row's place in its block of 128
+  auto sf_at = [&](int row) { return (long long)(row >> 7) * nk64 * 512 + (row & 31) * 16 + ((row & 127) >> 5) * 4; };
+  const int r0 = min(n0 + gr, p.N - 1), r1 = min(n0 + gr + 8, p.N - 1);  // rows past N are computed and dropped
+  const uint8_t *w0 = p.b + r0 * kb, *w1 = p.b + r1 * kb;
+  const uint8_t *s0 = p.sb + sf_at(r0), *s1 = p.sb + sf_at(r1);
+  float c[NT][4];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[t][i] = 0.0f;
+#pragma unroll 2
+  for (int u = warp * 4 + q; u - q < units; u += kWarps * 4) {
+    const bool in = u < units;
+    const long long so = (long long)(u >> 1) * 512 + (u & 1) * 2;
+    uint4 d0 = make_uint4(0, 0, 0, 0), d1 = d0, dx[NT];
+    uint32_t f0 = 0, f1 = 0, fx[NT];
+    if (in) {
+      d0 = __ldcs(reinterpret_cast<const uint4*>(w0 + (long long)u * 16));
+      d1 = __ldcs(reinterpret_cast<const uint4*>(w1 + (long long)u * 16));
+      f0 = *reinterpret_cast<const uint16_t*>(s0 + so);
+      f1 = *reinterpret_cast<const uint16_t*>(s1 + so);
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      dx[t] = make_uint4(0, 0, 0, 0);
+      fx[t] = 0;
+      const int row = t * 8 + gr;
+      if (in && row < p.M) {
+        dx[t] = *reinterpret_cast<const uint4*>(p.a + row * kb + (long long)u * 16);
+        fx[t] = *reinterpret_cast<const uint16_t*>(p.sa + sf_at(row) + so);
+      }
+    }
+    uint32_t h0[16], h1[16];
+    widen32(d0, f0, h0);
+    widen32(d1, f1, h1);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      uint32_t hx[16];
+      widen32(dx[t], fx[t], hx);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mma_16x8x16(c[t], h0[2 * j], h1[2 * j], h0[2 * j + 1], h1[2 * j + 1], hx[2 * j], hx[2 * j + 1]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    red[warp][gr][t * 8 + q * 2] = c[t][0];
+    red[warp][gr][t * 8 + q * 2 + 1] = c[t][1];
+    red[warp][gr + 8][t * 8 + q * 2] = c[t][2];
+    red[warp][gr + 8][t * 8 + q * 2 + 1] = c[t][3];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * NT * 8; i += kWarps * 32) {
+    const int j = i & 15, m = i >> 4, n = n0 + j;
+    if (m >= p.M || n >= p.N) continue;
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) s += red[w][j][m];
+    for (int r = 0; r < p.R; ++r)
+      s = fmaf(__bfloat162float(p.a2[m * p.lda2 + r]), __bfloat162float(p.b2[n * p.ldb2 + r]), s);
+    const float b = p.bias != nullptr ? __bfloat162float(p.bias[n]) : 0.0f;
+    p.out[m * p.ldo + n] = __float2bfloat16_rn(fmaf(s * p.rs[m], p.cs[n], b));
+  }
+}
+
+constexpr uint32_t smem_bytes() { return (uint32_t)sizeof(Smem) + 1024; }
+static_assert(smem_bytes() <= 227 * 1024, "shared memory");
+
+static cudaError_t launch_pair(const Params& p, cudaStream_t st) {
+  // per device: the attribute and the number of resident pairs belong to it
+  constexpr int kMaxDevices = 64;
+  static int max_pairs[kMaxDevices] = {};
+  static std::mutex mu;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2, 1, 1);
+  cfg.blockDim = dim3(NUM_THREADS, 1, 1);
+  cfg.dynamicSmemBytes = smem_bytes();
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  int pairs_max = 0;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (max_pairs[dev] == 0) {
+      e = cudaFuncSetAttribute(pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes());
+      if (e != cudaSuccess) return e;
+      int nsm = 0;
+      e = cudaDeviceGetAttribute(&nsm, cudaDevAttrMultiProcessorCount, dev);
+      if (e != cudaSuccess) return e;
+      cfg.gridDim = dim3((unsigned)(nsm & ~1), 1, 1);
+      // Persistent: no more pairs than can be resident at once (a pair needs two
+      // SMs of one GPC, so this can be below nsm/2).
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, pair_kernel, &cfg) != cudaSuccess || n <= 0) {
+        cudaGetLastError();
+        n = nsm / 2;
+      }
+      max_pairs[dev] = n;
+    }
+    pairs_max = max_pairs[dev];
+  }
+  const long long tiles = (long long)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
+  cfg.gridDim = dim3((unsigned)(2 * std::min<long long>(tiles, pairs_max)), 1, 1);
+  return cudaLaunchKernelEx(&cfg, pair_kernel, p);
+}
+
+static int map_rows(CUtensorMap* map, CUtensorMapDataType type, int es, const void* base, long long inner, long long rows,
+                    long long pitch_bytes) {
+  const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)pitch_bytes};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / es), (cuuint32_t)HALF};
+  const cuuint32_t estr[2] = {1u, 1u};
+  return encode_tiled(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+static int map_scales(CUtensorMap* map, const void* base, long long K, long long rows) {
+  const long long nk64 = (K + 63) / 64;
+  const cuuint64_t dims[3] = {128, (cuuint64_t)nk64, (cuuint64_t)((rows + 127) / 128)};
+  const cuuint64_t strides[2] = {SF_BLOCK, (cuuint64_t)(nk64 * SF_BLOCK)};
+  const cuuint32_t box[3] = {128, 4, 1};
+  const cuuint32_t estr[3] = {1u, 1u, 1u};
+  return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(base), dims, strides, box, estr,
+                      CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+static cudaError_t launch_small(const SmallParams& p, cudaStream_t st) {
+  const unsigned grid = (unsigned)((p.N + 15) / 16);
+  if (p.M <= 8) small_kernel<1><<<grid, kWarps * 32, 0, st>>>(p);
+  else if (p.M <= 16) small_kernel<2><<<grid, kWarps * 32, 0, st>>>(p);
+  else small_kernel<4><<<grid, kWarps * 32, 0, st>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace fp4gemm
+}  // namespace mh3
+
+using namespace mh3;
+
+extern "C" int mh3_fp4_gemm(const mh3_fp4_gemm_args* a, void* stream) {
+  const mh3::NvtxRange nvtx_range("mh3_fp4_gemm");
+  if (a == nullptr) return fail(MH3_ERR_INVALID, "mh3_fp4_gemm: null args");
+  if (a->M < 0 || a->N <= 0 || a->K <= 0 || a->R < 0) return fail(MH3_ERR_INVALID, "mh3_fp4_gemm: sizes must be positive");
+  if (a->K % 32) return fail(MH3_ERR_INVALID, "mh3_fp4_gemm: K must be a multiple of 32");
+  if (a->N % 8 || a->ldo % 8 || a->ldo < a->N) return fail(MH3_ERR_INVALID, "mh3_fp4_gemm: N and ldo must be multiples of 8, ldo >= N");
+  if (a->M > 0x7fffff00LL || a->N > 0x7fffff00LL || a->K > (1ll << 30) || a->R > (1ll << 20))
+    return fail(MH3_ERR_TOO_LARGE, "mh3_fp4_gemm: dimension too large");
+  if (a->M == 0) return MH3_OK;
+  if (((a->M + 255) / 256) * ((a->N + 255) / 256) > 0x7fff0000LL) return fail(MH3_ERR_TOO_LARGE, "mh3_fp4_gemm: too many tiles");
+  if (!a->a || !a->a_blocks || !a->a_scale || !a->b || !a->b_blocks || !a->b_scale || !a->out)
+    return fail(MH3_ERR_INVALID, "mh3_fp4_gemm: null pointer");
+  auto al16 = [](const void* p_) { return ((uintptr_t)p_ & 15u) == 0; };
+  if (!al16(a->a) || !al16(a->a_blocks) || !al16(a->b) || !al16(a->b_blocks) || !al16(a->out))
+    return fail(MH3_ERR_INVALID, "mh3_fp4_gemm: operands and out must be 16-byte aligned");
+  if (a->R > 0) {
+    if (!a->a2 || !a->b2) return fail(MH3_ERR_INVALID, "mh3_fp4_gemm: R > 0 needs a2 and b2");
+    if (a->R % 8 || a->lda2 % 8 || a->ldb2 % 8 || !al16(a->a2) || !al16(a->b2) || a->lda2 < a->R || a->ldb2 < a->R)
+      return fail(MH3_ERR_INVALID, "mh3_fp4_gemm: R and the strides of a2/b2 must be multiples of 8, 16-byte aligned");
+  }
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (a->M <= fp4gemm::kSmallM) {
+    fp4gemm::SmallParams p;
+    p.a = static_cast<const uint8_t*>(a->a);
+    p.sa = static_cast<const uint8_t*>(a->a_blocks);
+    p.b = static_cast<const uint8_t*>(a->b);
+    p.sb = static_cast<const uint8_t*>(a->b_blocks);
+    p.rs = a->a_scale;
+    p.cs = a->b_scale;
+    p.bias = static_cast<const __nv_bfloat16*>(a->bias);
+    p.a2 = static_cast<const __nv_bfloat16*>(a->a2);
+    p.b2 = static_cast<const __nv_bfloat16*>(a->b2);
+    p.lda2 = a->lda2;
+    p.ldb2 = a->ldb2;
+    p.ldo = a->ldo;
+    p.out = static_cast<__nv_bfloat16*>(a->out);
+    p.M = (int)a->M;
+    p.N = (int)a->N;
+    p.K = (int)a->K;
+    p.R = (int)a->R;
+    e = fp4gemm::launch_small(p, st);
+  } else {
+    fp4gemm::Params p;
+    memset(&p, 0, sizeof(p));
+    int rc = fp4gemm::map_rows(&p.tma_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a->a, a->K / 2, a->M, a->K / 2);
+    if (!rc) rc = fp4gemm::map_rows(&p.tma_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a->b, a->K / 2, a->N, a->K / 2);
+    if (!rc) rc = fp4gemm::map_scales(&p.tma_sa, a->a_blocks, a->K, a->M);
+    if (!rc) rc = fp4gemm::map_scales(&p.tma_sb, a->b_blocks, a->K, a->N);
+    if (!rc && a->R > 0) rc = fp4gemm::map_rows(&p.tma_a2, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a->a2, a->R, a->M, a->lda2 * 2);
+    if (!rc && a->R > 0) rc = fp4gemm::map_rows(&p.tma_b2, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a->b2, a->R, a->N, a->ldb2 * 2);
+    if (rc) return rc;
+    const cuuint64_t dims[2] = {(cuuint64_t)a->N, (cuuint64_t)a->M};
+    const cuuint64_t strides[1] = {(cuuint64_t)(a->ldo * 2)};
+    const cuuint32_t box[2] = {32u, 32u};
+    const cuuint32_t estr[2] = {1u, 1u};
+    rc = encode_tiled(&p.tma_out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a->out, dims, strides, box, estr,
+                      CU_TENSOR_MAP_SWIZZLE_64B);
+    if (rc) return rc;
+    p.M = (int)a->M;
+    p.N = (int)a->N;
+    p.K = (int)a->K;
+    p.R = (int)a->R;
+    p.rs = a->a_scale;
+    p.cs = a->b_scale;
+    p.bias = static_cast<const __nv_bfloat16*>(a->bias);
+    p.err = a->err ? a->err : device_error_word();
+    p.timeout_ns = a->timeout_ns ? a->timeout_ns : 4000000000ull;
+    p.test_flags = a->test_flags;
+    e = fp4gemm::launch_pair(p, st);
+  }
+  return e == cudaSuccess ? MH3_OK : fail_cuda(e, "mh3_fp4_gemm launch");
+}

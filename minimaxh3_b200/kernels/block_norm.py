@@ -1,0 +1,241 @@
+"""The norms before and after a transformer block, with modulation, gate and residual.
+
+A diffusion transformer's block normalises its stream, scales and shifts it by
+the timestep's modulation, and adds its gated output back; the model does this
+between the linears and attention that this package replaces (the reference has
+no kernel for it).  ``norm_modulate`` is the norm before a block;
+``gated_residual_norm`` joins the norm on a block's output, the gate, the
+residual and the next block's ``norm_modulate`` in one pass (csrc/block_norm.cu).
+Both are differentiable in every tensor argument.
+
+The modulation belongs to a batch item, to a packed sequence (``cu_seqlens``, as
+``fp8_attention_varlen``) or to each token.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import ops as _ops
+
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_MODS = "Tensor x, Tensor? y, Tensor? gate, Tensor? scale, Tensor? shift, Tensor? weight, Tensor? bias, Tensor? y_weight, Tensor? cu"
+_CONF = "int norm, int y_norm, float eps, float alpha, bool per_token"
+_LIB = torch.library.Library("mh3", "FRAGMENT")
+_LIB.define(f"block_norm({_MODS}, {_CONF}, bool want_stats) -> (Tensor, Tensor, Tensor)")
+_LIB.define(f"block_norm_backward(Tensor? dr, Tensor? dh, {_MODS}, Tensor stats, {_CONF}, bool[] want) -> Tensor[]")
+
+
+def _backward_cuda(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu, stats, norm, y_norm, eps, alpha, per_token, want):
+    grads = _ops.block_norm_bwd(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu, stats, norm, y_norm, eps, alpha,
+                                per_token, want)
+    return [x.new_empty(0) if g is None else g for g in grads]
+
+
+_LIB.impl("block_norm", _ops.block_norm_fwd, "CUDA")
+_LIB.impl("block_norm_backward", _backward_cuda, "CUDA")
+
+
+@torch.library.register_fake("mh3::block_norm", lib=_LIB)
+def _(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_norm, eps, alpha, per_token, want_stats):
+    rows = 1
+    for n in x.shape[:-1]:
+        rows = rows * n
+    none = x.new_empty(0)
+    return (x.new_empty(x.shape) if y is not None else none, x.new_empty(x.shape) if norm else none.clone(),
+            x.new_empty((rows, 4), dtype=torch.float32) if want_stats else none.clone())
+
+
+@torch.library.register_fake("mh3::block_norm_backward", lib=_LIB)
+def _(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu, stats, norm, y_norm, eps, alpha, per_token, want):
+    ts = (x, y, gate, scale, shift, weight, bias, y_weight)
+    return [t.new_empty(t.shape) if w and t is not None else x.new_empty(0) for t, w in zip(ts, want)]
+
+
+class _BlockNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_norm, eps, alpha, per_token):
+        r, h, stats = torch.ops.mh3.block_norm(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_norm, eps, alpha,
+                                               per_token, True)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, y, gate, scale, shift, weight, bias, y_weight, cu, stats)
+        ctx.conf = (norm, y_norm, eps, alpha, per_token)
+        return r, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dr, dh):
+        x, y, gate, scale, shift, weight, bias, y_weight, cu, stats = ctx.saved_tensors
+        if y is None:
+            dr = None
+        if not ctx.conf[0]:
+            dh = None
+        if dr is None and dh is None:
+            return (None,) * 14
+        want = [bool(n) and t is not None for n, t in zip(ctx.needs_input_grad, (x, y, gate, scale, shift, weight, bias, y_weight))]
+        grads = torch.ops.mh3.block_norm_backward(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu, stats, *ctx.conf, want)
+        return tuple(g if w else None for g, w in zip(grads, want)) + (None,) * 6
+
+
+def _check_stream(what, name, t, like=None):
+    if not isinstance(t, torch.Tensor) or t.dim() not in (2, 3) or t.dtype not in _TYPES:
+        raise ValueError(f"{what}: {name} must be a bf16, f16 or f32 tensor [B, S, C] or [T, C]")
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{what}: {name} must have x's shape, dtype and device")
+
+
+def _check_cu(what, x, cu):
+    if cu is None:
+        return
+    if not isinstance(cu, torch.Tensor) or cu.dtype != torch.int32 or cu.dim() != 1 or cu.numel() < 2 or cu.device != x.device:
+        raise ValueError(f"{what}: cu_seqlens must be an int32 tensor [nseq+1] on x's device")
+    if x.dim() != 2:
+        raise ValueError(f"{what}: cu_seqlens needs packed x [T, C]")
+
+
+def _modulation(what, x, cu, mods):
+    """The named modulation tensors as [groups, C] each, or of x's shape each if one of them has a row for each token."""
+    C = x.shape[-1]
+    groups = cu.numel() - 1 if cu is not None else x.shape[0] if x.dim() == 3 else 1
+    out, per_token = {}, False
+    for name, m in mods.items():
+        if m is None:
+            out[name] = None
+            continue
+        if not isinstance(m, torch.Tensor) or m.dtype not in _TYPES or m.device != x.device or m.dim() < 1 or m.shape[-1] != C:
+            raise ValueError(f"{what}: {name} must be a bf16, f16 or f32 tensor [..., C] on x's device")
+        lead = tuple(m.shape[:-1])
+        if x.dim() == 3:
+            B, S = x.shape[:2]
+            if len(lead) == 2 and lead[1] == 1 and lead[0] in (1, B):
+                m, kind = m[:, 0], "group"
+            elif lead in ((), (1,), (B,)):
+                kind = "group"
+            elif len(lead) == 2 and lead[0] in (1, B) and lead[1] == S:
+                kind = "token"
+            else:
+                raise ValueError(f"{what}: {name} must be [C], [B, C], [B, 1, C] or [B, S, C]")
+        elif lead in ((), (1,), (groups,)):
+            kind = "group"
+        elif lead == (x.shape[0],):
+            kind = "token"
+        else:
+            raise ValueError(f"{what}: {name} must be [C], [T, C], or with cu_seqlens [nseq, C]")
+        per_token = per_token or kind == "token"
+        out[name] = (kind, m)
+    for name, km in out.items():
+        if km is None:
+            continue
+        kind, m = km
+        if not per_token:
+            m = m.expand(groups, C)
+        elif kind == "token":
+            m = m.expand(x.shape)
+        elif cu is not None and m.dim() == 2 and m.shape[0] != 1:
+            raise ValueError(f"{what}: {name} is per sequence while another modulation is per token")
+        else:
+            m = (m if m.dim() == 1 or x.dim() == 2 else m.unsqueeze(1)).expand(x.shape)
+        out[name] = m
+    return out, per_token
+
+
+def _channels(what, x, vecs):
+    for name, v in vecs.items():
+        if v is not None and (not isinstance(v, torch.Tensor) or v.dtype not in _TYPES or tuple(v.shape) != (x.shape[-1],)
+                              or v.device != x.device):
+            raise ValueError(f"{what}: {name} must be a bf16, f16 or f32 tensor [C] on x's device")
+
+
+def _run(x, y, m, weight, bias, y_weight, cu, norm, y_norm, eps, alpha, per_token):
+    args = (x, y, m.get("gate"), m["scale"], m["shift"], weight, bias, y_weight, cu, norm, y_norm, float(eps), float(alpha),
+            per_token)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:8]):
+        return _BlockNormFn.apply(*args)
+    return torch.ops.mh3.block_norm(*args, False)[:2]
+
+
+def _finish_checks(what, x, eps):
+    if not 1 <= x.shape[-1] <= 8192:
+        raise ValueError(f"{what}: 1 to 8192 channels")
+    if not float(eps) >= 0.0:
+        raise ValueError(f"{what}: eps must not be negative")
+    if not x.is_cuda:
+        raise ValueError(f"{what}: expected CUDA tensors")
+
+
+def norm_modulate(
+    x: torch.Tensor,
+    scale: torch.Tensor | None = None,
+    shift: torch.Tensor | None = None,
+    *,
+    weight: torch.Tensor | None = None,
+    bias: torch.Tensor | None = None,
+    norm: str = "layer",
+    eps: float = 1e-6,
+    cu_seqlens: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``(norm(x) * weight + bias) * (1 + scale) + shift`` over the last dimension, in x's dtype.
+
+    x [B, S, C] or [T, C], bf16, f16 or f32, C <= 8192; ``norm`` "layer" or
+    "rms".  scale / shift: [C], [B, C], [B, 1, C], or a row for each token
+    ([B, S, C] / [T, C]); with ``cu_seqlens`` (int32 [nseq+1] on the device) also
+    [nseq, C], and rows outside every sequence give zeros.  weight / bias [C].
+    Modulation and weights may be of other float types than x (kept in f32
+    beside a bf16 stream); None leaves that term out.  Statistics and sums are
+    f32, the result is rounded once.
+    """
+    what = "norm_modulate"
+    _check_stream(what, "x", x)
+    _check_cu(what, x, cu_seqlens)
+    if norm not in ("layer", "rms"):
+        raise ValueError(f"{what}: norm must be 'layer' or 'rms'")
+    m, per_token = _modulation(what, x, cu_seqlens, {"scale": scale, "shift": shift})
+    _channels(what, x, {"weight": weight, "bias": bias})
+    _finish_checks(what, x, eps)
+    cu = None if cu_seqlens is None else cu_seqlens.contiguous()
+    return _run(x, None, m, weight, bias, None, cu, _ops.NORM_KINDS[norm], 0, eps, 1.0, per_token)[1]
+
+
+def gated_residual_norm(
+    x: torch.Tensor,
+    y: torch.Tensor,
+    gate: torch.Tensor | None = None,
+    scale: torch.Tensor | None = None,
+    shift: torch.Tensor | None = None,
+    *,
+    weight: torch.Tensor | None = None,
+    bias: torch.Tensor | None = None,
+    norm: str = "layer",
+    y_norm: str = "none",
+    y_weight: torch.Tensor | None = None,
+    residual_scale: float = 1.0,
+    eps: float = 1e-6,
+    cu_seqlens: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """The stream after a block and the next block's normed input, ``(r, h)``:
+
+    ``r = residual_scale * x + gate * (y_norm(y) * y_weight)`` and
+    ``h = (norm(r) * weight + bias) * (1 + scale) + shift``.
+
+    x is the stream, y the block's output (same shape and dtype).  ``y_norm``
+    "none", "rms" or "layer" is a norm on the block's output; y_weight [C] needs
+    one.  ``norm="none"`` leaves h out (returns ``(r, None)``).  gate takes the
+    forms of scale and shift; see ``norm_modulate`` for the rest.  h is computed
+    from r before r is rounded to x's dtype.
+    """
+    what = "gated_residual_norm"
+    _check_stream(what, "x", x)
+    _check_stream(what, "y", y, x)
+    _check_cu(what, x, cu_seqlens)
+    if norm not in _ops.NORM_KINDS or y_norm not in _ops.NORM_KINDS:
+        raise ValueError(f"{what}: norm and y_norm must be 'none', 'rms' or 'layer'")
+    if norm == "none" and any(t is not None for t in (scale, shift, weight, bias)):
+        raise ValueError(f"{what}: scale, shift, weight and bias need a norm")
+    if y_norm == "none" and y_weight is not None:
+        raise ValueError(f"{what}: y_weight needs y_norm")
+    m, per_token = _modulation(what, x, cu_seqlens, {"gate": gate, "scale": scale, "shift": shift})
+    _channels(what, x, {"weight": weight, "bias": bias, "y_weight": y_weight})
+    _finish_checks(what, x, eps)
+    cu = None if cu_seqlens is None else cu_seqlens.contiguous()
+    r, h = _run(x, y, m, weight, bias, y_weight, cu, _ops.NORM_KINDS[norm], _ops.NORM_KINDS[y_norm], eps, residual_scale, per_token)
+    return r, None if norm == "none" else h

@@ -1,0 +1,123 @@
+"""4-bit linear layers beside the FP8 ones: microscaled e2m1 weights and activations.
+
+The same place, policy and LoRA contract as ``fp8_linear`` (the reference's
+``kernels/fp8_linear.py``, which stops at 8 bits): ``FP4Linear`` replaces an
+``nn.Linear``, keeps the mutable ``adapters`` list of ``(A, B, scale)`` and runs
+an activation rounding plus one tcgen05 GEMM that applies the scales, the bias
+and every adapter's delta and writes bf16 once.  Weights take 0.5625 bytes each.
+
+A 4-bit matrix is three tensors ``(values, blocks, scale)``: see ``quantize_fp4``.
+Registered as ``torch.ops.mh3.fp4_linear`` with a fake implementation for
+``torch.compile``.  Inference only: no gradient is defined.
+"""
+from __future__ import annotations
+
+import torch
+import torch.nn as nn
+
+from .. import ops as _ops
+from .fp8_linear import convert_linears
+
+_LIB = torch.library.Library("mh3", "FRAGMENT")
+_LIB.define("fp4_linear(Tensor x2d, Tensor w4, Tensor w_blocks, Tensor w_scale, Tensor? bias, Tensor[] lora_a, "
+            "Tensor[] lora_b, float[] lora_scale) -> Tensor")
+
+
+def _fp4_linear_cuda(x2d, w4, w_blocks, w_scale, bias, lora_a, lora_b, lora_scale):
+    return _ops.fp4_linear(x2d, w4, w_blocks, w_scale, bias, list(zip(lora_a, lora_b, lora_scale)))
+
+
+_LIB.impl("fp4_linear", _fp4_linear_cuda, "CUDA")
+
+
+@torch.library.register_fake("mh3::fp4_linear", lib=_LIB)
+def _(x2d, w4, w_blocks, w_scale, bias, lora_a, lora_b, lora_scale):
+    return x2d.new_empty((x2d.shape[0], w4.shape[0]), dtype=torch.bfloat16)
+
+
+def quantize_fp4(x2d: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """x2d [M, K] (bf16, f16 or f32, K a multiple of 32) rounded to 4 bits: ``(values, blocks, scale)``.
+
+    values uint8 [M, K/2]: element 2j in the low half of byte j, 2j+1 in the high
+    half, e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign).  blocks
+    float8_e4m3fn [ceil(M/128), ceil(K/64), 32, 4, 4]: the scale of elements
+    16b..16b+15 of row m at [m // 128, b // 4, m % 32, m % 128 // 32, b % 4].
+    scale float32 [M, 1]: a power of two that puts the row's largest block scale
+    at the upper end of e4m3.  The value is code * block * scale; all roundings
+    are to nearest even.  A row that holds an infinity or NaN gets scale NaN.
+    """
+    return _ops.quantize_fp4(x2d)
+
+
+def dequantize_fp4(values: torch.Tensor, blocks: torch.Tensor, scale: torch.Tensor,
+                   dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The [M, K] numbers that a 4-bit matrix stands for (exact in bfloat16 and float32)."""
+    return _ops.dequantize_fp4(values, blocks, scale, dtype)
+
+
+def fp4_matmul(a, b, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """bf16 ``a b^T + bias`` of two 4-bit matrices ``(values, blocks, scale)``, a [M, K], b [N, K], N a multiple of 8."""
+    return _ops.fp4_gemm(tuple(a), tuple(b), bias=bias)
+
+
+def fp4_linear(x: torch.Tensor, w4: torch.Tensor, w_blocks: torch.Tensor, w_scale: torch.Tensor,
+               bias: torch.Tensor | None = None, adapters=()) -> torch.Tensor:
+    """bf16 ``x W^T + bias + sum_i scale_i (x A_i^T) B_i^T`` with W [N, K] in 4 bits and x [..., K] rounded to 4 bits.
+
+    (w4, w_blocks, w_scale) is ``quantize_fp4(W)``; adapters are
+    ``(A [r, K], B [N, r], scale)`` and see the unrounded x.  One to 32 rows run a
+    kernel that streams W once; more run on the tensor cores' 4-bit rate.
+    """
+    N, K = _ops.check_fp4(w4, w_blocks, w_scale, "fp4_linear weight")
+    if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.shape[-1] != K or not x.is_floating_point():
+        raise ValueError(f"fp4_linear: x must be a float tensor [..., {K}]")
+    if N % 8 or N == 0:
+        raise ValueError("fp4_linear: the number of output features must be a positive multiple of 8")
+    if not x.is_cuda or x.device != w4.device:
+        raise ValueError("fp4_linear: x and the weight must be on one CUDA device")
+    out = torch.ops.mh3.fp4_linear(x.reshape(-1, K), w4, w_blocks, w_scale, bias, [a for a, _, _ in adapters],
+                                   [b for _, b, _ in adapters], [float(s) for _, _, s in adapters])
+    return out.reshape(*x.shape[:-1], N)
+
+
+class FP4Linear(nn.Module):
+    """e2m1 weights with e4m3 block scales; fused scaled GEMM forward (the 4-bit ``FP8Linear``)."""
+
+    def __init__(self, in_features: int, out_features: int) -> None:
+        super().__init__()
+        self.in_features = in_features
+        self.out_features = out_features
+        self.adapters: list[tuple[torch.Tensor, torch.Tensor, float]] = []
+
+    @classmethod
+    @torch.no_grad()
+    def from_linear(cls, linear: nn.Linear) -> "FP4Linear":
+        """Round ``linear``'s weight once and free it (buffers ``w4``, ``w_blocks``, ``w_scale``, ``bias``)."""
+        if linear.in_features % 32 or linear.out_features % 8:
+            raise ValueError("FP4Linear needs in_features a multiple of 32 and out_features a multiple of 8")
+        mod = cls(linear.in_features, linear.out_features)
+        weight = linear.weight.detach()
+        if not weight.is_cuda:
+            weight = weight.cuda()
+        if weight.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+            weight = weight.to(torch.float32)
+        for name, t in zip(("w4", "w_blocks", "w_scale"), quantize_fp4(weight)):
+            mod.register_buffer(name, t)
+        bias = None
+        if linear.bias is not None:
+            bias = linear.bias.detach().to(device=mod.w4.device, dtype=torch.bfloat16).contiguous()
+        mod.register_buffer("bias", bias)
+        if isinstance(getattr(linear, "adapters", None), list):
+            mod.adapters = list(linear.adapters)
+        linear.weight = None
+        linear.bias = None
+        return mod
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return fp4_linear(x, self.w4, self.w_blocks, self.w_scale, self.bias, self.adapters).to(x.dtype)
+
+
+def convert_transformer_to_fp4(transformer: nn.Module, exclude_patterns, keep_edge_blocks: int) -> int:
+    """``convert_transformer_to_fp8``'s policy with ``FP4Linear``: in features a multiple of 32, out features of 16."""
+    return convert_linears(transformer, exclude_patterns, keep_edge_blocks, FP4Linear.from_linear,
+                           lambda m: m.in_features % 32 == 0 and m.out_features % 16 == 0)

@@ -43,6 +43,7 @@ import torch
 import os
 
 from .. import ops as _ops
+from .rotary import Rotary, rotary_axes
 
 LOG2E = 1.4426950408889634
 
@@ -198,6 +199,7 @@ def fp8_attention_varlen(
     cu_seqlens_k: torch.Tensor,
     max_seqlen_q: int,
     scale: float | None = None,
+    rotary: Rotary | None = None,
 ) -> torch.Tensor:
     """Non-causal FP8 attention over packed sequences.
 
@@ -209,7 +211,11 @@ def fp8_attention_varlen(
     V/scale for the f16 PV product unless ``MH3_PV_DTYPE=e4m3``).  Returns
     [Tq, H, D] in q's dtype; rows outside every sequence are not written
     (their values are unspecified).  ``scale`` defaults to 1/sqrt(D).
+    ``rotary`` (self-attention, Tq == Tk): q and k are turned by their tokens'
+    positions first (``rotary_axes``, positions [Tq, axes]).
     """
     _check_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q)
+    if rotary is not None:
+        q, k = rotary_axes(q, k, rotary.positions, rotary.axes_dim, rotary.theta, rotary.interleaved)
     return torch.ops.mh3.fp8_attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k, int(max_seqlen_q),
                                               math.nan if scale is None else float(scale))

@@ -125,13 +125,9 @@ def _patterns(exclude_patterns) -> list[str]:
     return [p.strip().lower() for p in items if p.strip()]
 
 
-def convert_transformer_to_fp8(transformer: nn.Module, exclude_patterns, keep_edge_blocks: int) -> int:
-    """Swap eligible ``nn.Linear`` layers of the primary blocks for ``FP8Linear`` (:125-162).
-
-    Eligible: inside blocks [keep, n-keep) of the primary block list, in and
-    out features both multiples of 16, and no exclusion pattern occurring in
-    the lower-cased dotted path ``<list>.<idx>.<sub>``.  Returns the count.
-    """
+def convert_linears(transformer: nn.Module, exclude_patterns, keep_edge_blocks: int, make, fits) -> int:
+    """Swap the ``nn.Linear`` layers of the primary blocks that ``fits`` accepts for ``make(linear)``
+    (the policy of ``convert_transformer_to_fp8``).  Returns the count."""
     pats = _patterns(exclude_patterns)
     list_name, blocks = find_primary_block_list(transformer)
     n = len(blocks)
@@ -143,12 +139,12 @@ def convert_transformer_to_fp8(transformer: nn.Module, exclude_patterns, keep_ed
         for sub_name, sub in list(block.named_modules()):
             if not isinstance(sub, nn.Linear):
                 continue
-            if sub.in_features % 16 or sub.out_features % 16:
+            if not fits(sub):
                 continue
             path = (f"{list_name}.{idx}.{sub_name}" if sub_name else f"{list_name}.{idx}").lower()
             if any(p in path for p in pats):
                 continue
-            new = FP8Linear.from_linear(sub)
+            new = make(sub)
             if not sub_name:
                 blocks[idx] = new
             else:
@@ -159,3 +155,14 @@ def convert_transformer_to_fp8(transformer: nn.Module, exclude_patterns, keep_ed
     if torch.cuda.is_available():
         torch.cuda.empty_cache()
     return count
+
+
+def convert_transformer_to_fp8(transformer: nn.Module, exclude_patterns, keep_edge_blocks: int) -> int:
+    """Swap eligible ``nn.Linear`` layers of the primary blocks for ``FP8Linear`` (:125-162).
+
+    Eligible: inside blocks [keep, n-keep) of the primary block list, in and
+    out features both multiples of 16, and no exclusion pattern occurring in
+    the lower-cased dotted path ``<list>.<idx>.<sub>``.  Returns the count.
+    """
+    return convert_linears(transformer, exclude_patterns, keep_edge_blocks, FP8Linear.from_linear,
+                           lambda m: m.in_features % 16 == 0 and m.out_features % 16 == 0)

@@ -8,7 +8,7 @@ GEMM, then per adapter two skinny matmuls and a read-modify-write of the
 whole output (fp8_linear.py:45-55).
 
 ``attach_lora_registry`` keeps that function's contract (a registry of every
-``nn.Linear`` / ``FP8Linear`` by name, an ``adapters`` list on each, the
+``nn.Linear`` / ``FP8Linear`` / ``FP4Linear`` by name, an ``adapters`` list on each, the
 ``nn.Linear`` forwards wrapped once, ``_lora_wrapped`` set) but the wrapped
 forward runs ``torch.ops.mh3.linear_lora``: the adapters' rank-r product is
 accumulated into the same tcgen05 accumulator as ``x W^T`` and the output is
@@ -24,6 +24,7 @@ import torch
 import torch.nn as nn
 
 from .. import ops as _ops
+from .fp4_linear import FP4Linear
 from .fp8_linear import FP8Linear, apply_lora_adapters
 
 
@@ -61,7 +62,7 @@ def attach_lora_registry(transformer: nn.Module) -> dict[str, nn.Module]:
     """runtime/lora.py:206-226 with the fused forward for ``nn.Linear`` layers."""
     registry: dict[str, nn.Module] = {}
     for name, mod in transformer.named_modules():
-        if isinstance(mod, (nn.Linear, FP8Linear)):
+        if isinstance(mod, (nn.Linear, FP8Linear, FP4Linear)):
             registry[name] = mod
             if not hasattr(mod, "adapters") or not isinstance(mod.adapters, list):
                 mod.adapters = []

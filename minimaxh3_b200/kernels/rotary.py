@@ -1,0 +1,121 @@
+"""Rotary positions with several axes (time, height, width) for video, images and audio.
+
+The model turns Q and K by their tokens' positions between the projection and
+attention; the reference's kernels take them already turned, so this has no
+counterpart there.  ``rotary_axes`` does both tensors in one launch
+(csrc/rotary.cu), on the layouts the attention entry points take, and is
+differentiable (the gradient is the inverse rotation, the same kernel).
+``fp8_attention_varlen(..., rotary=Rotary(...))`` applies it on the way in.
+"""
+from __future__ import annotations
+
+import typing
+
+import torch
+
+from .. import ops as _ops
+
+_LIB = torch.library.Library("mh3", "FRAGMENT")
+_LIB.define("rotary_axes(Tensor q, Tensor? k, Tensor positions, int[] axes_dim, float[] theta, bool interleaved, "
+            "bool inverse) -> (Tensor, Tensor)")
+
+
+def _rotary_cuda(q, k, positions, axes_dim, theta, interleaved, inverse):
+    oq, ok = _ops.rotary(q, k, positions, axes_dim, theta, interleaved, inverse)
+    return oq, q.new_empty(0) if ok is None else ok
+
+
+_LIB.impl("rotary_axes", _rotary_cuda, "CUDA")
+
+
+@torch.library.register_fake("mh3::rotary_axes", lib=_LIB)
+def _(q, k, positions, axes_dim, theta, interleaved, inverse):
+    return torch.empty_like(q), q.new_empty(0) if k is None else torch.empty_like(k)
+
+
+class _RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, axes_dim, theta, interleaved, inverse):
+        ctx.save_for_backward(positions)
+        ctx.rest = (axes_dim, theta, interleaved)
+        ctx.inverse, ctx.has_k = inverse, k is not None
+        return torch.ops.mh3.rotary_axes(q, k, positions, axes_dim, theta, interleaved, inverse)
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        (positions,) = ctx.saved_tensors
+        dq, dk = _RotaryFn.apply(gq, gk if ctx.has_k else None, positions, *ctx.rest, not ctx.inverse)
+        return dq, dk if ctx.has_k else None, None, None, None, None, None
+
+
+class Rotary(typing.NamedTuple):
+    """What ``rotary_axes`` takes beside the tensors."""
+
+    positions: torch.Tensor
+    axes_dim: typing.Sequence[int]
+    theta: typing.Union[float, typing.Sequence[float]] = 10000.0
+    interleaved: bool = True
+
+
+def _check(q, k, positions, axes_dim, theta):
+    for name, t in (("q", q), ("k", k)):
+        if name == "k" and t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or t.dim() not in (3, 4):
+            raise ValueError(f"rotary_axes: {name} must be a tensor [B, H, S, D] or packed [T, H, D]")
+        if t.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+            raise ValueError(f"rotary_axes: unsupported dtype {t.dtype} (bf16, f16 or f32)")
+    packed = q.dim() == 3
+    tokens = q.shape[0] if packed else q.shape[2]
+    if k is not None:
+        if k.dim() != q.dim() or k.dtype != q.dtype or k.device != q.device or k.shape[-1] != q.shape[-1]:
+            raise ValueError("rotary_axes: q and k must agree in dimensions, dtype, device and head dim")
+        if (k.shape[0] if packed else k.shape[2]) != tokens or (not packed and k.shape[0] != q.shape[0]):
+            raise ValueError("rotary_axes: q and k must have the same tokens")
+    axes = [int(d) for d in axes_dim]
+    if not 1 <= len(axes) <= 4 or any(d < 0 or d % 2 for d in axes) or not 0 < sum(axes) <= q.shape[-1]:
+        raise ValueError("rotary_axes: axes_dim is 1 to 4 even widths whose sum is positive and at most the head dim")
+    if q.shape[-1] > 256:
+        raise ValueError("rotary_axes: the head dim must be at most 256")
+    thetas = [float(theta)] * len(axes) if isinstance(theta, (int, float)) else [float(t) for t in theta]
+    if len(thetas) != len(axes) or any(not 0.0 < t <= 1e300 for t in thetas):
+        raise ValueError("rotary_axes: theta is one positive number, or one for each axis")
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64, torch.float32):
+        raise ValueError("rotary_axes: positions must be an int32, int64 or float32 tensor")
+    lead = tuple(positions.shape[:-1])
+    if positions.dim() not in (2, 3) or positions.shape[-1] != len(axes) or lead not in (
+            ((tokens,),) if packed else ((tokens,), (1, tokens), (q.shape[0], tokens))):
+        raise ValueError("rotary_axes: positions must be [S, axes] or [B, S, axes] (packed: [T, axes])")
+    if positions.device != q.device:
+        raise ValueError("rotary_axes: positions must be on q's device")
+    if not q.is_cuda:
+        raise ValueError("rotary_axes: expected CUDA tensors")
+    return axes, thetas
+
+
+def rotary_axes(
+    q: torch.Tensor,
+    k: torch.Tensor | None,
+    positions: torch.Tensor,
+    axes_dim: typing.Sequence[int],
+    theta: float | typing.Sequence[float] = 10000.0,
+    interleaved: bool = True,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Q and K turned by their tokens' positions; new tensors of the same shapes and dtype.
+
+    q [B, H, S, D] and k [B, Hk, S, D] (any strides with contiguous channels; the
+    head counts may differ; k may be None), or packed [T, H, D] as
+    ``fp8_attention_varlen`` takes them; bf16, f16 or f32, D <= 256.
+    ``positions`` [S, axes], [B, S, axes] or packed [T, axes]: int32, int64, or
+    float32 for tokens between grid points (audio beside video).  ``axes_dim``:
+    the even number of channels each axis turns, in order; channels past their
+    sum are copied.  The j-th of an axis's d/2 pairs turns by position *
+    theta^(-2j/d).  A pair is two neighbouring channels, or with
+    ``interleaved=False`` channels p and p + sum(axes_dim)/2.
+    """
+    axes, thetas = _check(q, k, positions, axes_dim, theta)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        oq, ok = _RotaryFn.apply(q, k, positions, axes, thetas, bool(interleaved), False)
+    else:
+        oq, ok = torch.ops.mh3.rotary_axes(q, k, positions, axes, thetas, bool(interleaved), False)
+    return oq, None if k is None else ok

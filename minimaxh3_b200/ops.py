@@ -56,6 +56,9 @@ def _dtype_code(dt: torch.dtype) -> int:
     raise ValueError(f"unsupported dtype {dt} (bf16 or fp16)")
 
 
+_FLOAT_CODE = {torch.bfloat16: _lib.MH3_DTYPE_BF16, torch.float16: _lib.MH3_DTYPE_F16, torch.float32: _lib.MH3_DTYPE_F32}
+
+
 def _require_cuda(*ts):
     for t in ts:
         if t is not None and not t.is_cuda:
@@ -667,6 +670,335 @@ def linear_lora(x2d: torch.Tensor, weight: torch.Tensor, bias, adapters) -> torc
         A_cat, b2 = _lora_operands(adapters, N, K, x2d.device)
         a2 = scaled_gemm(x2d, A_cat)
     return scaled_gemm(x2d, w, bias=bias, a2=a2, b2=b2)
+
+
+# ---------------------------------------------------------------------------
+# microscaled 4-bit rows and their product
+# ---------------------------------------------------------------------------
+
+
+def _fp4_blocks_shape(M: int, K: int):
+    return (_cdiv(M, BLOCK), _cdiv(K, 64), 32, 4, 4)
+
+
+def check_fp4(x4, blocks, scale, what: str):
+    """(M, K) of a 4-bit matrix (see ``quantize_fp4``); raises ValueError for anything else."""
+    for name, t, dt in (("values", x4, torch.uint8), ("block scales", blocks, E4M3), ("row scales", scale, torch.float32)):
+        if not isinstance(t, torch.Tensor) or t.dtype != dt:
+            raise ValueError(f"{what}: {name} must be a {dt} tensor")
+    if x4.dim() != 2 or x4.shape[1] == 0 or x4.shape[1] % 16:
+        raise ValueError(f"{what}: values must be [M, K/2] bytes with K a multiple of 32")
+    M, K = x4.shape[0], 2 * x4.shape[1]
+    if tuple(blocks.shape) != _fp4_blocks_shape(M, K):
+        raise ValueError(f"{what}: block scales must be of shape {_fp4_blocks_shape(M, K)}, got {tuple(blocks.shape)}")
+    if scale.numel() != M:
+        raise ValueError(f"{what}: need one row scale for each of {M} rows")
+    if blocks.device != x4.device or scale.device != x4.device:
+        raise ValueError(f"{what}: values and scales must be on one device")
+    if not (x4.is_contiguous() and blocks.is_contiguous() and scale.is_contiguous()):
+        raise ValueError(f"{what}: values and scales must be contiguous")
+    return M, K
+
+
+def _check_fp4_aligned(x4, blocks, what: str):
+    if x4.data_ptr() % 16 or blocks.data_ptr() % 16:
+        raise ValueError(f"{what}: values and block scales must be 16-byte aligned")
+
+
+def quantize_fp4(x2d: torch.Tensor):
+    """x2d [M,K] (bf16, f16 or f32) as 4-bit rows (``mh3_quantize_fp4``): ``(x4, blocks, scale)``.
+
+    x4 uint8 [M, K/2], two e2m1 codes a byte; blocks float8_e4m3fn
+    [ceil(M/128), ceil(K/64), 32, 4, 4], row 32 i + j of a block of 128 at
+    [j, i], one scale for 16 elements; scale float32 [M, 1], a power of two."""
+    if not isinstance(x2d, torch.Tensor) or x2d.dim() != 2:
+        raise ValueError("quantize_fp4 expects a 2D CUDA tensor")
+    if x2d.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError(f"quantize_fp4: unsupported dtype {x2d.dtype} (bf16, f16 or f32)")
+    M, K = x2d.shape
+    if K == 0 or K % 32:
+        raise ValueError("quantize_fp4: K must be a positive multiple of 32")
+    if not x2d.is_cuda:
+        raise ValueError("quantize_fp4 expects a 2D CUDA tensor")
+    if x2d.stride(1) != 1:
+        x2d = x2d.contiguous()
+    lib = _lib.load()
+    dev = x2d.device
+    x4 = torch.empty((M, K // 2), dtype=torch.uint8, device=dev)
+    blocks = torch.empty(_fp4_blocks_shape(M, K), dtype=E4M3, device=dev)
+    scale = torch.empty((M, 1), dtype=torch.float32, device=dev)
+    if M:
+        with torch.cuda.device(dev):
+            rc = lib.mh3_quantize_fp4(x2d.data_ptr(), x2d.stride(0), _FLOAT_CODE[x2d.dtype], M, K, x4.data_ptr(),
+                                      blocks.data_ptr(), scale.data_ptr(), _stream(dev))
+        _lib.check(rc, "mh3_quantize_fp4")
+    return x4, blocks, scale
+
+
+def dequantize_fp4(x4: torch.Tensor, blocks: torch.Tensor, scale: torch.Tensor,
+                   dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The [M, K] values of a 4-bit matrix, exact in bf16 and float32 (``mh3_dequantize_fp4``)."""
+    M, K = check_fp4(x4, blocks, scale, "dequantize_fp4")
+    _check_fp4_aligned(x4, blocks, "dequantize_fp4")
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("dequantize_fp4: dtype must be bfloat16 or float32")
+    _require_cuda(x4)
+    lib = _lib.load()
+    out = torch.empty((M, K), dtype=dtype, device=x4.device)
+    if M:
+        with torch.cuda.device(x4.device):
+            rc = lib.mh3_dequantize_fp4(x4.data_ptr(), blocks.data_ptr(), scale.data_ptr(), M, K, _FLOAT_CODE[dtype],
+                                        out.data_ptr(), _stream(x4.device))
+        _lib.check(rc, "mh3_dequantize_fp4")
+    return out
+
+
+def fp4_gemm(a, b, bias=None, a2=None, b2=None, out: torch.Tensor | None = None, err: torch.Tensor | None = None,
+             timeout_ns: int = 0, test_flags: int = 0) -> torch.Tensor:
+    """``mh3_fp4_gemm``: bf16 [M,N] of two 4-bit matrices ``(values, blocks, scale)``, a [M,K] and b [N,K].
+
+    bias: [N], used in bf16; a2 [M,R], b2 [N,R] bf16: a low-rank product added
+    before the row scales are applied; ``err``, ``timeout_ns`` and
+    ``test_flags`` as in ``scaled_gemm``."""
+    M, K = check_fp4(*a, "fp4_gemm a")
+    N, Kb = check_fp4(*b, "fp4_gemm b")
+    if K != Kb:
+        raise ValueError("fp4_gemm: a is [M,K] and b is [N,K]")
+    _check_fp4_aligned(*a[:2], "fp4_gemm a")
+    _check_fp4_aligned(*b[:2], "fp4_gemm b")
+    if N == 0 or N % 8:
+        raise ValueError("fp4_gemm: N must be a positive multiple of 8")
+    dev = a[0].device
+    _require_cuda(a[0], b[0])
+    g = _lib.Fp4GemmArgs()
+    g.M, g.N, g.K = M, N, K
+    g.a, g.a_blocks, g.a_scale = (t.data_ptr() for t in a)
+    g.b, g.b_blocks, g.b_scale = (t.data_ptr() for t in b)
+    for name, t in (("b", b[0]), ("bias", bias), ("a2", a2), ("b2", b2), ("out", out), ("err", err)):
+        if t is not None and t.device != dev:
+            raise ValueError(f"fp4_gemm: {name} must be on a's device")
+    if bias is not None:
+        bias = bias.reshape(-1).to(torch.bfloat16).contiguous()
+        if bias.numel() != N:
+            raise ValueError("bias must have N elements")
+        g.bias = bias.data_ptr()
+    if a2 is not None or b2 is not None:
+        if a2 is None or b2 is None or a2.dtype != torch.bfloat16 or b2.dtype != torch.bfloat16:
+            raise ValueError("a2/b2 must both be bfloat16")
+        if a2.dim() != 2 or b2.dim() != 2 or a2.shape[0] != M or b2.shape[0] != N or a2.shape[1] != b2.shape[1]:
+            raise ValueError("a2 is [M,R] and b2 is [N,R]")
+        if a2.stride(1) != 1 or b2.stride(1) != 1:
+            raise ValueError("a2 and b2 need a contiguous last dimension")
+        g.R = a2.shape[1]
+        g.a2, g.lda2, g.b2, g.ldb2 = a2.data_ptr(), max(a2.stride(0), g.R), b2.data_ptr(), max(b2.stride(0), g.R)
+    if out is None:
+        out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+    elif tuple(out.shape) != (M, N) or out.dtype != torch.bfloat16 or out.stride(1) != 1:
+        raise ValueError("out must be a bfloat16 tensor [M,N] with contiguous rows")
+    g.out, g.ldo = out.data_ptr(), max(out.stride(0), N)
+    if err is not None:
+        if err.dtype != torch.int32 or not err.is_cuda:
+            raise ValueError("err must be a CUDA int32 tensor")
+        g.err = err.data_ptr()
+    g.timeout_ns = int(timeout_ns)
+    g.test_flags = int(test_flags)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        rc = lib.mh3_fp4_gemm(g, _stream(dev))
+    _lib.check(rc, "mh3_fp4_gemm")
+    return out
+
+
+@nvtx("mh3.fp4_linear")
+def fp4_linear(x2d: torch.Tensor, w4: torch.Tensor, w_blocks: torch.Tensor, w_scale: torch.Tensor, bias,
+               adapters) -> torch.Tensor:
+    """FP4Linear forward: 4-bit activations (``quantize_fp4``) and one fused GEMM, bf16 out.
+
+    The adapters' delta is folded into the GEMM as in ``fp8_linear``:
+    a2 = (x A_cat^T) / x_scale, b2 = (scale*B)_cat / w_scale, both scales powers
+    of two."""
+    if x2d.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        x2d = x2d.to(torch.float32)
+    M, K = x2d.shape
+    N = w4.shape[0]
+    xq = quantize_fp4(x2d)
+    a2 = b2 = None
+    if adapters:
+        xb = x2d.to(torch.bfloat16).contiguous()
+        A_cat, b2 = _lora_operands(adapters, N, K, x2d.device, col_scale=w_scale.reshape(-1), scale_src=w_scale)
+        a2 = scaled_gemm(xb, A_cat, row_scale=xq[2], row_scale_inv=True)
+    return fp4_gemm(xq, (w4, w_blocks, w_scale), bias=bias, a2=a2, b2=b2)
+
+
+# ---------------------------------------------------------------------------
+# rotary positions
+# ---------------------------------------------------------------------------
+_POS_KIND = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+def _bhsd_strides(t: torch.Tensor):
+    """Strides (batch, head, token) of [B,H,S,D] or packed [T,H,D]."""
+    return (t.stride(0), t.stride(1), t.stride(2)) if t.dim() == 4 else (0, t.stride(1), t.stride(0))
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axes_dim, theta, interleaved: bool = True,
+           inverse: bool = False, out_q: torch.Tensor | None = None, out_k: torch.Tensor | None = None):
+    """``mh3_rotary`` on q and k, both [B,H,S,D] or both packed [T,H,D]; ``(q', k')``, k' None without k.
+
+    ``axes_dim`` and ``theta`` are sequences of one value per axis, positions
+    [S, axes] / [B, S, axes] (packed: [T, axes]).  Outputs take the inputs'
+    dimension order; ``out_q`` / ``out_k`` may be q / k themselves."""
+    ts = [t for t in (q, k) if t is not None]
+    a = _lib.RotaryArgs()
+    ins, outs = [], []
+    for t, o in ((q, out_q), (k, out_k)):
+        if t is None:
+            ins.append(None)
+            outs.append(None)
+            continue
+        if t.stride(-1) != 1 and t.shape[-1] != 1:
+            t = t.contiguous()
+        if o is None:
+            o = torch.empty_like(t)
+            if o.stride(-1) != 1 and o.shape[-1] != 1:
+                o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        elif o.shape != t.shape or o.dtype != t.dtype or o.device != t.device or o.stride(-1) != 1:
+            raise ValueError("rotary: an output must match its input, with contiguous channels")
+        ins.append(t)
+        outs.append(o)
+    q, k = ins
+    packed = q.dim() == 3
+    a.batch, a.seqlen = (1, q.shape[0]) if packed else (q.shape[0], q.shape[2])
+    a.heads_q, a.heads_k, a.head_dim = q.shape[1], 0 if k is None else k.shape[1], q.shape[-1]
+    a.dtype, a.pos_kind, a.n_axes = _FLOAT_CODE[q.dtype], _POS_KIND[positions.dtype], len(axes_dim)
+    a.interleaved, a.inverse = int(interleaved), int(inverse)
+    for i, (d, th) in enumerate(zip(axes_dim, theta)):
+        a.axes_dim[i], a.theta[i] = int(d), float(th)
+    if positions.stride(-1) != 1 and positions.shape[-1] != 1:
+        positions = positions.contiguous()
+    a.positions = positions.data_ptr()
+    a.pos_stride_s = positions.stride(-2)
+    a.pos_stride_b = positions.stride(0) if positions.dim() == 3 and positions.shape[0] > 1 else 0
+    a.q, a.q_out = q.data_ptr(), outs[0].data_ptr()
+    a.q_stride_b, a.q_stride_h, a.q_stride_s = _bhsd_strides(q)
+    a.qo_stride_b, a.qo_stride_h, a.qo_stride_s = _bhsd_strides(outs[0])
+    if k is not None:
+        a.k, a.k_out = k.data_ptr(), outs[1].data_ptr()
+        a.k_stride_b, a.k_stride_h, a.k_stride_s = _bhsd_strides(k)
+        a.ko_stride_b, a.ko_stride_h, a.ko_stride_s = _bhsd_strides(outs[1])
+    lib = _lib.load()
+    with torch.cuda.device(ts[0].device):
+        rc = lib.mh3_rotary(a, _stream(ts[0].device))
+    _lib.check(rc, "mh3_rotary")
+    return outs[0], outs[1]
+
+
+# ---------------------------------------------------------------------------
+# norms before and after a block
+# ---------------------------------------------------------------------------
+NORM_KINDS = {"none": 0, "rms": 1, "layer": 2}
+
+
+def _rows2d(t: torch.Tensor) -> torch.Tensor:
+    """[..., C] as [rows, C] with contiguous channels."""
+    t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _norm_args(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_norm, eps, alpha, per_token):
+    """The C arguments that the forward and the backward pass share, and the tensors they point into."""
+    a = _lib.BlockNormArgs()
+    keep = [x, y, cu]
+    C = x.shape[-1]
+    S = x.shape[1] if x.dim() == 3 else x.shape[0]
+    a.channels, a.dtype, a.norm, a.y_norm = C, _FLOAT_CODE[x.dtype], norm, y_norm
+    a.groups, a.group_rows = (cu.numel() - 1, 0) if cu is not None else (x.shape[0], S) if x.dim() == 3 else (1, S)
+    if a.groups == 0:
+        a.groups, a.group_rows = 1, 0  # an empty batch
+    a.per_row = int(per_token)
+    a.eps, a.residual_scale = float(eps), float(alpha)
+    if cu is not None:
+        a.cu_seqlens = cu.data_ptr()
+    x2 = _rows2d(x)
+    keep.append(x2)
+    a.rows = x2.shape[0]
+    a.x, a.x_stride = x2.data_ptr(), x2.stride(0)
+    if y is not None:
+        y2 = _rows2d(y)
+        keep.append(y2)
+        a.y, a.y_stride = y2.data_ptr(), y2.stride(0)
+    for name, m in (("gate", gate), ("scale", scale), ("shift", shift)):
+        if m is None:
+            continue
+        if m.stride(-1) != 1 and C != 1:
+            m = m.contiguous()
+        keep.append(m)
+        f = getattr(a, name)
+        f.ptr, f.dtype = m.data_ptr(), _FLOAT_CODE[m.dtype]
+        if not per_token:
+            f.stride_group, f.stride_row = m.stride(0), 0
+        elif m.dim() == 3:  # element (b, s): row b S + s
+            f.stride_group, f.stride_row = m.stride(0) - S * m.stride(1), m.stride(1)
+        else:
+            f.stride_group, f.stride_row = 0, m.stride(0)
+    for name, m in (("weight", weight), ("bias", bias), ("y_weight", y_weight)):
+        if m is not None:
+            m = m.contiguous()
+            keep.append(m)
+            f = getattr(a, name)
+            f.ptr, f.dtype = m.data_ptr(), _FLOAT_CODE[m.dtype]
+    return a, keep
+
+
+def block_norm_fwd(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm: int, y_norm: int, eps: float, alpha: float,
+                   per_token: bool, want_stats: bool):
+    """``mh3_block_norm_fwd``: (r, h, stats); r is empty without y, h with norm 0, stats when not wanted.
+
+    gate, scale, shift: [groups, C] (any stride), or with ``per_token`` of x's shape."""
+    a, keep = _norm_args(x, y, gate, scale, shift, weight, bias, y_weight, cu, max(norm, 1), y_norm, eps, alpha, per_token)
+    none = x.new_empty(0)
+    r = torch.empty(x.shape, dtype=x.dtype, device=x.device) if y is not None else none
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if norm else none
+    stats = torch.empty((a.rows, 4), dtype=torch.float32, device=x.device) if want_stats else none
+    if y is not None:
+        a.r = r.data_ptr()
+    if norm:
+        a.h = h.data_ptr()
+    if want_stats:
+        a.stats = stats.data_ptr()
+    lib = _lib.load()
+    with torch.cuda.device(x.device):
+        rc = lib.mh3_block_norm_fwd(a, _stream(x.device))
+    _lib.check(rc, "mh3_block_norm_fwd")
+    return r, h, stats
+
+
+def block_norm_bwd(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu, stats, norm: int, y_norm: int, eps: float,
+                   alpha: float, per_token: bool, want):
+    """``mh3_block_norm_bwd``: the gradients of (x, y, gate, scale, shift, weight, bias, y_weight) whose
+    entry of ``want`` is true, None for the others; dr or dh may be None."""
+    a, keep = _norm_args(x, y, gate, scale, shift, weight, bias, y_weight, cu, max(norm, 1), y_norm, eps, alpha, per_token)
+    if dr is not None:
+        dr = _rows2d(dr.to(x.dtype))
+        a.dr, a.dr_stride = dr.data_ptr(), dr.stride(0)
+    if dh is not None:
+        dh = _rows2d(dh.to(x.dtype))
+        a.dh, a.dh_stride = dh.data_ptr(), dh.stride(0)
+    names = ("dx", "dy", "dgate", "dscale", "dshift", "dweight", "dbias", "dy_weight")
+    grads = []
+    for name, t, w in zip(names, (x, y, gate, scale, shift, weight, bias, y_weight), want):
+        d = torch.empty(t.shape, dtype=t.dtype, device=t.device) if w and t is not None else None
+        if d is not None and d.numel():
+            setattr(a, name, d.data_ptr())
+        grads.append(d)
+    lib = _lib.load()
+    ws = torch.empty(max(16, int(lib.mh3_block_norm_workspace_bytes(a.rows, a.channels, a.groups))), dtype=torch.uint8,
+                     device=x.device)
+    a.stats, a.workspace = stats.data_ptr(), ws.data_ptr()
+    with torch.cuda.device(x.device):
+        rc = lib.mh3_block_norm_bwd(a, _stream(x.device))
+    _lib.check(rc, "mh3_block_norm_bwd")
+    return grads
 
 
 # ---------------------------------------------------------------------------
