@@ -14,9 +14,10 @@
 // computed into shared memory and used by every head of Q and K, so the two
 // double operations and the sincospi are 1/80th of a vector's work at 40 heads.
 //
-// Bound: HBM.  Q and K are read and written once by 16-byte vectors; a thread
-// keeps the same channels for every head it visits, so it needs one row of
-// angles per token, and issues kUnroll rows' loads before it rotates any.
+// Bound: HBM.  Q and K are read and written once by 16-byte vectors.  A thread
+// keeps the same channels for every (token, head) row it visits; its rows stream
+// through its own part of a three-stage ring in shared memory (cp.async, no
+// barrier), and the first stages are on their way before the angles are computed.
 #include <math.h>
 
 #include "mh3_b200.h"
@@ -28,8 +29,9 @@ namespace rotary {
 
 constexpr int kThreads = 256;
 constexpr int kMaxPairs = 128;  // head_dim <= 256
-constexpr int kUnroll = 5;      // head rows whose loads are in flight per thread
-constexpr int kMaxTokens = 8;   // tokens per CTA
+constexpr int kMaxTokens = 16;  // tokens per CTA
+constexpr int kStages = 3;
+constexpr int kVectors = 4;     // 16-byte vectors of a thread in a stage
 
 struct Params {
   const char *q, *k;
@@ -64,115 +66,179 @@ struct __align__(sizeof(T) * V) Vec {
   T e[V];
 };
 
-// V: channels per vector (16 bytes), or 1 for layouts that vectors do not fit.
-// INTER: pairs are neighbouring channels (2p, 2p+1); else (p, p + R/2).
-// A thread's unit is one vector of the row: V/2 pairs when INTER (those past R/2
-// pass), V pairs in two vectors when not, or V passing channels.
-template <typename T, int V, bool INTER>
-__global__ void __launch_bounds__(kThreads) kernel(const __grid_constant__ Params p) {
-  extern __shared__ float2 cs[];  // [tile][npair] (cos, sin)
-  const int npair = INTER ? (p.D + 1) / 2 : p.R2;  // INTER: a vector may reach past R/2
-  const long long t0 = (long long)blockIdx.x * p.tile;
-  const int nt = (int)min((long long)p.tile, p.tokens - t0);
+// (cos, sin) of the CTA's tokens, [nt][npair]; pairs past R/2 are not used.
+__device__ __forceinline__ void angles(const Params& p, float2* cs, long long t0, int nt, int npair) {
   for (int i = threadIdx.x; i < nt * npair; i += kThreads) {
     const int t = i / npair, j = i - t * npair;
-    float2 r = make_float2(1.0f, 0.0f);
-    if (j < p.R2) {
-      const long long tok = t0 + t;
-      const long long b = tok / p.S, s = tok - b * p.S;
-      const long long at = b * p.pos_sb + s * p.pos_ss + p.axis[j];
-      const double pos = p.pos_kind == 0   ? (double)static_cast<const int*>(p.pos)[at]
-                         : p.pos_kind == 1 ? (double)static_cast<const long long*>(p.pos)[at]
-                                           : (double)static_cast<const float*>(p.pos)[at];
-      double turn = pos * p.rate[j];
-      turn -= rint(turn);
-      float sn, c;
-      sincospif(2.0f * (float)turn, &sn, &c);
-      r = make_float2(c, sn * p.sign);
-    }
-    cs[i] = r;
-  }
-  __syncthreads();
-
-  // units of a row, and the rows that this CTA's threads visit side by side
-  const int units = !INTER ? p.R2 / V + (p.D - 2 * p.R2) / V : V > 1 ? p.D / V : npair;
-  const int rot_units = INTER ? (V > 1 ? units : p.R2) : p.R2 / V;
-  const int lanes = min(units, kThreads);
-  const int side = kThreads / lanes;
-  const int row0 = threadIdx.x / lanes;
-  if (row0 >= side) return;
-  const int rows = p.Hq + p.Hk;
-  for (int u = threadIdx.x - row0 * lanes; u < units; u += lanes) {
-    const bool rot = u < rot_units;
-    // first channel of the unit, and the distance to its second vector
-    const int c0 = INTER ? (V > 1 ? u * V : 2 * u) : (rot ? u * V : 2 * p.R2 + (u - rot_units) * V);
-    const int dist = INTER ? 1 : p.R2;
-    const bool two = INTER ? (V == 1 && c0 + 1 < p.D) : rot;  // a second vector (every rotated pair of V == 1 has one)
-    for (int t = 0; t < nt; ++t) {
-      const long long tok = t0 + t;
-      const long long b = tok / p.S, s = tok - b * p.S;
-      const T* qp = reinterpret_cast<const T*>(p.q) + b * p.q_sb + s * p.q_ss + c0;
-      const T* kp = reinterpret_cast<const T*>(p.k) + b * p.k_sb + s * p.k_ss + c0;
-      T* qo = reinterpret_cast<T*>(p.qo) + b * p.qo_sb + s * p.qo_ss + c0;
-      T* ko = reinterpret_cast<T*>(p.ko) + b * p.ko_sb + s * p.ko_ss + c0;
-      constexpr int NP = INTER ? (V > 1 ? V / 2 : 1) : V;  // pairs of a unit
-      float2 a[NP];
-#pragma unroll
-      for (int j = 0; j < NP; ++j)
-        a[j] = rot ? cs[t * npair + u * NP + j] : make_float2(1.0f, 0.0f);
-      for (int r = row0; r < rows; r += side * kUnroll) {
-        Vec<T, V> x[kUnroll], y[kUnroll];
-#pragma unroll
-        for (int i = 0; i < kUnroll; ++i) {
-          const int h = r + i * side;
-          if (h < rows) {
-            const T* at = h < p.Hq ? qp + h * p.q_sh : kp + (h - p.Hq) * p.k_sh;
-            x[i] = *reinterpret_cast<const Vec<T, V>*>(at);
-            if ((V == 1 || !INTER) && two) y[i] = *reinterpret_cast<const Vec<T, V>*>(at + dist);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kUnroll; ++i) {
-          const int h = r + i * side;
-          if (h >= rows) break;
-          T* to = h < p.Hq ? qo + h * p.qo_sh : ko + (h - p.Hq) * p.ko_sh;
-          if constexpr (INTER && V > 1) {
-#pragma unroll
-            for (int j = 0; j < NP; ++j) {
-              if (u * NP + j >= p.R2) break;
-              const float v0 = to_f(x[i].e[2 * j]), v1 = to_f(x[i].e[2 * j + 1]);
-              x[i].e[2 * j] = from_f<T>(v0 * a[j].x - v1 * a[j].y);
-              x[i].e[2 * j + 1] = from_f<T>(v0 * a[j].y + v1 * a[j].x);
-            }
-          } else if (rot) {
-#pragma unroll
-            for (int j = 0; j < NP; ++j) {
-              const float v0 = to_f(x[i].e[j]), v1 = to_f(y[i].e[j]);
-              x[i].e[j] = from_f<T>(v0 * a[j].x - v1 * a[j].y);
-              y[i].e[j] = from_f<T>(v0 * a[j].y + v1 * a[j].x);
-            }
-          }
-          *reinterpret_cast<Vec<T, V>*>(to) = x[i];
-          if ((V == 1 || !INTER) && two) *reinterpret_cast<Vec<T, V>*>(to + dist) = y[i];
-        }
-      }
-    }
+    if (j >= p.R2) continue;
+    const long long tok = t0 + t;
+    const long long b = tok / p.S, s = tok - b * p.S;
+    const long long at = b * p.pos_sb + s * p.pos_ss + p.axis[j];
+    const double pos = p.pos_kind == 0   ? (double)static_cast<const int*>(p.pos)[at]
+                       : p.pos_kind == 1 ? (double)static_cast<const long long*>(p.pos)[at]
+                                         : (double)static_cast<const float*>(p.pos)[at];
+    double turn = pos * p.rate[j];
+    turn -= rint(turn);
+    float sn, c;
+    sincospif(2.0f * (float)turn, &sn, &c);
+    cs[i] = make_float2(c, sn * p.sign);
   }
 }
 
-template <typename T, int V, bool INTER>
-static cudaError_t launch(const Params& p, cudaStream_t st) {
-  const int npair = INTER ? (p.D + 1) / 2 : p.R2;
-  const unsigned grid = (unsigned)((p.tokens + p.tile - 1) / p.tile);
-  kernel<T, V, INTER><<<grid, kThreads, (size_t)p.tile * npair * sizeof(float2), st>>>(p);
-  return cudaGetLastError();
+// Row i of the CTA's tokens x heads: token i / rows, Q's heads first.
+struct Row {
+  long long in, out;  // element offsets
+  int t;
+  bool k;
+};
+__device__ __forceinline__ Row locate(const Params& p, long long t0, int i) {
+  const int rows = p.Hq + p.Hk;
+  Row r;
+  r.t = (int)((unsigned)i / (unsigned)rows);
+  const int h = i - r.t * rows;
+  const long long tok = t0 + r.t;
+  long long b = 0, s = tok;
+  if (tok >= p.S) {
+    b = p.tokens <= 0xffffffffll ? (long long)((unsigned)tok / (unsigned)p.S) : tok / p.S;
+    s = tok - b * p.S;
+  }
+  r.k = h >= p.Hq;
+  if (r.k) {
+    r.in = b * p.k_sb + s * p.k_ss + (h - p.Hq) * p.k_sh;
+    r.out = b * p.ko_sb + s * p.ko_ss + (h - p.Hq) * p.ko_sh;
+  } else {
+    r.in = b * p.q_sb + s * p.q_ss + h * p.q_sh;
+    r.out = b * p.qo_sb + s * p.qo_ss + h * p.qo_sh;
+  }
+  return r;
 }
 
 template <typename T>
-static cudaError_t launch_type(const Params& p, bool vec, bool inter, cudaStream_t st) {
+__device__ __forceinline__ void rotate(T& x0, T& x1, float2 a) {
+  const float v0 = to_f(x0), v1 = to_f(x1);
+  x0 = from_f<T>(v0 * a.x - v1 * a.y);
+  x1 = from_f<T>(v0 * a.y + v1 * a.x);
+}
+
+// INTER: pairs are neighbouring channels (2p, 2p+1); else (p, p + R/2).
+// A thread's unit is one 16-byte vector of the row when INTER (pairs past R/2
+// pass), and when not the two vectors of V pairs, or V passing channels.
+template <typename T, bool INTER>
+__global__ void __launch_bounds__(kThreads) stream_kernel(const __grid_constant__ Params p) {
   constexpr int V = 16 / sizeof(T);
-  if (vec) return inter ? launch<T, V, true>(p, st) : launch<T, V, false>(p, st);
-  return inter ? launch<T, 1, true>(p, st) : launch<T, 1, false>(p, st);
+  constexpr int W = INTER ? 1 : 2;       // vectors of a unit
+  constexpr int U = kVectors / W;        // rows of a stage
+  constexpr int NP = INTER ? V / 2 : V;  // pairs of a unit
+  extern __shared__ uint4 smem[];
+  uint4* ring = smem + threadIdx.x;  // [kStages][kVectors][kThreads]
+  float2* cs = reinterpret_cast<float2*>(smem + kStages * kVectors * kThreads);
+  const int npair = INTER ? p.D / 2 : p.R2;
+  const long long t0 = (long long)blockIdx.x * p.tile;
+  const int nt = (int)min((long long)p.tile, p.tokens - t0);
+  const int rot_units = INTER ? p.D / V : p.R2 / V;
+  const int units = INTER ? rot_units : rot_units + (p.D - 2 * p.R2) / V;
+  const int side = kThreads / units;  // rows visited side by side (units <= 64)
+  const int row0 = threadIdx.x / units, u = threadIdx.x - row0 * units;
+  const bool rot = u < rot_units;
+  const int c0 = rot ? u * V : 2 * p.R2 + (u - rot_units) * V;
+  const int n = row0 < side ? nt * (p.Hq + p.Hk) : 0;  // rows of the CTA
+  auto issue = [&](int i, int st) {
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int j = i + k * side;
+      if (j < n) {
+        const Row r = locate(p, t0, j);
+        const T* src = reinterpret_cast<const T*>(r.k ? p.k : p.q) + r.in + c0;
+        uint4* dst = ring + (st * kVectors + k * W) * kThreads;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+        if (!INTER && rot)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst + kThreads)), "l"(src + p.R2) : "memory");
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int j = 0; j < kStages - 1; ++j) issue(row0 + j * U * side, j);
+  angles(p, cs, t0, nt, npair);
+  __syncthreads();
+  int st = 0;
+  for (int i = row0; i < n; i += U * side) {
+    issue(i + (kStages - 1) * U * side, st == 0 ? kStages - 1 : st - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int j = i + k * side;
+      if (j >= n) break;
+      const Row r = locate(p, t0, j);
+      T* to = reinterpret_cast<T*>(r.k ? p.ko : p.qo) + r.out + c0;
+      const uint4* src = ring + (st * kVectors + k * W) * kThreads;
+      Vec<T, V> x, y;
+      x = *reinterpret_cast<const Vec<T, V>*>(src);
+      if (rot) {
+        if (!INTER) y = *reinterpret_cast<const Vec<T, V>*>(src + kThreads);
+        const float4* ap = reinterpret_cast<const float4*>(cs + r.t * npair + u * NP);
+#pragma unroll
+        for (int q = 0; q < NP / 2; ++q) {
+          const float4 a = ap[q];
+          if (INTER) {
+            if (u * NP + 2 * q < p.R2) rotate(x.e[4 * q], x.e[4 * q + 1], make_float2(a.x, a.y));
+            if (u * NP + 2 * q + 1 < p.R2) rotate(x.e[4 * q + 2], x.e[4 * q + 3], make_float2(a.z, a.w));
+          } else {
+            rotate(x.e[2 * q], y.e[2 * q], make_float2(a.x, a.y));
+            rotate(x.e[2 * q + 1], y.e[2 * q + 1], make_float2(a.z, a.w));
+          }
+        }
+      }
+      *reinterpret_cast<Vec<T, V>*>(to) = x;
+      if (!INTER && rot) *reinterpret_cast<Vec<T, V>*>(to + p.R2) = y;
+    }
+    st = st + 1 == kStages ? 0 : st + 1;
+  }
+}
+
+// Layouts that 16-byte vectors do not fit: a unit is one pair or one passing channel.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) scalar_kernel(const __grid_constant__ Params p, int inter) {
+  extern __shared__ uint4 smem[];
+  float2* cs = reinterpret_cast<float2*>(smem);
+  const long long t0 = (long long)blockIdx.x * p.tile;
+  const int nt = (int)min((long long)p.tile, p.tokens - t0);
+  angles(p, cs, t0, nt, p.R2);
+  __syncthreads();
+  const int units = p.D - p.R2;
+  const int total = nt * (p.Hq + p.Hk) * units;
+  for (int i = threadIdx.x; i < total; i += kThreads) {
+    const int row = i / units, u = i - row * units;
+    const Row r = locate(p, t0, row);
+    const T* src = reinterpret_cast<const T*>(r.k ? p.k : p.q) + r.in;
+    T* to = reinterpret_cast<T*>(r.k ? p.ko : p.qo) + r.out;
+    if (u < p.R2) {
+      const int c0 = inter ? 2 * u : u, c1 = inter ? 2 * u + 1 : u + p.R2;
+      T x0 = src[c0], x1 = src[c1];
+      rotate(x0, x1, cs[r.t * p.R2 + u]);
+      to[c0] = x0;
+      to[c1] = x1;
+    } else {
+      to[u + p.R2] = src[u + p.R2];
+    }
+  }
+}
+
+template <typename T>
+static cudaError_t launch(const Params& p, bool vec, bool inter, cudaStream_t st) {
+  const unsigned grid = (unsigned)((p.tokens + p.tile - 1) / p.tile);
+  if (!vec) {
+    scalar_kernel<T><<<grid, kThreads, (size_t)p.tile * p.R2 * sizeof(float2), st>>>(p, inter ? 1 : 0);
+    return cudaGetLastError();
+  }
+  const size_t smem = (size_t)kStages * kVectors * kThreads * 16 + (size_t)p.tile * (inter ? p.D / 2 : p.R2) * sizeof(float2);
+  auto kern = inter ? stream_kernel<T, true> : stream_kernel<T, false>;
+  if (smem > 40 * 1024) {  // with the static part, past the 48 KB default
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  kern<<<grid, kThreads, smem, st>>>(p);
+  return cudaGetLastError();
 }
 
 }  // namespace rotary
@@ -207,7 +273,8 @@ extern "C" int mh3_rotary(const mh3_rotary_args* a, void* stream) {
   if (tokens == 0 || a->heads_q + (long long)a->heads_k == 0) return MH3_OK;
   if (!a->positions || (a->heads_q > 0 && (!a->q || !a->q_out)) || (a->heads_k > 0 && (!a->k || !a->k_out)))
     return fail(MH3_ERR_INVALID, "mh3_rotary: null pointer");
-  if ((long long)a->heads_q + a->heads_k > (1 << 24) || tokens > (1ll << 40))
+  // rows and units of a CTA are counted in 32 bits: 16 tokens x heads x 256
+  if ((long long)a->heads_q + a->heads_k > (1 << 18) || tokens > (1ll << 34))
     return fail(MH3_ERR_TOO_LARGE, "mh3_rotary: too many heads or tokens");
   const bool inter = a->interleaved != 0;
   const int es = a->dtype == MH3_DTYPE_F32 ? 4 : 2, V = 16 / es;
@@ -238,16 +305,16 @@ extern "C" int mh3_rotary(const mh3_rotary_args* a, void* stream) {
   p.pos_sb = a->pos_stride_b;
   p.pos_ss = a->pos_stride_s;
   p.sign = a->inverse ? -1.0f : 1.0f;
-  // Tokens per CTA: enough for 40 KB of Q and K, which hides the angles'
-  // latency, while 148 SMs still get several CTAs each.
+  // Tokens per CTA: enough for 80 KB of Q and K (five stages of the ring), while
+  // 148 SMs still get four CTAs each.
   const long long token_bytes = ((long long)a->heads_q + a->heads_k) * a->head_dim * es;
   int tile = 1;
-  while (tile < rotary::kMaxTokens && tile * token_bytes < 40960 && tokens / (2 * tile) >= 148 * 8) tile *= 2;
+  while (tile < rotary::kMaxTokens && tile * token_bytes < 81920 && tokens / (2 * tile) >= 148 * 4) tile *= 2;
   p.tile = tile;
   if ((tokens + tile - 1) / tile > 0x7fffffffLL) return fail(MH3_ERR_TOO_LARGE, "mh3_rotary: too many tokens");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const cudaError_t e = a->dtype == MH3_DTYPE_BF16  ? rotary::launch_type<__nv_bfloat16>(p, vec, inter, st)
-                        : a->dtype == MH3_DTYPE_F16 ? rotary::launch_type<__half>(p, vec, inter, st)
-                                                    : rotary::launch_type<float>(p, vec, inter, st);
+  const cudaError_t e = a->dtype == MH3_DTYPE_BF16  ? rotary::launch<__nv_bfloat16>(p, vec, inter, st)
+                        : a->dtype == MH3_DTYPE_F16 ? rotary::launch<__half>(p, vec, inter, st)
+                                                    : rotary::launch<float>(p, vec, inter, st);
   return e == cudaSuccess ? MH3_OK : fail_cuda(e, "mh3_rotary launch");
 }
