@@ -18,12 +18,17 @@
 // It recomputes xhat and yhat from x, y and the rows' saved (mean, rstd).
 //
 // Bound: HBM (4 bytes a bf16 element for norm_modulate, 8 for the gated form;
-// backward 6 and 12).  One CTA holds a row, eight channels a thread, and walks a
+// backward 6 and 12).  A CTA spans a row, eight channels a thread, and walks a
 // contiguous range of rows, so the modulation is read and combined once per
-// group (kept in the thread's own slots of shared memory) and the next row's
-// vectors are loaded before the current row is reduced.  Column sums stay in
+// group (kept in the thread's own slots of shared memory).  The rows stream
+// through a ring of two or three stages in shared memory: each thread copies its
+// own sixteen bytes with cp.async and reads back only what it copied, so the ring
+// needs no barrier, and 80 KB per SM are in flight whatever the registers hold.  A
+// stage is several rows, whose sums share one barrier.  Column sums stay in
 // registers over the range; each (CTA, group) writes one partial row and a second
 // kernel adds the partials in a fixed order: no atomics, the same bits every time.
+// Rows that vectors do not fit, a modulation for each row, and rows too long for
+// two stages take the general kernels, one row at a time through registers.
 #include <algorithm>
 
 #include "mh3_b200.h"
@@ -59,7 +64,7 @@ struct Params {
   float* gsum;       // [G][3][C]
   long long rows, S; // S: rows of a group (dense)
   const int* cu;     // packed: [G + 1]
-  int C, G, ynorm, norm, ctas;
+  int C, G, ynorm, norm, ctas, stages;
   float eps, alpha;
 };
 
@@ -174,7 +179,7 @@ __device__ __forceinline__ void slot_get(const float4* s, float (&v)[8]) {
 // of ``buf`` in turn, so one barrier per call is enough: a warp can reach the
 // second-next call only when every warp has left this one.
 template <int N>
-__device__ __forceinline__ void block_sum(float (&v)[N], float (*buf)[2][32], int& turn) {
+__device__ __forceinline__ void block_sum(float (&v)[N], float (*buf)[4][32], int& turn) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
@@ -196,7 +201,7 @@ __device__ __forceinline__ void block_sum(float (&v)[N], float (*buf)[2][32], in
 }
 
 // (mean, rstd) of the row held as v (n valid channels in this thread).
-__device__ __forceinline__ float2 row_stats(const float (&v)[8], int n, int C, int kind, float eps, float (*buf)[2][32],
+__device__ __forceinline__ float2 row_stats(const float (&v)[8], int n, int C, int kind, float eps, float (*buf)[4][32],
                                             int& turn) {
   float mean = 0.0f, s[1];
   if (kind == kLayer) {
@@ -254,7 +259,7 @@ __device__ __forceinline__ int group_of(const Params& p, long long row, int g, l
 template <typename T, bool VEC, bool PT>
 __global__ void __launch_bounds__(1024) fwd_kernel(const __grid_constant__ Params p) {
   extern __shared__ float4 slots[];
-  __shared__ float red[2][2][32];
+  __shared__ float red[2][4][32];
   float4* sA = slots;                    // w (1 + scale)        (PT: w)
   float4* sB = slots + 2 * blockDim.x;   // b (1 + scale) + shift (PT: b)
   float4* sG = slots + 4 * blockDim.x;   // gate wy              (PT: wy); only with y
@@ -368,7 +373,7 @@ __global__ void __launch_bounds__(1024) fwd_kernel(const __grid_constant__ Param
 template <typename T, bool VEC, bool PT>
 __global__ void __launch_bounds__(1024) bwd_kernel(const __grid_constant__ Params p) {
   extern __shared__ float4 slots[];
-  __shared__ float red[2][2][32];
+  __shared__ float red[2][4][32];
   float4* sA = slots;                   // w (1 + scale)  (PT: w)
   float4* sG = slots + 2 * blockDim.x;  // gate wy        (PT: wy); only with y
   const int c = threadIdx.x * 8;
@@ -551,11 +556,394 @@ __global__ void __launch_bounds__(1024) bwd_kernel(const __grid_constant__ Param
   else if (g >= 0 && g < p.G) flush(g);
 }
 
-// Column sums of group blockIdx.y..: 32 channels x 8 partials at a time.  PT: one
+// ---------------------------------------------------------------------------
+// The streaming kernels: rows in vectors, modulation by group
+// ---------------------------------------------------------------------------
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A thread's eight channels of a row, to and from its place in the ring (``at``:
+// the place of the row and tensor, in 16-byte units times the CTA's threads).
+template <typename T>
+struct Ring {
+  static constexpr int W = sizeof(T) == 4 ? 2 : 1;  // 16-byte units of eight channels
+  uint4* base;
+  __device__ __forceinline__ void copy(int at, const T* src) const {
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(base + (at * W + w) * (int)blockDim.x + threadIdx.x)),
+                   "l"(reinterpret_cast<const uint4*>(src) + w)
+                   : "memory");
+  }
+  __device__ __forceinline__ void get(int at, float (&v)[8]) const {
+    Raw<T> r;
+#pragma unroll
+    for (int w = 0; w < W; ++w) r.u[w] = base[(at * W + w) * (int)blockDim.x + threadIdx.x];
+    unpack(r, v);
+  }
+};
+
+// (mean, rstd) of R rows at once (channels of threads past the row are 0).
+template <int R>
+__device__ __forceinline__ void rows_stats(const float (&v)[R][8], bool live, int C, int kind, float eps, float (*buf)[4][32],
+                                           int& turn, float2 (&out)[R]) {
+  float s[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) out[i].x = 0.0f;
+  if (kind == kLayer) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      s[i] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s[i] += v[i][k];
+    }
+    block_sum(s, buf, turn);
+#pragma unroll
+    for (int i = 0; i < R; ++i) out[i].x = s[i] / (float)C;
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    s[i] = 0.0f;
+    if (live) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float d = v[i][k] - out[i].x;
+        s[i] = fmaf(d, d, s[i]);
+      }
+    }
+  }
+  block_sum(s, buf, turn);
+#pragma unroll
+  for (int i = 0; i < R; ++i) out[i].y = rsqrtf(s[i] / (float)C + eps);
+}
+
+template <typename T, bool Y, int R, int MAXT>
+__global__ void __launch_bounds__(MAXT) fwd_stream_kernel(const __grid_constant__ Params p) {
+  extern __shared__ float4 slots[];
+  __shared__ float red[2][4][32];
+  constexpr int NT = Y ? 2 : 1;              // tensors of a stage
+  float4* sA = slots;                        // w (1 + scale)
+  float4* sB = slots + 2 * blockDim.x;       // b (1 + scale) + shift
+  float4* sG = slots + 4 * blockDim.x;       // gate wy; only with y
+  const Ring<T> ring{reinterpret_cast<uint4*>(slots + (Y ? 6 : 4) * blockDim.x)};
+  const int c = threadIdx.x * 8;
+  const bool live = c < p.C;
+  const long long lo = p.rows * blockIdx.x / p.ctas, hi = p.rows * (blockIdx.x + 1) / p.ctas;
+  int turn = 0, g = -1;
+  long long end = lo;
+  auto issue = [&](long long row, int st) {  // rows [row, row + R) into stage st
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (row + i < hi) {
+          ring.copy((st * NT) * R + i, static_cast<const T*>(p.x) + (row + i) * p.x_s + c);
+          if (Y) ring.copy((st * NT + 1) * R + i, static_cast<const T*>(p.y) + (row + i) * p.y_s + c);
+        }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int j = 0; j < p.stages - 1; ++j) issue(lo + (long long)j * R, j);
+  int st = 0;
+  for (long long row = lo; row < hi; row += R) {
+    issue(row + (long long)(p.stages - 1) * R, st == 0 ? p.stages - 1 : st - 1);
+    if (p.stages == 3) cp_wait<2>();
+    else cp_wait<1>();
+    const int cnt = (int)min((long long)R, hi - row);
+    for (int j = 0; j < cnt;) {  // the stage's rows, a group at a time
+      if (row + j >= end) {
+        g = group_of(p, row + j, g == p.G ? -1 : g, end);
+        if (live && g < p.G) {
+          float w[8], b[8], t[8];
+          mod8<true>(p.w.p, p.w.dt, c, 8, 1.0f, w);
+          mod8<true>(p.b.p, p.b.dt, c, 8, 0.0f, b);
+          mod8<true>(p.scale.p, p.scale.dt, g * p.scale.sg + c, 8, 0.0f, t);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            w[k] *= 1.0f + t[k];
+            b[k] *= 1.0f + t[k];
+          }
+          mod8<true>(p.shift.p, p.shift.dt, g * p.shift.sg + c, 8, 0.0f, t);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) b[k] += t[k];
+          slot_put(sA, w);
+          slot_put(sB, b);
+          if (Y) {
+            mod8<true>(p.wy.p, p.wy.dt, c, 8, 1.0f, w);
+            mod8<true>(p.gate.p, p.gate.dt, g * p.gate.sg + c, 8, 1.0f, t);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] *= t[k];
+            slot_put(sG, w);
+          }
+        }
+      }
+      const int n = (int)min((long long)cnt, end - row);
+      float v[R][8];
+      float2 sy[R], sr[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        sy[i] = sr[i] = make_float2(0.0f, 1.0f);
+        if (live && i >= j && i < n) ring.get((st * NT) * R + i, v[i]);
+        else
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[i][k] = 0.0f;
+      }
+      if (g >= p.G) {  // outside every packed sequence: zeros
+        const float z[8] = {};
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+          if (i >= j && i < n) {
+            if (live && p.r) store8<T, true>(static_cast<T*>(p.r) + (row + i) * p.C + c, 8, z);
+            if (live && p.h) store8<T, true>(static_cast<T*>(p.h) + (row + i) * p.C + c, 8, z);
+            if (threadIdx.x == 0 && p.stats) p.stats[row + i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          }
+        j = n;
+        continue;
+      }
+      if (Y) {
+        float y[R][8], a[8];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          if (live && i >= j && i < n) ring.get((st * NT + 1) * R + i, y[i]);
+          else
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[i][k] = 0.0f;
+        }
+        if (p.ynorm != kNone) rows_stats<R>(y, live, p.C, p.ynorm, p.eps, red, turn, sy);
+        if (live) {
+          slot_get(sG, a);
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[i][k] = fmaf(a[k], (y[i][k] - sy[i].x) * sy[i].y, p.alpha * v[i][k]);
+            if (i >= j && i < n) store8<T, true>(static_cast<T*>(p.r) + (row + i) * p.C + c, 8, v[i]);
+          }
+        }
+      }
+      if (p.h != nullptr) {
+        rows_stats<R>(v, live, p.C, p.norm, p.eps, red, turn, sr);
+        if (live) {
+          float a[8], b[8];
+          slot_get(sA, a);
+          slot_get(sB, b);
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[i][k] = fmaf((v[i][k] - sr[i].x) * sr[i].y, a[k], b[k]);
+            if (i >= j && i < n) store8<T, true>(static_cast<T*>(p.h) + (row + i) * p.C + c, 8, v[i]);
+          }
+        }
+      }
+      if (threadIdx.x == 0 && p.stats)
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+          if (i >= j && i < n) p.stats[row + i] = make_float4(sy[i].x, sy[i].y, sr[i].x, sr[i].y);
+      j = n;
+    }
+    st = st + 1 == p.stages ? 0 : st + 1;
+  }
+}
+
+template <typename T, bool Y, int R, int MAXT>
+__global__ void __launch_bounds__(MAXT) bwd_stream_kernel(const __grid_constant__ Params p) {
+  extern __shared__ float4 slots[];
+  __shared__ float red[2][4][32];
+  constexpr int NT = Y ? 4 : 2;          // x, dh, y, dr
+  float4* sA = slots;                    // w (1 + scale)
+  float4* sG = slots + 2 * blockDim.x;   // gate wy; only with y
+  const Ring<T> ring{reinterpret_cast<uint4*>(slots + (Y ? 4 : 2) * blockDim.x)};
+  const int c = threadIdx.x * 8;
+  const bool live = c < p.C;
+  const long long lo = p.rows * blockIdx.x / p.ctas, hi = p.rows * (blockIdx.x + 1) / p.ctas;
+  const bool has_dr = Y && p.dr != nullptr, has_dh = p.dh != nullptr;
+  int turn = 0, g = -1;
+  long long end = lo;
+  float a1[8] = {}, a2[8] = {}, a3[8] = {};  // column sums of dh xhat, dh and d yhat
+  float4 nst[R];                             // the next stage's row statistics
+  auto flush = [&](int grp) {
+    if (!live) return;
+    float* o = p.part + (long long)(blockIdx.x + grp) * 3 * p.C + c;
+    store8<float, true>(o, 8, a1);
+    store8<float, true>(o + p.C, 8, a2);
+    store8<float, true>(o + 2 * p.C, 8, a3);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a1[k] = a2[k] = a3[k] = 0.0f;
+  };
+  auto issue = [&](long long row, int st) {
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (row + i < hi) {
+          const int at = st * NT * R + i;
+          ring.copy(at, static_cast<const T*>(p.x) + (row + i) * p.x_s + c);
+          if (has_dh) ring.copy(at + R, static_cast<const T*>(p.dh) + (row + i) * p.dh_s + c);
+          if (Y) ring.copy(at + 2 * R, static_cast<const T*>(p.y) + (row + i) * p.y_s + c);
+          if (has_dr) ring.copy(at + 3 * R, static_cast<const T*>(p.dr) + (row + i) * p.dr_s + c);
+        }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto fetch_stats = [&](long long row) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) nst[i] = row + i < hi ? __ldg(p.stats + row + i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  };
+  for (int j = 0; j < p.stages - 1; ++j) issue(lo + (long long)j * R, j);
+  fetch_stats(lo);
+  int st = 0;
+  for (long long row = lo; row < hi; row += R) {
+    issue(row + (long long)(p.stages - 1) * R, st == 0 ? p.stages - 1 : st - 1);
+    float4 rs[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) rs[i] = nst[i];
+    fetch_stats(row + R);
+    if (p.stages == 3) cp_wait<2>();
+    else cp_wait<1>();
+    const int cnt = (int)min((long long)R, hi - row);
+    for (int j = 0; j < cnt;) {
+      if (row + j >= end) {
+        const int was = g;
+        g = group_of(p, row + j, g == p.G ? -1 : g, end);
+        if (was >= 0 && was < p.G) flush(was);
+        if (live && g < p.G) {
+          float w[8], t[8];
+          mod8<true>(p.w.p, p.w.dt, c, 8, 1.0f, w);
+          mod8<true>(p.scale.p, p.scale.dt, g * p.scale.sg + c, 8, 0.0f, t);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) w[k] *= 1.0f + t[k];
+          slot_put(sA, w);
+          if (Y) {
+            mod8<true>(p.wy.p, p.wy.dt, c, 8, 1.0f, w);
+            mod8<true>(p.gate.p, p.gate.dt, g * p.gate.sg + c, 8, 1.0f, t);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] *= t[k];
+            slot_put(sG, w);
+          }
+        }
+      }
+      const int n = (int)min((long long)cnt, end - row);
+      if (g >= p.G) {  // outside every packed sequence: no gradient
+        const float z[8] = {};
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+          if (live && i >= j && i < n) {
+            if (p.dx) store8<T, true>(static_cast<T*>(p.dx) + (row + i) * p.C + c, 8, z);
+            if (p.dy) store8<T, true>(static_cast<T*>(p.dy) + (row + i) * p.C + c, 8, z);
+          }
+        j = n;
+        continue;
+      }
+      float d[R][8], yh[R][8], gt[8];
+      if (Y && live) slot_get(sG, gt);
+      {
+        float xh[R][8], s[2 * R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          s[2 * i] = s[2 * i + 1] = 0.0f;
+          const bool in = live && i >= j && i < n;
+          const int at = st * NT * R + i;
+          if (in) {
+            ring.get(at, xh[i]);
+            if (Y) {
+              ring.get(at + 2 * R, yh[i]);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                yh[i][k] = (yh[i][k] - rs[i].x) * rs[i].y;
+                xh[i][k] = fmaf(gt[k], yh[i][k], p.alpha * xh[i][k]);
+              }
+            }
+            if (has_dh) {
+              float t[8];
+              ring.get(at + R, t);
+              slot_get(sA, d[i]);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                xh[i][k] = (xh[i][k] - rs[i].z) * rs[i].w;
+                a1[k] = fmaf(t[k], xh[i][k], a1[k]);
+                a2[k] += t[k];
+                d[i][k] *= t[k];  // dn
+                s[2 * i] += d[i][k];
+                s[2 * i + 1] = fmaf(d[i][k], xh[i][k], s[2 * i + 1]);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) xh[i][k] = yh[i][k] = d[i][k] = 0.0f;
+          }
+        }
+        if (has_dh) {
+          block_sum(s, red, turn);
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+            const float m0 = p.norm == kLayer ? s[2 * i] / (float)p.C : 0.0f, m1 = s[2 * i + 1] / (float)p.C;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) d[i][k] = rs[i].w * (d[i][k] - m0 - xh[i][k] * m1);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) d[i][k] = 0.0f;
+        }
+      }
+      const float al = Y ? p.alpha : 1.0f;
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (live && i >= j && i < n) {
+          float t[8];
+          if (has_dr) {
+            ring.get(st * NT * R + i + 3 * R, t);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) d[i][k] += t[k];
+          }
+          if (p.dx) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t[k] = al * d[i][k];
+            store8<T, true>(static_cast<T*>(p.dx) + (row + i) * p.C + c, 8, t);
+          }
+        }
+      if (Y) {
+        float s[2 * R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          s[2 * i] = s[2 * i + 1] = 0.0f;
+          if (live && i >= j && i < n) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              a3[k] = fmaf(d[i][k], yh[i][k], a3[k]);
+              d[i][k] *= gt[k];
+              s[2 * i] += d[i][k];
+              s[2 * i + 1] = fmaf(d[i][k], yh[i][k], s[2 * i + 1]);
+            }
+          }
+        }
+        if (p.ynorm != kNone && p.dy) {
+          block_sum(s, red, turn);
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+            const float m0 = p.ynorm == kLayer ? s[2 * i] / (float)p.C : 0.0f, m1 = s[2 * i + 1] / (float)p.C;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) d[i][k] = rs[i].y * (d[i][k] - m0 - yh[i][k] * m1);
+          }
+        }
+        if (p.dy)
+#pragma unroll
+          for (int i = 0; i < R; ++i)
+            if (live && i >= j && i < n) store8<T, true>(static_cast<T*>(p.dy) + (row + i) * p.C + c, 8, d[i]);
+      }
+      j = n;
+    }
+    st = st + 1 == p.stages ? 0 : st + 1;
+  }
+  if (g >= 0 && g < p.G) flush(g);
+}
+
+// Column sums of group blockIdx.y..: 32 channels x 32 partials at a time.  PT: one
 // "group" holds every CTA's partial.
+constexpr int kParts = 32;
 template <bool PT>
-__global__ void __launch_bounds__(256) group_sum_kernel(const __grid_constant__ Params p) {
-  __shared__ float sh[3][8][32];
+__global__ void __launch_bounds__(32 * kParts) group_sum_kernel(const __grid_constant__ Params p) {
+  __shared__ float sh[3][kParts][32];
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   const int groups = PT ? 1 : p.G;
@@ -577,7 +965,7 @@ __global__ void __launch_bounds__(256) group_sum_kernel(const __grid_constant__ 
     float s[3] = {0.0f, 0.0f, 0.0f};
     if (c < p.C) {
 #pragma unroll 4
-      for (int i = i0 + part; i < i1; i += 8) {
+      for (int i = i0 + part; i < i1; i += kParts) {
         const float* q = p.part + (long long)(i + (PT ? 0 : g)) * 3 * p.C + c;
 #pragma unroll
         for (int k = 0; k < 3; ++k) s[k] += q[(long long)k * p.C];
@@ -591,7 +979,7 @@ __global__ void __launch_bounds__(256) group_sum_kernel(const __grid_constant__ 
       for (int k = 0; k < 3; ++k) {
         s[k] = 0.0f;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) s[k] += sh[k][q][lane];
+        for (int q = 0; q < kParts; ++q) s[k] += sh[k][q][lane];
         p.gsum[((long long)g * 3 + k) * p.C + c] = s[k];
       }
       if (!PT) {
@@ -628,45 +1016,84 @@ __global__ void __launch_bounds__(128) chan_kernel(const __grid_constant__ Param
 
 static int threads_of(int C) { return ((C + 7) / 8 + 31) / 32 * 32; }
 
-// CTAs: two of a 5120-channel row's 640 threads fill an SM's registers; narrow
-// rows get as many warps.
+// CTAs: one of a 5120-channel row's 640 threads per SM, narrow rows to as many
+// threads (up to 16 CTAs).  More CTAs only add partial rows of column sums.
 static int ctas_of(long long rows, int C) {
-  const int per = std::max(1, std::min(32, 1536 / threads_of(C)));
+  const int per = std::max(1, std::min(16, 640 / threads_of(C)));
   return (int)std::min<long long>(rows, (long long)kSMs * per);
 }
 
-template <typename T, bool VEC, bool PT>
-static cudaError_t launch_fwd(const Params& p, cudaStream_t st) {
-  const int nt = threads_of(p.C);
-  const size_t smem = (size_t)nt * 8 * sizeof(float) * (p.y ? 3 : 2);
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(fwd_kernel<T, VEC, PT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 98304);
+template <auto K>
+static cudaError_t start(const Params& p, size_t smem, cudaStream_t st) {
+  if (smem > 40 * 1024) {  // with the static part, past the 48 KB default
+    const cudaError_t e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
   }
-  fwd_kernel<T, VEC, PT><<<p.ctas, nt, smem, st>>>(p);
+  K<<<p.ctas, threads_of(p.C), smem, st>>>(p);
   return cudaGetLastError();
 }
 
+// Shared memory of a streaming kernel with ``mods`` slots and ``tensors`` x R rows a
+// stage; sets p.stages to 3, or 2 where three do not fit, and 0 where two do not.
+constexpr size_t kSmemMax = 226 * 1024;
+static size_t ring_bytes(Params& p, int mods, int tensors, int R, int es) {
+  const size_t nt = (size_t)threads_of(p.C);
+  const size_t fixed = nt * 32 * mods, stage = nt * 8 * es * tensors * R;
+  p.stages = fixed + 3 * stage <= kSmemMax ? 3 : fixed + 2 * stage <= kSmemMax ? 2 : 0;
+  return fixed + p.stages * stage;
+}
+
+// Rows a stage: 40 KB of a 5120-channel row's tensors where the values of a
+// stage fit the registers of 640 threads (four rows forward, two backward).
+template <typename T, bool Y>
+static cudaError_t stream_fwd(Params& p, cudaStream_t st, bool& done) {
+  constexpr int R = (sizeof(T) == 4 ? 2 : 4) / (Y ? 2 : 1);
+  const bool wide = threads_of(p.C) > 640;
+  const size_t smem = ring_bytes(p, Y ? 3 : 2, Y ? 2 : 1, wide ? 1 : R, sizeof(T));
+  done = p.stages != 0;
+  if (!done) return cudaSuccess;
+  return wide ? start<fwd_stream_kernel<T, Y, 1, 1024>>(p, smem, st) : start<fwd_stream_kernel<T, Y, R, 640>>(p, smem, st);
+}
+template <typename T, bool Y>
+static cudaError_t stream_bwd(Params& p, cudaStream_t st, bool& done) {
+  constexpr int R = sizeof(T) == 4 || Y ? 1 : 2;
+  const bool wide = threads_of(p.C) > 640;
+  const size_t smem = ring_bytes(p, Y ? 2 : 1, Y ? 4 : 2, wide ? 1 : R, sizeof(T));
+  done = p.stages != 0;
+  if (!done) return cudaSuccess;
+  return wide ? start<bwd_stream_kernel<T, Y, 1, 1024>>(p, smem, st) : start<bwd_stream_kernel<T, Y, R, 640>>(p, smem, st);
+}
+
 template <typename T, bool VEC, bool PT>
-static cudaError_t launch_bwd(const Params& p, cudaStream_t st) {
-  const int nt = threads_of(p.C);
-  const size_t smem = (size_t)nt * 8 * sizeof(float) * (p.y ? 2 : 1);
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(bwd_kernel<T, VEC, PT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536);
+static cudaError_t launch_fwd(Params& p, cudaStream_t st) {
+  if constexpr (VEC && !PT) {
+    bool done = false;
+    const cudaError_t e = p.y ? stream_fwd<T, true>(p, st, done) : stream_fwd<T, false>(p, st, done);
+    if (done) return e;
+  }
+  return start<fwd_kernel<T, VEC, PT>>(p, (size_t)threads_of(p.C) * 32 * (p.y ? 3 : 2), st);
+}
+
+template <typename T, bool VEC, bool PT>
+static cudaError_t launch_bwd(Params& p, cudaStream_t st) {
+  if (p.rows > 0) {
+    bool done = false;
+    cudaError_t e = cudaSuccess;
+    if constexpr (VEC && !PT) e = p.y ? stream_bwd<T, true>(p, st, done) : stream_bwd<T, false>(p, st, done);
+    if (!done) e = start<bwd_kernel<T, VEC, PT>>(p, (size_t)threads_of(p.C) * 32 * (p.y ? 2 : 1), st);
     if (e != cudaSuccess) return e;
   }
-  if (p.rows > 0) bwd_kernel<T, VEC, PT><<<p.ctas, nt, smem, st>>>(p);
   const bool chan = p.dw || p.db || p.dwy;
   if (chan || (!PT && (p.dscale || p.dshift || p.dgate))) {
     const dim3 grid((unsigned)((p.C + 31) / 32), (unsigned)std::min(PT ? 1 : p.G, 65535));
-    group_sum_kernel<PT><<<grid, 256, 0, st>>>(p);
+    group_sum_kernel<PT><<<grid, 32 * kParts, 0, st>>>(p);
     if (chan) chan_kernel<PT><<<(p.C + 127) / 128, 128, 0, st>>>(p);
   }
   return cudaGetLastError();
 }
 
 template <typename T>
-static cudaError_t launch(const Params& p, bool bwd, bool vec, bool pt, cudaStream_t st) {
+static cudaError_t launch(Params& p, bool bwd, bool vec, bool pt, cudaStream_t st) {
 #define MH3_BN(F)                                                              \
   return vec ? (pt ? F<T, true, true>(p, st) : F<T, true, false>(p, st))       \
              : (pt ? F<T, false, true>(p, st) : F<T, false, false>(p, st))
