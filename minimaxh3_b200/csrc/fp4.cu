@@ -17,9 +17,12 @@
 // 2^(E-11): the exponent is E - 11, one more if M > 1.3125 - integer compares.
 //
 // Bound: HBM, 2 bytes in and 0.5625 out per 16-bit element.  A thread owns the 16
-// elements of a block (32 contiguous bytes, kept in registers between the row's
-// reduction and the rounding), so the input is read once and the block's maximum
-// needs no exchange; rows longer than 1024 threads' blocks are read twice.
+// elements of a block, so the block's maximum needs no exchange and the input is
+// read once.  CTAs are persistent: rows stream through a ring of three stages in
+// shared memory (cp.async; a thread reads back only what it copied), so two rows
+// are on their way while one is reduced and rounded.  Rows longer than 1024
+// threads' blocks, and rows that 16-byte vectors do not fit, are read twice by the
+// general kernel.
 #include <algorithm>
 #include <string>
 
@@ -39,6 +42,13 @@ __device__ __forceinline__ float div_by(float x, float s, float r) {
 }
 
 template <typename T>
+__device__ __forceinline__ float to_float(T v) {
+  if constexpr (std::is_same<T, float>::value) return v;
+  else if constexpr (std::is_same<T, __half>::value) return __half2float(v);
+  else return __bfloat162float(v);
+}
+
+template <typename T>
 __device__ __forceinline__ void load16(const T* p, float (&v)[16], bool vec) {
   constexpr int NV = 16 * sizeof(T) / 16;
   T e[16];
@@ -52,11 +62,7 @@ __device__ __forceinline__ void load16(const T* p, float (&v)[16], bool vec) {
     for (int i = 0; i < 16; ++i) e[i] = p[i];
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    if constexpr (std::is_same<T, float>::value) v[i] = e[i];
-    else if constexpr (std::is_same<T, __half>::value) v[i] = __half2float(e[i]);
-    else v[i] = __bfloat162float(e[i]);
-  }
+  for (int i = 0; i < 16; ++i) v[i] = to_float(e[i]);
 }
 
 // Largest magnitude as the integer of its bits: an infinity or NaN orders above
@@ -100,73 +106,142 @@ __device__ __forceinline__ long long block_offset(long long row, int b, int nk64
   return ((row >> 7) * nk64 + (b >> 2)) * 512 + (row & 31) * 16 + ((row & 127) >> 5) * 4 + (b & 3);
 }
 
-// Blocks of 32 x warps threads per row, rows side by side in y.  ONE: a row has at
-// most blockDim.x blocks, which stay in registers.  Rows M.. of the last block of
-// 128 get zero scales, so the buffer is the same whatever the memory held.
-template <typename T, bool ONE>
+// One block: its scale byte and 16 codes, from the row's exponent.
+__device__ __forceinline__ uint32_t round_block(const float (&v)[16], float inv, uint2& code) {
+  // e4m3 of absmax / (6 scale): the division by 6 is the only rounding before it
+  const float raw = div_by(__uint_as_float(absmax16(v)) * inv, 6.0f, 1.0f / 6.0f);
+  const uint32_t s8 = cvt_e4m3x2_f32(0.0f, raw) & 0xffu;
+  if (s8 != 0) {
+    const float s = e4m3_value(s8), r = __frcp_rn(s);
+    float q[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) q[i] = div_by(v[i] * inv, s, r);
+    code = make_uint2(e2m1x8(q), e2m1x8(q + 8));
+  }
+  return s8;
+}
+
+// The four scales of neighbouring lanes as one word (b: the lane's scale index).
+__device__ __forceinline__ void put_scales(uint8_t* blocks, uint32_t s8, long long row, int b, int nk64) {
+  uint32_t word = s8 << (8 * (b & 3));
+  const uint32_t lanes = 0xfu << (threadIdx.x & 28);
+  word |= __shfl_xor_sync(lanes, word, 1);
+  word |= __shfl_xor_sync(lanes, word, 2);
+  if ((b & 3) == 0) *reinterpret_cast<uint32_t*>(blocks + block_offset(row, b, nk64)) = word;
+}
+
+// Maximum over a row's threads: all lanes of a warp, then its warps through two
+// halves of shared memory in turn (one barrier: the half is written again only
+// after the next call's).
+__device__ __forceinline__ uint32_t row_max(uint32_t top, uint32_t (*red)[32], int& turn) {
+  top = __reduce_max_sync(0xffffffffu, top);
+  const int warps = blockDim.x >> 5;
+  if (warps == 1) return top;
+  const int lane = threadIdx.x & 31;
+  uint32_t* r = red[turn] + threadIdx.y * warps;
+  if (lane == 0) r[threadIdx.x >> 5] = top;
+  __syncthreads();
+  top = __reduce_max_sync(0xffffffffu, lane < warps ? r[lane] : 0u);
+  turn ^= 1;
+  return top;
+}
+
+constexpr int kStages = 3;
+
+// Streaming: blockDim.x threads (a multiple of 32, at least the row's scales) per
+// row, blockDim.y rows at once.  Rows M.. of the last block of 128 get zero
+// scales, so the buffer is the same whatever the memory held.
+template <typename T>
+__global__ void __launch_bounds__(kMaxThreads) quantize_stream_kernel(const T* __restrict__ x, long long stride, long long M, int K,
+                                                                     uint8_t* __restrict__ x4, uint8_t* __restrict__ blocks,
+                                                                     float* __restrict__ scale) {
+  constexpr int W = sizeof(T);  // 16-byte vectors of a block
+  extern __shared__ uint4 ring[];
+  __shared__ uint32_t red[2][32];
+  const int nb = K / 16, nk64 = (K + 63) / 64, b = threadIdx.x;
+  const int nthr = blockDim.x * blockDim.y, tid = threadIdx.y * blockDim.x + threadIdx.x;
+  const bool mine = b < nb;
+  const long long step = (long long)gridDim.x * blockDim.y;
+  const long long padded = (M + 127) / 128 * 128;
+  auto issue = [&](long long row, int st) {
+    if (mine && row < M) {
+      const uint4* src = reinterpret_cast<const uint4*>(x + row * stride + b * 16);
+#pragma unroll
+      for (int w = 0; w < W; ++w)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(ring + (st * W + w) * nthr + tid)), "l"(src + w)
+                     : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const long long first = (long long)blockIdx.x * blockDim.y;
+#pragma unroll
+  for (int j = 0; j < kStages - 1; ++j) issue(first + threadIdx.y + j * step, j);
+  int st = 0, turn = 0;
+  for (long long base = first; base < padded; base += step) {  // the same trips for every thread of the CTA
+    const long long row = base + threadIdx.y;
+    issue(row + (kStages - 1) * step, st == 0 ? kStages - 1 : st - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    const bool live = row < M;
+    float v[16];
+    if (mine && live) {
+      uint4 u[W];
+#pragma unroll
+      for (int w = 0; w < W; ++w) u[w] = ring[(st * W + w) * nthr + tid];
+      T e[16];
+      memcpy(e, u, sizeof(e));
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = to_float(e[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+    }
+    const uint32_t top = row_max(absmax16(v), red, turn);
+    if (row < padded) {
+      const bool finite = top < 0x7f800000u;
+      const int e = row_exponent(top);
+      uint2 code = make_uint2(0, 0);
+      const uint32_t s8 = finite ? round_block(v, pow2f(-e), code) : 0u;  // e in [-100, 117]
+      if (live && b == 0) scale[row] = finite ? pow2f(e) : __uint_as_float(0x7fffffffu);
+      if (live && mine) *reinterpret_cast<uint2*>(x4 + row * (K / 2) + (long long)b * 8) = code;
+      if (b < nk64 * 4) put_scales(blocks, s8, row, b, nk64);
+    }
+    st = st + 1 == kStages ? 0 : st + 1;
+  }
+}
+
+// General: one row per CTA, read once for its maximum and once for the rounding.
+template <typename T>
 __global__ void __launch_bounds__(kMaxThreads) quantize_kernel(const T* __restrict__ x, long long stride, long long M, int K,
                                                               uint8_t* __restrict__ x4, uint8_t* __restrict__ blocks,
                                                               float* __restrict__ scale, int vec) {
-  __shared__ uint32_t red[32];
-  const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+  __shared__ uint32_t red[2][32];
+  const long long row = blockIdx.x;
   const int nb = K / 16, nk64 = (K + 63) / 64;
-  const int warps = blockDim.x >> 5;
   const T* xp = x + row * stride;
-  float v[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = 0.0f;
-  uint32_t top = 0, mine = 0;
-  if (row < M) {
-    if constexpr (ONE) {
-      if ((int)threadIdx.x < nb) load16(xp + threadIdx.x * 16, v, vec != 0);
-      top = mine = absmax16(v);
-    } else {
-      for (int b = threadIdx.x; b < nb; b += blockDim.x) {
-        load16(xp + (long long)b * 16, v, vec != 0);
-        top = max(top, absmax16(v));
-      }
-    }
-  }
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (warps > 1) {
-    const int w0 = threadIdx.y * warps;  // this row's partial maxima
-    if ((threadIdx.x & 31) == 0) red[w0 + (threadIdx.x >> 5)] = top;
-    __syncthreads();
-    top = 0;
-    for (int w = 0; w < warps; ++w) top = max(top, red[w0 + w]);
-  }
-  if (row >= (M + 127) / 128 * 128) return;  // whole warps: blockDim.x is a multiple of 32
   const bool live = row < M;
+  float v[16];
+  uint32_t top = 0;
+  int turn = 0;
+  if (live)
+    for (int b = threadIdx.x; b < nb; b += blockDim.x) {
+      load16(xp + (long long)b * 16, v, vec != 0);
+      top = max(top, absmax16(v));
+    }
+  top = row_max(top, red, turn);
   const bool finite = top < 0x7f800000u;
   const int e = row_exponent(top);
-  const float inv = pow2f(-e);  // e in [-100, 117]
   if (live && threadIdx.x == 0) scale[row] = finite ? pow2f(e) : __uint_as_float(0x7fffffffu);
-  for (int b = threadIdx.x; b < nk64 * 4; b += blockDim.x) {  // nk64 * 4: past K the scales are 0
+  for (int b = threadIdx.x; b < nk64 * 4; b += blockDim.x) {
     uint32_t s8 = 0;
     uint2 code = make_uint2(0, 0);
-    if (b < nb && live && finite) {
-      if constexpr (!ONE) {
+    if (b < nb && live) {
+      if (finite) {
         load16(xp + (long long)b * 16, v, vec != 0);
-        mine = absmax16(v);
+        s8 = round_block(v, pow2f(-e), code);
       }
-      // e4m3 of absmax / (6 scale): the division by 6 is the only rounding before it
-      const float raw = div_by(__uint_as_float(mine) * inv, 6.0f, 1.0f / 6.0f);
-      s8 = cvt_e4m3x2_f32(0.0f, raw) & 0xffu;
-      if (s8 != 0) {
-        const float s = e4m3_value(s8), r = __frcp_rn(s);
-        float q[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) q[i] = div_by(v[i] * inv, s, r);
-        code = make_uint2(e2m1x8(q), e2m1x8(q + 8));
-      }
+      *reinterpret_cast<uint2*>(x4 + row * (K / 2) + (long long)b * 8) = code;
     }
-    if (b < nb && live) *reinterpret_cast<uint2*>(x4 + row * (K / 2) + (long long)b * 8) = code;
-    // four neighbouring lanes hold the four scales of one word
-    uint32_t word = s8 << (8 * (b & 3));
-    const uint32_t lanes = 0xfu << (threadIdx.x & 28);
-    word |= __shfl_xor_sync(lanes, word, 1);
-    word |= __shfl_xor_sync(lanes, word, 2);
-    if ((b & 3) == 0) *reinterpret_cast<uint32_t*>(blocks + block_offset(row, b, nk64)) = word;
+    put_scales(blocks, s8, row, b, nk64);
   }
 }
 
@@ -229,14 +304,26 @@ static cudaError_t launch_quantize(const void* x, long long stride, long long M,
                                    cudaStream_t st) {
   const int nb4 = (K + 63) / 64 * 4;  // scales of a row, the last word filled up
   const int tx = std::min(kMaxThreads, (nb4 + 31) / 32 * 32);
-  const dim3 block((unsigned)tx, (unsigned)std::max(1, 256 / tx));
   const long long padded = (M + 127) / 128 * 128;
-  const unsigned grid = (unsigned)((padded + block.y - 1) / block.y);
   const int vec = ((uintptr_t)x & 15u) == 0 && stride * (long long)sizeof(T) % 16 == 0;
   const T* xp = static_cast<const T*>(x);
   uint8_t *c = static_cast<uint8_t*>(x4), *b = static_cast<uint8_t*>(blocks);
-  if (nb4 <= tx) quantize_kernel<T, true><<<grid, block, 0, st>>>(xp, stride, M, K, c, b, scale, vec);
-  else quantize_kernel<T, false><<<grid, block, 0, st>>>(xp, stride, M, K, c, b, scale, vec);
+  if (nb4 > tx || !vec) {
+    quantize_kernel<T><<<(unsigned)padded, tx, 0, st>>>(xp, stride, M, K, c, b, scale, vec);
+    return cudaGetLastError();
+  }
+  const dim3 block((unsigned)tx, (unsigned)std::max(1, 256 / tx));
+  const int nthr = tx * (int)block.y;
+  const size_t smem = (size_t)kStages * sizeof(T) * 16 * nthr;
+  if (smem > 40 * 1024) {  // with the static part, past the 48 KB default
+    const cudaError_t e =
+        cudaFuncSetAttribute(quantize_stream_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  // resident CTAs of 64 registers a thread, and of 224 KB of rings
+  const long long per = std::min<long long>(1024 / nthr, 224 * 1024 / (long long)smem);
+  const long long grid = std::min<long long>((padded + block.y - 1) / block.y, 148 * std::max(1ll, per));
+  quantize_stream_kernel<T><<<(unsigned)grid, block, smem, st>>>(xp, stride, M, K, c, b, scale);
   return cudaGetLastError();
 }
 
