@@ -564,6 +564,43 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// Eight channels as four pairs: the arithmetic below is in packed f32 pairs, which
+// halves its issue slots (these kernels are otherwise bound by instruction issue).
+struct V8 {
+  float2 e[4];
+};
+__device__ __forceinline__ void pair_get(const float4* s, V8& v) {
+  const float4 a = s[threadIdx.x], b = s[blockDim.x + threadIdx.x];
+  v.e[0] = make_float2(a.x, a.y);
+  v.e[1] = make_float2(a.z, a.w);
+  v.e[2] = make_float2(b.x, b.y);
+  v.e[3] = make_float2(b.z, b.w);
+}
+template <typename T>
+__device__ __forceinline__ void store_pairs(T* p, const V8& v) {
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v.e[0].x, v.e[0].y, v.e[1].x, v.e[1].y);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v.e[2].x, v.e[2].y, v.e[3].x, v.e[3].y);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(v.e[i].x, v.e[i].y);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v.e[i].x, v.e[i].y);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+__device__ __forceinline__ float sum8(const V8& v) {
+  const float2 s = fadd2(fadd2(v.e[0], v.e[1]), fadd2(v.e[2], v.e[3]));
+  return s.x + s.y;
+}
+
 // A thread's eight channels of a row, to and from its place in the ring (``at``:
 // the place of the row and tensor, in 16-byte units times the CTA's threads).
 template <typename T>
@@ -577,46 +614,88 @@ struct Ring {
                    "l"(reinterpret_cast<const uint4*>(src) + w)
                    : "memory");
   }
-  __device__ __forceinline__ void get(int at, float (&v)[8]) const {
+  __device__ __forceinline__ void get(int at, V8& v) const {
     Raw<T> r;
 #pragma unroll
     for (int w = 0; w < W; ++w) r.u[w] = base[(at * W + w) * (int)blockDim.x + threadIdx.x];
-    unpack(r, v);
+    float f[8];
+    unpack(r, f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v.e[i] = make_float2(f[2 * i], f[2 * i + 1]);
   }
 };
 
-// (mean, rstd) of R rows at once (channels of threads past the row are 0).
+// Sums over the CTA of N values per thread (1, 2 or 4).  The first exchanges hand
+// each lane one of the values (lane % N), so the rest of the tree carries one
+// value: 6 shuffles for 4 values, not 20.  The halves of ``buf`` take turns, as
+// in block_sum.
+template <int N>
+__device__ __forceinline__ void team_sum(float (&v)[N], float (*buf)[4][32], int& turn) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  float z;
+  if constexpr (N == 1) {
+    z = v[0] + __shfl_xor_sync(0xffffffffu, v[0], 1);
+    z += __shfl_xor_sync(0xffffffffu, z, 2);
+  } else {
+    const bool odd = lane & 1;
+    float a = odd ? v[1] : v[0];
+    a += __shfl_xor_sync(0xffffffffu, odd ? v[0] : v[1], 1);
+    if constexpr (N == 2) {
+      z = a + __shfl_xor_sync(0xffffffffu, a, 2);
+    } else {
+      float b = odd ? v[3] : v[2];
+      b += __shfl_xor_sync(0xffffffffu, odd ? v[2] : v[3], 1);
+      const bool high = lane & 2;
+      z = high ? b : a;
+      z += __shfl_xor_sync(0xffffffffu, high ? a : b, 2);
+    }
+  }
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+  if (nw > 1) {
+    float* r = &buf[turn][0][0];
+    if (lane < N) r[warp * N + lane] = z;
+    __syncthreads();
+    z = 0.0f;
+    for (int i = lane; i < nw * N; i += 32) z += r[i];  // i % N == lane % N
+#pragma unroll
+    for (int o = N; o < 32; o <<= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    turn ^= 1;
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = N == 1 ? z : __shfl_sync(0xffffffffu, z, k);
+}
+
+// Rows i of v to v - mean, and their (mean, rstd); threads past the row hold zeros
+// and add nothing.
 template <int R>
-__device__ __forceinline__ void rows_stats(const float (&v)[R][8], bool live, int C, int kind, float eps, float (*buf)[4][32],
-                                           int& turn, float2 (&out)[R]) {
+__device__ __forceinline__ void center(V8 (&v)[R], bool live, float inv_c, int kind, float eps, float (*buf)[4][32], int& turn,
+                                       float2 (&out)[R]) {
   float s[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) out[i].x = 0.0f;
   if (kind == kLayer) {
 #pragma unroll
+    for (int i = 0; i < R; ++i) s[i] = sum8(v[i]);
+    team_sum(s, buf, turn);
+#pragma unroll
     for (int i = 0; i < R; ++i) {
-      s[i] = 0.0f;
+      out[i].x = s[i] * inv_c;
+      if (live)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s[i] += v[i][k];
+        for (int k = 0; k < 4; ++k) v[i].e[k] = fadd2(v[i].e[k], both(-out[i].x));
     }
-    block_sum(s, buf, turn);
-#pragma unroll
-    for (int i = 0; i < R; ++i) out[i].x = s[i] / (float)C;
   }
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    s[i] = 0.0f;
-    if (live) {
+    float2 q = fmul2(v[i].e[0], v[i].e[0]);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float d = v[i][k] - out[i].x;
-        s[i] = fmaf(d, d, s[i]);
-      }
-    }
+    for (int k = 1; k < 4; ++k) q = ffma2(v[i].e[k], v[i].e[k], q);
+    s[i] = q.x + q.y;
   }
-  block_sum(s, buf, turn);
+  team_sum(s, buf, turn);
 #pragma unroll
-  for (int i = 0; i < R; ++i) out[i].y = rsqrtf(s[i] / (float)C + eps);
+  for (int i = 0; i < R; ++i) out[i].y = rsqrtf(fmaf(s[i], inv_c, eps));
 }
 
 template <typename T, bool Y, int R, int MAXT>
@@ -630,6 +709,7 @@ __global__ void __launch_bounds__(MAXT) fwd_stream_kernel(const __grid_constant_
   const Ring<T> ring{reinterpret_cast<uint4*>(slots + (Y ? 6 : 4) * blockDim.x)};
   const int c = threadIdx.x * 8;
   const bool live = c < p.C;
+  const float inv_c = 1.0f / (float)p.C;
   const long long lo = p.rows * blockIdx.x / p.ctas, hi = p.rows * (blockIdx.x + 1) / p.ctas;
   int turn = 0, g = -1;
   long long end = lo;
@@ -651,6 +731,55 @@ __global__ void __launch_bounds__(MAXT) fwd_stream_kernel(const __grid_constant_
     if (p.stages == 3) cp_wait<2>();
     else cp_wait<1>();
     const int cnt = (int)min((long long)R, hi - row);
+    // Rows [j, n) of the stage, all of one group; ALL: every row of it.
+    auto work = [&](auto all, int j, int n) {
+      constexpr bool ALL = decltype(all)::value;
+      V8 v[R];
+      float2 sy[R], sr[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        sy[i] = sr[i] = make_float2(0.0f, 1.0f);
+        v[i] = V8{};
+        if (live && (ALL || (i >= j && i < n))) ring.get((st * NT) * R + i, v[i]);
+      }
+      if (Y) {
+        V8 y[R], a;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          y[i] = V8{};
+          if (live && (ALL || (i >= j && i < n))) ring.get((st * NT + 1) * R + i, y[i]);
+        }
+        if (p.ynorm != kNone) center<R>(y, live, inv_c, p.ynorm, p.eps, red, turn, sy);
+        if (live) {
+          pair_get(sG, a);
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              v[i].e[k] = ffma2(fmul2(a.e[k], both(sy[i].y)), y[i].e[k], fmul2(v[i].e[k], both(p.alpha)));
+            if (p.r && (ALL || (i >= j && i < n))) store_pairs<T>(static_cast<T*>(p.r) + (row + i) * p.C + c, v[i]);
+          }
+        }
+      }
+      if (p.h != nullptr) {
+        center<R>(v, live, inv_c, p.norm, p.eps, red, turn, sr);
+        if (live) {
+          V8 a, b;
+          pair_get(sA, a);
+          pair_get(sB, b);
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[i].e[k] = ffma2(fmul2(v[i].e[k], both(sr[i].y)), a.e[k], b.e[k]);
+            if (ALL || (i >= j && i < n)) store_pairs<T>(static_cast<T*>(p.h) + (row + i) * p.C + c, v[i]);
+          }
+        }
+      }
+      if (threadIdx.x == 0 && p.stats)
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+          if (ALL || (i >= j && i < n)) p.stats[row + i] = make_float4(sy[i].x, sy[i].y, sr[i].x, sr[i].y);
+    };
     for (int j = 0; j < cnt;) {  // the stage's rows, a group at a time
       if (row + j >= end) {
         g = group_of(p, row + j, g == p.G ? -1 : g, end);
@@ -679,66 +808,18 @@ __global__ void __launch_bounds__(MAXT) fwd_stream_kernel(const __grid_constant_
         }
       }
       const int n = (int)min((long long)cnt, end - row);
-      float v[R][8];
-      float2 sy[R], sr[R];
-#pragma unroll
-      for (int i = 0; i < R; ++i) {
-        sy[i] = sr[i] = make_float2(0.0f, 1.0f);
-        if (live && i >= j && i < n) ring.get((st * NT) * R + i, v[i]);
-        else
-#pragma unroll
-          for (int k = 0; k < 8; ++k) v[i][k] = 0.0f;
-      }
       if (g >= p.G) {  // outside every packed sequence: zeros
-        const float z[8] = {};
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-          if (i >= j && i < n) {
-            if (live && p.r) store8<T, true>(static_cast<T*>(p.r) + (row + i) * p.C + c, 8, z);
-            if (live && p.h) store8<T, true>(static_cast<T*>(p.h) + (row + i) * p.C + c, 8, z);
-            if (threadIdx.x == 0 && p.stats) p.stats[row + i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          }
-        j = n;
-        continue;
-      }
-      if (Y) {
-        float y[R][8], a[8];
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-          if (live && i >= j && i < n) ring.get((st * NT + 1) * R + i, y[i]);
-          else
-#pragma unroll
-            for (int k = 0; k < 8; ++k) y[i][k] = 0.0f;
+        const V8 z = {};
+        for (int i = j; i < n; ++i) {
+          if (live && p.r) store_pairs<T>(static_cast<T*>(p.r) + (row + i) * p.C + c, z);
+          if (live && p.h) store_pairs<T>(static_cast<T*>(p.h) + (row + i) * p.C + c, z);
+          if (threadIdx.x == 0 && p.stats) p.stats[row + i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
-        if (p.ynorm != kNone) rows_stats<R>(y, live, p.C, p.ynorm, p.eps, red, turn, sy);
-        if (live) {
-          slot_get(sG, a);
-#pragma unroll
-          for (int i = 0; i < R; ++i) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[i][k] = fmaf(a[k], (y[i][k] - sy[i].x) * sy[i].y, p.alpha * v[i][k]);
-            if (i >= j && i < n) store8<T, true>(static_cast<T*>(p.r) + (row + i) * p.C + c, 8, v[i]);
-          }
-        }
+      } else if (n - j == R) {
+        work(std::true_type{}, 0, R);
+      } else {
+        work(std::false_type{}, j, n);
       }
-      if (p.h != nullptr) {
-        rows_stats<R>(v, live, p.C, p.norm, p.eps, red, turn, sr);
-        if (live) {
-          float a[8], b[8];
-          slot_get(sA, a);
-          slot_get(sB, b);
-#pragma unroll
-          for (int i = 0; i < R; ++i) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[i][k] = fmaf((v[i][k] - sr[i].x) * sr[i].y, a[k], b[k]);
-            if (i >= j && i < n) store8<T, true>(static_cast<T*>(p.h) + (row + i) * p.C + c, 8, v[i]);
-          }
-        }
-      }
-      if (threadIdx.x == 0 && p.stats)
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-          if (i >= j && i < n) p.stats[row + i] = make_float4(sy[i].x, sy[i].y, sr[i].x, sr[i].y);
       j = n;
     }
     st = st + 1 == p.stages ? 0 : st + 1;
@@ -755,20 +836,20 @@ __global__ void __launch_bounds__(MAXT) bwd_stream_kernel(const __grid_constant_
   const Ring<T> ring{reinterpret_cast<uint4*>(slots + (Y ? 4 : 2) * blockDim.x)};
   const int c = threadIdx.x * 8;
   const bool live = c < p.C;
+  const float inv_c = 1.0f / (float)p.C;
   const long long lo = p.rows * blockIdx.x / p.ctas, hi = p.rows * (blockIdx.x + 1) / p.ctas;
   const bool has_dr = Y && p.dr != nullptr, has_dh = p.dh != nullptr;
   int turn = 0, g = -1;
   long long end = lo;
-  float a1[8] = {}, a2[8] = {}, a3[8] = {};  // column sums of dh xhat, dh and d yhat
-  float4 nst[R];                             // the next stage's row statistics
+  V8 a1 = {}, a2 = {}, a3 = {};  // column sums of dh xhat, dh and d yhat
+  float4 nst[R];                 // the next stage's row statistics
   auto flush = [&](int grp) {
     if (!live) return;
     float* o = p.part + (long long)(blockIdx.x + grp) * 3 * p.C + c;
-    store8<float, true>(o, 8, a1);
-    store8<float, true>(o + p.C, 8, a2);
-    store8<float, true>(o + 2 * p.C, 8, a3);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) a1[k] = a2[k] = a3[k] = 0.0f;
+    store_pairs<float>(o, a1);
+    store_pairs<float>(o + p.C, a2);
+    store_pairs<float>(o + 2 * p.C, a3);
+    a1 = a2 = a3 = V8{};
   };
   auto issue = [&](long long row, int st) {
     if (live) {
@@ -823,83 +904,80 @@ __global__ void __launch_bounds__(MAXT) bwd_stream_kernel(const __grid_constant_
       }
       const int n = (int)min((long long)cnt, end - row);
       if (g >= p.G) {  // outside every packed sequence: no gradient
-        const float z[8] = {};
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-          if (live && i >= j && i < n) {
-            if (p.dx) store8<T, true>(static_cast<T*>(p.dx) + (row + i) * p.C + c, 8, z);
-            if (p.dy) store8<T, true>(static_cast<T*>(p.dy) + (row + i) * p.C + c, 8, z);
+        const V8 z = {};
+        for (int i = j; i < n; ++i)
+          if (live) {
+            if (p.dx) store_pairs<T>(static_cast<T*>(p.dx) + (row + i) * p.C + c, z);
+            if (p.dy) store_pairs<T>(static_cast<T*>(p.dy) + (row + i) * p.C + c, z);
           }
         j = n;
         continue;
       }
-      float d[R][8], yh[R][8], gt[8];
-      if (Y && live) slot_get(sG, gt);
+      V8 d[R], yh[R], gt = {};
+      if (Y && live) pair_get(sG, gt);
       {
-        float xh[R][8], s[2 * R];
+        V8 xh[R];
+        float s[2 * R];
 #pragma unroll
         for (int i = 0; i < R; ++i) {
           s[2 * i] = s[2 * i + 1] = 0.0f;
-          const bool in = live && i >= j && i < n;
+          xh[i] = yh[i] = d[i] = V8{};
           const int at = st * NT * R + i;
-          if (in) {
+          if (live && i >= j && i < n) {
             ring.get(at, xh[i]);
             if (Y) {
               ring.get(at + 2 * R, yh[i]);
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                yh[i][k] = (yh[i][k] - rs[i].x) * rs[i].y;
-                xh[i][k] = fmaf(gt[k], yh[i][k], p.alpha * xh[i][k]);
+              for (int k = 0; k < 4; ++k) {
+                yh[i].e[k] = fmul2(fadd2(yh[i].e[k], both(-rs[i].x)), both(rs[i].y));
+                xh[i].e[k] = ffma2(gt.e[k], yh[i].e[k], fmul2(xh[i].e[k], both(p.alpha)));
               }
             }
             if (has_dh) {
-              float t[8];
+              V8 t;
               ring.get(at + R, t);
-              slot_get(sA, d[i]);
+              pair_get(sA, d[i]);
+              float2 s0 = both(0.0f), s1 = s0;
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                xh[i][k] = (xh[i][k] - rs[i].z) * rs[i].w;
-                a1[k] = fmaf(t[k], xh[i][k], a1[k]);
-                a2[k] += t[k];
-                d[i][k] *= t[k];  // dn
-                s[2 * i] += d[i][k];
-                s[2 * i + 1] = fmaf(d[i][k], xh[i][k], s[2 * i + 1]);
+              for (int k = 0; k < 4; ++k) {
+                xh[i].e[k] = fmul2(fadd2(xh[i].e[k], both(-rs[i].z)), both(rs[i].w));
+                a1.e[k] = ffma2(t.e[k], xh[i].e[k], a1.e[k]);
+                a2.e[k] = fadd2(a2.e[k], t.e[k]);
+                d[i].e[k] = fmul2(d[i].e[k], t.e[k]);  // dn
+                s0 = fadd2(s0, d[i].e[k]);
+                s1 = ffma2(d[i].e[k], xh[i].e[k], s1);
               }
+              s[2 * i] = s0.x + s0.y;
+              s[2 * i + 1] = s1.x + s1.y;
             }
-          } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) xh[i][k] = yh[i][k] = d[i][k] = 0.0f;
           }
         }
         if (has_dh) {
-          block_sum(s, red, turn);
+          team_sum(s, red, turn);
 #pragma unroll
           for (int i = 0; i < R; ++i) {
-            const float m0 = p.norm == kLayer ? s[2 * i] / (float)p.C : 0.0f, m1 = s[2 * i + 1] / (float)p.C;
+            const float m0 = p.norm == kLayer ? -s[2 * i] * inv_c : 0.0f, m1 = -s[2 * i + 1] * inv_c;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) d[i][k] = rs[i].w * (d[i][k] - m0 - xh[i][k] * m1);
+            for (int k = 0; k < 4; ++k)
+              d[i].e[k] = fmul2(ffma2(xh[i].e[k], both(m1), fadd2(d[i].e[k], both(m0))), both(rs[i].w));
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < R; ++i)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) d[i][k] = 0.0f;
         }
       }
-      const float al = Y ? p.alpha : 1.0f;
 #pragma unroll
       for (int i = 0; i < R; ++i)
         if (live && i >= j && i < n) {
-          float t[8];
+          V8 t;
           if (has_dr) {
             ring.get(st * NT * R + i + 3 * R, t);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) d[i][k] += t[k];
+            for (int k = 0; k < 4; ++k) d[i].e[k] = fadd2(d[i].e[k], t.e[k]);
           }
           if (p.dx) {
+            t = d[i];
+            if (Y)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) t[k] = al * d[i][k];
-            store8<T, true>(static_cast<T*>(p.dx) + (row + i) * p.C + c, 8, t);
+              for (int k = 0; k < 4; ++k) t.e[k] = fmul2(t.e[k], both(p.alpha));
+            store_pairs<T>(static_cast<T*>(p.dx) + (row + i) * p.C + c, t);
           }
         }
       if (Y) {
@@ -908,28 +986,32 @@ __global__ void __launch_bounds__(MAXT) bwd_stream_kernel(const __grid_constant_
         for (int i = 0; i < R; ++i) {
           s[2 * i] = s[2 * i + 1] = 0.0f;
           if (live && i >= j && i < n) {
+            float2 s0 = both(0.0f), s1 = s0;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              a3[k] = fmaf(d[i][k], yh[i][k], a3[k]);
-              d[i][k] *= gt[k];
-              s[2 * i] += d[i][k];
-              s[2 * i + 1] = fmaf(d[i][k], yh[i][k], s[2 * i + 1]);
+            for (int k = 0; k < 4; ++k) {
+              a3.e[k] = ffma2(d[i].e[k], yh[i].e[k], a3.e[k]);
+              d[i].e[k] = fmul2(d[i].e[k], gt.e[k]);
+              s0 = fadd2(s0, d[i].e[k]);
+              s1 = ffma2(d[i].e[k], yh[i].e[k], s1);
             }
+            s[2 * i] = s0.x + s0.y;
+            s[2 * i + 1] = s1.x + s1.y;
           }
         }
         if (p.ynorm != kNone && p.dy) {
-          block_sum(s, red, turn);
+          team_sum(s, red, turn);
 #pragma unroll
           for (int i = 0; i < R; ++i) {
-            const float m0 = p.ynorm == kLayer ? s[2 * i] / (float)p.C : 0.0f, m1 = s[2 * i + 1] / (float)p.C;
+            const float m0 = p.ynorm == kLayer ? -s[2 * i] * inv_c : 0.0f, m1 = -s[2 * i + 1] * inv_c;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) d[i][k] = rs[i].y * (d[i][k] - m0 - yh[i][k] * m1);
+            for (int k = 0; k < 4; ++k)
+              d[i].e[k] = fmul2(ffma2(yh[i].e[k], both(m1), fadd2(d[i].e[k], both(m0))), both(rs[i].y));
           }
         }
         if (p.dy)
 #pragma unroll
           for (int i = 0; i < R; ++i)
-            if (live && i >= j && i < n) store8<T, true>(static_cast<T*>(p.dy) + (row + i) * p.C + c, 8, d[i]);
+            if (live && i >= j && i < n) store_pairs<T>(static_cast<T*>(p.dy) + (row + i) * p.C + c, d[i]);
       }
       j = n;
     }

@@ -106,19 +106,48 @@ __device__ __forceinline__ long long block_offset(long long row, int b, int nk64
   return ((row >> 7) * nk64 + (b >> 2)) * 512 + (row & 31) * 16 + ((row & 127) >> 5) * 4 + (b & 3);
 }
 
-// One block: its scale byte and 16 codes, from the row's exponent.
-__device__ __forceinline__ uint32_t round_block(const float (&v)[16], float inv, uint2& code) {
+// One block: its scale byte and 16 codes, from its absmax and the row's exponent.
+// The quotients are div_by in packed pairs, which halves their issue slots.
+__device__ __forceinline__ uint32_t round_block(const float (&v)[16], uint32_t top, float inv, uint2& code) {
   // e4m3 of absmax / (6 scale): the division by 6 is the only rounding before it
-  const float raw = div_by(__uint_as_float(absmax16(v)) * inv, 6.0f, 1.0f / 6.0f);
+  const float raw = div_by(__uint_as_float(top) * inv, 6.0f, 1.0f / 6.0f);
   const uint32_t s8 = cvt_e4m3x2_f32(0.0f, raw) & 0xffu;
   if (s8 != 0) {
     const float s = e4m3_value(s8), r = __frcp_rn(s);
+    const float2 r2 = both(r), ns2 = both(-s), inv2 = both(inv);
     float q[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) q[i] = div_by(v[i] * inv, s, r);
+    for (int i = 0; i < 16; i += 2) {
+      const float2 x = fmul2(make_float2(v[i], v[i + 1]), inv2);
+      const float2 a = fmul2(x, r2);
+      const float2 d = ffma2(ffma2(ns2, a, x), r2, a);
+      q[i] = d.x;
+      q[i + 1] = d.y;
+    }
     code = make_uint2(e2m1x8(q), e2m1x8(q + 8));
   }
   return s8;
+}
+
+// absmax16 of a block as loaded: 16-bit types compare two magnitudes at a time as
+// integers, and only the larger one is widened.
+template <typename T>
+__device__ __forceinline__ uint32_t absmax_raw(const uint4 (&u)[sizeof(T)]) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(u);
+  if constexpr (sizeof(T) == 4) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max(m, w[i] & 0x7fffffffu);
+    return m;
+  } else {
+    uint32_t m = w[0] & 0x7fff7fffu;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+    m = max(m & 0xffffu, m >> 16);
+    if constexpr (std::is_same<T, __half>::value)
+      return m >= 0x7c00u ? 0x7f800000u | m : __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+    return m << 16;
+  }
 }
 
 // The four scales of neighbouring lanes as one word (b: the lane's scale index).
@@ -182,25 +211,24 @@ __global__ void __launch_bounds__(kMaxThreads) quantize_stream_kernel(const T* _
     issue(row + (kStages - 1) * step, st == 0 ? kStages - 1 : st - 1);
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
     const bool live = row < M;
-    float v[16];
-    if (mine && live) {
-      uint4 u[W];
+    uint4 u[W];
 #pragma unroll
-      for (int w = 0; w < W; ++w) u[w] = ring[(st * W + w) * nthr + tid];
-      T e[16];
-      memcpy(e, u, sizeof(e));
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = to_float(e[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = 0.0f;
-    }
-    const uint32_t top = row_max(absmax16(v), red, turn);
+    for (int w = 0; w < W; ++w) u[w] = mine && live ? ring[(st * W + w) * nthr + tid] : make_uint4(0, 0, 0, 0);
+    const uint32_t own = absmax_raw<T>(u);
+    const uint32_t top = row_max(own, red, turn);
     if (row < padded) {
       const bool finite = top < 0x7f800000u;
       const int e = row_exponent(top);
       uint2 code = make_uint2(0, 0);
-      const uint32_t s8 = finite ? round_block(v, pow2f(-e), code) : 0u;  // e in [-100, 117]
+      uint32_t s8 = 0;
+      if (finite) {
+        T t[16];
+        float v[16];
+        memcpy(t, u, sizeof(t));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = to_float(t[i]);
+        s8 = round_block(v, own, pow2f(-e), code);  // e in [-100, 117]
+      }
       if (live && b == 0) scale[row] = finite ? pow2f(e) : __uint_as_float(0x7fffffffu);
       if (live && mine) *reinterpret_cast<uint2*>(x4 + row * (K / 2) + (long long)b * 8) = code;
       if (b < nk64 * 4) put_scales(blocks, s8, row, b, nk64);
@@ -237,7 +265,7 @@ __global__ void __launch_bounds__(kMaxThreads) quantize_kernel(const T* __restri
     if (b < nb && live) {
       if (finite) {
         load16(xp + (long long)b * 16, v, vec != 0);
-        s8 = round_block(v, pow2f(-e), code);
+        s8 = round_block(v, absmax16(v), pow2f(-e), code);
       }
       *reinterpret_cast<uint2*>(x4 + row * (K / 2) + (long long)b * 8) = code;
     }
@@ -257,44 +285,57 @@ __device__ __forceinline__ void e2m1x8_halves(uint32_t w, uint32_t (&h)[4]) {
       : "r"(w));
 }
 
-// One 16-element block per thread.
+// Eight elements per thread (16 bytes of bf16, neighbouring threads side by side),
+// kRows rows whose loads are issued together.
+constexpr int kRows = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ x4, const uint8_t* __restrict__ blocks,
-                                                         const float* __restrict__ scale, int nb, long long M, T* __restrict__ out) {
-  const int b = blockIdx.x * blockDim.x + threadIdx.x;
-  const int nk64 = (nb + 3) / 4;
-  if (b >= nb) return;
-  for (long long row = (long long)blockIdx.y * blockDim.y + threadIdx.y; row < M; row += (long long)gridDim.y * blockDim.y) {
-    const uint2 code = *reinterpret_cast<const uint2*>(x4 + (row * nb + b) * 8);
-    const float s = e4m3_value(blocks[block_offset(row, b, nk64)]) * scale[row];
-    uint32_t h[8];
-    {
-      uint32_t t[4];
-      e2m1x8_halves(code.x, t);
-      for (int i = 0; i < 4; ++i) h[i] = t[i];
-      e2m1x8_halves(code.y, t);
-      for (int i = 0; i < 4; ++i) h[4 + i] = t[i];
-    }
-    float v[16];
+                                                         const float* __restrict__ scale, int n8, long long M, T* __restrict__ out) {
+  const int c = blockIdx.x * blockDim.x + threadIdx.x;  // of the row's n8 = K / 8 pieces
+  const int nk64 = (n8 + 7) / 8;
+  if (c >= n8) return;
+  const long long step = (long long)gridDim.y * blockDim.y;
+  for (long long row = (long long)blockIdx.y * blockDim.y + threadIdx.y; row < M; row += step * kRows) {
+    uint32_t code[kRows], s8[kRows];
+    float rs[kRows];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-      v[2 * i] = f.x * s;
-      v[2 * i + 1] = f.y * s;
-    }
-    T* o = out + (row * nb + b) * 16;
-    if constexpr (std::is_same<T, float>::value) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(o)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    } else {
-      uint32_t w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&p);
+    for (int i = 0; i < kRows; ++i) {
+      const long long r = row + i * step;
+      code[i] = s8[i] = 0;
+      rs[i] = 0.0f;
+      if (r < M) {
+        code[i] = __ldcs(reinterpret_cast<const uint32_t*>(x4) + r * n8 + c);
+        s8[i] = blocks[block_offset(r, c >> 1, nk64)];
+        rs[i] = scale[r];
       }
-      reinterpret_cast<uint4*>(o)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-      reinterpret_cast<uint4*>(o)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const long long r = row + i * step;
+      if (r >= M) break;
+      const float s = e4m3_value(s8[i]) * rs[i];
+      uint32_t h[4];
+      e2m1x8_halves(code[i], h);
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[k]));
+        v[2 * k] = f.x * s;
+        v[2 * k + 1] = f.y * s;
+      }
+      T* o = out + (r * n8 + c) * 8;
+      if constexpr (std::is_same<T, float>::value) {
+        reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+      } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+          w[k] = *reinterpret_cast<const uint32_t*>(&p);
+        }
+        *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
     }
   }
 }
@@ -376,16 +417,19 @@ extern "C" int mh3_dequantize_fp4(const void* x4, const void* blocks, const floa
     return fail(MH3_ERR_INVALID, "mh3_dequantize_fp4: out_dtype must be bf16 or f32");
   if (M == 0) return MH3_OK;
   if (!out || ((uintptr_t)out & 15u)) return fail(MH3_ERR_INVALID, "mh3_dequantize_fp4: out must be 16-byte aligned and not null");
-  const int nb = (int)(K / 16);
-  const int tx = std::min(256, (nb + 31) / 32 * 32);
+  const int n8 = (int)(K / 8);
+  const int tx = std::min(256, (n8 + 31) / 32 * 32);
   const dim3 block((unsigned)tx, (unsigned)std::max(1, 256 / tx));
-  const dim3 grid((unsigned)((nb + tx - 1) / tx), (unsigned)std::min<int64_t>((M + block.y - 1) / block.y, 65535));
+  const int64_t rows = (M + block.y - 1) / block.y;  // CTA rows; kRows of them per CTA once the SMs are full
+  const int64_t gx = (n8 + tx - 1) / tx;
+  const int64_t gy = std::max<int64_t>((rows + fp4::kRows - 1) / fp4::kRows, std::min<int64_t>(rows, 148 * 4 / gx));
+  const dim3 grid((unsigned)gx, (unsigned)std::min<int64_t>(gy, 65535));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const uint8_t *c = static_cast<const uint8_t*>(x4), *b = static_cast<const uint8_t*>(blocks);
   if (out_dtype == MH3_DTYPE_F32)
-    fp4::dequantize_kernel<float><<<grid, block, 0, st>>>(c, b, scale, nb, M, static_cast<float*>(out));
+    fp4::dequantize_kernel<float><<<grid, block, 0, st>>>(c, b, scale, n8, M, static_cast<float*>(out));
   else
-    fp4::dequantize_kernel<__nv_bfloat16><<<grid, block, 0, st>>>(c, b, scale, nb, M, static_cast<__nv_bfloat16*>(out));
+    fp4::dequantize_kernel<__nv_bfloat16><<<grid, block, 0, st>>>(c, b, scale, n8, M, static_cast<__nv_bfloat16*>(out));
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? MH3_OK : fail_cuda(e, "mh3_dequantize_fp4 launch");
 }

@@ -40,6 +40,7 @@ struct Params {
   long long qo_sb, qo_sh, qo_ss, ko_sb, ko_sh, ko_ss;
   long long tokens;  // batch * seqlen
   int S, Hq, Hk, D, R2, tile;
+  unsigned magic;  // 2^32 / (Hq + Hk) + 1; 0 for one head
   const void* pos;
   int pos_kind;  // 0 int32, 1 int64, 2 float
   long long pos_sb, pos_ss;
@@ -85,32 +86,31 @@ __device__ __forceinline__ void angles(const Params& p, float2* cs, long long t0
   }
 }
 
-// Row i of the CTA's tokens x heads: token i / rows, Q's heads first.
-struct Row {
-  long long in, out;  // element offsets
-  int t;
-  bool k;
+// Row i of the CTA's tokens x heads is head i % rows of token i / rows, Q's heads
+// first.  Its addresses come from a table of the CTA's tokens: head 0's address of Q
+// and of the output, and for K the address that its first head would have if K's
+// heads were numbered from 0 too - so a row costs a division (a multiplication by
+// the host's 2^32 / rows + 1, exact below 2^32 / rows), a select and one product.
+struct Token {
+  const char *q, *k;
+  char *qo, *ko;
 };
-__device__ __forceinline__ Row locate(const Params& p, long long t0, int i) {
-  const int rows = p.Hq + p.Hk;
-  Row r;
-  r.t = (int)((unsigned)i / (unsigned)rows);
-  const int h = i - r.t * rows;
-  const long long tok = t0 + r.t;
-  long long b = 0, s = tok;
-  if (tok >= p.S) {
-    b = p.tokens <= 0xffffffffll ? (long long)((unsigned)tok / (unsigned)p.S) : tok / p.S;
-    s = tok - b * p.S;
+__device__ __forceinline__ void token_table(const Params& p, Token* tab, long long t0, int nt, int es) {
+  if ((int)threadIdx.x < nt) {
+    const long long tok = t0 + threadIdx.x;
+    const long long b = tok / p.S, s = tok - b * p.S;
+    Token t;
+    t.q = p.q + (b * p.q_sb + s * p.q_ss) * es;
+    t.k = p.k + (b * p.k_sb + s * p.k_ss - p.Hq * p.k_sh) * es;
+    t.qo = p.qo + (b * p.qo_sb + s * p.qo_ss) * es;
+    t.ko = p.ko + (b * p.ko_sb + s * p.ko_ss - p.Hq * p.ko_sh) * es;
+    tab[threadIdx.x] = t;
   }
-  r.k = h >= p.Hq;
-  if (r.k) {
-    r.in = b * p.k_sb + s * p.k_ss + (h - p.Hq) * p.k_sh;
-    r.out = b * p.ko_sb + s * p.ko_ss + (h - p.Hq) * p.ko_sh;
-  } else {
-    r.in = b * p.q_sb + s * p.q_ss + h * p.q_sh;
-    r.out = b * p.qo_sb + s * p.qo_ss + h * p.qo_sh;
-  }
-  return r;
+}
+__device__ __forceinline__ int row_token(const Params& p, int i, int& h) {
+  const int t = p.magic != 0 ? (int)__umulhi((unsigned)i, p.magic) : i;
+  h = i - t * (p.Hq + p.Hk);
+  return t;
 }
 
 template <typename T>
@@ -132,6 +132,7 @@ __global__ void __launch_bounds__(kThreads) stream_kernel(const __grid_constant_
   extern __shared__ uint4 smem[];
   uint4* ring = smem + threadIdx.x;  // [kStages][kVectors][kThreads]
   float2* cs = reinterpret_cast<float2*>(smem + kStages * kVectors * kThreads);
+  __shared__ Token tab[kMaxTokens];
   const int npair = INTER ? p.D / 2 : p.R2;
   const long long t0 = (long long)blockIdx.x * p.tile;
   const int nt = (int)min((long long)p.tile, p.tokens - t0);
@@ -147,8 +148,9 @@ __global__ void __launch_bounds__(kThreads) stream_kernel(const __grid_constant_
     for (int k = 0; k < U; ++k) {
       const int j = i + k * side;
       if (j < n) {
-        const Row r = locate(p, t0, j);
-        const T* src = reinterpret_cast<const T*>(r.k ? p.k : p.q) + r.in + c0;
+        int h;
+        const Token& tk = tab[row_token(p, j, h)];
+        const T* src = reinterpret_cast<const T*>(h < p.Hq ? tk.q : tk.k) + h * (h < p.Hq ? p.q_sh : p.k_sh) + c0;
         uint4* dst = ring + (st * kVectors + k * W) * kThreads;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
         if (!INTER && rot)
@@ -157,6 +159,8 @@ __global__ void __launch_bounds__(kThreads) stream_kernel(const __grid_constant_
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  token_table(p, tab, t0, nt, sizeof(T));
+  __syncthreads();
 #pragma unroll
   for (int j = 0; j < kStages - 1; ++j) issue(row0 + j * U * side, j);
   angles(p, cs, t0, nt, npair);
@@ -169,14 +173,16 @@ __global__ void __launch_bounds__(kThreads) stream_kernel(const __grid_constant_
     for (int k = 0; k < U; ++k) {
       const int j = i + k * side;
       if (j >= n) break;
-      const Row r = locate(p, t0, j);
-      T* to = reinterpret_cast<T*>(r.k ? p.ko : p.qo) + r.out + c0;
+      int h;
+      const int t = row_token(p, j, h);
+      const Token& tk = tab[t];
+      T* to = reinterpret_cast<T*>(h < p.Hq ? tk.qo : tk.ko) + h * (h < p.Hq ? p.qo_sh : p.ko_sh) + c0;
       const uint4* src = ring + (st * kVectors + k * W) * kThreads;
       Vec<T, V> x, y;
       x = *reinterpret_cast<const Vec<T, V>*>(src);
       if (rot) {
         if (!INTER) y = *reinterpret_cast<const Vec<T, V>*>(src + kThreads);
-        const float4* ap = reinterpret_cast<const float4*>(cs + r.t * npair + u * NP);
+        const float4* ap = reinterpret_cast<const float4*>(cs + t * npair + u * NP);
 #pragma unroll
         for (int q = 0; q < NP / 2; ++q) {
           const float4 a = ap[q];
@@ -201,21 +207,25 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) scalar_kernel(const __grid_constant__ Params p, int inter) {
   extern __shared__ uint4 smem[];
   float2* cs = reinterpret_cast<float2*>(smem);
+  __shared__ Token tab[kMaxTokens];
   const long long t0 = (long long)blockIdx.x * p.tile;
   const int nt = (int)min((long long)p.tile, p.tokens - t0);
+  token_table(p, tab, t0, nt, sizeof(T));
   angles(p, cs, t0, nt, p.R2);
   __syncthreads();
   const int units = p.D - p.R2;
   const int total = nt * (p.Hq + p.Hk) * units;
   for (int i = threadIdx.x; i < total; i += kThreads) {
     const int row = i / units, u = i - row * units;
-    const Row r = locate(p, t0, row);
-    const T* src = reinterpret_cast<const T*>(r.k ? p.k : p.q) + r.in;
-    T* to = reinterpret_cast<T*>(r.k ? p.ko : p.qo) + r.out;
+    int h;
+    const int t = row_token(p, row, h);
+    const bool isq = h < p.Hq;
+    const T* src = reinterpret_cast<const T*>(isq ? tab[t].q : tab[t].k) + h * (isq ? p.q_sh : p.k_sh);
+    T* to = reinterpret_cast<T*>(isq ? tab[t].qo : tab[t].ko) + h * (isq ? p.qo_sh : p.ko_sh);
     if (u < p.R2) {
       const int c0 = inter ? 2 * u : u, c1 = inter ? 2 * u + 1 : u + p.R2;
       T x0 = src[c0], x1 = src[c1];
-      rotate(x0, x1, cs[r.t * p.R2 + u]);
+      rotate(x0, x1, cs[t * p.R2 + u]);
       to[c0] = x0;
       to[c1] = x1;
     } else {
@@ -273,8 +283,9 @@ extern "C" int mh3_rotary(const mh3_rotary_args* a, void* stream) {
   if (tokens == 0 || a->heads_q + (long long)a->heads_k == 0) return MH3_OK;
   if (!a->positions || (a->heads_q > 0 && (!a->q || !a->q_out)) || (a->heads_k > 0 && (!a->k || !a->k_out)))
     return fail(MH3_ERR_INVALID, "mh3_rotary: null pointer");
-  // rows and units of a CTA are counted in 32 bits: 16 tokens x heads x 256
-  if ((long long)a->heads_q + a->heads_k > (1 << 18) || tokens > (1ll << 34))
+  // A CTA's rows are divided by their number per token with a 32-bit product: exact
+  // while 16 (heads)^2 < 2^32.
+  if ((long long)a->heads_q + a->heads_k > 8192 || tokens > (1ll << 34))
     return fail(MH3_ERR_TOO_LARGE, "mh3_rotary: too many heads or tokens");
   const bool inter = a->interleaved != 0;
   const int es = a->dtype == MH3_DTYPE_F32 ? 4 : 2, V = 16 / es;
@@ -298,6 +309,7 @@ extern "C" int mh3_rotary(const mh3_rotary_args* a, void* stream) {
   p.S = a->seqlen;
   p.Hq = a->heads_q;
   p.Hk = a->heads_k;
+  p.magic = p.Hq + p.Hk == 1 ? 0u : (unsigned)((1ull << 32) / (unsigned)(p.Hq + p.Hk)) + 1u;
   p.D = a->head_dim;
   p.R2 = r2;
   p.pos = a->positions;

@@ -138,9 +138,10 @@ def test_norm_modulate_forward(B, S, C, dtype, mod, norm):
     # the same modulation as [B, 1, C] and as a row for each token
     full = norm_modulate(x, sc, sh, norm=norm)
     assert torch.equal(norm_modulate(x, sc[:, None], sh[:, None], norm=norm), full)
+    c = Case(x, scale=sc, shift=sh, norm=norm, rows_of=per)  # another kernel, another order of the sums: the same bound
     tok = norm_modulate(x, per(sc).contiguous(), per(sh).contiguous(), norm=norm)
-    assert torch.equal(tok, full)
-    assert torch.equal(norm_modulate(x, per(sc).contiguous(), sh, norm=norm), full)
+    _close(tok, c.h, c.eh)
+    assert torch.equal(norm_modulate(x, per(sc).contiguous(), sh, norm=norm), tok)
 
 
 @pytest.mark.parametrize("B,S,C", [(1, 1, 8), (3, 37, 104), (2, 9, 7), (1, 70, 1544), (2, 11, 5120)])
