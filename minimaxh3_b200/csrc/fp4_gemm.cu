@@ -10,11 +10,14 @@
 //   A stage is 256 elements of K: per CTA 128 rows of A and of B (128 bytes each),
 //   2 KB of A's scales and 4 KB of B's (every CTA needs the scales of all 256
 //   columns).  Bound: the tensor cores' 4-bit rate and the power limit.
-//   Tensor memory (512 columns): the block scales take 2 x 48 columns, so two whole
-//   256-column accumulators do not fit; they overlap in 96 columns.  The epilogue
-//   takes those 96 into registers first and hands them over, then drains the other
-//   160 while the next tile's MMAs run.  A scale buffer is rewritten only after the
-//   MMAs that read it two stages earlier have completed.
+//   Tensor memory (512 columns): one 256-column accumulator and, for each of the
+//   five stages, 48 columns of block scales.  A stage's scale columns are rewritten
+//   when its shared memory is refilled, which the full barrier already orders after
+//   the MMAs that read both; with two accumulators there is room for two scale
+//   buffers only, and waiting for the MMAs two stages back cost 11 % (1.18 ms
+//   against 1.05 without the wait at 32760 x 13824 x 5120).  Eight epilogue warps take
+//   the whole accumulator into registers and hand it over before they scale and
+//   store it, so the next tile's MMAs run meanwhile.
 // * small_kernel (M <= kSmallM): bound by reading b once.  A CTA takes 16 rows of b,
 //   its warps split K; codes are widened to f16 with their block scale (6
 //   significant bits: exact) and multiplied by mma.sync.m16n8k16 with f32 sums.
@@ -30,7 +33,8 @@
 namespace mh3 {
 namespace fp4gemm {
 
-constexpr int NUM_THREADS = 192;
+constexpr int NUM_THREADS = 320;
+constexpr int EPI_WARPS = 8;
 constexpr int STAGES = 5;
 constexpr int STAGE_K = 256;                  // elements of K per stage (128 bytes)
 constexpr int BM = 256, BN = 256, HALF = 128;  // tile; rows of A and B per CTA
@@ -38,9 +42,7 @@ constexpr int TILE_BYTES = HALF * 128;
 constexpr int SF_BLOCK = 512;                  // scales of 128 rows x 64 elements
 constexpr int EPI_BOX = 32 * 32 * 2;
 constexpr int kGroupM = 8;                     // 256-row blocks per raster group
-constexpr int ACC1 = 160;                      // first column of the second accumulator
-constexpr int OVERLAP = 3;                     // shared 32-column chunks
-constexpr int SF_COL = 416, SF_COLS = 48;      // scale buffers: 4 x 4 columns of A, 4 x 8 of B
+constexpr int SF_COL = 256, SF_COLS = 48;      // scales of a stage: 4 x 4 columns of A, 4 x 8 of B
 constexpr int kSmallM = 32;
 
 struct Params {
@@ -61,13 +63,13 @@ struct __align__(1024) Smem {
   uint8_t b[STAGES][TILE_BYTES];
   uint8_t sa[STAGES][4 * SF_BLOCK];
   uint8_t sb[STAGES][2][4 * SF_BLOCK];
-  uint8_t epi[4][2][EPI_BOX];
-  float col_scale[2][BN];
-  float col_bias[2][BN];
+  uint8_t epi[EPI_WARPS][2][EPI_BOX];
+  float col_scale[BN];
+  float col_bias[BN];
   uint64_t full[STAGES];  // used in the leader
   uint64_t empty[STAGES];
-  uint64_t acc_full[2];
-  uint64_t acc_part;      // used in the leader: the overlapping columns are drained (4 warps x 2 CTAs)
+  uint64_t acc_full;
+  uint64_t acc_empty;     // used in the leader: the accumulator is in registers (8 warps x 2 CTAs)
   uint64_t mma_done;
   uint64_t bar_never;     // nothing arrives on it (test hook)
   uint32_t tmem_base;
@@ -103,8 +105,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) pair_kernel(const __grid_const
       mbar_init(smem_u32(&sm.full[i]), 1);
       mbar_init(smem_u32(&sm.empty[i]), 1);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&sm.acc_full[i]), 1);
-    mbar_init(smem_u32(&sm.acc_part), 8);
+    mbar_init(smem_u32(&sm.acc_full), 1);
+    mbar_init(smem_u32(&sm.acc_empty), 2 * EPI_WARPS);
     mbar_init(smem_u32(&sm.mma_done), 1);
     mbar_init(smem_u32(&sm.bar_never), 1);
     sm.abort_flag = 0;
@@ -129,7 +131,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) pair_kernel(const __grid_const
       tma_prefetch_desc(&p.tma_sb);
     }
     __syncwarp();
-    int it = 0, last_issued = -1;
+    int it = 0, last_issued = -1, st = 0;
+    uint32_t phase = 1u;
     bool ok = true;
     if (p.test_flags & MH3_TEST_STALL_PRODUCER) {  // a wait that nothing ends runs out first
       bool w = true;
@@ -142,9 +145,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) pair_kernel(const __grid_const
       const int row_a = mb * BM + (int)crank * HALF;
       const int row_b = nb * BN + (int)crank * HALF;
       for (int s = 0; s < kst; ++s, ++it) {
-        const int st = it % STAGES;
         bool w = true;
-        if (lane == 0) w = mbar_wait(smem_u32(&sm.empty[st]), ((uint32_t)(it / STAGES) & 1u) ^ 1u, g);
+        if (lane == 0) w = mbar_wait(smem_u32(&sm.empty[st]), phase, g);
         if (!__shfl_sync(0xffffffffu, w ? 1 : 0, 0)) {
           ok = false;
           break;
@@ -168,6 +170,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) pair_kernel(const __grid_const
           }
         }
         __syncwarp();
+        if (++st == STAGES) {
+          st = 0;
+          phase ^= 1u;
+        }
       }
     }
     // Teardown (leader): the last copies counted on each stage must land.
@@ -175,61 +181,74 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) pair_kernel(const __grid_const
       for (int i = max(0, last_issued - STAGES + 1); i <= last_issued; ++i)
         mbar_wait_teardown(smem_u32(&sm.full[i % STAGES]), (uint32_t)(i / STAGES) & 1u);
   } else if (warp == 1) {
-    if (crank == 0) {
-      // -------------------------------------------------------------- MMA issuer (leader)
+    // ---------------------------------------------------------------- MMA issuer (leader)
+    // One thread, and as few instructions per MMA as it takes: its issue is what
+    // keeps the tensor cores fed.  With descriptors built per MMA and a division per
+    // stage a 512-cycle stage took 750 to 900 cycles; with descriptors that only
+    // count up, the twelve scale copies and the commit hide behind the MMAs (513).
+    if (crank == 0 && elect_one_sync()) {
       constexpr uint32_t kIdF4 = idesc_nvf4(BM, BN);
       constexpr uint32_t kIdBF = idesc_bf16(BM, BN, false, false);
-      int it = 0, tcount = 0, nsf = 0;
-      int used[2] = {-STAGES, -STAGES};  // the stage whose MMAs last read each scale buffer
-      for (int t = pair; t < num_tiles; t += npairs, ++tcount) {
-        const int acc = tcount & 1;
-        const uint32_t d_tmem = tmem + (uint32_t)(acc * ACC1);
-        // The previous tile's epilogue has read the shared columns, and with them
-        // the whole of the tile before it.
-        if (tcount > 0) mbar_wait_cluster(smem_u32(&sm.acc_part), (uint32_t)(tcount - 1) & 1u, g);
-        tc_fence_after();
-        for (int s = 0; s < kst; ++s, ++it) {
-          const int st = it % STAGES;
-          mbar_wait(smem_u32(&sm.full[st]), (uint32_t)(it / STAGES) & 1u, g);
-          const bool main = s < kst_main;
-          if (main) {
-            // A stage number that has come round again was filled only after its
-            // MMAs were done; a younger one is waited for here.
-            const int u = used[nsf & 1];
-            if (u >= 0 && it < u + STAGES) mbar_wait(smem_u32(&sm.empty[u % STAGES]), (uint32_t)(u / STAGES) & 1u, g);
-            used[nsf & 1] = it;
-          }
-          tc_fence_after();
-          __syncwarp();
-          if (elect_one_sync()) {
-            if (main) {
-              const int nmma = min(4, nk64 - s * 4);  // 64 elements each
-              const uint32_t sfa = tmem + SF_COL + (uint32_t)(nsf & 1) * SF_COLS, sfb = sfa + 16;
-              for (int kk = 0; kk < nmma; ++kk) {
-                tmem_cp_scales_pair(sfa + kk * 4, smem_desc(smem_u32(sm.sa[st]) + kk * SF_BLOCK, 0, 128, kLayoutNone));
-                tmem_cp_scales_pair(sfb + kk * 8, smem_desc(smem_u32(sm.sb[st][0]) + kk * SF_BLOCK, 0, 128, kLayoutNone));
-                tmem_cp_scales_pair(sfb + kk * 8 + 4, smem_desc(smem_u32(sm.sb[st][1]) + kk * SF_BLOCK, 0, 128, kLayoutNone));
-              }
-              for (int kk = 0; kk < nmma; ++kk)
-                mma_nvf4_ss_pair(d_tmem, smem_desc(smem_u32(sm.a[st]) + kk * 32, 16, 1024, kLayoutSW128),
-                                 smem_desc(smem_u32(sm.b[st]) + kk * 32, 16, 1024, kLayoutSW128), kIdF4, sfa + kk * 4,
-                                 sfb + kk * 8, (s > 0 || kk > 0) ? 1u : 0u);
-            } else {
-              for (int kk = 0; kk < 4; ++kk)  // 16 bf16 each
-                mma_f16_ss_pair(d_tmem, smem_desc(smem_u32(sm.a[st]) + kk * 32, 16, 1024, kLayoutSW128),
-                                smem_desc(smem_u32(sm.b[st]) + kk * 32, 16, 1024, kLayoutSW128), kIdBF, 1u);
-            }
-            mma_commit_pair(smem_u32(&sm.empty[st]), 0x3);
-          }
-          if (main) ++nsf;
-          __syncwarp();
+      const uint64_t da0 = smem_desc(smem_u32(sm.a[0]), 16, 1024, kLayoutSW128);
+      const uint64_t db0 = smem_desc(smem_u32(sm.b[0]), 16, 1024, kLayoutSW128);
+      const uint64_t dsa0 = smem_desc(smem_u32(sm.sa[0]), 0, 128, kLayoutNone);
+      const uint64_t dsb0 = smem_desc(smem_u32(sm.sb[0][0]), 0, 128, kLayoutNone);
+      const uint32_t full0 = smem_u32(&sm.full[0]), empty0 = smem_u32(&sm.empty[0]);
+      const int tail = nk64 - (kst_main - 1) * 4;  // 64-element steps of the last main stage
+      int st = 0;
+      uint32_t phase = 0, tphase = 0, fresh = 0;
+      uint64_t da = da0, db = db0;  // 16-byte units: 1024 a stage, 2 an MMA
+      auto next = [&] {
+        mma_commit_pair(empty0 + st * 8, 0x3);
+        da += TILE_BYTES / 16;
+        db += TILE_BYTES / 16;
+        if (++st == STAGES) {
+          st = 0;
+          phase ^= 1u;
+          da = da0;
+          db = db0;
         }
-        if (elect_one_sync()) mma_commit_pair(smem_u32(&sm.acc_full[acc]), 0x3);
-        __syncwarp();
+      };
+      auto main_stage = [&](auto whole, int n, bool first) {
+        mbar_wait(full0 + st * 8, phase, g);
+        tc_fence_after();
+        const uint64_t dsa = dsa0 + (uint64_t)(st * (4 * SF_BLOCK / 16)), dsb = dsb0 + (uint64_t)(st * (8 * SF_BLOCK / 16));
+        const uint32_t sfa = tmem + SF_COL + (uint32_t)(st * SF_COLS), sfb = sfa + 16;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          if (decltype(whole)::value || kk < n) {
+            tmem_cp_scales_pair(sfa + kk * 4, dsa + kk * (SF_BLOCK / 16));
+            tmem_cp_scales_pair(sfb + kk * 8, dsb + kk * (SF_BLOCK / 16));
+            tmem_cp_scales_pair(sfb + kk * 8 + 4, dsb + (4 + kk) * (SF_BLOCK / 16));
+          }
+        if (first && fresh) {  // the epilogue has taken the previous tile
+          mbar_wait_cluster(smem_u32(&sm.acc_empty), tphase, g);
+          tphase ^= 1u;
+          tc_fence_after();
+        }
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          if (decltype(whole)::value || kk < n)
+            mma_nvf4_ss_pair(tmem, da + 2 * kk, db + 2 * kk, kIdF4, sfa + kk * 4, sfb + kk * 8, first && kk == 0 ? 0u : 1u);
+        next();
+      };
+      for (int t = pair; t < num_tiles; t += npairs) {
+        const int whole = tail == 4 ? kst_main : kst_main - 1;
+        for (int s = 0; s < whole; ++s) main_stage(std::true_type{}, 4, s == 0);
+        if (whole < kst_main) main_stage(std::false_type{}, tail, whole == 0);
+        for (int s = kst_main; s < kst; ++s) {
+          mbar_wait(full0 + st * 8, phase, g);
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) mma_f16_ss_pair(tmem, da + 2 * kk, db + 2 * kk, kIdBF, 1u);  // 16 bf16 each
+          next();
+        }
+        mma_commit_pair(smem_u32(&sm.acc_full), 0x3);
+        fresh = 1u;
       }
-      if (elect_one_sync()) mma_commit_pair(smem_u32(&sm.mma_done), 0x3);
-      __syncwarp();
+      mma_commit_pair(smem_u32(&sm.mma_done), 0x3);
     }
+    __syncwarp();
     // Both CTAs: every pair MMA (they write both CTAs' TMEM) must be
     // finished before TMEM is freed, also on the abort path.
     if (lane == 0) mbar_wait_teardown(smem_u32(&sm.mma_done), 0);
@@ -237,47 +256,56 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) pair_kernel(const __grid_const
   } else {
     // ------------------------------------------------------------------ epilogue (both CTAs)
     const int q = warp & 3;           // TMEM lane quarter of this warp
-    const int et = threadIdx.x - 64;  // 0..127 over the 4 epilogue warps
-    const uint32_t lane_off = (uint32_t)(q * 32) << 16;
+    const int ew = warp - 2;          // 0..7: warps q and q + 4 of a quarter take a half of the columns each
+    const int half = ew >> 2;
+    const int et = threadIdx.x - 64;  // 0..255 over the epilogue warps
+    const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * 128);
     int tcount = 0, buf = 0;
     for (int t = pair; t < num_tiles; t += npairs, ++tcount) {
       int mb, nb;
       coords(t, mb, nb);
-      const int acc = tcount & 1;
       const int n0 = nb * BN;
-      for (int j = et; j < BN; j += 128) {
-        const int n = n0 + j;
+      named_barrier_sync(1, 32 * EPI_WARPS);  // the last tile's column values have been read
+      {
+        const int n = n0 + et;
         const bool in = n < p.N;
-        sm.col_scale[acc][j] = in ? __ldg(p.cs + n) : 0.0f;
-        sm.col_bias[acc][j] = (p.bias != nullptr && in) ? __bfloat162float(p.bias[n]) : 0.0f;
+        sm.col_scale[et] = in ? __ldg(p.cs + n) : 0.0f;
+        sm.col_bias[et] = (p.bias != nullptr && in) ? __bfloat162float(p.bias[n]) : 0.0f;
       }
-      named_barrier_sync(1, 128);
-      const int m0 = mb * BM + (int)crank * HALF + q * 32;  // first row of this warp's box
+      named_barrier_sync(1, 32 * EPI_WARPS);
+      const int m0 = mb * BM + (int)crank * HALF + q * 32;  // first row of this warp's boxes
       const int m = m0 + lane;
       const float rsv = m < p.M ? __ldg(p.rs + m) : 0.0f;
-      mbar_wait(smem_u32(&sm.acc_full[acc]), (uint32_t)(tcount >> 1) & 1u, g);
+      mbar_wait(smem_u32(&sm.acc_full), (uint32_t)tcount & 1u, g);
       tc_fence_after();
-      const uint32_t base = tmem + (uint32_t)(acc * ACC1) + lane_off;
-      // One 32-column chunk of the tile to its output box.
-      auto put = [&](int c, const uint32_t (&v)[32]) {
-        if (n0 + c * 32 >= p.N || m0 >= p.M) return;  // warp-uniform: box wholly outside
-        const float* cs = &sm.col_scale[acc][c * 32];
-        const float* bs = &sm.col_bias[acc][c * 32];
+      uint32_t v[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(base + (uint32_t)c * 32, v[c]);
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&sm.acc_empty), 0));
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int col = half * 128 + c * 32;
+        if (n0 + col >= p.N || m0 >= p.M) continue;  // warp-uniform: box wholly outside
+        const float* cs = &sm.col_scale[col];
+        const float* bs = &sm.col_bias[col];
         uint32_t packed[16];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float4 c4 = *reinterpret_cast<const float4*>(cs + 4 * i);
           const float4 b4 = *reinterpret_cast<const float4*>(bs + 4 * i);
-          const __nv_bfloat162 h0 = __floats2bfloat162_rn(fmaf(__uint_as_float(v[4 * i + 0]) * rsv, c4.x, b4.x),
-                                                          fmaf(__uint_as_float(v[4 * i + 1]) * rsv, c4.y, b4.y));
-          const __nv_bfloat162 h1 = __floats2bfloat162_rn(fmaf(__uint_as_float(v[4 * i + 2]) * rsv, c4.z, b4.z),
-                                                          fmaf(__uint_as_float(v[4 * i + 3]) * rsv, c4.w, b4.w));
+          const __nv_bfloat162 h0 = __floats2bfloat162_rn(fmaf(__uint_as_float(v[c][4 * i + 0]) * rsv, c4.x, b4.x),
+                                                          fmaf(__uint_as_float(v[c][4 * i + 1]) * rsv, c4.y, b4.y));
+          const __nv_bfloat162 h1 = __floats2bfloat162_rn(fmaf(__uint_as_float(v[c][4 * i + 2]) * rsv, c4.z, b4.z),
+                                                          fmaf(__uint_as_float(v[c][4 * i + 3]) * rsv, c4.w, b4.w));
           packed[2 * i] = *reinterpret_cast<const uint32_t*>(&h0);
           packed[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&h1);
         }
         if (lane == 0) bulk_wait_group_read<1>();  // the store that last read this box is done
         __syncwarp();
-        uint8_t* box = sm.epi[q][buf];
+        uint8_t* box = sm.epi[ew][buf];
 #pragma unroll
         for (int j = 0; j < 4; ++j)  // 64B swizzle: 16-byte piece j of row ``lane``
           *reinterpret_cast<uint4*>(box + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) =
@@ -285,34 +313,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) pair_kernel(const __grid_const
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          tma_store_2d(&p.tma_out, smem_u32(box), n0 + c * 32, m0);
+          tma_store_2d(&p.tma_out, smem_u32(box), n0 + col, m0);
           bulk_commit_group();
         }
         buf ^= 1;
-      };
-      // the chunks that the next tile's accumulator shares: the last three of the
-      // first accumulator, the first three of the second
-      const int c0 = acc == 0 ? BN / 32 - OVERLAP : 0;
-      {
-        uint32_t v[OVERLAP][32];
-#pragma unroll
-        for (int i = 0; i < OVERLAP; ++i) tmem_ld32(base + (uint32_t)(c0 + i) * 32, v[i]);
-        tmem_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&sm.acc_part), 0));
-#pragma unroll
-        for (int i = 0; i < OVERLAP; ++i) put(c0 + i, v[i]);
       }
-      const int c1 = acc == 0 ? 0 : OVERLAP;
-#pragma unroll 1
-      for (int c = c1; c < c1 + BN / 32 - OVERLAP; ++c) {
-        uint32_t v[32];
-        tmem_ld32(base + (uint32_t)c * 32, v);
-        tmem_wait_ld();
-        put(c, v);
-      }
-      tc_fence_before();
     }
     if (lane == 0) bulk_wait_group<0>();  // stores complete before the CTA's shared memory goes
     __syncwarp();
