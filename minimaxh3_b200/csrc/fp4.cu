@@ -16,13 +16,15 @@
 // definition.  With M in [1, 2) and absmax = M 2^E, absmax / 2688 = (M / 1.3125)
 // 2^(E-11): the exponent is E - 11, one more if M > 1.3125 - integer compares.
 //
-// Bound: HBM, 2 bytes in and 0.5625 out per 16-bit element.  A thread owns the 16
-// elements of a block, so the block's maximum needs no exchange and the input is
-// read once.  CTAs are persistent: rows stream through a ring of three stages in
-// shared memory (cp.async; a thread reads back only what it copied), so two rows
-// are on their way while one is reduced and rounded.  Rows longer than 1024
-// threads' blocks, and rows that 16-byte vectors do not fit, are read twice by the
-// general kernel.
+// Bound: HBM, 2 bytes in and 0.5625 out per 16-bit element, once the instructions
+// of a block (about 110) fit beside it.  A thread owns the 16 elements of a block, so
+// the block's maximum needs no exchange.  CTAs are persistent and take four rows 32
+// apart at a time: their maxima share one barrier, and their block scales for 64
+// elements are the 16 neighbouring bytes of the scale layout, written as one
+// vector.  The rows stream through a two-stage ring in shared memory (cp.async; a
+// thread reads back only what it copied, once for the maxima and once for the
+// rounding).  Rows too long for that ring, and rows that 16-byte vectors do not fit, are read
+// twice by the general kernel.
 #include <algorithm>
 #include <string>
 
@@ -63,6 +65,12 @@ __device__ __forceinline__ void load16(const T* p, float (&v)[16], bool vec) {
   }
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = to_float(e[i]);
+}
+
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // Largest magnitude as the integer of its bits: an infinity or NaN orders above
@@ -107,13 +115,16 @@ __device__ __forceinline__ long long block_offset(long long row, int b, int nk64
 }
 
 // One block: its scale byte and 16 codes, from its absmax and the row's exponent.
-// The quotients are div_by in packed pairs, which halves their issue slots.
+// The quotients are div_by in packed pairs, which halves their issue slots; an
+// approximate reciprocal serves: where the true quotient is a border it has a few
+// bits, the remainder is exact, and the corrected quotient lands on it; where it is
+// not, 16-bit input is at least 2^-13 of it away.
 __device__ __forceinline__ uint32_t round_block(const float (&v)[16], uint32_t top, float inv, uint2& code) {
   // e4m3 of absmax / (6 scale): the division by 6 is the only rounding before it
   const float raw = div_by(__uint_as_float(top) * inv, 6.0f, 1.0f / 6.0f);
   const uint32_t s8 = cvt_e4m3x2_f32(0.0f, raw) & 0xffu;
   if (s8 != 0) {
-    const float s = e4m3_value(s8), r = __frcp_rn(s);
+    const float s = e4m3_value(s8), r = rcp_approx(s);
     const float2 r2 = both(r), ns2 = both(-s), inv2 = both(inv);
     float q[16];
 #pragma unroll
@@ -140,9 +151,11 @@ __device__ __forceinline__ uint32_t absmax_raw(const uint4 (&u)[sizeof(T)]) {
     for (int i = 0; i < 16; ++i) m = max(m, w[i] & 0x7fffffffu);
     return m;
   } else {
-    uint32_t m = w[0] & 0x7fff7fffu;
-#pragma unroll
-    for (int i = 1; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+    constexpr uint32_t kAbs = 0x7fff7fffu;
+    uint32_t m = __vimax3_u16x2(w[0] & kAbs, w[1] & kAbs, w[2] & kAbs);
+    m = __vimax3_u16x2(m, w[3] & kAbs, w[4] & kAbs);
+    m = __vimax3_u16x2(m, w[5] & kAbs, w[6] & kAbs);
+    m = __vimax3_u16x2(m, w[7] & kAbs, 0u);
     m = max(m & 0xffffu, m >> 16);
     if constexpr (std::is_same<T, __half>::value)
       return m >= 0x7c00u ? 0x7f800000u | m : __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
@@ -175,10 +188,12 @@ __device__ __forceinline__ uint32_t row_max(uint32_t top, uint32_t (*red)[32], i
   return top;
 }
 
-constexpr int kStages = 3;
+constexpr int kQuad = 4;    // rows r, r + 32, r + 64, r + 96 of a block of 128
+constexpr int kStages = 2;
+constexpr size_t kRingMax = 224 * 1024;
 
 // Streaming: blockDim.x threads (a multiple of 32, at least the row's scales) per
-// row, blockDim.y rows at once.  Rows M.. of the last block of 128 get zero
+// row, blockDim.y quads at once.  Rows M.. of the last block of 128 get zero
 // scales, so the buffer is the same whatever the memory held.
 template <typename T>
 __global__ void __launch_bounds__(kMaxThreads) quantize_stream_kernel(const T* __restrict__ x, long long stride, long long M, int K,
@@ -186,54 +201,101 @@ __global__ void __launch_bounds__(kMaxThreads) quantize_stream_kernel(const T* _
                                                                      float* __restrict__ scale) {
   constexpr int W = sizeof(T);  // 16-byte vectors of a block
   extern __shared__ uint4 ring[];
-  __shared__ uint32_t red[2][32];
+  __shared__ uint4 red[2][32];  // a warp's four maxima
   const int nb = K / 16, nk64 = (K + 63) / 64, b = threadIdx.x;
-  const int nthr = blockDim.x * blockDim.y, tid = threadIdx.y * blockDim.x + threadIdx.x;
-  const bool mine = b < nb;
-  const long long step = (long long)gridDim.x * blockDim.y;
-  const long long padded = (M + 127) / 128 * 128;
-  auto issue = [&](long long row, int st) {
-    if (mine && row < M) {
-      const uint4* src = reinterpret_cast<const uint4*>(x + row * stride + b * 16);
+  const int nthr = blockDim.x * blockDim.y, warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+  uint4* mine = ring + threadIdx.y * blockDim.x + threadIdx.x;  // [kStages][kQuad][W][nthr]
+  const bool in = b < nb;
+  const int quads = (int)((M + 127) / 128 * 32);  // of 32 in each block of 128 rows
+  const int step = gridDim.x * blockDim.y;
+  auto first_row = [](int q) { return (long long)(q >> 5) * 128 + (q & 31); };
+  auto issue = [&](int q, int st) {
+    if (in && q < quads) {
+      long long row = first_row(q);
+      const T* src = x + row * stride + b * 16;
 #pragma unroll
-      for (int w = 0; w < W; ++w)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(ring + (st * W + w) * nthr + tid)), "l"(src + w)
-                     : "memory");
+      for (int i = 0; i < kQuad; ++i, row += 32, src += 32 * stride)
+        if (row < M)
+#pragma unroll
+          for (int w = 0; w < W; ++w)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(mine + ((st * kQuad + i) * W + w) * nthr)),
+                         "l"(reinterpret_cast<const uint4*>(src) + w)
+                         : "memory");
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  const long long first = (long long)blockIdx.x * blockDim.y;
-#pragma unroll
-  for (int j = 0; j < kStages - 1; ++j) issue(first + threadIdx.y + j * step, j);
-  int st = 0, turn = 0;
-  for (long long base = first; base < padded; base += step) {  // the same trips for every thread of the CTA
-    const long long row = base + threadIdx.y;
-    issue(row + (kStages - 1) * step, st == 0 ? kStages - 1 : st - 1);
+  const int q0 = blockIdx.x * blockDim.y;
+  issue(q0 + threadIdx.y, 0);
+  int st = 0;
+  for (int base = q0; base < quads; base += step) {  // the same trips for every thread of the CTA
+    const int q = base + threadIdx.y;
+    issue(q + step, st ^ 1);
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-    const bool live = row < M;
-    uint4 u[W];
+    const long long row0 = first_row(q);
+    auto load = [&](int i, uint4(&u)[W]) {
 #pragma unroll
-    for (int w = 0; w < W; ++w) u[w] = mine && live ? ring[(st * W + w) * nthr + tid] : make_uint4(0, 0, 0, 0);
-    const uint32_t own = absmax_raw<T>(u);
-    const uint32_t top = row_max(own, red, turn);
-    if (row < padded) {
-      const bool finite = top < 0x7f800000u;
-      const int e = row_exponent(top);
-      uint2 code = make_uint2(0, 0);
-      uint32_t s8 = 0;
-      if (finite) {
-        T t[16];
-        float v[16];
-        memcpy(t, u, sizeof(t));
+      for (int w = 0; w < W; ++w) u[w] = mine[((st * kQuad + i) * W + w) * nthr];
+    };
+    uint32_t own[kQuad], top[kQuad];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = to_float(t[i]);
-        s8 = round_block(v, own, pow2f(-e), code);  // e in [-100, 117]
+    for (int i = 0; i < kQuad; ++i) {
+      own[i] = 0;
+      if (in && q < quads && row0 + 32 * i < M) {
+        uint4 u[W];
+        load(i, u);
+        own[i] = absmax_raw<T>(u);
       }
-      if (live && b == 0) scale[row] = finite ? pow2f(e) : __uint_as_float(0x7fffffffu);
-      if (live && mine) *reinterpret_cast<uint2*>(x4 + row * (K / 2) + (long long)b * 8) = code;
-      if (b < nk64 * 4) put_scales(blocks, s8, row, b, nk64);
+      top[i] = __reduce_max_sync(0xffffffffu, own[i]);
     }
-    st = st + 1 == kStages ? 0 : st + 1;
+    if (warps > 1) {
+      uint4* r = red[st] + threadIdx.y * warps;
+      if (lane == 0) r[threadIdx.x >> 5] = make_uint4(top[0], top[1], top[2], top[3]);
+      __syncthreads();  // one per trip: this half is written again only after the next trip's
+      const uint4 t = lane < warps ? r[lane] : make_uint4(0, 0, 0, 0);
+      top[0] = __reduce_max_sync(0xffffffffu, t.x);
+      top[1] = __reduce_max_sync(0xffffffffu, t.y);
+      top[2] = __reduce_max_sync(0xffffffffu, t.z);
+      top[3] = __reduce_max_sync(0xffffffffu, t.w);
+    }
+    if (q < quads) {
+      uint32_t words[kQuad];
+      uint8_t* xo = x4 + row0 * (K / 2) + (long long)b * 8;
+#pragma unroll
+      for (int i = 0; i < kQuad; ++i, xo += 16ll * K) {
+        const bool live = row0 + 32 * i < M;
+        const bool finite = top[i] < 0x7f800000u;
+        const int e = row_exponent(top[i]);
+        uint2 code = make_uint2(0, 0);
+        uint32_t s8 = 0;
+        if (live && in) {
+          if (finite) {
+            uint4 u[W];
+            load(i, u);
+            T t[16];
+            float v[16];
+            memcpy(t, u, sizeof(t));
+#pragma unroll
+            for (int k = 0; k < 16; ++k) v[k] = to_float(t[k]);
+            s8 = round_block(v, own[i], pow2f(-e), code);  // e in [-100, 117]
+          }
+          *reinterpret_cast<uint2*>(xo) = code;
+          if (b == 0) scale[row0 + 32 * i] = finite ? pow2f(e) : __uint_as_float(0x7fffffffu);
+        }
+        words[i] = s8 << (8 * (b & 3));
+      }
+      if (b < nk64 * 4) {  // four lanes hold the four scales of each row's word
+        const uint32_t lanes = 0xfu << (lane & 28);
+#pragma unroll
+        for (int i = 0; i < kQuad; ++i) {
+          words[i] |= __shfl_xor_sync(lanes, words[i], 1);
+          words[i] |= __shfl_xor_sync(lanes, words[i], 2);
+        }
+        if ((b & 3) == 0)
+          *reinterpret_cast<uint4*>(blocks + ((long long)(q >> 5) * nk64 + (b >> 2)) * 512 + (q & 31) * 16) =
+              make_uint4(words[0], words[1], words[2], words[3]);
+      }
+    }
+    st ^= 1;
   }
 }
 
@@ -285,56 +347,52 @@ __device__ __forceinline__ void e2m1x8_halves(uint32_t w, uint32_t (&h)[4]) {
       : "r"(w));
 }
 
-// Eight elements per thread (16 bytes of bf16, neighbouring threads side by side),
-// kRows rows whose loads are issued together.
-constexpr int kRows = 4;
+// Eight elements per thread (16 bytes of bf16, neighbouring threads side by side) of
+// the four rows whose scales lie in one vector.
 template <typename T>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ x4, const uint8_t* __restrict__ blocks,
                                                          const float* __restrict__ scale, int n8, long long M, T* __restrict__ out) {
   const int c = blockIdx.x * blockDim.x + threadIdx.x;  // of the row's n8 = K / 8 pieces
   const int nk64 = (n8 + 7) / 8;
   if (c >= n8) return;
-  const long long step = (long long)gridDim.y * blockDim.y;
-  for (long long row = (long long)blockIdx.y * blockDim.y + threadIdx.y; row < M; row += step * kRows) {
-    uint32_t code[kRows], s8[kRows];
-    float rs[kRows];
+  const int quads = (int)((M + 127) / 128 * 32);
+  const int byte = 8 * ((c >> 1) & 3);
+  for (int q = blockIdx.y * blockDim.y + threadIdx.y; q < quads; q += gridDim.y * blockDim.y) {
+    const long long row0 = (long long)(q >> 5) * 128 + (q & 31);
+    if (row0 >= M) continue;
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(x4) + row0 * n8 + c;
+    T* o = out + (row0 * n8 + c) * 8;
+    uint32_t code[kQuad];
+    float rs[kQuad];
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const long long r = row + i * step;
-      code[i] = s8[i] = 0;
-      rs[i] = 0.0f;
-      if (r < M) {
-        code[i] = __ldcs(reinterpret_cast<const uint32_t*>(x4) + r * n8 + c);
-        s8[i] = blocks[block_offset(r, c >> 1, nk64)];
-        rs[i] = scale[r];
-      }
+    for (int i = 0; i < kQuad; ++i) {
+      const bool live = row0 + 32 * i < M;
+      code[i] = live ? __ldcs(src + 32ll * i * n8) : 0u;
+      rs[i] = live ? scale[row0 + 32 * i] : 0.0f;
     }
+    const uint4 s4 = *reinterpret_cast<const uint4*>(blocks + ((long long)(q >> 5) * nk64 + (c >> 3)) * 512 + (q & 31) * 16);
+    const uint32_t sw[kQuad] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const long long r = row + i * step;
-      if (r >= M) break;
-      const float s = e4m3_value(s8[i]) * rs[i];
+    for (int i = 0; i < kQuad; ++i) {
+      if (row0 + 32 * i >= M) break;
+      const float2 s = both(e4m3_value((sw[i] >> byte) & 0xffu) * rs[i]);
       uint32_t h[4];
       e2m1x8_halves(code[i], h);
-      float v[8];
+      float2 v[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[k]));
-        v[2 * k] = f.x * s;
-        v[2 * k + 1] = f.y * s;
-      }
-      T* o = out + (r * n8 + c) * 8;
+      for (int k = 0; k < 4; ++k) v[k] = fmul2(__half22float2(*reinterpret_cast<const __half2*>(&h[k])), s);
+      T* to = o + 256ll * i * n8;
       if constexpr (std::is_same<T, float>::value) {
-        reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        reinterpret_cast<float4*>(to)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+        reinterpret_cast<float4*>(to)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
       } else {
         uint32_t w[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+          const __nv_bfloat162 p = __floats2bfloat162_rn(v[k].x, v[k].y);
           w[k] = *reinterpret_cast<const uint32_t*>(&p);
         }
-        *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
   }
@@ -349,22 +407,22 @@ static cudaError_t launch_quantize(const void* x, long long stride, long long M,
   const int vec = ((uintptr_t)x & 15u) == 0 && stride * (long long)sizeof(T) % 16 == 0;
   const T* xp = static_cast<const T*>(x);
   uint8_t *c = static_cast<uint8_t*>(x4), *b = static_cast<uint8_t*>(blocks);
-  if (nb4 > tx || !vec) {
+  const int ty = std::max(1, 256 / tx);
+  const int nthr = tx * ty;
+  const size_t smem = (size_t)kStages * kQuad * sizeof(T) * 16 * nthr;
+  if (nb4 > tx || !vec || smem > kRingMax) {
     quantize_kernel<T><<<(unsigned)padded, tx, 0, st>>>(xp, stride, M, K, c, b, scale, vec);
     return cudaGetLastError();
   }
-  const dim3 block((unsigned)tx, (unsigned)std::max(1, 256 / tx));
-  const int nthr = tx * (int)block.y;
-  const size_t smem = (size_t)kStages * sizeof(T) * 16 * nthr;
   if (smem > 40 * 1024) {  // with the static part, past the 48 KB default
     const cudaError_t e =
         cudaFuncSetAttribute(quantize_stream_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
   }
-  // resident CTAs of 64 registers a thread, and of 224 KB of rings
-  const long long per = std::min<long long>(1024 / nthr, 224 * 1024 / (long long)smem);
-  const long long grid = std::min<long long>((padded + block.y - 1) / block.y, 148 * std::max(1ll, per));
-  quantize_stream_kernel<T><<<(unsigned)grid, block, smem, st>>>(xp, stride, M, K, c, b, scale);
+  // resident CTAs of 64 registers a thread and their rings
+  const long long per = std::max<long long>(1, std::min<long long>(1024 / nthr, (long long)(kRingMax / smem)));
+  const long long grid = std::min<long long>((padded / kQuad + ty - 1) / ty, 148 * per);
+  quantize_stream_kernel<T><<<(unsigned)grid, dim3((unsigned)tx, (unsigned)ty), smem, st>>>(xp, stride, M, K, c, b, scale);
   return cudaGetLastError();
 }
 
@@ -420,9 +478,8 @@ extern "C" int mh3_dequantize_fp4(const void* x4, const void* blocks, const floa
   const int n8 = (int)(K / 8);
   const int tx = std::min(256, (n8 + 31) / 32 * 32);
   const dim3 block((unsigned)tx, (unsigned)std::max(1, 256 / tx));
-  const int64_t rows = (M + block.y - 1) / block.y;  // CTA rows; kRows of them per CTA once the SMs are full
   const int64_t gx = (n8 + tx - 1) / tx;
-  const int64_t gy = std::max<int64_t>((rows + fp4::kRows - 1) / fp4::kRows, std::min<int64_t>(rows, 148 * 4 / gx));
+  const int64_t gy = ((M + 127) / 128 * 32 + block.y - 1) / block.y;  // quads
   const dim3 grid((unsigned)gx, (unsigned)std::min<int64_t>(gy, 65535));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const uint8_t *c = static_cast<const uint8_t*>(x4), *b = static_cast<const uint8_t*>(blocks);
