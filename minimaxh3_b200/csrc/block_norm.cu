@@ -564,64 +564,134 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Eight channels as four pairs: the arithmetic below is in packed f32 pairs, which
-// halves its issue slots (these kernels are otherwise bound by instruction issue).
-struct V8 {
-  float2 e[4];
+// A thread's CH channels of a row are P pieces of E channels (16 bytes), the CTA's
+// pieces side by side: piece q of thread t holds channels (q nt + t) E.. - so every
+// copy and store of a warp is one run of 512 bytes, in 16 and in 32 bits.  The
+// arithmetic is in packed f32 pairs, which halves its issue slots: these kernels
+// were bound by instruction issue before they were bound by HBM.
+template <typename T, int CH>
+struct Lay {
+  static constexpr int E = 16 / sizeof(T);
+  static constexpr int P = CH / E;
+  static __device__ __forceinline__ int at(int q) { return (q * (int)blockDim.x + (int)threadIdx.x) * E; }
 };
-__device__ __forceinline__ void pair_get(const float4* s, V8& v) {
-  const float4 a = s[threadIdx.x], b = s[blockDim.x + threadIdx.x];
-  v.e[0] = make_float2(a.x, a.y);
-  v.e[1] = make_float2(a.z, a.w);
-  v.e[2] = make_float2(b.x, b.y);
-  v.e[3] = make_float2(b.z, b.w);
-}
-template <typename T>
-__device__ __forceinline__ void store_pairs(T* p, const V8& v) {
-  if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v.e[0].x, v.e[0].y, v.e[1].x, v.e[1].y);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v.e[2].x, v.e[2].y, v.e[3].x, v.e[3].y);
-  } else {
-    uint32_t w[4];
+template <int CH>
+struct Vals {
+  float2 e[CH / 2];
+};
+
+// E modulation values from a 16-byte or smaller vector of any of the three types.
+template <int E>
+__device__ __forceinline__ void mod_piece(const void* p, int dt, long long at, float dflt, float* v) {
+  if (p == nullptr) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (std::is_same<T, __half>::value) {
-        const __half2 h = __floats2half2_rn(v.e[i].x, v.e[i].y);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-      } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v.e[i].x, v.e[i].y);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    for (int i = 0; i < E; ++i) v[i] = dflt;
+  } else if (dt == MH3_DTYPE_F32) {
+#pragma unroll
+    for (int i = 0; i < E; i += 4) {
+      const float4 f = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + i);
+      v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; i += 4) {
+      const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at + i);
+      const uint32_t w[2] = {u.x, u.y};
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float2 f = dt == MH3_DTYPE_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[k]))
+                                             : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
+        v[i + 2 * k] = f.x;
+        v[i + 2 * k + 1] = f.y;
       }
     }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   }
-}
-__device__ __forceinline__ float sum8(const V8& v) {
-  const float2 s = fadd2(fadd2(v.e[0], v.e[1]), fadd2(v.e[2], v.e[3]));
-  return s.x + s.y;
 }
 
-// A thread's eight channels of a row, to and from its place in the ring (``at``:
-// the place of the row and tensor, in 16-byte units times the CTA's threads).
-template <typename T>
-struct Ring {
-  static constexpr int W = sizeof(T) == 4 ? 2 : 1;  // 16-byte units of eight channels
-  uint4* base;
-  __device__ __forceinline__ void copy(int at, const T* src) const {
+// f(piece index, its first channel, E values of up to three tensors) for the thread's
+// pieces inside the row; results go to slots.
+template <int CH>
+__device__ __forceinline__ void slots_put(float4* s, const float (&v)[CH]) {
 #pragma unroll
-    for (int w = 0; w < W; ++w)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(base + (at * W + w) * (int)blockDim.x + threadIdx.x)),
-                   "l"(reinterpret_cast<const uint4*>(src) + w)
-                   : "memory");
+  for (int i = 0; i < CH / 4; ++i) s[i * blockDim.x + threadIdx.x] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+}
+template <int CH>
+__device__ __forceinline__ void slots_get(const float4* s, Vals<CH>& v) {
+#pragma unroll
+  for (int i = 0; i < CH / 4; ++i) {
+    const float4 f = s[i * blockDim.x + threadIdx.x];
+    v.e[2 * i] = make_float2(f.x, f.y);
+    v.e[2 * i + 1] = make_float2(f.z, f.w);
   }
-  __device__ __forceinline__ void get(int at, V8& v) const {
-    Raw<T> r;
+}
+template <typename T, int CH>
+__device__ __forceinline__ void mods(const void* p, int dt, long long at, int C, float dflt, float (&v)[CH]) {
+  using L = Lay<T, CH>;
 #pragma unroll
-    for (int w = 0; w < W; ++w) r.u[w] = base[(at * W + w) * (int)blockDim.x + threadIdx.x];
-    float f[8];
-    unpack(r, f);
+  for (int q = 0; q < L::P; ++q)
+    if (L::at(q) < C) mod_piece<L::E>(p, dt, at + L::at(q), dflt, v + q * L::E);
+}
+
+// A row of the output, from its first channel.
+template <typename T, int CH>
+__device__ __forceinline__ void store_row(T* row, int C, const Vals<CH>& v) {
+  using L = Lay<T, CH>;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v.e[i] = make_float2(f[2 * i], f[2 * i + 1]);
+  for (int q = 0; q < L::P; ++q) {
+    if (L::at(q) >= C) continue;
+    const float2* e = v.e + q * (L::E / 2);
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(row + L::at(q)) = make_float4(e[0].x, e[0].y, e[1].x, e[1].y);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __half>::value) {
+          const __half2 h = __floats2half2_rn(e[i].x, e[i].y);
+          w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(e[i].x, e[i].y);
+          w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
+      *reinterpret_cast<uint4*>(row + L::at(q)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+// A thread's pieces in the ring; ``slot``: the place of a stage's row and tensor.
+template <typename T, int CH>
+struct Ring {
+  using L = Lay<T, CH>;
+  uint4* base;  // of the thread
+  int C;
+  __device__ __forceinline__ void copy(int slot, const T* row) const {
+#pragma unroll
+    for (int q = 0; q < L::P; ++q)
+      if (L::at(q) < C)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(base + (slot * L::P + q) * (int)blockDim.x)),
+                     "l"(row + L::at(q))
+                     : "memory");
+  }
+  // channels past the row are 0
+  __device__ __forceinline__ void get(int slot, Vals<CH>& v) const {
+#pragma unroll
+    for (int q = 0; q < L::P; ++q) {
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (L::at(q) < C) u = base[(slot * L::P + q) * (int)blockDim.x];
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      float2* e = v.e + q * (L::E / 2);
+      if constexpr (sizeof(T) == 4) {
+        e[0] = make_float2(__uint_as_float(w[0]), __uint_as_float(w[1]));
+        e[1] = make_float2(__uint_as_float(w[2]), __uint_as_float(w[3]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (std::is_same<T, __half>::value) e[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          else e[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+        }
+      }
+    }
   }
 };
 
@@ -666,113 +736,148 @@ __device__ __forceinline__ void team_sum(float (&v)[N], float (*buf)[4][32], int
   for (int k = 0; k < N; ++k) v[k] = N == 1 ? z : __shfl_sync(0xffffffffu, z, k);
 }
 
-// Rows i of v to v - mean, and their (mean, rstd); threads past the row hold zeros
-// and add nothing.
-template <int R>
-__device__ __forceinline__ void center(V8 (&v)[R], bool live, float inv_c, int kind, float eps, float (*buf)[4][32], int& turn,
+// Rows i of v to v - mean, and their (mean, rstd); channels past the row stay 0.
+template <typename T, int CH, int R>
+__device__ __forceinline__ void center(Vals<CH> (&v)[R], int C, float inv_c, int kind, float eps, float (*buf)[4][32], int& turn,
                                        float2 (&out)[R]) {
+  using L = Lay<T, CH>;
   float s[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) out[i].x = 0.0f;
   if (kind == kLayer) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) s[i] = sum8(v[i]);
+    for (int i = 0; i < R; ++i) {
+      float2 t = v[i].e[0];
+#pragma unroll
+      for (int k = 1; k < CH / 2; ++k) t = fadd2(t, v[i].e[k]);
+      s[i] = t.x + t.y;
+    }
     team_sum(s, buf, turn);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       out[i].x = s[i] * inv_c;
-      if (live)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[i].e[k] = fadd2(v[i].e[k], both(-out[i].x));
+      for (int q = 0; q < L::P; ++q)
+        if (L::at(q) < C)
+#pragma unroll
+          for (int k = 0; k < L::E / 2; ++k) v[i].e[q * (L::E / 2) + k] = fadd2(v[i].e[q * (L::E / 2) + k], both(-out[i].x));
     }
   }
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    float2 q = fmul2(v[i].e[0], v[i].e[0]);
+    float2 t = fmul2(v[i].e[0], v[i].e[0]);
 #pragma unroll
-    for (int k = 1; k < 4; ++k) q = ffma2(v[i].e[k], v[i].e[k], q);
-    s[i] = q.x + q.y;
+    for (int k = 1; k < CH / 2; ++k) t = ffma2(v[i].e[k], v[i].e[k], t);
+    s[i] = t.x + t.y;
   }
   team_sum(s, buf, turn);
 #pragma unroll
   for (int i = 0; i < R; ++i) out[i].y = rsqrtf(fmaf(s[i], inv_c, eps));
 }
 
-template <typename T, bool Y, int R, int MAXT>
-__global__ void __launch_bounds__(MAXT) fwd_stream_kernel(const __grid_constant__ Params p) {
+// The modulation of group g for the thread's channels, combined into its slots.
+template <typename T, int CH, bool SHIFT, bool Y>
+__device__ __forceinline__ void load_mods(const Params& p, int g, float4* sA, float4* sB, float4* sG) {
+  float w[CH] = {}, t[CH] = {};
+  mods<T, CH>(p.scale.p, p.scale.dt, g * p.scale.sg, p.C, 0.0f, t);
+  mods<T, CH>(p.w.p, p.w.dt, 0, p.C, 1.0f, w);
+#pragma unroll
+  for (int k = 0; k < CH; ++k) w[k] *= 1.0f + t[k];
+  slots_put<CH>(sA, w);
+  if (SHIFT) {
+    mods<T, CH>(p.b.p, p.b.dt, 0, p.C, 0.0f, w);
+#pragma unroll
+    for (int k = 0; k < CH; ++k) w[k] *= 1.0f + t[k];
+    mods<T, CH>(p.shift.p, p.shift.dt, g * p.shift.sg, p.C, 0.0f, t);
+#pragma unroll
+    for (int k = 0; k < CH; ++k) w[k] += t[k];
+    slots_put<CH>(sB, w);
+  }
+  if (Y) {
+    mods<T, CH>(p.wy.p, p.wy.dt, 0, p.C, 1.0f, w);
+    mods<T, CH>(p.gate.p, p.gate.dt, g * p.gate.sg, p.C, 1.0f, t);
+#pragma unroll
+    for (int k = 0; k < CH; ++k) w[k] *= t[k];
+    slots_put<CH>(sG, w);
+  }
+}
+
+template <typename T, bool Y, int CH, int R, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) fwd_stream_kernel(const __grid_constant__ Params p) {
   extern __shared__ float4 slots[];
   __shared__ float red[2][4][32];
-  constexpr int NT = Y ? 2 : 1;              // tensors of a stage
-  float4* sA = slots;                        // w (1 + scale)
-  float4* sB = slots + 2 * blockDim.x;       // b (1 + scale) + shift
-  float4* sG = slots + 4 * blockDim.x;       // gate wy; only with y
-  const Ring<T> ring{reinterpret_cast<uint4*>(slots + (Y ? 6 : 4) * blockDim.x)};
-  const int c = threadIdx.x * 8;
-  const bool live = c < p.C;
+  constexpr int NT = Y ? 2 : 1;               // tensors of a stage
+  constexpr int S = CH / 4;                   // float4 of a thread's channels
+  float4* sA = slots;                         // w (1 + scale)
+  float4* sB = slots + S * blockDim.x;        // b (1 + scale) + shift
+  float4* sG = slots + 2 * S * blockDim.x;    // gate wy; only with y
+  const Ring<T, CH> ring{reinterpret_cast<uint4*>(slots + (Y ? 3 : 2) * S * blockDim.x) + threadIdx.x, p.C};
   const float inv_c = 1.0f / (float)p.C;
-  const long long lo = p.rows * blockIdx.x / p.ctas, hi = p.rows * (blockIdx.x + 1) / p.ctas;
+  const int lo = (int)(p.rows * blockIdx.x / p.ctas), hi = (int)(p.rows * (blockIdx.x + 1) / p.ctas);
   int turn = 0, g = -1;
   long long end = lo;
-  auto issue = [&](long long row, int st) {  // rows [row, row + R) into stage st
-    if (live) {
+  const T* xs = static_cast<const T*>(p.x) + lo * p.x_s;  // the next row to copy
+  const T* ys = static_cast<const T*>(p.y) + (Y ? lo * p.y_s : 0);
+  int ahead = lo;
+  auto issue = [&](int st) {  // the next R rows into stage st
 #pragma unroll
-      for (int i = 0; i < R; ++i)
-        if (row + i < hi) {
-          ring.copy((st * NT) * R + i, static_cast<const T*>(p.x) + (row + i) * p.x_s + c);
-          if (Y) ring.copy((st * NT + 1) * R + i, static_cast<const T*>(p.y) + (row + i) * p.y_s + c);
-        }
+    for (int i = 0; i < R; ++i, ++ahead) {
+      if (ahead < hi) {
+        ring.copy(st * NT * R + i, xs);
+        if (Y) ring.copy((st * NT + 1) * R + i, ys);
+      }
+      xs += p.x_s;
+      if (Y) ys += p.y_s;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  for (int j = 0; j < p.stages - 1; ++j) issue(lo + (long long)j * R, j);
+  for (int j = 0; j < p.stages - 1; ++j) issue(j);
   int st = 0;
-  for (long long row = lo; row < hi; row += R) {
-    issue(row + (long long)(p.stages - 1) * R, st == 0 ? p.stages - 1 : st - 1);
+  T* ro = static_cast<T*>(p.r) + (p.r ? (long long)lo * p.C : 0);
+  T* ho = static_cast<T*>(p.h) + (p.h ? (long long)lo * p.C : 0);
+  for (int row = lo; row < hi; row += R, ro += (long long)R * p.C, ho += (long long)R * p.C) {
+    issue(st == 0 ? p.stages - 1 : st - 1);
     if (p.stages == 3) cp_wait<2>();
     else cp_wait<1>();
-    const int cnt = (int)min((long long)R, hi - row);
+    const int cnt = min(R, hi - row);
     // Rows [j, n) of the stage, all of one group; ALL: every row of it.
     auto work = [&](auto all, int j, int n) {
       constexpr bool ALL = decltype(all)::value;
-      V8 v[R];
+      Vals<CH> v[R];
       float2 sy[R], sr[R];
 #pragma unroll
       for (int i = 0; i < R; ++i) {
         sy[i] = sr[i] = make_float2(0.0f, 1.0f);
-        v[i] = V8{};
-        if (live && (ALL || (i >= j && i < n))) ring.get((st * NT) * R + i, v[i]);
+        if (ALL || (i >= j && i < n)) ring.get(st * NT * R + i, v[i]);
+        else v[i] = Vals<CH>{};
       }
       if (Y) {
-        V8 y[R], a;
+        Vals<CH> y[R], a;
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-          y[i] = V8{};
-          if (live && (ALL || (i >= j && i < n))) ring.get((st * NT + 1) * R + i, y[i]);
+          if (ALL || (i >= j && i < n)) ring.get((st * NT + 1) * R + i, y[i]);
+          else y[i] = Vals<CH>{};
         }
-        if (p.ynorm != kNone) center<R>(y, live, inv_c, p.ynorm, p.eps, red, turn, sy);
-        if (live) {
-          pair_get(sG, a);
+        if (p.ynorm != kNone) center<T, CH, R>(y, p.C, inv_c, p.ynorm, p.eps, red, turn, sy);
+        slots_get<CH>(sG, a);
 #pragma unroll
-          for (int i = 0; i < R; ++i) {
+        for (int i = 0; i < R; ++i) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              v[i].e[k] = ffma2(fmul2(a.e[k], both(sy[i].y)), y[i].e[k], fmul2(v[i].e[k], both(p.alpha)));
-            if (p.r && (ALL || (i >= j && i < n))) store_pairs<T>(static_cast<T*>(p.r) + (row + i) * p.C + c, v[i]);
-          }
+          for (int k = 0; k < CH / 2; ++k)
+            v[i].e[k] = ffma2(fmul2(a.e[k], both(sy[i].y)), y[i].e[k], fmul2(v[i].e[k], both(p.alpha)));
+          if (p.r && (ALL || (i >= j && i < n))) store_row<T, CH>(ro + (long long)i * p.C, p.C, v[i]);
         }
       }
       if (p.h != nullptr) {
-        center<R>(v, live, inv_c, p.norm, p.eps, red, turn, sr);
-        if (live) {
-          V8 a, b;
-          pair_get(sA, a);
-          pair_get(sB, b);
+        center<T, CH, R>(v, p.C, inv_c, p.norm, p.eps, red, turn, sr);
+        Vals<CH> a, b;
+        slots_get<CH>(sA, a);
+        slots_get<CH>(sB, b);
 #pragma unroll
-          for (int i = 0; i < R; ++i) {
+        for (int i = 0; i < R; ++i) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[i].e[k] = ffma2(fmul2(v[i].e[k], both(sr[i].y)), a.e[k], b.e[k]);
-            if (ALL || (i >= j && i < n)) store_pairs<T>(static_cast<T*>(p.h) + (row + i) * p.C + c, v[i]);
-          }
+          for (int k = 0; k < CH / 2; ++k) v[i].e[k] = ffma2(fmul2(v[i].e[k], both(sr[i].y)), a.e[k], b.e[k]);
+          if (ALL || (i >= j && i < n)) store_row<T, CH>(ho + (long long)i * p.C, p.C, v[i]);
         }
       }
       if (threadIdx.x == 0 && p.stats)
@@ -783,36 +888,14 @@ __global__ void __launch_bounds__(MAXT) fwd_stream_kernel(const __grid_constant_
     for (int j = 0; j < cnt;) {  // the stage's rows, a group at a time
       if (row + j >= end) {
         g = group_of(p, row + j, g == p.G ? -1 : g, end);
-        if (live && g < p.G) {
-          float w[8], b[8], t[8];
-          mod8<true>(p.w.p, p.w.dt, c, 8, 1.0f, w);
-          mod8<true>(p.b.p, p.b.dt, c, 8, 0.0f, b);
-          mod8<true>(p.scale.p, p.scale.dt, g * p.scale.sg + c, 8, 0.0f, t);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            w[k] *= 1.0f + t[k];
-            b[k] *= 1.0f + t[k];
-          }
-          mod8<true>(p.shift.p, p.shift.dt, g * p.shift.sg + c, 8, 0.0f, t);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) b[k] += t[k];
-          slot_put(sA, w);
-          slot_put(sB, b);
-          if (Y) {
-            mod8<true>(p.wy.p, p.wy.dt, c, 8, 1.0f, w);
-            mod8<true>(p.gate.p, p.gate.dt, g * p.gate.sg + c, 8, 1.0f, t);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) w[k] *= t[k];
-            slot_put(sG, w);
-          }
-        }
+        if (g < p.G) load_mods<T, CH, true, Y>(p, g, sA, sB, sG);
       }
       const int n = (int)min((long long)cnt, end - row);
       if (g >= p.G) {  // outside every packed sequence: zeros
-        const V8 z = {};
+        const Vals<CH> z = {};
         for (int i = j; i < n; ++i) {
-          if (live && p.r) store_pairs<T>(static_cast<T*>(p.r) + (row + i) * p.C + c, z);
-          if (live && p.h) store_pairs<T>(static_cast<T*>(p.h) + (row + i) * p.C + c, z);
+          if (p.r) store_row<T, CH>(ro + (long long)i * p.C, p.C, z);
+          if (p.h) store_row<T, CH>(ho + (long long)i * p.C, p.C, z);
           if (threadIdx.x == 0 && p.stats) p.stats[row + i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
       } else if (n - j == R) {
@@ -828,118 +911,111 @@ __global__ void __launch_bounds__(MAXT) fwd_stream_kernel(const __grid_constant_
 
 template <typename T, bool Y, int R, int MAXT>
 __global__ void __launch_bounds__(MAXT) bwd_stream_kernel(const __grid_constant__ Params p) {
+  constexpr int CH = 8;
+  using L = Lay<T, CH>;
   extern __shared__ float4 slots[];
   __shared__ float red[2][4][32];
   constexpr int NT = Y ? 4 : 2;          // x, dh, y, dr
   float4* sA = slots;                    // w (1 + scale)
   float4* sG = slots + 2 * blockDim.x;   // gate wy; only with y
-  const Ring<T> ring{reinterpret_cast<uint4*>(slots + (Y ? 4 : 2) * blockDim.x)};
-  const int c = threadIdx.x * 8;
-  const bool live = c < p.C;
+  const Ring<T, CH> ring{reinterpret_cast<uint4*>(slots + (Y ? 4 : 2) * blockDim.x) + threadIdx.x, p.C};
   const float inv_c = 1.0f / (float)p.C;
-  const long long lo = p.rows * blockIdx.x / p.ctas, hi = p.rows * (blockIdx.x + 1) / p.ctas;
+  const int lo = (int)(p.rows * blockIdx.x / p.ctas), hi = (int)(p.rows * (blockIdx.x + 1) / p.ctas);
   const bool has_dr = Y && p.dr != nullptr, has_dh = p.dh != nullptr;
   int turn = 0, g = -1;
   long long end = lo;
-  V8 a1 = {}, a2 = {}, a3 = {};  // column sums of dh xhat, dh and d yhat
-  float4 nst[R];                 // the next stage's row statistics
+  Vals<CH> a1 = {}, a2 = {}, a3 = {};  // column sums of dh xhat, dh and d yhat
+  float4 nst[R];                       // the next stage's row statistics
   auto flush = [&](int grp) {
-    if (!live) return;
-    float* o = p.part + (long long)(blockIdx.x + grp) * 3 * p.C + c;
-    store_pairs<float>(o, a1);
-    store_pairs<float>(o + p.C, a2);
-    store_pairs<float>(o + 2 * p.C, a3);
-    a1 = a2 = a3 = V8{};
-  };
-  auto issue = [&](long long row, int st) {
-    if (live) {
+    float* o = p.part + (long long)(blockIdx.x + grp) * 3 * p.C;
+    const Vals<CH>* a[3] = {&a1, &a2, &a3};
 #pragma unroll
-      for (int i = 0; i < R; ++i)
-        if (row + i < hi) {
-          const int at = st * NT * R + i;
-          ring.copy(at, static_cast<const T*>(p.x) + (row + i) * p.x_s + c);
-          if (has_dh) ring.copy(at + R, static_cast<const T*>(p.dh) + (row + i) * p.dh_s + c);
-          if (Y) ring.copy(at + 2 * R, static_cast<const T*>(p.y) + (row + i) * p.y_s + c);
-          if (has_dr) ring.copy(at + 3 * R, static_cast<const T*>(p.dr) + (row + i) * p.dr_s + c);
-        }
-    }
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+      for (int q = 0; q < L::P; ++q)
+        if (L::at(q) < p.C)
+#pragma unroll
+          for (int i = 0; i < L::E / 2; i += 2) {
+            const float2* e = a[k]->e + q * (L::E / 2) + i;
+            *reinterpret_cast<float4*>(o + (long long)k * p.C + L::at(q) + 2 * i) = make_float4(e[0].x, e[0].y, e[1].x, e[1].y);
+          }
+    a1 = a2 = a3 = Vals<CH>{};
+  };
+  int ahead = lo;
+  auto issue = [&](int st) {
+#pragma unroll
+    for (int i = 0; i < R; ++i, ++ahead)
+      if (ahead < hi) {
+        const int slot = st * NT * R + i;
+        ring.copy(slot, static_cast<const T*>(p.x) + ahead * p.x_s);
+        if (has_dh) ring.copy(slot + R, static_cast<const T*>(p.dh) + ahead * p.dh_s);
+        if (Y) ring.copy(slot + 2 * R, static_cast<const T*>(p.y) + ahead * p.y_s);
+        if (has_dr) ring.copy(slot + 3 * R, static_cast<const T*>(p.dr) + ahead * p.dr_s);
+      }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  auto fetch_stats = [&](long long row) {
+  auto fetch_stats = [&](int row) {
 #pragma unroll
     for (int i = 0; i < R; ++i) nst[i] = row + i < hi ? __ldg(p.stats + row + i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   };
-  for (int j = 0; j < p.stages - 1; ++j) issue(lo + (long long)j * R, j);
+  for (int j = 0; j < p.stages - 1; ++j) issue(j);
   fetch_stats(lo);
   int st = 0;
-  for (long long row = lo; row < hi; row += R) {
-    issue(row + (long long)(p.stages - 1) * R, st == 0 ? p.stages - 1 : st - 1);
+  for (int row = lo; row < hi; row += R) {
+    issue(st == 0 ? p.stages - 1 : st - 1);
     float4 rs[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) rs[i] = nst[i];
     fetch_stats(row + R);
     if (p.stages == 3) cp_wait<2>();
     else cp_wait<1>();
-    const int cnt = (int)min((long long)R, hi - row);
+    const int cnt = min(R, hi - row);
     for (int j = 0; j < cnt;) {
       if (row + j >= end) {
         const int was = g;
         g = group_of(p, row + j, g == p.G ? -1 : g, end);
         if (was >= 0 && was < p.G) flush(was);
-        if (live && g < p.G) {
-          float w[8], t[8];
-          mod8<true>(p.w.p, p.w.dt, c, 8, 1.0f, w);
-          mod8<true>(p.scale.p, p.scale.dt, g * p.scale.sg + c, 8, 0.0f, t);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) w[k] *= 1.0f + t[k];
-          slot_put(sA, w);
-          if (Y) {
-            mod8<true>(p.wy.p, p.wy.dt, c, 8, 1.0f, w);
-            mod8<true>(p.gate.p, p.gate.dt, g * p.gate.sg + c, 8, 1.0f, t);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) w[k] *= t[k];
-            slot_put(sG, w);
-          }
-        }
+        if (g < p.G) load_mods<T, CH, false, Y>(p, g, sA, nullptr, sG);
       }
       const int n = (int)min((long long)cnt, end - row);
       if (g >= p.G) {  // outside every packed sequence: no gradient
-        const V8 z = {};
-        for (int i = j; i < n; ++i)
-          if (live) {
-            if (p.dx) store_pairs<T>(static_cast<T*>(p.dx) + (row + i) * p.C + c, z);
-            if (p.dy) store_pairs<T>(static_cast<T*>(p.dy) + (row + i) * p.C + c, z);
-          }
+        const Vals<CH> z = {};
+        for (int i = j; i < n; ++i) {
+          if (p.dx) store_row<T, CH>(static_cast<T*>(p.dx) + (long long)(row + i) * p.C, p.C, z);
+          if (p.dy) store_row<T, CH>(static_cast<T*>(p.dy) + (long long)(row + i) * p.C, p.C, z);
+        }
         j = n;
         continue;
       }
-      V8 d[R], yh[R], gt = {};
-      if (Y && live) pair_get(sG, gt);
+      // Channels past the row: x, y, dh and dr read as 0, the slots hold 0 there, so
+      // their terms of every sum are 0 (xhat, yhat are not, but multiply a 0).
+      Vals<CH> d[R], yh[R], gt = {};
+      if (Y) slots_get<CH>(sG, gt);
       {
-        V8 xh[R];
+        Vals<CH> xh[R];
         float s[2 * R];
 #pragma unroll
         for (int i = 0; i < R; ++i) {
           s[2 * i] = s[2 * i + 1] = 0.0f;
-          xh[i] = yh[i] = d[i] = V8{};
-          const int at = st * NT * R + i;
-          if (live && i >= j && i < n) {
-            ring.get(at, xh[i]);
+          xh[i] = yh[i] = d[i] = Vals<CH>{};
+          const int slot = st * NT * R + i;
+          if (i >= j && i < n) {
+            ring.get(slot, xh[i]);
             if (Y) {
-              ring.get(at + 2 * R, yh[i]);
+              ring.get(slot + 2 * R, yh[i]);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
+              for (int k = 0; k < CH / 2; ++k) {
                 yh[i].e[k] = fmul2(fadd2(yh[i].e[k], both(-rs[i].x)), both(rs[i].y));
                 xh[i].e[k] = ffma2(gt.e[k], yh[i].e[k], fmul2(xh[i].e[k], both(p.alpha)));
               }
             }
             if (has_dh) {
-              V8 t;
-              ring.get(at + R, t);
-              pair_get(sA, d[i]);
+              Vals<CH> t;
+              ring.get(slot + R, t);
+              slots_get<CH>(sA, d[i]);
               float2 s0 = both(0.0f), s1 = s0;
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
+              for (int k = 0; k < CH / 2; ++k) {
                 xh[i].e[k] = fmul2(fadd2(xh[i].e[k], both(-rs[i].z)), both(rs[i].w));
                 a1.e[k] = ffma2(t.e[k], xh[i].e[k], a1.e[k]);
                 a2.e[k] = fadd2(a2.e[k], t.e[k]);
@@ -958,45 +1034,44 @@ __global__ void __launch_bounds__(MAXT) bwd_stream_kernel(const __grid_constant_
           for (int i = 0; i < R; ++i) {
             const float m0 = p.norm == kLayer ? -s[2 * i] * inv_c : 0.0f, m1 = -s[2 * i + 1] * inv_c;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < CH / 2; ++k)
               d[i].e[k] = fmul2(ffma2(xh[i].e[k], both(m1), fadd2(d[i].e[k], both(m0))), both(rs[i].w));
           }
         }
       }
 #pragma unroll
       for (int i = 0; i < R; ++i)
-        if (live && i >= j && i < n) {
-          V8 t;
+        if (i >= j && i < n) {
+          Vals<CH> t;
           if (has_dr) {
             ring.get(st * NT * R + i + 3 * R, t);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) d[i].e[k] = fadd2(d[i].e[k], t.e[k]);
+            for (int k = 0; k < CH / 2; ++k) d[i].e[k] = fadd2(d[i].e[k], t.e[k]);
           }
           if (p.dx) {
             t = d[i];
             if (Y)
 #pragma unroll
-              for (int k = 0; k < 4; ++k) t.e[k] = fmul2(t.e[k], both(p.alpha));
-            store_pairs<T>(static_cast<T*>(p.dx) + (row + i) * p.C + c, t);
+              for (int k = 0; k < CH / 2; ++k) t.e[k] = fmul2(t.e[k], both(p.alpha));
+            store_row<T, CH>(static_cast<T*>(p.dx) + (long long)(row + i) * p.C, p.C, t);
           }
         }
       if (Y) {
         float s[2 * R];
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-          s[2 * i] = s[2 * i + 1] = 0.0f;
-          if (live && i >= j && i < n) {
-            float2 s0 = both(0.0f), s1 = s0;
+          float2 s0 = both(0.0f), s1 = s0;
+          if (i >= j && i < n) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < CH / 2; ++k) {
               a3.e[k] = ffma2(d[i].e[k], yh[i].e[k], a3.e[k]);
               d[i].e[k] = fmul2(d[i].e[k], gt.e[k]);
               s0 = fadd2(s0, d[i].e[k]);
               s1 = ffma2(d[i].e[k], yh[i].e[k], s1);
             }
-            s[2 * i] = s0.x + s0.y;
-            s[2 * i + 1] = s1.x + s1.y;
           }
+          s[2 * i] = s0.x + s0.y;
+          s[2 * i + 1] = s1.x + s1.y;
         }
         if (p.ynorm != kNone && p.dy) {
           team_sum(s, red, turn);
@@ -1004,14 +1079,14 @@ __global__ void __launch_bounds__(MAXT) bwd_stream_kernel(const __grid_constant_
           for (int i = 0; i < R; ++i) {
             const float m0 = p.ynorm == kLayer ? -s[2 * i] * inv_c : 0.0f, m1 = -s[2 * i + 1] * inv_c;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < CH / 2; ++k)
               d[i].e[k] = fmul2(ffma2(yh[i].e[k], both(m1), fadd2(d[i].e[k], both(m0))), both(rs[i].y));
           }
         }
         if (p.dy)
 #pragma unroll
           for (int i = 0; i < R; ++i)
-            if (live && i >= j && i < n) store_pairs<T>(static_cast<T*>(p.dy) + (row + i) * p.C + c, d[i]);
+            if (i >= j && i < n) store_row<T, CH>(static_cast<T*>(p.dy) + (long long)(row + i) * p.C, p.C, d[i]);
       }
       j = n;
     }
@@ -1096,7 +1171,7 @@ __global__ void __launch_bounds__(128) chan_kernel(const __grid_constant__ Param
   if (p.dwy) put1(p.dwy, p.wy.dt, c, sy);
 }
 
-static int threads_of(int C) { return ((C + 7) / 8 + 31) / 32 * 32; }
+static int threads_of(int C, int ch = 8) { return ((C + ch - 1) / ch + 31) / 32 * 32; }
 
 // CTAs: one of a 5120-channel row's 640 threads per SM, narrow rows to as many
 // threads (up to 16 CTAs).  More CTAs only add partial rows of column sums.
@@ -1106,54 +1181,74 @@ static int ctas_of(long long rows, int C) {
 }
 
 template <auto K>
-static cudaError_t start(const Params& p, size_t smem, cudaStream_t st) {
+static cudaError_t start(const Params& p, int threads, size_t smem, cudaStream_t st) {
   if (smem > 40 * 1024) {  // with the static part, past the 48 KB default
     const cudaError_t e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
   }
-  K<<<p.ctas, threads_of(p.C), smem, st>>>(p);
+  K<<<p.ctas, threads, smem, st>>>(p);
   return cudaGetLastError();
 }
 
 // Shared memory of a streaming kernel with ``mods`` slots and ``tensors`` x R rows a
 // stage; sets p.stages to 3, or 2 where three do not fit, and 0 where two do not.
-constexpr size_t kSmemMax = 226 * 1024;
-static size_t ring_bytes(Params& p, int mods, int tensors, int R, int es) {
-  const size_t nt = (size_t)threads_of(p.C);
-  const size_t fixed = nt * 32 * mods, stage = nt * 8 * es * tensors * R;
-  p.stages = fixed + 3 * stage <= kSmemMax ? 3 : fixed + 2 * stage <= kSmemMax ? 2 : 0;
+constexpr size_t kSmemMax = 224 * 1024;
+static size_t ring_bytes(Params& p, int threads, int ch, int mods, int rows, int es, size_t most) {
+  const size_t fixed = (size_t)threads * ch * 4 * mods, stage = (size_t)threads * ch * es * rows;
+  p.stages = fixed + 3 * stage <= most ? 3 : fixed + 2 * stage <= most ? 2 : 0;
   return fixed + p.stages * stage;
 }
 
-// Rows a stage: 40 KB of a 5120-channel row's tensors where the values of a
-// stage fit the registers of 640 threads (four rows forward, two backward).
-template <typename T, bool Y>
+// norm_modulate: 16 channels a thread and two rows a stage, two CTAs of a
+// 5120-channel row per SM (146 us with 8 channels and four rows in one CTA, at
+// 32760 x 5120: the reductions' instructions per channel halve).  The gated form
+// holds three modulation slots and two tensors, so one CTA with 8 channels.
+template <typename T>
 static cudaError_t stream_fwd(Params& p, cudaStream_t st, bool& done) {
-  constexpr int R = (sizeof(T) == 4 ? 2 : 4) / (Y ? 2 : 1);
-  const bool wide = threads_of(p.C) > 640;
-  const size_t smem = ring_bytes(p, Y ? 3 : 2, Y ? 2 : 1, wide ? 1 : R, sizeof(T));
+  constexpr int R = 2;
+  const int nt = threads_of(p.C, 16);
+  int per = std::max(1, std::min(16, 640 / nt));  // CTAs per SM, fewer where their rings do not fit
+  size_t smem = 0;
+  for (;; --per) {
+    smem = ring_bytes(p, nt, 16, 2, R, sizeof(T), kSmemMax / per - 2048);
+    if (p.stages != 0 || per == 1) break;
+  }
   done = p.stages != 0;
   if (!done) return cudaSuccess;
-  return wide ? start<fwd_stream_kernel<T, Y, 1, 1024>>(p, smem, st) : start<fwd_stream_kernel<T, Y, R, 640>>(p, smem, st);
+  p.ctas = (int)std::min<long long>(p.rows, (long long)kSMs * per);
+  return nt <= 320 ? start<fwd_stream_kernel<T, false, 16, R, 320, 2>>(p, nt, smem, st)
+                   : start<fwd_stream_kernel<T, false, 16, R, 512, 1>>(p, nt, smem, st);
+}
+template <typename T>
+static cudaError_t stream_fwd_gated(Params& p, cudaStream_t st, bool& done) {
+  constexpr int R = sizeof(T) == 4 ? 1 : 2;
+  const int nt = threads_of(p.C);
+  const bool wide = nt > 640;
+  const size_t smem = ring_bytes(p, nt, 8, 3, 2 * (wide ? 1 : R), sizeof(T), kSmemMax);
+  done = p.stages != 0;
+  if (!done) return cudaSuccess;
+  return wide ? start<fwd_stream_kernel<T, true, 8, 1, 1024, 1>>(p, nt, smem, st)
+              : start<fwd_stream_kernel<T, true, 8, R, 640, 1>>(p, nt, smem, st);
 }
 template <typename T, bool Y>
 static cudaError_t stream_bwd(Params& p, cudaStream_t st, bool& done) {
   constexpr int R = sizeof(T) == 4 || Y ? 1 : 2;
-  const bool wide = threads_of(p.C) > 640;
-  const size_t smem = ring_bytes(p, Y ? 2 : 1, Y ? 4 : 2, wide ? 1 : R, sizeof(T));
+  const int nt = threads_of(p.C);
+  const bool wide = nt > 640;
+  const size_t smem = ring_bytes(p, nt, 8, Y ? 2 : 1, (Y ? 4 : 2) * (wide ? 1 : R), sizeof(T), kSmemMax);
   done = p.stages != 0;
   if (!done) return cudaSuccess;
-  return wide ? start<bwd_stream_kernel<T, Y, 1, 1024>>(p, smem, st) : start<bwd_stream_kernel<T, Y, R, 640>>(p, smem, st);
+  return wide ? start<bwd_stream_kernel<T, Y, 1, 1024>>(p, nt, smem, st) : start<bwd_stream_kernel<T, Y, R, 640>>(p, nt, smem, st);
 }
 
 template <typename T, bool VEC, bool PT>
 static cudaError_t launch_fwd(Params& p, cudaStream_t st) {
   if constexpr (VEC && !PT) {
     bool done = false;
-    const cudaError_t e = p.y ? stream_fwd<T, true>(p, st, done) : stream_fwd<T, false>(p, st, done);
+    const cudaError_t e = p.y ? stream_fwd_gated<T>(p, st, done) : stream_fwd<T>(p, st, done);
     if (done) return e;
   }
-  return start<fwd_kernel<T, VEC, PT>>(p, (size_t)threads_of(p.C) * 32 * (p.y ? 3 : 2), st);
+  return start<fwd_kernel<T, VEC, PT>>(p, threads_of(p.C), (size_t)threads_of(p.C) * 32 * (p.y ? 3 : 2), st);
 }
 
 template <typename T, bool VEC, bool PT>
@@ -1162,7 +1257,7 @@ static cudaError_t launch_bwd(Params& p, cudaStream_t st) {
     bool done = false;
     cudaError_t e = cudaSuccess;
     if constexpr (VEC && !PT) e = p.y ? stream_bwd<T, true>(p, st, done) : stream_bwd<T, false>(p, st, done);
-    if (!done) e = start<bwd_kernel<T, VEC, PT>>(p, (size_t)threads_of(p.C) * 32 * (p.y ? 2 : 1), st);
+    if (!done) e = start<bwd_kernel<T, VEC, PT>>(p, threads_of(p.C), (size_t)threads_of(p.C) * 32 * (p.y ? 2 : 1), st);
     if (e != cudaSuccess) return e;
   }
   const bool chan = p.dw || p.db || p.dwy;
@@ -1192,7 +1287,7 @@ static int run(const mh3_block_norm_args* a, bool bwd, void* stream) {
   if (a == nullptr) return fail(MH3_ERR_INVALID, "mh3_block_norm: null args");
   if (a->rows < 0 || a->channels <= 0 || a->groups <= 0) return fail(MH3_ERR_INVALID, "mh3_block_norm: bad sizes");
   if (a->channels > kMaxC) return fail(MH3_ERR_TOO_LARGE, "mh3_block_norm: at most 8192 channels");
-  if (a->rows > (1ll << 40)) return fail(MH3_ERR_TOO_LARGE, "mh3_block_norm: too many rows");
+  if (a->rows > 0x7fff0000ll) return fail(MH3_ERR_TOO_LARGE, "mh3_block_norm: too many rows");
   if (!float_type(a->dtype)) return fail(MH3_ERR_INVALID, "mh3_block_norm: dtype must be bf16, f16 or f32");
   if (a->norm != kRms && a->norm != kLayer) return fail(MH3_ERR_INVALID, "mh3_block_norm: norm must be 1 (rms) or 2 (layer)");
   if (a->y_norm < kNone || a->y_norm > kLayer) return fail(MH3_ERR_INVALID, "mh3_block_norm: y_norm must be 0, 1 or 2");
