@@ -543,6 +543,17 @@ typedef struct mh3_fp4_gemm_args {
 
 MH3_API int mh3_fp4_gemm(const mh3_fp4_gemm_args* args, void* stream);
 
+/*
+ * mh3_quantize_fp4 of x [M,K] (bf16, f16 or f32, row stride x_stride) and
+ * mh3_fp4_gemm of the result with the 4-bit weight [N,K], in one call; for a
+ * few rows (workspace_bytes 0) in one launch.  workspace:
+ * mh3_fp4_linear_workspace_bytes() bytes, 16-byte aligned.
+ */
+MH3_API uint64_t mh3_fp4_linear_workspace_bytes(int64_t M, int64_t K);
+MH3_API int mh3_fp4_linear(const void* x, int64_t x_stride, int32_t in_dtype, int64_t M, int64_t N, int64_t K,
+                           const void* w4, const void* w_blocks, const float* w_scale, const void* bias, void* out,
+                           int64_t ldo, void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

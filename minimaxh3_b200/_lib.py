@@ -169,6 +169,8 @@ _SIGNATURES = {
     "mh3_quantize_fp4": (c_i32, [c_ptr, c_i64, c_i32, c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_ptr]),
     "mh3_dequantize_fp4": (c_i32, [c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i32, c_ptr, c_ptr]),
     "mh3_fp4_gemm": (c_i32, [ctypes.POINTER(Fp4GemmArgs), c_ptr]),
+    "mh3_fp4_linear_workspace_bytes": (c_u64, [c_i64, c_i64]),
+    "mh3_fp4_linear": (c_i32, [c_ptr, c_i64, c_i32, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_ptr, c_ptr]),
     "mh3_step_diff_workspace_bytes": (c_u64, []),
     "mh3_step_diff": (c_i32, [c_ptr, c_ptr, c_i32, c_i64, c_i32, c_ptr, c_ptr, c_ptr]),
 }

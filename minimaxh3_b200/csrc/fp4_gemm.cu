@@ -18,14 +18,19 @@
 //   against 1.05 without the wait at 32760 x 13824 x 5120).  Eight epilogue warps take
 //   the whole accumulator into registers and hand it over before they scale and
 //   store it, so the next tile's MMAs run meanwhile.
-// * small_kernel (M <= kSmallM): bound by reading b once.  A CTA takes 16 rows of b,
-//   its warps split K; codes are widened to f16 with their block scale (6
-//   significant bits: exact) and multiplied by mma.sync.m16n8k16 with f32 sums.
-//   The weights are the 16-row operand, up to 32 tokens the narrow one, and both
-//   sides use the same permutation of k, so a lane loads 32 consecutive codes.
+// * small_kernel (M <= kSmallM): reads b once.  A CTA takes 16 rows of b, its warps
+//   split K; codes are widened to f16 with their block scale (6 significant bits:
+//   exact) and multiplied by mma.sync.m16n8k16 with f32 sums.  The weights are the
+//   16-row operand, up to 16 tokens the narrow one, and both sides use the same
+//   permutation of k, so a lane loads 32 consecutive codes.  Bound: widening the
+//   codes (about one instruction each) beside the latency of a chain of a few loads;
+//   above 16 rows the pair kernel takes no longer (11.7 us at 17 rows of 5120 x 5120
+//   against 9.4 here at 16; 15.6 against 17.3 at 13824 x 5120).
+
 #include <algorithm>
 #include <mutex>
 
+#include "fp4.cuh"
 #include "mh3_b200.h"
 #include "mh3_internal.h"
 #include "ptx.cuh"
@@ -43,7 +48,7 @@ constexpr int SF_BLOCK = 512;                  // scales of 128 rows x 64 elemen
 constexpr int EPI_BOX = 32 * 32 * 2;
 constexpr int kGroupM = 8;                     // 256-row blocks per raster group
 constexpr int SF_COL = 256, SF_COLS = 48;      // scales of a stage: 4 x 4 columns of A, 4 x 8 of B
-constexpr int kSmallM = 32;
+constexpr int kSmallM = 16;
 
 struct Params {
   CUtensorMap tma_a, tma_b;    // bytes (K/2, rows), box (128, 128), 128B swizzle
@@ -335,9 +340,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) pair_kernel(const __grid_const
 // ---------------------------------------------------------------------------
 // Few rows
 // ---------------------------------------------------------------------------
+// Warps of a CTA, which split K, and its rows of b.  16 rows by 8 warps took 6.9 us at
+// one row of 5120 x 5120 (32 rows: 8.1; 4 warps: 10.0) and 13.2 us at 13824 x 5120
+// (11.4; 12.4): more rows share a's widening, but leave too few warps per SM.
 constexpr int kWarps = 8;
+constexpr int kRowsW = 16;
 
 struct SmallParams {
+  const void* x;  // FUSED: the rows to round, [M, K] with stride x_s
+  long long x_s;
   const uint8_t *a, *sa, *b, *sb;
   const float *rs, *cs;
   const __nv_bfloat16 *bias, *a2, *b2;
@@ -356,14 +367,7 @@ __device__ __forceinline__ void widen32(const uint4& code, uint32_t sf, uint32_t
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint32_t t[4];
-    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-        "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
-        : "=r"(t[0]), "=r"(t[1]), "=r"(t[2]), "=r"(t[3])
-        : "r"(w[i]));
+    fp4::e2m1x8_halves(w[i], t);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&t[j]), i < 2 ? lo : hi);
@@ -380,76 +384,145 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// NT: groups of 8 rows of a.
-template <int NT>
+// NT: groups of 8 rows of a.  X: void, a is given in 4 bits; or the type of x, which
+// every CTA rounds for itself into shared memory while its weights are on their way to
+// L2 - one launch and no workspace for the calls where latency counts (8.3 us at one
+// row of 5120 x 5120 against 2.3 + 6.9; from three rows on the CTAs' copies of x cost
+// more than the launch).
+constexpr int kFusedRows = 2;
+constexpr int kFusedBytes = 96 * 1024;  // of codes and scales
+
+template <int NT, typename X>
 __global__ void __launch_bounds__(kWarps * 32) small_kernel(const __grid_constant__ SmallParams p) {
-  __shared__ float red[kWarps][16][NT * 8 + 1];
+  constexpr bool FUSED = !std::is_same<X, void>::value;
+  __shared__ float red[kWarps][kRowsW][NT * 8 + 1];
+  extern __shared__ uint4 own[];  // FUSED: codes [M][K/2], then scales [M][K/16]
+  __shared__ uint32_t top[FUSED ? kFusedRows : 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n0 = blockIdx.x * 16;
+  const int n0 = blockIdx.x * kRowsW;
   const int gr = lane >> 2, q = lane & 3;
   const int units = p.K / 32, nk64 = (p.K + 63) / 64;
   const long long kb = p.K / 2;
   // scale word of 32 codes: two bytes of the row's place in its block of 128
   auto sf_at = [&](int row) { return (long long)(row >> 7) * nk64 * 512 + (row & 31) * 16 + ((row & 127) >> 5) * 4; };
-  const int r0 = min(n0 + gr, p.N - 1), r1 = min(n0 + gr + 8, p.N - 1);  // rows past N are computed and dropped
-  const uint8_t *w0 = p.b + r0 * kb, *w1 = p.b + r1 * kb;
-  const uint8_t *s0 = p.sb + sf_at(r0), *s1 = p.sb + sf_at(r1);
-  float c[NT][4];
+  const uint8_t *w[kRowsW / 8], *sw[kRowsW / 8];  // the lane's rows, 8 apart; those past N are computed and dropped
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c[t][i] = 0.0f;
-#pragma unroll 2
-  for (int u = warp * 4 + q; u - q < units; u += kWarps * 4) {
-    const bool in = u < units;
+  for (int i = 0; i < kRowsW / 8; ++i) {
+    const int r = min(n0 + gr + 8 * i, p.N - 1);
+    w[i] = p.b + r * kb;
+    sw[i] = p.sb + sf_at(r);
+  }
+  const uint8_t* xs = reinterpret_cast<const uint8_t*>(own) + p.M * kb;
+  float c[kRowsW / 16][NT][4] = {};
+  uint4 d[kRowsW / 8];  // a unit's codes and scales
+  uint32_t f[kRowsW / 8];
+  auto fetch = [&](int u) {
     const long long so = (long long)(u >> 1) * 512 + (u & 1) * 2;
-    uint4 d0 = make_uint4(0, 0, 0, 0), d1 = d0, dx[NT];
-    uint32_t f0 = 0, f1 = 0, fx[NT];
-    if (in) {
-      d0 = __ldcs(reinterpret_cast<const uint4*>(w0 + (long long)u * 16));
-      d1 = __ldcs(reinterpret_cast<const uint4*>(w1 + (long long)u * 16));
-      f0 = *reinterpret_cast<const uint16_t*>(s0 + so);
-      f1 = *reinterpret_cast<const uint16_t*>(s1 + so);
-    }
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      dx[t] = make_uint4(0, 0, 0, 0);
-      fx[t] = 0;
-      const int row = t * 8 + gr;
-      if (in && row < p.M) {
-        dx[t] = *reinterpret_cast<const uint4*>(p.a + row * kb + (long long)u * 16);
-        fx[t] = *reinterpret_cast<const uint16_t*>(p.sa + sf_at(row) + so);
+    for (int i = 0; i < kRowsW / 8; ++i) {
+      d[i] = u < units ? __ldcs(reinterpret_cast<const uint4*>(w[i] + (long long)u * 16)) : make_uint4(0, 0, 0, 0);
+      f[i] = u < units ? *reinterpret_cast<const uint16_t*>(sw[i] + so) : 0;
+    }
+  };
+  fetch(warp * 4 + q);
+  if constexpr (FUSED) {
+    // this CTA's rows of weights towards L2
+    const int lines = (int)((kb + 127) / 128);
+    for (int i = threadIdx.x; i < kRowsW * lines; i += kWarps * 32) {
+      const int row = min(n0 + i / lines, p.N - 1);
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.b + row * kb + (long long)(i % lines) * 128));
+    }
+    const int nb = p.K / 16, total = p.M * nb;
+    const X* x = static_cast<const X*>(p.x);
+    const bool vec = (reinterpret_cast<uintptr_t>(p.x) & 15u) == 0 && p.x_s * (long long)sizeof(X) % 16 == 0;
+    if ((int)threadIdx.x < p.M) top[threadIdx.x] = 0;
+    __syncthreads();
+    uint32_t most[kFusedRows] = {};
+    for (int b = threadIdx.x; b < nb; b += kWarps * 32)
+#pragma unroll
+      for (int m = 0; m < kFusedRows; ++m)
+        if (m < p.M) {
+          float v[16];
+          fp4::load16(x + m * p.x_s + b * 16, v, vec);
+          most[m] = max(most[m], fp4::absmax16(v));
+        }
+#pragma unroll
+    for (int m = 0; m < kFusedRows; ++m)
+      if (m < p.M) {
+        most[m] = __reduce_max_sync(0xffffffffu, most[m]);
+        if (lane == 0) atomicMax(&top[m], most[m]);
       }
+    __syncthreads();
+    for (int i = threadIdx.x; i < total; i += kWarps * 32) {
+      const int m = i / nb, b = i - m * nb;
+      uint2 code = make_uint2(0, 0);
+      uint32_t s8 = 0;
+      if (top[m] < 0x7f800000u) {
+        float v[16];
+        fp4::load16(x + m * p.x_s + b * 16, v, vec);
+        s8 = fp4::round_block(v, fp4::absmax16(v), fp4::pow2f(-fp4::row_exponent(top[m])), code);
+      }
+      reinterpret_cast<uint2*>(own)[i] = code;
+      const_cast<uint8_t*>(xs)[i] = (uint8_t)s8;
     }
-    uint32_t h0[16], h1[16];
-    widen32(d0, f0, h0);
-    widen32(d1, f1, h1);
+    __syncthreads();
+  }
+  for (int u = warp * 4 + q; u - q < units; u += kWarps * 4) {
+    uint32_t hx[NT][16];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      uint32_t hx[16];
-      widen32(dx[t], fx[t], hx);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) mma_16x8x16(c[t], h0[2 * j], h1[2 * j], h0[2 * j + 1], h1[2 * j + 1], hx[2 * j], hx[2 * j + 1]);
+      uint4 dx = make_uint4(0, 0, 0, 0);
+      uint32_t fx = 0;
+      const int row = t * 8 + gr;
+      if (u < units && row < p.M) {
+        if constexpr (FUSED) {
+          dx = own[row * units + u];
+          fx = *reinterpret_cast<const uint16_t*>(xs + (row * units + u) * 2);
+        } else {
+          dx = *reinterpret_cast<const uint4*>(p.a + row * kb + (long long)u * 16);
+          fx = *reinterpret_cast<const uint16_t*>(p.sa + sf_at(row) + (long long)(u >> 1) * 512 + (u & 1) * 2);
+        }
+      }
+      widen32(dx, fx, hx[t]);
     }
+#pragma unroll
+    for (int i = 0; i < kRowsW / 16; ++i) {
+      uint32_t h0[16], h1[16];
+      widen32(d[2 * i], f[2 * i], h0);
+      widen32(d[2 * i + 1], f[2 * i + 1], h1);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          mma_16x8x16(c[i][t], h0[2 * j], h1[2 * j], h0[2 * j + 1], h1[2 * j + 1], hx[t][2 * j], hx[t][2 * j + 1]);
+    }
+    fetch(u + kWarps * 4);
   }
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    red[warp][gr][t * 8 + q * 2] = c[t][0];
-    red[warp][gr][t * 8 + q * 2 + 1] = c[t][1];
-    red[warp][gr + 8][t * 8 + q * 2] = c[t][2];
-    red[warp][gr + 8][t * 8 + q * 2 + 1] = c[t][3];
-  }
+  for (int i = 0; i < kRowsW / 16; ++i)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float* r0 = &red[warp][16 * i + gr][t * 8 + q * 2];
+      float* r1 = &red[warp][16 * i + gr + 8][t * 8 + q * 2];
+      r0[0] = c[i][t][0];
+      r0[1] = c[i][t][1];
+      r1[0] = c[i][t][2];
+      r1[1] = c[i][t][3];
+    }
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * NT * 8; i += kWarps * 32) {
-    const int j = i & 15, m = i >> 4, n = n0 + j;
+  for (int i = threadIdx.x; i < kRowsW * NT * 8; i += kWarps * 32) {
+    const int j = i % kRowsW, m = i / kRowsW, n = n0 + j;
     if (m >= p.M || n >= p.N) continue;
     float s = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) s += red[w][j][m];
+    for (int k = 0; k < kWarps; ++k) s += red[k][j][m];
     for (int r = 0; r < p.R; ++r)
       s = fmaf(__bfloat162float(p.a2[m * p.lda2 + r]), __bfloat162float(p.b2[n * p.ldb2 + r]), s);
+    float rs;
+    if constexpr (FUSED) rs = top[m] < 0x7f800000u ? fp4::pow2f(fp4::row_exponent(top[m])) : __uint_as_float(0x7fffffffu);
+    else rs = p.rs[m];
     const float b = p.bias != nullptr ? __bfloat162float(p.bias[n]) : 0.0f;
-    p.out[m * p.ldo + n] = __float2bfloat16_rn(fmaf(s * p.rs[m], p.cs[n], b));
+    p.out[m * p.ldo + n] = __float2bfloat16_rn(fmaf(s * rs, p.cs[n], b));
   }
 }
 
@@ -523,10 +596,23 @@ static int map_scales(CUtensorMap* map, const void* base, long long K, long long
 }
 
 static cudaError_t launch_small(const SmallParams& p, cudaStream_t st) {
-  const unsigned grid = (unsigned)((p.N + 15) / 16);
-  if (p.M <= 8) small_kernel<1><<<grid, kWarps * 32, 0, st>>>(p);
-  else if (p.M <= 16) small_kernel<2><<<grid, kWarps * 32, 0, st>>>(p);
-  else small_kernel<4><<<grid, kWarps * 32, 0, st>>>(p);
+  const unsigned grid = (unsigned)((p.N + kRowsW - 1) / kRowsW);
+  if (p.M <= 8) small_kernel<1, void><<<grid, kWarps * 32, 0, st>>>(p);
+  else small_kernel<2, void><<<grid, kWarps * 32, 0, st>>>(p);
+  return cudaGetLastError();
+}
+
+// Whether a linear of M rows runs as one launch.
+static bool fused(long long M, long long K) { return M <= kFusedRows && M * (K / 2 + K / 16) <= kFusedBytes; }
+
+template <typename X>
+static cudaError_t launch_fused(const SmallParams& p, cudaStream_t st) {
+  const size_t smem = (size_t)p.M * (p.K / 2 + p.K / 16);
+  if (smem > 32 * 1024) {  // with the static part, past the 48 KB default
+    const cudaError_t e = cudaFuncSetAttribute(small_kernel<1, X>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  small_kernel<1, X><<<(unsigned)((p.N + kRowsW - 1) / kRowsW), kWarps * 32, smem, st>>>(p);
   return cudaGetLastError();
 }
 
@@ -558,7 +644,7 @@ extern "C" int mh3_fp4_gemm(const mh3_fp4_gemm_args* a, void* stream) {
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (a->M <= fp4gemm::kSmallM) {
-    fp4gemm::SmallParams p;
+    fp4gemm::SmallParams p = {};
     p.a = static_cast<const uint8_t*>(a->a);
     p.sa = static_cast<const uint8_t*>(a->a_blocks);
     p.b = static_cast<const uint8_t*>(a->b);
@@ -607,4 +693,63 @@ extern "C" int mh3_fp4_gemm(const mh3_fp4_gemm_args* a, void* stream) {
     e = fp4gemm::launch_pair(p, st);
   }
   return e == cudaSuccess ? MH3_OK : fail_cuda(e, "mh3_fp4_gemm launch");
+}
+
+extern "C" uint64_t mh3_fp4_linear_workspace_bytes(int64_t M, int64_t K) {
+  if (M <= 0 || K <= 0 || fp4gemm::fused(M, K)) return 0;
+  // codes, block scales, row scales, each on a 16-byte boundary
+  return (uint64_t)M * (uint64_t)(K / 2) + mh3_fp4_block_bytes(M, K) + ((uint64_t)M * 4 + 15) / 16 * 16;
+}
+
+extern "C" int mh3_fp4_linear(const void* x, int64_t x_stride, int32_t in_dtype, int64_t M, int64_t N, int64_t K,
+                              const void* w4, const void* w_blocks, const float* w_scale, const void* bias, void* out,
+                              int64_t ldo, void* workspace, void* stream) {
+  const mh3::NvtxRange nvtx_range("mh3_fp4_linear");
+  if (M < 0 || N <= 0 || K <= 0 || K % 32) return fail(MH3_ERR_INVALID, "mh3_fp4_linear: K must be a positive multiple of 32");
+  if (in_dtype != MH3_DTYPE_BF16 && in_dtype != MH3_DTYPE_F16 && in_dtype != MH3_DTYPE_F32)
+    return fail(MH3_ERR_INVALID, "mh3_fp4_linear: in_dtype must be bf16, f16 or f32");
+  mh3_fp4_gemm_args g;
+  memset(&g, 0, sizeof(g));
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.b = w4;
+  g.b_blocks = w_blocks;
+  g.b_scale = w_scale;
+  g.bias = bias;
+  g.out = out;
+  g.ldo = ldo;
+  if (M == 0 || !fp4gemm::fused(M, K)) {
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    if (M > 0 && (!ws || ((uintptr_t)ws & 15u)))
+      return fail(MH3_ERR_INVALID, "mh3_fp4_linear: needs a 16-byte aligned workspace");
+    g.a = ws;
+    g.a_blocks = ws + M * (K / 2);
+    g.a_scale = reinterpret_cast<const float*>(ws + M * (K / 2) + mh3_fp4_block_bytes(M, K));
+    const int rc = mh3_quantize_fp4(x, x_stride, in_dtype, M, K, ws, ws + M * (K / 2),
+                                    reinterpret_cast<float*>(ws + M * (K / 2) + mh3_fp4_block_bytes(M, K)), stream);
+    return rc ? rc : mh3_fp4_gemm(&g, stream);
+  }
+  if (N % 8 || ldo % 8 || ldo < N) return fail(MH3_ERR_INVALID, "mh3_fp4_linear: N and ldo must be multiples of 8, ldo >= N");
+  if (N > 0x7fffff00LL || K > (1ll << 30)) return fail(MH3_ERR_TOO_LARGE, "mh3_fp4_linear: dimension too large");
+  if (!x || !w4 || !w_blocks || !w_scale || !out) return fail(MH3_ERR_INVALID, "mh3_fp4_linear: null pointer");
+  if (((uintptr_t)w4 & 15u) || ((uintptr_t)w_blocks & 15u) || ((uintptr_t)out & 15u))
+    return fail(MH3_ERR_INVALID, "mh3_fp4_linear: the weight and out must be 16-byte aligned");
+  fp4gemm::SmallParams p = {};
+  p.x = x;
+  p.x_s = x_stride;
+  p.b = static_cast<const uint8_t*>(w4);
+  p.sb = static_cast<const uint8_t*>(w_blocks);
+  p.cs = w_scale;
+  p.bias = static_cast<const __nv_bfloat16*>(bias);
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.ldo = ldo;
+  p.M = (int)M;
+  p.N = (int)N;
+  p.K = (int)K;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const cudaError_t e = in_dtype == MH3_DTYPE_BF16 ? fp4gemm::launch_fused<__nv_bfloat16>(p, st)
+                        : in_dtype == MH3_DTYPE_F16 ? fp4gemm::launch_fused<__half>(p, st)
+                                                    : fp4gemm::launch_fused<float>(p, st);
+  return e == cudaSuccess ? MH3_OK : fail_cuda(e, "mh3_fp4_linear launch");
 }

@@ -97,6 +97,9 @@ def _modulation(what, x, cu, mods):
     """The named modulation tensors as [groups, C] each, or of x's shape each if one of them has a row for each token."""
     C = x.shape[-1]
     groups = cu.numel() - 1 if cu is not None else x.shape[0] if x.dim() == 3 else 1
+    if all(m is None or (isinstance(m, torch.Tensor) and m.shape == (groups, C) and m.dtype in _TYPES and m.device == x.device)
+           for m in mods.values()):  # the common form
+        return mods, False
     out, per_token = {}, False
     for name, m in mods.items():
         if m is None:

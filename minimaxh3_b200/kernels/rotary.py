@@ -15,6 +15,8 @@ import torch
 
 from .. import ops as _ops
 
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_POS_TYPES = (torch.int32, torch.int64, torch.float32)
 _LIB = torch.library.Library("mh3", "FRAGMENT")
 _LIB.define("rotary_axes(Tensor q, Tensor? k, Tensor positions, int[] axes_dim, float[] theta, bool interleaved, "
             "bool inverse) -> (Tensor, Tensor)")
@@ -57,36 +59,45 @@ class Rotary(typing.NamedTuple):
     interleaved: bool = True
 
 
+def _plan(axes_dim: tuple, theta) -> tuple[list[int], list[float]]:
+    """The axes' widths and thetas as lists, checked."""
+    axes = [int(d) for d in axes_dim]
+    if not 1 <= len(axes) <= 4 or any(d < 0 or d % 2 for d in axes) or not 0 < sum(axes):
+        raise ValueError("rotary_axes: axes_dim is 1 to 4 even widths whose sum is positive and at most the head dim")
+    thetas = [float(t) for t in theta] if isinstance(theta, tuple) else [float(theta)] * len(axes)
+    if len(thetas) != len(axes) or any(not 0.0 < t <= 1e300 for t in thetas):
+        raise ValueError("rotary_axes: theta is one positive number, or one for each axis")
+    return axes, thetas
+
+
 def _check(q, k, positions, axes_dim, theta):
     for name, t in (("q", q), ("k", k)):
-        if name == "k" and t is None:
+        if t is None and name == "k":
             continue
         if not isinstance(t, torch.Tensor) or t.dim() not in (3, 4):
             raise ValueError(f"rotary_axes: {name} must be a tensor [B, H, S, D] or packed [T, H, D]")
-        if t.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        if t.dtype not in _TYPES:
             raise ValueError(f"rotary_axes: unsupported dtype {t.dtype} (bf16, f16 or f32)")
-    packed = q.dim() == 3
-    tokens = q.shape[0] if packed else q.shape[2]
+    shape, dev = q.shape, q.device
+    packed = len(shape) == 3
+    tokens, D = shape[0] if packed else shape[2], shape[-1]
     if k is not None:
-        if k.dim() != q.dim() or k.dtype != q.dtype or k.device != q.device or k.shape[-1] != q.shape[-1]:
+        ks = k.shape
+        if len(ks) != len(shape) or k.dtype != q.dtype or k.device != dev or ks[-1] != D:
             raise ValueError("rotary_axes: q and k must agree in dimensions, dtype, device and head dim")
-        if (k.shape[0] if packed else k.shape[2]) != tokens or (not packed and k.shape[0] != q.shape[0]):
+        if (ks[0] if packed else ks[2]) != tokens or (not packed and ks[0] != shape[0]):
             raise ValueError("rotary_axes: q and k must have the same tokens")
-    axes = [int(d) for d in axes_dim]
-    if not 1 <= len(axes) <= 4 or any(d < 0 or d % 2 for d in axes) or not 0 < sum(axes) <= q.shape[-1]:
+    axes, thetas = _plan(tuple(axes_dim), theta if isinstance(theta, (int, float)) else tuple(theta))
+    if sum(axes) > D:
         raise ValueError("rotary_axes: axes_dim is 1 to 4 even widths whose sum is positive and at most the head dim")
-    if q.shape[-1] > 256:
+    if D > 256:
         raise ValueError("rotary_axes: the head dim must be at most 256")
-    thetas = [float(theta)] * len(axes) if isinstance(theta, (int, float)) else [float(t) for t in theta]
-    if len(thetas) != len(axes) or any(not 0.0 < t <= 1e300 for t in thetas):
-        raise ValueError("rotary_axes: theta is one positive number, or one for each axis")
-    if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64, torch.float32):
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in _POS_TYPES:
         raise ValueError("rotary_axes: positions must be an int32, int64 or float32 tensor")
-    lead = tuple(positions.shape[:-1])
-    if positions.dim() not in (2, 3) or positions.shape[-1] != len(axes) or lead not in (
-            ((tokens,),) if packed else ((tokens,), (1, tokens), (q.shape[0], tokens))):
+    ps = positions.shape
+    if len(ps) not in (2, 3) or ps[-1] != len(axes) or ps[-2] != tokens or (len(ps) == 3 and (packed or ps[0] not in (1, shape[0]))):
         raise ValueError("rotary_axes: positions must be [S, axes] or [B, S, axes] (packed: [T, axes])")
-    if positions.device != q.device:
+    if positions.device != dev:
         raise ValueError("rotary_axes: positions must be on q's device")
     if not q.is_cuda:
         raise ValueError("rotary_axes: expected CUDA tensors")

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import collections
 import functools
+import struct
 
 import torch
 
@@ -54,6 +55,19 @@ def _dtype_code(dt: torch.dtype) -> int:
     if dt == torch.float16:
         return _lib.MH3_DTYPE_F16
     raise ValueError(f"unsupported dtype {dt} (bf16 or fp16)")
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _launch(dev: torch.device, fn, *args) -> int:
+    """``fn(*args, stream)`` with ``dev`` current, on its current stream.  The small calls' time is
+    the host's: the device is switched only where it has to be."""
+    index = dev.index
+    if _raw_stream is not None and index == torch.cuda.current_device():
+        return fn(*args, _raw_stream(index))
+    with torch.cuda.device(dev):
+        return fn(*args, _stream(dev))
 
 
 _FLOAT_CODE = {torch.bfloat16: _lib.MH3_DTYPE_BF16, torch.float16: _lib.MH3_DTYPE_F16, torch.float32: _lib.MH3_DTYPE_F32}
@@ -686,14 +700,16 @@ def check_fp4(x4, blocks, scale, what: str):
     for name, t, dt in (("values", x4, torch.uint8), ("block scales", blocks, E4M3), ("row scales", scale, torch.float32)):
         if not isinstance(t, torch.Tensor) or t.dtype != dt:
             raise ValueError(f"{what}: {name} must be a {dt} tensor")
-    if x4.dim() != 2 or x4.shape[1] == 0 or x4.shape[1] % 16:
+    shape = x4.shape
+    if len(shape) != 2 or shape[1] == 0 or shape[1] % 16:
         raise ValueError(f"{what}: values must be [M, K/2] bytes with K a multiple of 32")
-    M, K = x4.shape[0], 2 * x4.shape[1]
-    if tuple(blocks.shape) != _fp4_blocks_shape(M, K):
+    M, K = shape[0], 2 * shape[1]
+    if blocks.shape != _fp4_blocks_shape(M, K):
         raise ValueError(f"{what}: block scales must be of shape {_fp4_blocks_shape(M, K)}, got {tuple(blocks.shape)}")
     if scale.numel() != M:
         raise ValueError(f"{what}: need one row scale for each of {M} rows")
-    if blocks.device != x4.device or scale.device != x4.device:
+    dev = x4.device
+    if blocks.device != dev or scale.device != dev:
         raise ValueError(f"{what}: values and scales must be on one device")
     if not (x4.is_contiguous() and blocks.is_contiguous() and scale.is_contiguous()):
         raise ValueError(f"{what}: values and scales must be contiguous")
@@ -728,9 +744,8 @@ def quantize_fp4(x2d: torch.Tensor):
     blocks = torch.empty(_fp4_blocks_shape(M, K), dtype=E4M3, device=dev)
     scale = torch.empty((M, 1), dtype=torch.float32, device=dev)
     if M:
-        with torch.cuda.device(dev):
-            rc = lib.mh3_quantize_fp4(x2d.data_ptr(), x2d.stride(0), _FLOAT_CODE[x2d.dtype], M, K, x4.data_ptr(),
-                                      blocks.data_ptr(), scale.data_ptr(), _stream(dev))
+        rc = _launch(dev, lib.mh3_quantize_fp4, x2d.data_ptr(), x2d.stride(0), _FLOAT_CODE[x2d.dtype], M, K, x4.data_ptr(),
+                     blocks.data_ptr(), scale.data_ptr())
         _lib.check(rc, "mh3_quantize_fp4")
     return x4, blocks, scale
 
@@ -746,9 +761,8 @@ def dequantize_fp4(x4: torch.Tensor, blocks: torch.Tensor, scale: torch.Tensor,
     lib = _lib.load()
     out = torch.empty((M, K), dtype=dtype, device=x4.device)
     if M:
-        with torch.cuda.device(x4.device):
-            rc = lib.mh3_dequantize_fp4(x4.data_ptr(), blocks.data_ptr(), scale.data_ptr(), M, K, _FLOAT_CODE[dtype],
-                                        out.data_ptr(), _stream(x4.device))
+        rc = _launch(x4.device, lib.mh3_dequantize_fp4, x4.data_ptr(), blocks.data_ptr(), scale.data_ptr(), M, K,
+                     _FLOAT_CODE[dtype], out.data_ptr())
         _lib.check(rc, "mh3_dequantize_fp4")
     return out
 
@@ -803,8 +817,7 @@ def fp4_gemm(a, b, bias=None, a2=None, b2=None, out: torch.Tensor | None = None,
     g.timeout_ns = int(timeout_ns)
     g.test_flags = int(test_flags)
     lib = _lib.load()
-    with torch.cuda.device(dev):
-        rc = lib.mh3_fp4_gemm(g, _stream(dev))
+    rc = _launch(dev, lib.mh3_fp4_gemm, g)
     _lib.check(rc, "mh3_fp4_gemm")
     return out
 
@@ -812,22 +825,42 @@ def fp4_gemm(a, b, bias=None, a2=None, b2=None, out: torch.Tensor | None = None,
 @nvtx("mh3.fp4_linear")
 def fp4_linear(x2d: torch.Tensor, w4: torch.Tensor, w_blocks: torch.Tensor, w_scale: torch.Tensor, bias,
                adapters) -> torch.Tensor:
-    """FP4Linear forward: 4-bit activations (``quantize_fp4``) and one fused GEMM, bf16 out.
+    """FP4Linear forward: 4-bit activations and one GEMM (``mh3_fp4_linear``), bf16 out.
 
     The adapters' delta is folded into the GEMM as in ``fp8_linear``:
     a2 = (x A_cat^T) / x_scale, b2 = (scale*B)_cat / w_scale, both scales powers
     of two."""
-    if x2d.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+    if x2d.dtype not in _FLOAT_CODE:
         x2d = x2d.to(torch.float32)
     M, K = x2d.shape
     N = w4.shape[0]
-    xq = quantize_fp4(x2d)
-    a2 = b2 = None
+    dev = x2d.device
     if adapters:
+        xq = quantize_fp4(x2d)
         xb = x2d.to(torch.bfloat16).contiguous()
-        A_cat, b2 = _lora_operands(adapters, N, K, x2d.device, col_scale=w_scale.reshape(-1), scale_src=w_scale)
+        A_cat, b2 = _lora_operands(adapters, N, K, dev, col_scale=w_scale.reshape(-1), scale_src=w_scale)
         a2 = scaled_gemm(xb, A_cat, row_scale=xq[2], row_scale_inv=True)
-    return fp4_gemm(xq, (w4, w_blocks, w_scale), bias=bias, a2=a2, b2=b2)
+        return fp4_gemm(xq, (w4, w_blocks, w_scale), bias=bias, a2=a2, b2=b2)
+    if check_fp4(w4, w_blocks, w_scale, "fp4_linear weight")[1] != K:
+        raise ValueError("fp4_linear: x is [M,K] and the weight [N,K]")
+    if w4.device != dev:
+        raise ValueError("fp4_linear: x and the weight must be on one device")
+    if K != 1 and x2d.stride(1) != 1:
+        x2d = x2d.contiguous()
+    if bias is not None:
+        if bias.numel() != N or bias.device != dev:
+            raise ValueError("fp4_linear: bias must have N elements on x's device")
+        if bias.dtype != torch.bfloat16 or not bias.is_contiguous():
+            bias = bias.to(torch.bfloat16).contiguous()
+    lib = _lib.load()
+    out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+    nbytes = lib.mh3_fp4_linear_workspace_bytes(M, K)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    rc = _launch(dev, lib.mh3_fp4_linear, x2d.data_ptr(), x2d.stride(0), _FLOAT_CODE[x2d.dtype], M, N, K, w4.data_ptr(),
+                 w_blocks.data_ptr(), w_scale.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), N,
+                 None if ws is None else ws.data_ptr())
+    _lib.check(rc, "mh3_fp4_linear")
+    return out
 
 
 # ---------------------------------------------------------------------------
@@ -836,9 +869,8 @@ def fp4_linear(x2d: torch.Tensor, w4: torch.Tensor, w_blocks: torch.Tensor, w_sc
 _POS_KIND = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
 
-def _bhsd_strides(t: torch.Tensor):
-    """Strides (batch, head, token) of [B,H,S,D] or packed [T,H,D]."""
-    return (t.stride(0), t.stride(1), t.stride(2)) if t.dim() == 4 else (0, t.stride(1), t.stride(0))
+# mh3_rotary_args in one packing: filling it field by field takes as long as the launch
+_ROTARY = struct.Struct("@10i4i4d" + "P3q" * 4 + "P2q")
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axes_dim, theta, interleaved: bool = True,
@@ -848,12 +880,10 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
     ``axes_dim`` and ``theta`` are sequences of one value per axis, positions
     [S, axes] / [B, S, axes] (packed: [T, axes]).  Outputs take the inputs'
     dimension order; ``out_q`` / ``out_k`` may be q / k themselves."""
-    ts = [t for t in (q, k) if t is not None]
-    a = _lib.RotaryArgs()
-    ins, outs = [], []
+    ptrs, outs, copies = [], [], []
     for t, o in ((q, out_q), (k, out_k)):
         if t is None:
-            ins.append(None)
+            ptrs += [0] * 8
             outs.append(None)
             continue
         if t.stride(-1) != 1 and t.shape[-1] != 1:
@@ -864,31 +894,29 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
                 o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
         elif o.shape != t.shape or o.dtype != t.dtype or o.device != t.device or o.stride(-1) != 1:
             raise ValueError("rotary: an output must match its input, with contiguous channels")
-        ins.append(t)
+        s, so = t.stride(), o.stride()
+        if len(s) == 4:
+            ptrs += [t.data_ptr(), s[0], s[1], s[2], o.data_ptr(), so[0], so[1], so[2]]
+        else:  # packed [T, H, D]
+            ptrs += [t.data_ptr(), 0, s[1], s[0], o.data_ptr(), 0, so[1], so[0]]
         outs.append(o)
-    q, k = ins
-    packed = q.dim() == 3
-    a.batch, a.seqlen = (1, q.shape[0]) if packed else (q.shape[0], q.shape[2])
-    a.heads_q, a.heads_k, a.head_dim = q.shape[1], 0 if k is None else k.shape[1], q.shape[-1]
-    a.dtype, a.pos_kind, a.n_axes = _FLOAT_CODE[q.dtype], _POS_KIND[positions.dtype], len(axes_dim)
-    a.interleaved, a.inverse = int(interleaved), int(inverse)
-    for i, (d, th) in enumerate(zip(axes_dim, theta)):
-        a.axes_dim[i], a.theta[i] = int(d), float(th)
+        if t is not q and t is not k:
+            copies.append(t)  # alive until the launch
+    shape = q.shape
+    if len(shape) == 3:
+        batch, seqlen = 1, shape[0]
+    else:
+        batch, seqlen = shape[0], shape[2]
     if positions.stride(-1) != 1 and positions.shape[-1] != 1:
         positions = positions.contiguous()
-    a.positions = positions.data_ptr()
-    a.pos_stride_s = positions.stride(-2)
-    a.pos_stride_b = positions.stride(0) if positions.dim() == 3 and positions.shape[0] > 1 else 0
-    a.q, a.q_out = q.data_ptr(), outs[0].data_ptr()
-    a.q_stride_b, a.q_stride_h, a.q_stride_s = _bhsd_strides(q)
-    a.qo_stride_b, a.qo_stride_h, a.qo_stride_s = _bhsd_strides(outs[0])
-    if k is not None:
-        a.k, a.k_out = k.data_ptr(), outs[1].data_ptr()
-        a.k_stride_b, a.k_stride_h, a.k_stride_s = _bhsd_strides(k)
-        a.ko_stride_b, a.ko_stride_h, a.ko_stride_s = _bhsd_strides(outs[1])
-    lib = _lib.load()
-    with torch.cuda.device(ts[0].device):
-        rc = lib.mh3_rotary(a, _stream(ts[0].device))
+    ps = positions.stride()
+    pos_b = ps[0] if len(ps) == 3 and positions.shape[0] > 1 else 0
+    n = len(axes_dim)
+    a = _lib.RotaryArgs.from_buffer_copy(_ROTARY.pack(
+        batch, seqlen, shape[1], 0 if k is None else k.shape[1], shape[-1], _FLOAT_CODE[q.dtype], _POS_KIND[positions.dtype], n,
+        int(interleaved), int(inverse), *axes_dim, *(0,) * (4 - n), *theta, *(0.0,) * (4 - n),
+        *ptrs[0:4], *ptrs[8:12], *ptrs[4:8], *ptrs[12:16], positions.data_ptr(), pos_b, ps[-2]))
+    rc = _launch(q.device, _lib.load().mh3_rotary, a)
     _lib.check(rc, "mh3_rotary")
     return outs[0], outs[1]
 
@@ -899,54 +927,66 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
 NORM_KINDS = {"none": 0, "rms": 1, "layer": 2}
 
 
+# mh3_block_norm_args in one packing (see _ROTARY)
+_NORM = struct.Struct("@2q6i2fP" + "Pq" * 2 + "P2q2i" * 6 + "3P" + "Pq" * 2 + "9P")
+_NO_MOD = (0, 0, 0, 0, 0)
+
+
 def _rows2d(t: torch.Tensor) -> torch.Tensor:
     """[..., C] as [rows, C] with contiguous channels."""
-    t = t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-def _norm_args(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_norm, eps, alpha, per_token):
-    """The C arguments that the forward and the backward pass share, and the tensors they point into."""
-    a = _lib.BlockNormArgs()
-    keep = [x, y, cu]
-    C = x.shape[-1]
-    S = x.shape[1] if x.dim() == 3 else x.shape[0]
-    a.channels, a.dtype, a.norm, a.y_norm = C, _FLOAT_CODE[x.dtype], norm, y_norm
-    a.groups, a.group_rows = (cu.numel() - 1, 0) if cu is not None else (x.shape[0], S) if x.dim() == 3 else (1, S)
-    if a.groups == 0:
-        a.groups, a.group_rows = 1, 0  # an empty batch
-    a.per_row = int(per_token)
-    a.eps, a.residual_scale = float(eps), float(alpha)
-    if cu is not None:
-        a.cu_seqlens = cu.data_ptr()
-    x2 = _rows2d(x)
-    keep.append(x2)
-    a.rows = x2.shape[0]
-    a.x, a.x_stride = x2.data_ptr(), x2.stride(0)
-    if y is not None:
-        y2 = _rows2d(y)
-        keep.append(y2)
-        a.y, a.y_stride = y2.data_ptr(), y2.stride(0)
-    for name, m in (("gate", gate), ("scale", scale), ("shift", shift)):
+def _norm_args(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_norm, eps, alpha, per_token, r, h, stats,
+               dr=None, dh=None, grads=(None,) * 8, workspace=None):
+    """The C arguments, and the tensors they point into.  ``workspace``: a function of (rows, channels, groups)."""
+    shape = x.shape
+    C = shape[-1]
+    S = shape[1] if len(shape) == 3 else shape[0]
+    groups, group_rows = (cu.numel() - 1, 0) if cu is not None else (shape[0], S) if len(shape) == 3 else (1, S)
+    if groups == 0:
+        groups, group_rows = 1, 0  # an empty batch
+    keep = []
+
+    def rows(t):
+        if t is None:
+            return (0, 0)
+        t = _rows2d(t)
+        keep.append(t)
+        return (t.data_ptr(), t.stride(0))
+
+    def mod(m):
         if m is None:
-            continue
+            return _NO_MOD
         if m.stride(-1) != 1 and C != 1:
             m = m.contiguous()
         keep.append(m)
-        f = getattr(a, name)
-        f.ptr, f.dtype = m.data_ptr(), _FLOAT_CODE[m.dtype]
+        s = m.stride()
         if not per_token:
-            f.stride_group, f.stride_row = m.stride(0), 0
-        elif m.dim() == 3:  # element (b, s): row b S + s
-            f.stride_group, f.stride_row = m.stride(0) - S * m.stride(1), m.stride(1)
+            sg, sr = s[0], 0
+        elif len(s) == 3:  # element (b, s): row b S + s
+            sg, sr = s[0] - S * s[1], s[1]
         else:
-            f.stride_group, f.stride_row = 0, m.stride(0)
-    for name, m in (("weight", weight), ("bias", bias), ("y_weight", y_weight)):
-        if m is not None:
-            m = m.contiguous()
-            keep.append(m)
-            f = getattr(a, name)
-            f.ptr, f.dtype = m.data_ptr(), _FLOAT_CODE[m.dtype]
+            sg, sr = 0, s[0]
+        return (m.data_ptr(), sg, sr, _FLOAT_CODE[m.dtype], 0)
+
+    def chan(v):
+        if v is None:
+            return _NO_MOD
+        v = v.contiguous()
+        keep.append(v)
+        return (v.data_ptr(), 0, 0, _FLOAT_CODE[v.dtype], 0)
+
+    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731  (an empty tensor's is null)
+    nrows = x.numel() // C
+    ws = None if workspace is None else workspace(nrows, C, groups)
+    a = _lib.BlockNormArgs.from_buffer_copy(_NORM.pack(
+        nrows, group_rows, C, groups, _FLOAT_CODE[x.dtype], norm, y_norm, int(per_token), eps, alpha, ptr(cu), *rows(x), *rows(y),
+        *mod(gate), *mod(scale), *mod(shift), *chan(weight), *chan(bias), *chan(y_weight), ptr(r), ptr(h), ptr(stats),
+        *rows(dr), *rows(dh), *map(ptr, grads), ptr(ws)))
+    keep.append(ws)
     return a, keep
 
 
@@ -955,48 +995,31 @@ def block_norm_fwd(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm: i
     """``mh3_block_norm_fwd``: (r, h, stats); r is empty without y, h with norm 0, stats when not wanted.
 
     gate, scale, shift: [groups, C] (any stride), or with ``per_token`` of x's shape."""
-    a, keep = _norm_args(x, y, gate, scale, shift, weight, bias, y_weight, cu, max(norm, 1), y_norm, eps, alpha, per_token)
-    none = x.new_empty(0)
-    r = torch.empty(x.shape, dtype=x.dtype, device=x.device) if y is not None else none
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if norm else none
-    stats = torch.empty((a.rows, 4), dtype=torch.float32, device=x.device) if want_stats else none
-    if y is not None:
-        a.r = r.data_ptr()
-    if norm:
-        a.h = h.data_ptr()
-    if want_stats:
-        a.stats = stats.data_ptr()
-    lib = _lib.load()
-    with torch.cuda.device(x.device):
-        rc = lib.mh3_block_norm_fwd(a, _stream(x.device))
+    r = torch.empty(x.shape, dtype=x.dtype, device=x.device) if y is not None else None
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if norm else None
+    stats = torch.empty((x.numel() // x.shape[-1], 4), dtype=torch.float32, device=x.device) if want_stats else None
+    a, keep = _norm_args(x, y, gate, scale, shift, weight, bias, y_weight, cu, max(norm, 1), y_norm, eps, alpha, per_token, r, h,
+                         stats)
+    rc = _launch(x.device, _lib.load().mh3_block_norm_fwd, a)
     _lib.check(rc, "mh3_block_norm_fwd")
-    return r, h, stats
+    return tuple(x.new_empty(0) if t is None else t for t in (r, h, stats))
 
 
 def block_norm_bwd(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu, stats, norm: int, y_norm: int, eps: float,
                    alpha: float, per_token: bool, want):
     """``mh3_block_norm_bwd``: the gradients of (x, y, gate, scale, shift, weight, bias, y_weight) whose
     entry of ``want`` is true, None for the others; dr or dh may be None."""
-    a, keep = _norm_args(x, y, gate, scale, shift, weight, bias, y_weight, cu, max(norm, 1), y_norm, eps, alpha, per_token)
-    if dr is not None:
-        dr = _rows2d(dr.to(x.dtype))
-        a.dr, a.dr_stride = dr.data_ptr(), dr.stride(0)
-    if dh is not None:
-        dh = _rows2d(dh.to(x.dtype))
-        a.dh, a.dh_stride = dh.data_ptr(), dh.stride(0)
-    names = ("dx", "dy", "dgate", "dscale", "dshift", "dweight", "dbias", "dy_weight")
-    grads = []
-    for name, t, w in zip(names, (x, y, gate, scale, shift, weight, bias, y_weight), want):
-        d = torch.empty(t.shape, dtype=t.dtype, device=t.device) if w and t is not None else None
-        if d is not None and d.numel():
-            setattr(a, name, d.data_ptr())
-        grads.append(d)
+    dr, dh = (None if d is None else d.to(x.dtype) for d in (dr, dh))
+    ts = (x, y, gate, scale, shift, weight, bias, y_weight)
+    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if w and t is not None else None for t, w in zip(ts, want)]
     lib = _lib.load()
-    ws = torch.empty(max(16, int(lib.mh3_block_norm_workspace_bytes(a.rows, a.channels, a.groups))), dtype=torch.uint8,
-                     device=x.device)
-    a.stats, a.workspace = stats.data_ptr(), ws.data_ptr()
-    with torch.cuda.device(x.device):
-        rc = lib.mh3_block_norm_bwd(a, _stream(x.device))
+
+    def workspace(rows, C, groups):
+        nbytes = max(16, lib.mh3_block_norm_workspace_bytes(rows, C, groups))
+        return torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+
+    a, keep = _norm_args(*ts, cu, max(norm, 1), y_norm, eps, alpha, per_token, None, None, stats, dr, dh, grads, workspace)
+    rc = _launch(x.device, lib.mh3_block_norm_bwd, a)
     _lib.check(rc, "mh3_block_norm_bwd")
     return grads
 
