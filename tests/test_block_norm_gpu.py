@@ -380,3 +380,57 @@ def test_compiled():
     d = torch.ones_like(h)
     for a, b in zip(torch.autograd.grad((r, h), (x, y, g), (d, d)), torch.autograd.grad((er, eh), (x, y, g), (d, d))):
         assert torch.equal(a, b)
+
+
+def test_modulation_forms_of_packed_rows():
+    """x [T, C]: one row for all, a row for each token, and both at once; other float types beside x."""
+    from minimaxh3_b200.kernels.block_norm import gated_residual_norm, norm_modulate
+
+    T, C, f = 33, 136, torch.float32
+    x, y = _rand(100, T, C), _rand(101, T, C)
+    one, tok, g = _rand(102, C, dtype=f, scale=0.3), _rand(103, T, C, scale=0.3), _rand(104, 1, C, dtype=torch.float16)
+    per = lambda t: t.expand(T, C)
+    for sc, sh in ((one, one), (one[None], tok), (tok, one), (tok, tok)):
+        c = Case(x, scale=per(sc), shift=per(sh))
+        _close(norm_modulate(x, sc, sh), c.h, c.eh)
+        c = Case(x, y, gate=per(g), scale=per(sc), shift=per(sh), y_norm="layer")
+        r, h = gated_residual_norm(x, y, g, sc, sh, y_norm="layer")
+        _close(r, c.r, c.er, "r")
+        _close(h, c.h, c.eh, "h")
+    # gradients of a token's modulation beside one that all tokens share
+    leaf = lambda t: t.detach().clone().requires_grad_(True)
+    lo, lt, lg = leaf(one), leaf(tok), leaf(g)
+    dr, dh = _rand(105, T, C), _rand(106, T, C)
+    r, h = gated_residual_norm(x, y, lg, lo, lt)
+    go, gt, gg = torch.autograd.grad((r, h), (lo, lt, lg), (dr, dh))
+    c = Case(x, y, gate=per(g), scale=per(one), shift=per(tok))
+    want = c.grads(dr, dh, lambda t: t)
+    _close(gt, *want["shift"])
+    # those of the shared rows are rounded per token to their type before they are added: one half step of it each
+    for got, name in ((go, "scale"), (gg, "gate")):
+        ref, err = want[name]
+        err = (err + torch.finfo(got.dtype).eps / 2 * ref.abs()).sum(0) + T * torch.finfo(got.dtype).eps / 2 * ref.abs().sum(0)
+        _close(got.view(-1), ref.sum(0), err, name)
+    # an 8-wide row that no vector fits, and strides of the modulation
+    wide = _rand(107, 2, 3, 4 * 24 + 1, dtype=f)
+    c = Case(x.view(1, T, C)[:, :3, :24].expand(2, 3, 24), scale=wide[..., 1:25], shift=wide[..., 25:49])
+    _close(norm_modulate(x.view(1, T, C)[:, :3, :24].expand(2, 3, 24), wide[..., 1:25], wide[..., 25:49]), c.h, c.eh)
+
+
+def test_long_and_short_sequences_share_a_stage():
+    """Sequences that end inside the rows a CTA takes at once, and many empty ones."""
+    from minimaxh3_b200.kernels.block_norm import norm_modulate
+
+    lens = [1, 0, 0, 2, 1, 3, 700, 1, 1, 0, 5000, 2, 1]
+    n, T, C, f = len(lens), sum(lens), 64, torch.float32
+    cu = torch.tensor([sum(lens[:i]) for i in range(n + 1)], dtype=torch.int32, device=DEV)
+    rep = torch.repeat_interleave(torch.arange(n), torch.tensor(lens)).to(DEV)
+    x, sc = _rand(110, T, C).requires_grad_(True), _rand(111, n, C, dtype=f).requires_grad_(True)
+    h = norm_modulate(x, sc, cu_seqlens=cu)
+    c = Case(x, scale=sc, rows_of=lambda t: t[rep])
+    _close(h, c.h, c.eh)
+    dh = _rand(112, T, C)
+    dx, ds = torch.autograd.grad(h, (x, sc), dh)
+    want = c.grads(None, dh, lambda t: torch.zeros(n, C, dtype=t.dtype, device=DEV).index_add_(0, rep, t))
+    _close(dx, *want["x"], "x")
+    _close(ds, *want["scale"], "scale")

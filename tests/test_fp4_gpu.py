@@ -210,6 +210,25 @@ def test_linear_types_empty_and_nan_rows():
     assert fp4_linear(torch.empty(0, 96, device=DEV), *w).shape == (0, 64)
 
 
+def test_linear_of_few_rows_strides_and_outputs():
+    """The one-launch form (one and two rows) against the two steps it stands for, on rows that vectors fit or not."""
+    from minimaxh3_b200 import ops
+    from minimaxh3_b200.kernels.fp4_linear import fp4_linear, fp4_matmul, quantize_fp4
+
+    for K, N in ((32, 8), (96, 40), (5120, 264), (40000, 24), (200000, 8)):
+        w = quantize_fp4(_rand(54, N, K, scale=0.05).to(DEV))
+        for dtype in (torch.bfloat16, torch.float32):
+            wide = _rand(55, 3, K + 9, dtype=dtype).to(DEV)
+            for x in (wide[:1, 1:K + 1], wide[:2, 8:K + 8], wide[1:, 1:K + 1], wide[:3, :K]):
+                got = fp4_linear(x, *w)
+                assert torch.equal(got, fp4_matmul(quantize_fp4(x), w))
+    for M in (2, 12, 300):  # a strided output, its other elements left as they were
+        a, b, av, bv = _pair(M, 264, 96)
+        out = torch.full((M, 280), 7.0, dtype=torch.bfloat16, device=DEV)
+        ops.fp4_gemm(a, b, out=out[:, :264])
+        assert torch.equal(out[:, :264], fp4_matmul(a, b)) and bool((out[:, 264:] == 7).all())
+
+
 def test_output_offsets_past_32_bits():
     from minimaxh3_b200.kernels.fp4_linear import fp4_matmul, quantize_fp4
 
