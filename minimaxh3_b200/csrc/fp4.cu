@@ -153,12 +153,9 @@ __global__ void __launch_bounds__(kMaxThreads) quantize_stream_kernel(const T* _
           if (finite) {
             uint4 u[W];
             load(i, u);
-            T t[16];
-            float v[16];
-            memcpy(t, u, sizeof(t));
-#pragma unroll
-            for (int k = 0; k < 16; ++k) v[k] = to_float(t[k]);
-            s8 = round_block(v, own[i], pow2f(-e), code);  // e in [-100, 117]
+            float2 v[8];
+            pairs16<T>(u, v);
+            s8 = round_block(v, own[i], e, code);
           }
           *reinterpret_cast<uint2*>(xo) = code;
           if (b == 0) scale[row0 + 32 * i] = finite ? pow2f(e) : __uint_as_float(0x7fffffffu);
@@ -192,7 +189,7 @@ __global__ void __launch_bounds__(kMaxThreads) quantize_kernel(const T* __restri
   const int nb = K / 16, nk64 = (K + 63) / 64;
   const T* xp = x + row * stride;
   const bool live = row < M;
-  float v[16];
+  float2 v[8];
   uint32_t top = 0;
   int turn = 0;
   if (live)
@@ -210,7 +207,7 @@ __global__ void __launch_bounds__(kMaxThreads) quantize_kernel(const T* __restri
     if (b < nb && live) {
       if (finite) {
         load16(xp + (long long)b * 16, v, vec != 0);
-        s8 = round_block(v, absmax16(v), pow2f(-e), code);
+        s8 = round_block(v, absmax16(v), e, code);
       }
       *reinterpret_cast<uint2*>(x4 + row * (K / 2) + (long long)b * 8) = code;
     }

@@ -22,7 +22,7 @@ __device__ __forceinline__ float to_float(T v) {
 }
 
 template <typename T>
-__device__ __forceinline__ void load16(const T* p, float (&v)[16], bool vec) {
+__device__ __forceinline__ void load16(const T* p, float2 (&v)[8], bool vec) {
   constexpr int NV = 16 * sizeof(T) / 16;
   T e[16];
   if (vec) {
@@ -35,7 +35,7 @@ __device__ __forceinline__ void load16(const T* p, float (&v)[16], bool vec) {
     for (int i = 0; i < 16; ++i) e[i] = p[i];
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = to_float(e[i]);
+  for (int i = 0; i < 8; ++i) v[i] = make_float2(to_float(e[2 * i]), to_float(e[2 * i + 1]));
 }
 
 __device__ __forceinline__ float rcp_approx(float x) {
@@ -44,12 +44,14 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return y;
 }
 
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
 // Largest magnitude as the integer of its bits: an infinity or NaN orders above
 // every finite value, so none is lost.
-__device__ __forceinline__ uint32_t absmax16(const float (&v)[16]) {
+__device__ __forceinline__ uint32_t absmax16(const float2 (&v)[8]) {
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  for (int i = 0; i < 8; ++i) m = max(m, max(__float_as_uint(v[i].x) & 0x7fffffffu, __float_as_uint(v[i].y) & 0x7fffffffu));
   return m;
 }
 
@@ -79,36 +81,51 @@ __device__ __forceinline__ int row_exponent(uint32_t bits) {
   return max(e, -100);
 }
 
-__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 __device__ __forceinline__ long long block_offset(long long row, int b, int nk64) {
   return ((row >> 7) * nk64 + (b >> 2)) * 512 + (row & 31) * 16 + ((row & 127) >> 5) * 4 + (b & 3);
 }
 
 // One block: its scale byte and 16 codes, from its absmax and the row's exponent.
-// The quotients are div_by in packed pairs, which halves their issue slots; an
-// approximate reciprocal serves: where the true quotient is a border it has a few
-// bits, the remainder is exact, and the corrected quotient lands on it; where it is
-// not, 16-bit input is at least 2^-13 of it away.
-__device__ __forceinline__ uint32_t round_block(const float (&v)[16], uint32_t top, float inv, uint2& code) {
+// The quotients x / (block scale) are div_by in packed pairs, which halves their issue
+// slots; an approximate reciprocal serves: where the true quotient is a border it has
+// a few bits, the remainder is exact, and the corrected quotient lands on it; where it
+// is not, 16-bit input is at least 2^-13 of it away.  Divisor and reciprocal carry the
+// row's power of two; rows so small that the remainder could leave the normal range
+// (e < -60) are first scaled by 2^64.
+__device__ __forceinline__ uint32_t round_block(const float2 (&x)[8], uint32_t top, int e, uint2& code) {
   // e4m3 of absmax / (6 scale): the division by 6 is the only rounding before it
-  const float raw = div_by(__uint_as_float(top) * inv, 6.0f, 1.0f / 6.0f);
+  const float raw = div_by(__uint_as_float(top) * pow2f(-e), 6.0f, 1.0f / 6.0f);
   const uint32_t s8 = cvt_e4m3x2_f32(0.0f, raw) & 0xffu;
   if (s8 != 0) {
-    const float s = e4m3_value(s8), r = rcp_approx(s);
-    const float2 r2 = both(r), ns2 = both(-s), inv2 = both(inv);
+    const float s = e4m3_value(s8);
+    const bool tiny = e < -60;
+    const int f = tiny ? e + 64 : e;  // [-36, 117]
+    const float2 d2 = both(-s * pow2f(f)), r2 = both(rcp_approx(s) * pow2f(-f));
     float q[16];
 #pragma unroll
-    for (int i = 0; i < 16; i += 2) {
-      const float2 x = fmul2(make_float2(v[i], v[i + 1]), inv2);
-      const float2 a = fmul2(x, r2);
-      const float2 d = ffma2(ffma2(ns2, a, x), r2, a);
-      q[i] = d.x;
-      q[i + 1] = d.y;
+    for (int i = 0; i < 8; ++i) {
+      const float2 v = tiny ? fmul2(x[i], both(0x1p64f)) : x[i];
+      const float2 a = fmul2(v, r2);
+      const float2 c = ffma2(ffma2(d2, a, v), r2, a);
+      q[2 * i] = c.x;
+      q[2 * i + 1] = c.y;
     }
     code = make_uint2(e2m1x8(q), e2m1x8(q + 8));
   }
   return s8;
+}
+
+// A block as loaded, in pairs.
+template <typename T>
+__device__ __forceinline__ void pairs16(const uint4 (&u)[sizeof(T)], float2 (&v)[8]) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(u);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (sizeof(T) == 4) v[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    else if constexpr (std::is_same<T, __half>::value) v[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    else v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  }
 }
 
 // absmax16 of a block as loaded: 16-bit types compare two magnitudes at a time as

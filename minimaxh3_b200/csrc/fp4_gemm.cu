@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(kWarps * 32) small_kernel(const __grid_constan
 #pragma unroll
       for (int m = 0; m < kFusedRows; ++m)
         if (m < p.M) {
-          float v[16];
+          float2 v[8];
           fp4::load16(x + m * p.x_s + b * 16, v, vec);
           most[m] = max(most[m], fp4::absmax16(v));
         }
@@ -458,9 +458,9 @@ __global__ void __launch_bounds__(kWarps * 32) small_kernel(const __grid_constan
       uint2 code = make_uint2(0, 0);
       uint32_t s8 = 0;
       if (top[m] < 0x7f800000u) {
-        float v[16];
+        float2 v[8];
         fp4::load16(x + m * p.x_s + b * 16, v, vec);
-        s8 = fp4::round_block(v, fp4::absmax16(v), fp4::pow2f(-fp4::row_exponent(top[m])), code);
+        s8 = fp4::round_block(v, fp4::absmax16(v), fp4::row_exponent(top[m]), code);
       }
       reinterpret_cast<uint2*>(own)[i] = code;
       const_cast<uint8_t*>(xs)[i] = (uint8_t)s8;

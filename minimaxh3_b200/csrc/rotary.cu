@@ -15,10 +15,12 @@
 // double operations and the sincospi are 1/80th of a vector's work at 40 heads.
 //
 // Bound: HBM.  Q and K are read and written once by 16-byte vectors.  A thread
-// keeps the same channels for every (token, head) row it visits and steps through
-// the heads by a fixed stride, so a row costs two pointer increments, and a token
-// one read of its angles.  Its rows stream through its own part of a ring in shared
-// memory (cp.async, no barrier); the first are on their way before the angles are computed.
+// keeps the same channels of the same one to four heads for every token of its
+// CTA, so a vector costs two pointer increments and about forty instructions in
+// all (with the head looked up per vector it was 160, and the kernel issue-bound:
+// 326 us at 32760 tokens x 80 heads x 128).  Its vectors stream through its own part
+// of a ring in shared memory (cp.async, no barrier); the first tokens are on their
+// way before the angles are computed.
 #include <math.h>
 
 #include <algorithm>
@@ -30,11 +32,11 @@
 namespace mh3 {
 namespace rotary {
 
-constexpr int kThreads = 256;    // of the scalar kernel; the most of the streaming one is kMaxThreads
-constexpr int kMaxThreads = 384;
-constexpr int kMaxPairs = 128;  // head_dim <= 256
-constexpr int kMaxTokens = 16;  // tokens per CTA
-constexpr int kDepth = 8;       // 16-byte vectors of a thread in the ring
+constexpr int kThreads = 256;     // of the scalar kernel
+constexpr int kMaxThreads = 384;  // of the streaming kernel
+constexpr int kMaxPairs = 128;    // head_dim <= 256
+constexpr int kMaxTokens = 16;    // tokens per CTA
+constexpr int kDepth = 4;         // tokens in the ring
 
 struct Params {
   const char *q, *k;
@@ -42,7 +44,8 @@ struct Params {
   long long q_sb, q_sh, q_ss, k_sb, k_sh, k_ss;      // element strides
   long long qo_sb, qo_sh, qo_ss, ko_sb, ko_sh, ko_ss;
   long long tokens;  // batch * seqlen
-  int S, Hq, Hk, D, R2, tile, side;
+  int S, Hq, Hk, D, R2, tile;
+  int side;  // rows (heads of Q, then of K) that a CTA visits side by side
   const void* pos;
   int pos_kind;  // 0 int32, 1 int64, 2 float
   long long pos_sb, pos_ss;
@@ -64,10 +67,16 @@ __device__ __forceinline__ T from_f(float v) {
   else return __float2bfloat16_rn(v);
 }
 
-template <typename T, int V>
-struct __align__(sizeof(T) * V) Vec {
-  T e[V];
-};
+// Batch item and place of a token.
+__device__ __forceinline__ long long split(const Params& p, long long tok, int& s) {
+  if (tok < p.S) {
+    s = (int)tok;
+    return 0;
+  }
+  const long long b = p.tokens <= 0xffffffffll ? (long long)((unsigned)tok / (unsigned)p.S) : tok / p.S;
+  s = (int)(tok - b * p.S);
+  return b;
+}
 
 // cos and sin of the CTA's tokens, [nt][npair] each; pairs past R/2 have the angle 0.
 __device__ __forceinline__ void angles(const Params& p, float* cos_, float* sin_, long long t0, int nt, int npair) {
@@ -78,8 +87,8 @@ __device__ __forceinline__ void angles(const Params& p, float* cos_, float* sin_
       sin_[i] = 0.0f;
       continue;
     }
-    const long long tok = t0 + t;
-    const long long b = tok / p.S, s = tok - b * p.S;
+    int s;
+    const long long b = split(p, t0 + t, s);
     const long long at = b * p.pos_sb + s * p.pos_ss + p.axis[j];
     const double pos = p.pos_kind == 0   ? (double)static_cast<const int*>(p.pos)[at]
                        : p.pos_kind == 1 ? (double)static_cast<const long long*>(p.pos)[at]
@@ -93,25 +102,6 @@ __device__ __forceinline__ void angles(const Params& p, float* cos_, float* sin_
   }
 }
 
-// Addresses of head 0 of the CTA's tokens.
-struct Token {
-  const char *q, *k;
-  char *qo, *ko;
-};
-__device__ __forceinline__ void token_table(const Params& p, Token* tab, long long t0, int nt, int es) {
-  if ((int)threadIdx.x < nt) {
-    const long long tok = t0 + threadIdx.x;
-    const long long b = tok / p.S, s = tok - b * p.S;
-    Token t;
-    t.q = p.q + (b * p.q_sb + s * p.q_ss) * es;
-    t.k = p.k + (b * p.k_sb + s * p.k_ss) * es;
-    t.qo = p.qo + (b * p.qo_sb + s * p.qo_ss) * es;
-    t.ko = p.ko + (b * p.ko_sb + s * p.ko_ss) * es;
-    tab[threadIdx.x] = t;
-  }
-  if ((int)threadIdx.x == nt) tab[nt] = Token{};  // read, not followed, past the last token
-}
-
 template <typename T>
 __device__ __forceinline__ void rotate(T& x0, T& x1, float2 a) {
   const float v0 = to_f(x0), v1 = to_f(x1);
@@ -119,129 +109,167 @@ __device__ __forceinline__ void rotate(T& x0, T& x1, float2 a) {
   x1 = from_f<T>(fmaf(v1, a.x, __fmul_rn(v0, a.y)));
 }
 
-// A thread's way through its rows: tokens t, Q's then K's heads h, h + side, ..
-// ``P``: char of the inputs or of the outputs.
-template <typename P>
-struct Cursor {
-  P* at;
-  int t, h;
-  bool k;
+// Eight or four values of a vector as pairs (2i, 2i+1), and back.
+template <typename T>
+struct Pairs {
+  static constexpr int N = 8 / sizeof(T);
+  float2 e[N];
+  __device__ __forceinline__ explicit Pairs(const uint4& u) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (sizeof(T) == 4) e[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+      else if constexpr (std::is_same<T, __half>::value) e[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      else e[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    }
+  }
+  __device__ __forceinline__ uint4 vec() const {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        w[2 * i] = __float_as_uint(e[i].x);
+        w[2 * i + 1] = __float_as_uint(e[i].y);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(e[i].x, e[i].y);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(e[i].x, e[i].y);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
 };
 
 // The units of a row: one 16-byte vector when INTER (pairs past R/2 pass), and when
-// not the two vectors of V pairs, or V passing channels.
-template <typename T, bool INTER>
+// not the two vectors of V pairs, or V passing channels.  A CTA: ``side`` x M rows of
+// ``tile`` tokens.
+template <typename T, bool INTER, int M>
 __global__ void __launch_bounds__(kMaxThreads) stream_kernel(const __grid_constant__ Params p) {
-  constexpr int V = 16 / sizeof(T);
+  constexpr int V = 16 / sizeof(T), ES = sizeof(T);
   constexpr int W = INTER ? 1 : 2;       // vectors of a unit
-  constexpr int D = kDepth / W;          // rows of a thread in the ring
   constexpr int NP = INTER ? V / 2 : V;  // pairs of a unit
   extern __shared__ uint4 smem[];
-  uint4* ring = smem + threadIdx.x;  // [D][W][threads]
+  uint4* ring = smem + threadIdx.x;  // [kDepth][M][W][threads]
   const int nthr = blockDim.x;
-  float* cos_ = reinterpret_cast<float*>(smem + kDepth * nthr);
-  __shared__ Token tab[kMaxTokens + 1];
+  float* cos_ = reinterpret_cast<float*>(smem + kDepth * M * W * nthr);
   const int npair = INTER ? p.D / 2 : p.R2;
   float* sin_ = cos_ + p.tile * npair;
   const long long t0 = (long long)blockIdx.x * p.tile;
   const int nt = (int)min((long long)p.tile, p.tokens - t0);
   const int rot_units = INTER ? p.D / V : p.R2 / V;
   const int units = INTER ? rot_units : rot_units + (p.D - 2 * p.R2) / V;
-  const int side = p.side;  // rows visited side by side
   const int row0 = threadIdx.x / units, u = threadIdx.x - row0 * units;
   const bool rot = u < rot_units;
   const int c0 = rot ? u * V : 2 * p.R2 + (u - rot_units) * V;
-  const bool has_q = row0 < p.Hq && row0 < side, has_k = row0 < p.Hk && row0 < side;
-  // the thread's first Q and K rows, and a step of ``side`` heads, in bytes
-  constexpr int ES = sizeof(T);
-  const long long q0 = (row0 * p.q_sh + c0) * ES, k0 = (row0 * p.k_sh + c0) * ES;
-  const long long qo0 = (row0 * p.qo_sh + c0) * ES, ko0 = (row0 * p.ko_sh + c0) * ES;
-  const long long qs = side * p.q_sh * ES, ks = side * p.k_sh * ES, qos = side * p.qo_sh * ES, kos = side * p.ko_sh * ES;
-  token_table(p, tab, t0, nt, ES);
-  __syncthreads();
-  auto enter = [&](auto& c) {  // the first row of c's token and tensor
-    c.h = row0;
-    if constexpr (std::is_same<std::decay_t<decltype(c)>, Cursor<const char>>::value)
-      c.at = c.k ? tab[c.t].k + k0 : tab[c.t].q + q0;
-    else
-      c.at = c.k ? tab[c.t].ko + ko0 : tab[c.t].qo + qo0;
-  };
-  auto advance = [&](auto& c, long long qstep, long long kstep) {
-    c.h += side;
-    c.at += c.k ? kstep : qstep;
-    if (c.h >= (c.k ? p.Hk : p.Hq)) {
-      if (c.k || !has_k) ++c.t;
-      c.k = has_q ? (has_k && !c.k) : true;
-      enter(c);  // past the last token: a row of the table that is not followed
+  int s_in;
+  const long long b0 = split(p, t0, s_in);
+  int s_out = s_in;
+  const char* in[M];
+  char* out[M];
+  unsigned own = 0, isq = 0;  // bit j: the thread has row j; it is one of Q's
+#pragma unroll
+  for (int j = 0; j < M; ++j) {
+    const int r = blockIdx.y * (M * p.side) + j * p.side + row0;
+    const int h = r < p.Hq ? r : r - p.Hq;
+    if (r < p.Hq) {
+      isq |= 1u << j;
+      in[j] = p.q + (b0 * p.q_sb + s_in * p.q_ss + h * p.q_sh + c0) * ES;
+      out[j] = p.qo + (b0 * p.qo_sb + s_in * p.qo_ss + h * p.qo_sh + c0) * ES;
+    } else {
+      in[j] = p.k + (b0 * p.k_sb + s_in * p.k_ss + h * p.k_sh + c0) * ES;
+      out[j] = p.ko + (b0 * p.ko_sb + s_in * p.ko_ss + h * p.ko_sh + c0) * ES;
     }
-  };
-  const int per_q = has_q ? (p.Hq - row0 + side - 1) / side : 0, per_k = has_k ? (p.Hk - row0 + side - 1) / side : 0;
-  const int n = nt * (per_q + per_k);  // the thread's rows
-  Cursor<const char> in{nullptr, 0, 0, !has_q};
-  Cursor<char> out{nullptr, 0, 0, !has_q};
-  enter(in);
-  enter(out);
-  int issued = 0;
-  auto issue = [&](int slot) {
-    if (issued < n) {
-      uint4* dst = ring + slot * W * nthr;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(in.at) : "memory");
-      if (!INTER && rot)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst + nthr)), "l"(in.at + p.R2 * ES) : "memory");
-      ++issued;
-      advance(in, qs, ks);
+    if (row0 < p.side && r < p.Hq + p.Hk) own |= 1u << j;
+  }
+  int ahead = 0;
+  auto issue = [&](int slot) {  // the next token's vectors into the ring
+    if (ahead < nt) {
+      ++ahead;
+      const bool wrap = ++s_in == p.S;
+      if (wrap) s_in = 0;
+#pragma unroll
+      for (int j = 0; j < M; ++j) {
+        const bool mine = own >> j & 1u, q = isq >> j & 1u;
+        uint4* dst = ring + (slot * M + j) * W * nthr;
+        if (mine) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(in[j]) : "memory");
+          if (!INTER && rot)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst + nthr)), "l"(in[j] + p.R2 * ES) : "memory");
+        }
+        in[j] += (q ? p.q_ss : p.k_ss) * ES;
+        if (wrap) in[j] += (q ? p.q_sb - p.S * p.q_ss : p.k_sb - p.S * p.k_ss) * ES;  // the next batch item
+      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int j = 0; j < D - 1; ++j) issue(j);
+  for (int j = 0; j < kDepth - 1; ++j) issue(j);
   angles(p, cos_, sin_, t0, nt, npair);
   __syncthreads();
-  float2 cs[NP / 2], sn[NP / 2];  // of the current token's pairs 2 i, 2 i + 1 of the unit
   const int whole = INTER ? max(0, min(NP, p.R2 - u * NP)) : (rot ? NP : 0);  // rotated pairs of the unit
-  int slot = 0, token = -1;
-  for (int i = 0; i < n; ++i) {
-    issue(slot == 0 ? D - 1 : slot - 1);
-    asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
-    if (out.t != token) {
-      token = out.t;
-      if (whole)
-#pragma unroll
-        for (int q = 0; q < NP / 2; ++q) {
-          cs[q] = *reinterpret_cast<const float2*>(cos_ + token * npair + u * NP + 2 * q);
-          sn[q] = *reinterpret_cast<const float2*>(sin_ + token * npair + u * NP + 2 * q);
-        }
-    }
-    const uint4* src = ring + slot * W * nthr;
-    Vec<T, V> x = *reinterpret_cast<const Vec<T, V>*>(src), y;
-    if (!INTER && rot) y = *reinterpret_cast<const Vec<T, V>*>(src + nthr);
+  const float *cp = cos_ + u * NP, *sp = sin_ + u * NP;
+  int slot = 0;
+  for (int t = 0; t < nt; ++t, cp += npair, sp += npair) {
+    issue(slot == 0 ? kDepth - 1 : slot - 1);
+    float2 cs[NP / 2], sn[NP / 2], ns[NP / 2];  // of pairs 2i and 2i + 1
     if (whole) {
-      const Vec<T, V> keep = x;
 #pragma unroll
-      for (int q = 0; q < NP / 2; ++q) {
-        // pairs 2 q and 2 q + 1, in packed f32
-        T &a0 = INTER ? x.e[4 * q] : x.e[2 * q], &a1 = INTER ? x.e[4 * q + 2] : x.e[2 * q + 1];
-        T &b0 = INTER ? x.e[4 * q + 1] : y.e[2 * q], &b1 = INTER ? x.e[4 * q + 3] : y.e[2 * q + 1];
-        const float2 a = make_float2(to_f(a0), to_f(a1)), b = make_float2(to_f(b0), to_f(b1));
-        const float2 ms = make_float2(-sn[q].x, -sn[q].y);
-        const float2 r = ffma2(b, ms, fmul2(a, cs[q])), s = ffma2(b, cs[q], fmul2(a, sn[q]));
-        a0 = from_f<T>(r.x);
-        a1 = from_f<T>(r.y);
-        b0 = from_f<T>(s.x);
-        b1 = from_f<T>(s.y);
+      for (int i = 0; i < NP / 2; ++i) {
+        cs[i] = *reinterpret_cast<const float2*>(cp + 2 * i);
+        sn[i] = *reinterpret_cast<const float2*>(sp + 2 * i);
+        ns[i] = make_float2(-sn[i].x, -sn[i].y);
       }
-      if (INTER && whole < NP)  // the unit where the rotated channels end: its others pass untouched
-#pragma unroll
-        for (int q = 0; q < NP; ++q)
-          if (q >= whole) {
-            x.e[2 * q] = keep.e[2 * q];
-            x.e[2 * q + 1] = keep.e[2 * q + 1];
-          }
     }
-    *reinterpret_cast<Vec<T, V>*>(out.at) = x;
-    if (!INTER && rot) *reinterpret_cast<Vec<T, V>*>(out.at + p.R2 * ES) = y;
-    advance(out, qos, kos);
-    slot = slot + 1 == D ? 0 : slot + 1;
+    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+    const bool wrap = ++s_out == p.S;
+    if (wrap) s_out = 0;
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+      const bool q = isq >> j & 1u;
+      if (own >> j & 1u) {
+        const uint4* src = ring + (slot * M + j) * W * nthr;
+        uint4 x = src[0];
+        if (whole) {
+          if constexpr (INTER) {
+            Pairs<T> v(x);
+#pragma unroll
+            for (int i = 0; i < NP / 2; ++i) {  // the first and second channels of two pairs, side by side
+              const float2 a = make_float2(v.e[2 * i].x, v.e[2 * i + 1].x), b = make_float2(v.e[2 * i].y, v.e[2 * i + 1].y);
+              const float2 r = ffma2(b, ns[i], fmul2(a, cs[i])), w = ffma2(b, cs[i], fmul2(a, sn[i]));
+              v.e[2 * i] = make_float2(r.x, w.x);
+              v.e[2 * i + 1] = make_float2(r.y, w.y);
+            }
+            const uint4 y = v.vec();
+            if (whole == NP) {
+              x = y;
+            } else {  // the unit where the rotated channels end: its others pass untouched
+              constexpr int WP = ES == 4 ? 2 : 1;  // words of a pair
+              const uint32_t old[4] = {x.x, x.y, x.z, x.w}, now[4] = {y.x, y.y, y.z, y.w};
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) w[i] = i / WP < whole ? now[i] : old[i];
+              x = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else {
+            Pairs<T> a(x), b(src[nthr]);
+#pragma unroll
+            for (int i = 0; i < NP / 2; ++i) {
+              const float2 r = ffma2(b.e[i], ns[i], fmul2(a.e[i], cs[i]));
+              b.e[i] = ffma2(b.e[i], cs[i], fmul2(a.e[i], sn[i]));
+              a.e[i] = r;
+            }
+            x = a.vec();
+            *reinterpret_cast<uint4*>(out[j] + p.R2 * ES) = b.vec();
+          }
+        }
+        *reinterpret_cast<uint4*>(out[j]) = x;
+      }
+      out[j] += (q ? p.qo_ss : p.ko_ss) * ES;
+      if (wrap) out[j] += (q ? p.qo_sb - p.S * p.qo_ss : p.ko_sb - p.S * p.ko_ss) * ES;
+    }
+    slot = slot + 1 == kDepth ? 0 : slot + 1;
   }
 }
 
@@ -251,10 +279,8 @@ __global__ void __launch_bounds__(kThreads) scalar_kernel(const __grid_constant_
   extern __shared__ uint4 smem[];
   float* cos_ = reinterpret_cast<float*>(smem);
   float* sin_ = cos_ + p.tile * p.R2;
-  __shared__ Token tab[kMaxTokens + 1];
   const long long t0 = (long long)blockIdx.x * p.tile;
   const int nt = (int)min((long long)p.tile, p.tokens - t0);
-  token_table(p, tab, t0, nt, sizeof(T));
   angles(p, cos_, sin_, t0, nt, p.R2);
   __syncthreads();
   const int units = p.D - p.R2;
@@ -265,8 +291,10 @@ __global__ void __launch_bounds__(kThreads) scalar_kernel(const __grid_constant_
     int h = row - t * (p.Hq + p.Hk);
     const bool isq = h < p.Hq;
     h -= isq ? 0 : p.Hq;
-    const T* src = reinterpret_cast<const T*>(isq ? tab[t].q : tab[t].k) + h * (isq ? p.q_sh : p.k_sh);
-    T* to = reinterpret_cast<T*>(isq ? tab[t].qo : tab[t].ko) + h * (isq ? p.qo_sh : p.ko_sh);
+    int sq;
+    const long long b = split(p, t0 + t, sq);
+    const T* src = reinterpret_cast<const T*>(isq ? p.q : p.k) + (isq ? b * p.q_sb + sq * p.q_ss + h * p.q_sh : b * p.k_sb + sq * p.k_ss + h * p.k_sh);
+    T* to = reinterpret_cast<T*>(isq ? p.qo : p.ko) + (isq ? b * p.qo_sb + sq * p.qo_ss + h * p.qo_sh : b * p.ko_sb + sq * p.ko_ss + h * p.ko_sh);
     if (u < p.R2) {
       const int c0 = inter ? 2 * u : u, c1 = inter ? 2 * u + 1 : u + p.R2;
       T x0 = src[c0], x1 = src[c1];
@@ -286,15 +314,23 @@ static cudaError_t launch(const Params& p, bool vec, bool inter, cudaStream_t st
     scalar_kernel<T><<<grid, kThreads, (size_t)p.tile * p.R2 * sizeof(float2), st>>>(p, inter ? 1 : 0);
     return cudaGetLastError();
   }
+  // Rows per thread: the fewest of 1, 2 and 4 with which the CTA's threads hold all heads
+  // (half as many when a unit is two vectors); more heads than that in further CTAs.
   constexpr int V = 16 / sizeof(T);
-  const int threads = (p.side * (inter ? p.D / V : (p.D - p.R2) / V) + 31) / 32 * 32;
-  const size_t smem = (size_t)kDepth * threads * 16 + (size_t)p.tile * (inter ? p.D / 2 : p.R2) * sizeof(float2);
-  auto kern = inter ? stream_kernel<T, true> : stream_kernel<T, false>;
-  if (smem > 40 * 1024) {  // with the static part, past the 48 KB default
+  const int units = inter ? p.D / V : (p.D - p.R2) / V, rows = p.Hq + p.Hk, most = inter ? 4 : 2;
+  int m = 1;
+  while (m < most && (rows + m - 1) / m * units > kMaxThreads) m *= 2;
+  Params q = p;
+  q.side = std::min((rows + m - 1) / m, kMaxThreads / units);
+  const int threads = (q.side * units + 31) / 32 * 32;
+  const size_t smem = (size_t)kDepth * m * (inter ? 1 : 2) * threads * 16 + (size_t)p.tile * (inter ? p.D / 2 : p.R2) * sizeof(float2);
+  auto kern = inter ? (m == 1 ? stream_kernel<T, true, 1> : m == 2 ? stream_kernel<T, true, 2> : stream_kernel<T, true, 4>)
+                    : (m == 1 ? stream_kernel<T, false, 1> : stream_kernel<T, false, 2>);
+  if (smem > 40 * 1024) {  // past the 48 KB default
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
   }
-  kern<<<grid, threads, smem, st>>>(p);
+  kern<<<dim3(grid, (unsigned)((rows + m * q.side - 1) / (m * q.side))), threads, smem, st>>>(q);
   return cudaGetLastError();
 }
 
@@ -361,29 +397,12 @@ extern "C" int mh3_rotary(const mh3_rotary_args* a, void* stream) {
   p.pos_sb = a->pos_stride_b;
   p.pos_ss = a->pos_stride_s;
   p.sign = a->inverse ? -1.0f : 1.0f;
-  // Tokens per CTA: enough for 80 KB of Q and K (five stages of the ring), while
-  // 148 SMs still get four CTAs each.
+  // Tokens per CTA: up to 160 KB of Q and K (two rounds of the ring), while 148 SMs
+  // still get four CTAs each.
   const long long token_bytes = ((long long)a->heads_q + a->heads_k) * a->head_dim * es;
   int tile = 1;
-  while (tile < rotary::kMaxTokens && tile * token_bytes < 81920 && tokens / (2 * tile) >= 148 * 4) tile *= 2;
+  while (tile < rotary::kMaxTokens && tile * token_bytes < 163840 && tokens / (2 * tile) >= 148 * 4) tile *= 2;
   p.tile = tile;
-  // Heads side by side: of the counts that fill 192 to 384 threads (fewer where a row
-  // has too few heads), the one that leaves the fewest lanes without a row - 20 for
-  // 40 heads of 128 channels.
-  const int units = inter ? a->head_dim / V : (a->head_dim - r2) / V;
-  p.side = 1;
-  if (vec) {
-    const int most = std::max(1, std::min(rotary::kMaxThreads / units, std::max(a->heads_q, a->heads_k)));
-    const int least = std::max(1, std::min(192 / units, most));
-    long long best = -1;
-    for (int side = most; side >= least; --side) {
-      const long long lost = (side - a->heads_q % side) % side + (side - a->heads_k % side) % side;
-      if (best < 0 || lost < best) {
-        best = lost;
-        p.side = side;
-      }
-    }
-  }
   if ((tokens + tile - 1) / tile > 0x7fffffffLL) return fail(MH3_ERR_TOO_LARGE, "mh3_rotary: too many tokens");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const cudaError_t e = a->dtype == MH3_DTYPE_BF16  ? rotary::launch<__nv_bfloat16>(p, vec, inter, st)
