@@ -569,11 +569,13 @@ __device__ __forceinline__ void cp_wait() {
 // copy and store of a warp is one run of 512 bytes, in 16 and in 32 bits.  The
 // arithmetic is in packed f32 pairs, which halves its issue slots: these kernels
 // were bound by instruction issue before they were bound by HBM.
-template <typename T, int CH>
+// FIT: the threads' channels are the row's, so no piece is past it.
+template <typename T, int CH, bool FIT>
 struct Lay {
   static constexpr int E = 16 / sizeof(T);
   static constexpr int P = CH / E;
   static __device__ __forceinline__ int at(int q) { return (q * (int)blockDim.x + (int)threadIdx.x) * E; }
+  static __device__ __forceinline__ bool in(int q, int C) { return FIT || at(q) < C; }
 };
 template <int CH>
 struct Vals {
@@ -626,19 +628,19 @@ __device__ __forceinline__ void slots_get(const float4* s, Vals<CH>& v) {
 }
 template <typename T, int CH>
 __device__ __forceinline__ void mods(const void* p, int dt, long long at, int C, float dflt, float (&v)[CH]) {
-  using L = Lay<T, CH>;
+  using L = Lay<T, CH, false>;
 #pragma unroll
   for (int q = 0; q < L::P; ++q)
-    if (L::at(q) < C) mod_piece<L::E>(p, dt, at + L::at(q), dflt, v + q * L::E);
+    if (L::in(q, C)) mod_piece<L::E>(p, dt, at + L::at(q), dflt, v + q * L::E);
 }
 
 // A row of the output, from its first channel.
-template <typename T, int CH>
+template <typename T, int CH, bool FIT = false>
 __device__ __forceinline__ void store_row(T* row, int C, const Vals<CH>& v) {
-  using L = Lay<T, CH>;
+  using L = Lay<T, CH, FIT>;
 #pragma unroll
   for (int q = 0; q < L::P; ++q) {
-    if (L::at(q) >= C) continue;
+    if (!L::in(q, C)) continue;
     const float2* e = v.e + q * (L::E / 2);
     if constexpr (sizeof(T) == 4) {
       *reinterpret_cast<float4*>(row + L::at(q)) = make_float4(e[0].x, e[0].y, e[1].x, e[1].y);
@@ -660,15 +662,15 @@ __device__ __forceinline__ void store_row(T* row, int C, const Vals<CH>& v) {
 }
 
 // A thread's pieces in the ring; ``slot``: the place of a stage's row and tensor.
-template <typename T, int CH>
+template <typename T, int CH, bool FIT = false>
 struct Ring {
-  using L = Lay<T, CH>;
+  using L = Lay<T, CH, FIT>;
   uint4* base;  // of the thread
   int C;
   __device__ __forceinline__ void copy(int slot, const T* row) const {
 #pragma unroll
     for (int q = 0; q < L::P; ++q)
-      if (L::at(q) < C)
+      if (L::in(q, C))
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(base + (slot * L::P + q) * (int)blockDim.x)),
                      "l"(row + L::at(q))
                      : "memory");
@@ -678,7 +680,7 @@ struct Ring {
 #pragma unroll
     for (int q = 0; q < L::P; ++q) {
       uint4 u = make_uint4(0, 0, 0, 0);
-      if (L::at(q) < C) u = base[(slot * L::P + q) * (int)blockDim.x];
+      if (L::in(q, C)) u = base[(slot * L::P + q) * (int)blockDim.x];
       const uint32_t w[4] = {u.x, u.y, u.z, u.w};
       float2* e = v.e + q * (L::E / 2);
       if constexpr (sizeof(T) == 4) {
@@ -737,10 +739,10 @@ __device__ __forceinline__ void team_sum(float (&v)[N], float (*buf)[4][32], int
 }
 
 // Rows i of v to v - mean, and their (mean, rstd); channels past the row stay 0.
-template <typename T, int CH, int R>
+template <typename T, int CH, int R, bool FIT>
 __device__ __forceinline__ void center(Vals<CH> (&v)[R], int C, float inv_c, int kind, float eps, float (*buf)[4][32], int& turn,
                                        float2 (&out)[R]) {
-  using L = Lay<T, CH>;
+  using L = Lay<T, CH, FIT>;
   float s[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) out[i].x = 0.0f;
@@ -758,7 +760,7 @@ __device__ __forceinline__ void center(Vals<CH> (&v)[R], int C, float inv_c, int
       out[i].x = s[i] * inv_c;
 #pragma unroll
       for (int q = 0; q < L::P; ++q)
-        if (L::at(q) < C)
+        if (L::in(q, C))
 #pragma unroll
           for (int k = 0; k < L::E / 2; ++k) v[i].e[q * (L::E / 2) + k] = fadd2(v[i].e[q * (L::E / 2) + k], both(-out[i].x));
     }
@@ -802,7 +804,7 @@ __device__ __forceinline__ void load_mods(const Params& p, int g, float4* sA, fl
   }
 }
 
-template <typename T, bool Y, int CH, int R, int MAXT, int MINB>
+template <typename T, bool Y, int CH, int R, bool FIT, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) fwd_stream_kernel(const __grid_constant__ Params p) {
   extern __shared__ float4 slots[];
   __shared__ float red[2][4][32];
@@ -811,7 +813,7 @@ __global__ void __launch_bounds__(MAXT, MINB) fwd_stream_kernel(const __grid_con
   float4* sA = slots;                         // w (1 + scale)
   float4* sB = slots + S * blockDim.x;        // b (1 + scale) + shift
   float4* sG = slots + 2 * S * blockDim.x;    // gate wy; only with y
-  const Ring<T, CH> ring{reinterpret_cast<uint4*>(slots + (Y ? 3 : 2) * S * blockDim.x) + threadIdx.x, p.C};
+  const Ring<T, CH, FIT> ring{reinterpret_cast<uint4*>(slots + (Y ? 3 : 2) * S * blockDim.x) + threadIdx.x, p.C};
   const float inv_c = 1.0f / (float)p.C;
   const int lo = (int)(p.rows * blockIdx.x / p.ctas), hi = (int)(p.rows * (blockIdx.x + 1) / p.ctas);
   int turn = 0, g = -1;
@@ -858,18 +860,18 @@ __global__ void __launch_bounds__(MAXT, MINB) fwd_stream_kernel(const __grid_con
           if (ALL || (i >= j && i < n)) ring.get((st * NT + 1) * R + i, y[i]);
           else y[i] = Vals<CH>{};
         }
-        if (p.ynorm != kNone) center<T, CH, R>(y, p.C, inv_c, p.ynorm, p.eps, red, turn, sy);
+        if (p.ynorm != kNone) center<T, CH, R, FIT>(y, p.C, inv_c, p.ynorm, p.eps, red, turn, sy);
         slots_get<CH>(sG, a);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
 #pragma unroll
           for (int k = 0; k < CH / 2; ++k)
             v[i].e[k] = ffma2(fmul2(a.e[k], both(sy[i].y)), y[i].e[k], fmul2(v[i].e[k], both(p.alpha)));
-          if (p.r && (ALL || (i >= j && i < n))) store_row<T, CH>(ro + (long long)i * p.C, p.C, v[i]);
+          if (p.r && (ALL || (i >= j && i < n))) store_row<T, CH, FIT>(ro + (long long)i * p.C, p.C, v[i]);
         }
       }
       if (p.h != nullptr) {
-        center<T, CH, R>(v, p.C, inv_c, p.norm, p.eps, red, turn, sr);
+        center<T, CH, R, FIT>(v, p.C, inv_c, p.norm, p.eps, red, turn, sr);
         Vals<CH> a, b;
         slots_get<CH>(sA, a);
         slots_get<CH>(sB, b);
@@ -877,7 +879,7 @@ __global__ void __launch_bounds__(MAXT, MINB) fwd_stream_kernel(const __grid_con
         for (int i = 0; i < R; ++i) {
 #pragma unroll
           for (int k = 0; k < CH / 2; ++k) v[i].e[k] = ffma2(fmul2(v[i].e[k], both(sr[i].y)), a.e[k], b.e[k]);
-          if (ALL || (i >= j && i < n)) store_row<T, CH>(ho + (long long)i * p.C, p.C, v[i]);
+          if (ALL || (i >= j && i < n)) store_row<T, CH, FIT>(ho + (long long)i * p.C, p.C, v[i]);
         }
       }
       if (threadIdx.x == 0 && p.stats)
@@ -894,8 +896,8 @@ __global__ void __launch_bounds__(MAXT, MINB) fwd_stream_kernel(const __grid_con
       if (g >= p.G) {  // outside every packed sequence: zeros
         const Vals<CH> z = {};
         for (int i = j; i < n; ++i) {
-          if (p.r) store_row<T, CH>(ro + (long long)i * p.C, p.C, z);
-          if (p.h) store_row<T, CH>(ho + (long long)i * p.C, p.C, z);
+          if (p.r) store_row<T, CH, FIT>(ro + (long long)i * p.C, p.C, z);
+          if (p.h) store_row<T, CH, FIT>(ho + (long long)i * p.C, p.C, z);
           if (threadIdx.x == 0 && p.stats) p.stats[row + i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
       } else if (n - j == R) {
@@ -912,7 +914,7 @@ __global__ void __launch_bounds__(MAXT, MINB) fwd_stream_kernel(const __grid_con
 template <typename T, bool Y, int R, int MAXT>
 __global__ void __launch_bounds__(MAXT) bwd_stream_kernel(const __grid_constant__ Params p) {
   constexpr int CH = 8;
-  using L = Lay<T, CH>;
+  using L = Lay<T, CH, false>;
   extern __shared__ float4 slots[];
   __shared__ float red[2][4][32];
   constexpr int NT = Y ? 4 : 2;          // x, dh, y, dr
@@ -933,7 +935,7 @@ __global__ void __launch_bounds__(MAXT) bwd_stream_kernel(const __grid_constant_
     for (int k = 0; k < 3; ++k)
 #pragma unroll
       for (int q = 0; q < L::P; ++q)
-        if (L::at(q) < p.C)
+        if (L::in(q, p.C))
 #pragma unroll
           for (int i = 0; i < L::E / 2; i += 2) {
             const float2* e = a[k]->e + q * (L::E / 2) + i;
@@ -1216,8 +1218,9 @@ static cudaError_t stream_fwd(Params& p, cudaStream_t st, bool& done) {
   done = p.stages != 0;
   if (!done) return cudaSuccess;
   p.ctas = (int)std::min<long long>(p.rows, (long long)kSMs * per);
-  return nt <= 320 ? start<fwd_stream_kernel<T, false, 16, R, 320, 2>>(p, nt, smem, st)
-                   : start<fwd_stream_kernel<T, false, 16, R, 512, 1>>(p, nt, smem, st);
+  if (nt > 320) return start<fwd_stream_kernel<T, false, 16, R, false, 512, 1>>(p, nt, smem, st);
+  return p.C == nt * 16 ? start<fwd_stream_kernel<T, false, 16, R, true, 320, 2>>(p, nt, smem, st)
+                        : start<fwd_stream_kernel<T, false, 16, R, false, 320, 2>>(p, nt, smem, st);
 }
 template <typename T>
 static cudaError_t stream_fwd_gated(Params& p, cudaStream_t st, bool& done) {
@@ -1227,8 +1230,9 @@ static cudaError_t stream_fwd_gated(Params& p, cudaStream_t st, bool& done) {
   const size_t smem = ring_bytes(p, nt, 8, 3, 2 * (wide ? 1 : R), sizeof(T), kSmemMax);
   done = p.stages != 0;
   if (!done) return cudaSuccess;
-  return wide ? start<fwd_stream_kernel<T, true, 8, 1, 1024, 1>>(p, nt, smem, st)
-              : start<fwd_stream_kernel<T, true, 8, R, 640, 1>>(p, nt, smem, st);
+  if (wide) return start<fwd_stream_kernel<T, true, 8, 1, false, 1024, 1>>(p, nt, smem, st);
+  return p.C == nt * 8 ? start<fwd_stream_kernel<T, true, 8, R, true, 640, 1>>(p, nt, smem, st)
+                       : start<fwd_stream_kernel<T, true, 8, R, false, 640, 1>>(p, nt, smem, st);
 }
 template <typename T, bool Y>
 static cudaError_t stream_bwd(Params& p, cudaStream_t st, bool& done) {

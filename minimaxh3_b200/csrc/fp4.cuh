@@ -91,23 +91,20 @@ __device__ __forceinline__ long long block_offset(long long row, int b, int nk64
 // slots; an approximate reciprocal serves: where the true quotient is a border it has
 // a few bits, the remainder is exact, and the corrected quotient lands on it; where it
 // is not, 16-bit input is at least 2^-13 of it away.  Divisor and reciprocal carry the
-// row's power of two; rows so small that the remainder could leave the normal range
-// (e < -60) are first scaled by 2^64.
+// row's power of two (2^-109 to 2^126 in magnitude); a remainder below the normal
+// range is off by 2^-150 at most, which the reciprocal makes 2^-41 of a code.
 __device__ __forceinline__ uint32_t round_block(const float2 (&x)[8], uint32_t top, int e, uint2& code) {
   // e4m3 of absmax / (6 scale): the division by 6 is the only rounding before it
   const float raw = div_by(__uint_as_float(top) * pow2f(-e), 6.0f, 1.0f / 6.0f);
   const uint32_t s8 = cvt_e4m3x2_f32(0.0f, raw) & 0xffu;
   if (s8 != 0) {
     const float s = e4m3_value(s8);
-    const bool tiny = e < -60;
-    const int f = tiny ? e + 64 : e;  // [-36, 117]
-    const float2 d2 = both(-s * pow2f(f)), r2 = both(rcp_approx(s) * pow2f(-f));
+    const float2 d2 = both(-s * pow2f(e)), r2 = both(rcp_approx(s) * pow2f(-e));  // e in [-100, 117]
     float q[16];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float2 v = tiny ? fmul2(x[i], both(0x1p64f)) : x[i];
-      const float2 a = fmul2(v, r2);
-      const float2 c = ffma2(ffma2(d2, a, v), r2, a);
+      const float2 a = fmul2(x[i], r2);
+      const float2 c = ffma2(ffma2(d2, a, x[i]), r2, a);
       q[2 * i] = c.x;
       q[2 * i + 1] = c.y;
     }
