@@ -8,8 +8,8 @@
 //
 // gate, scale and shift belong to a group of rows (a batch item or a packed
 // sequence) or to each row.  Every quantity between the inputs and r, h is fp32;
-// the variance is summed around the mean (a second pass over registers), so a
-// stream whose mean is far from zero loses nothing; r and h are rounded once.
+// the variance is summed around the mean where the mean is far from zero, so such
+// a stream loses nothing; r and h are rounded once.
 //
 // Backward, with dn = dh w (1 + scale), d = dr + rstd (dn - mean(dn) - xhat mean(dn xhat)):
 //   dx = alpha d,  dz = d gate,  dy = dz or the norm's gradient of dz wy,
@@ -739,42 +739,63 @@ __device__ __forceinline__ void team_sum(float (&v)[N], float (*buf)[4][32], int
 }
 
 // Rows i of v to v - mean, and their (mean, rstd); channels past the row stay 0.
-template <typename T, int CH, int R, bool FIT>
+// ONCE: a layer norm's sum and sum of squares share one barrier.  The variance q / C -
+// mean^2 loses mean^2 / variance of the sums' relative error, so where a row's is over 8
+// the variance is summed again around the mean, as it always is without ONCE.  At 16
+// channels a thread that takes norm_modulate from 126 to 115 us (32760 x 5120); the
+// gated form's 20 warps lose more in the wider tree than a barrier costs (327 against 372 us).
+template <typename T, int CH, int R, bool FIT, bool ONCE>
 __device__ __forceinline__ void center(Vals<CH> (&v)[R], int C, float inv_c, int kind, float eps, float (*buf)[4][32], int& turn,
                                        float2 (&out)[R]) {
   using L = Lay<T, CH, FIT>;
-  float s[R];
+  float var[R];
+  auto squares = [&](int i) {
+    float2 t = fmul2(v[i].e[0], v[i].e[0]);
 #pragma unroll
-  for (int i = 0; i < R; ++i) out[i].x = 0.0f;
+    for (int k = 1; k < CH / 2; ++k) t = ffma2(v[i].e[k], v[i].e[k], t);
+    return t.x + t.y;
+  };
+  auto around_mean = [&] {
+#pragma unroll
+    for (int i = 0; i < R; ++i) var[i] = squares(i);
+    team_sum(var, buf, turn);
+#pragma unroll
+    for (int i = 0; i < R; ++i) var[i] *= inv_c;
+  };
   if (kind == kLayer) {
+    constexpr int N = ONCE ? 2 : 1;
+    float s[N * R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       float2 t = v[i].e[0];
 #pragma unroll
       for (int k = 1; k < CH / 2; ++k) t = fadd2(t, v[i].e[k]);
-      s[i] = t.x + t.y;
+      s[N * i] = t.x + t.y;
+      if constexpr (ONCE) s[N * i + 1] = squares(i);
     }
     team_sum(s, buf, turn);
+    bool far = !ONCE;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      out[i].x = s[i] * inv_c;
+      out[i].x = s[N * i] * inv_c;
+      if constexpr (ONCE) {
+        var[i] = fmaf(-out[i].x, out[i].x, s[N * i + 1] * inv_c);
+        far = far || out[i].x * out[i].x > 8.0f * var[i];
+      }
 #pragma unroll
       for (int q = 0; q < L::P; ++q)
         if (L::in(q, C))
 #pragma unroll
           for (int k = 0; k < L::E / 2; ++k) v[i].e[q * (L::E / 2) + k] = fadd2(v[i].e[q * (L::E / 2) + k], both(-out[i].x));
     }
+    if (far) around_mean();  // the same answer in every thread
+  } else {
+#pragma unroll
+    for (int i = 0; i < R; ++i) out[i].x = 0.0f;
+    around_mean();
   }
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    float2 t = fmul2(v[i].e[0], v[i].e[0]);
-#pragma unroll
-    for (int k = 1; k < CH / 2; ++k) t = ffma2(v[i].e[k], v[i].e[k], t);
-    s[i] = t.x + t.y;
-  }
-  team_sum(s, buf, turn);
-#pragma unroll
-  for (int i = 0; i < R; ++i) out[i].y = rsqrtf(fmaf(s[i], inv_c, eps));
+  for (int i = 0; i < R; ++i) out[i].y = rsqrtf(var[i] + eps);
 }
 
 // The modulation of group g for the thread's channels, combined into its slots.
@@ -860,7 +881,7 @@ __global__ void __launch_bounds__(MAXT, MINB) fwd_stream_kernel(const __grid_con
           if (ALL || (i >= j && i < n)) ring.get((st * NT + 1) * R + i, y[i]);
           else y[i] = Vals<CH>{};
         }
-        if (p.ynorm != kNone) center<T, CH, R, FIT>(y, p.C, inv_c, p.ynorm, p.eps, red, turn, sy);
+        if (p.ynorm != kNone) center<T, CH, R, FIT, !Y>(y, p.C, inv_c, p.ynorm, p.eps, red, turn, sy);
         slots_get<CH>(sG, a);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
@@ -871,7 +892,7 @@ __global__ void __launch_bounds__(MAXT, MINB) fwd_stream_kernel(const __grid_con
         }
       }
       if (p.h != nullptr) {
-        center<T, CH, R, FIT>(v, p.C, inv_c, p.norm, p.eps, red, turn, sr);
+        center<T, CH, R, FIT, !Y>(v, p.C, inv_c, p.norm, p.eps, red, turn, sr);
         Vals<CH> a, b;
         slots_get<CH>(sA, a);
         slots_get<CH>(sB, b);

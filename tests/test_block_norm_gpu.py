@@ -368,6 +368,24 @@ def test_infinite_rows_keep_to_themselves():
     assert bool((norm_modulate(torch.full((2, 64), 3.0, device=DEV)) == 0).all())  # a constant row: its variance is 0
 
 
+@pytest.mark.parametrize("shift", [0.0, 2.8, 2.9, 40.0, -3000.0])
+@pytest.mark.parametrize("C", [64, 1000, 5120])
+def test_streams_far_from_zero(shift, C):
+    """Means on both sides of the border where the variance is summed again (8 times it), and far past it."""
+    from minimaxh3_b200.kernels.block_norm import gated_residual_norm, norm_modulate
+
+    f = torch.float32
+    x = _rand(95, 1, 41, C, dtype=f, shift=shift)
+    x[:, ::5] -= shift  # rows of both kinds side by side
+    c = Case(x)
+    _close(norm_modulate(x), c.h, c.eh)
+    y, g = _rand(96, 1, 41, C, dtype=f, shift=-shift), _rand(97, C, dtype=f)
+    c = Case(x, y, gate=g, y_norm="layer")
+    r, h = gated_residual_norm(x, y, g, y_norm="layer")
+    _close(r, c.r, c.er)
+    _close(h, c.h, c.eh)
+
+
 def test_compiled():
     from minimaxh3_b200.kernels.block_norm import gated_residual_norm
 
