@@ -1012,13 +1012,20 @@ def block_norm_bwd(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu,
     dr, dh = (None if d is None else d.to(x.dtype) for d in (dr, dh))
     ts = (x, y, gate, scale, shift, weight, bias, y_weight)
     grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if w and t is not None else None for t, w in zip(ts, want)]
+    written = list(grads)
+    if dh is None:  # h was not used: what only h depends on has the gradient 0
+        for i in (3, 4, 5, 6):
+            if grads[i] is not None:
+                grads[i].zero_()
+                written[i] = None
     lib = _lib.load()
 
     def workspace(rows, C, groups):
         nbytes = max(16, lib.mh3_block_norm_workspace_bytes(rows, C, groups))
         return torch.empty(nbytes, dtype=torch.uint8, device=x.device)
 
-    a, keep = _norm_args(*ts, cu, max(norm, 1), y_norm, eps, alpha, per_token, None, None, stats, dr, dh, grads, workspace)
+    a, keep = _norm_args(*ts, cu, max(norm, 1), y_norm, eps, alpha, per_token, None, None, stats, dr, dh, written,
+                         workspace)
     rc = _launch(x.device, lib.mh3_block_norm_bwd, a)
     _lib.check(rc, "mh3_block_norm_bwd")
     return grads

@@ -285,6 +285,15 @@ def test_broadcast_inputs_and_partial_gradients():
     r, h = gated_residual_norm(x, y, g)
     (dy,) = torch.autograd.grad(h, y, dh)
     _close(dy, *c.grads(None, dh, lambda t: t.sum(1))["y"])
+    # what only h depends on has the gradient 0 when h is not used, by group and by token
+    for lead in ((B,), (B, S)):
+        sc = _rand(77, *lead, C, dtype=f).requires_grad_(True)
+        w = _rand(78, C, dtype=f).requires_grad_(True)
+        r, _ = gated_residual_norm(x, y, g, sc, sc, weight=w)
+        ds, dw, dy2 = torch.autograd.grad(r, (sc, w, y), dh)
+        assert bool((ds == 0).all()) and bool((dw == 0).all())
+        want = Case(x, y, gate=g, rows_of=lambda t: t[:, None].expand(B, S, C)).grads(dh, None, lambda t: t.sum(1))
+        _close(dy2, *want["y"])
     # x and y are the same tensor, and an input is shared by two calls
     xs = _rand(76, B, S, C, dtype=f).requires_grad_(True)
     r, h = gated_residual_norm(xs, xs, g.detach())
