@@ -8,7 +8,7 @@ and every adapter's delta and writes bf16 once.  Weights take 0.5625 bytes each.
 
 A 4-bit matrix is three tensors ``(values, blocks, scale)``: see ``quantize_fp4``.
 Registered as ``torch.ops.mh3.fp4_linear`` with a fake implementation for
-``torch.compile``.  Inference only: no gradient is defined.
+``torch.compile``.  Inference only: asking for a gradient raises, as with ``FP8Linear``.
 """
 from __future__ import annotations
 
@@ -33,6 +33,18 @@ _LIB.impl("fp4_linear", _fp4_linear_cuda, "CUDA")
 @torch.library.register_fake("mh3::fp4_linear", lib=_LIB)
 def _(x2d, w4, w_blocks, w_scale, bias, lora_a, lora_b, lora_scale):
     return x2d.new_empty((x2d.shape[0], w4.shape[0]), dtype=torch.bfloat16)
+
+
+class _NoGradient(torch.autograd.Function):
+    """Passes a result on, tied to the inputs that ask for a gradient, so that asking for it raises."""
+
+    @staticmethod
+    def forward(ctx, out, *inputs):
+        return out.view_as(out)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("fp4_linear has no gradient: its 4-bit operands are for inference")
 
 
 def quantize_fp4(x2d: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -77,6 +89,10 @@ def fp4_linear(x: torch.Tensor, w4: torch.Tensor, w_blocks: torch.Tensor, w_scal
         raise ValueError("fp4_linear: x and the weight must be on one CUDA device")
     out = torch.ops.mh3.fp4_linear(x.reshape(-1, K), w4, w_blocks, w_scale, bias, [a for a, _, _ in adapters],
                                    [b for _, b, _ in adapters], [float(s) for _, _, s in adapters])
+    if torch.is_grad_enabled():
+        asks = [t for t in (x, *(t for a, b, _ in adapters for t in (a, b))) if t.requires_grad]
+        if asks:
+            out = _NoGradient.apply(out, *asks)
     return out.reshape(*x.shape[:-1], N)
 
 

@@ -193,6 +193,19 @@ def test_linear_with_adapters(M, ranks):
     _check(mod(x.to(DEV)).cpu(), xq @ wq.t() + bias.double(), mag, K)
 
 
+def test_linear_refuses_gradients():
+    from minimaxh3_b200.kernels.fp4_linear import fp4_linear, quantize_fp4
+
+    w = quantize_fp4(_rand(56, 64, 96).to(DEV))
+    x = _rand(57, 5, 96).to(DEV).requires_grad_(True)
+    A, B = _rand(58, 16, 96).to(DEV), _rand(59, 64, 16).to(DEV).requires_grad_(True)
+    for out in (fp4_linear(x, *w), fp4_linear(x.detach(), *w, adapters=[(A, B, 1.0)])):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            out.float().sum().backward()
+    with torch.no_grad():
+        assert not fp4_linear(x, *w).requires_grad
+
+
 def test_linear_types_empty_and_nan_rows():
     from minimaxh3_b200.kernels.fp4_linear import fp4_linear, quantize_fp4
 
