@@ -450,7 +450,8 @@ MH3_API int mh3_rotary(const mh3_rotary_args* args, void* stream);
  * modulation, and writes every gradient whose pointer is given: dx, dy
  * [rows, channels] in dtype; dgate, dscale, dshift [groups or rows, channels]
  * and dweight, dbias, dy_weight [channels], each in its tensor's type, all
- * contiguous.  Column sums are added in a fixed order.  workspace:
+ * contiguous (null dr or dh: that output was not used, its gradient is 0).
+ * Column sums are added in a fixed order.  workspace:
  * mh3_block_norm_workspace_bytes() bytes, 16-byte aligned.
  * No reference counterpart (the model's blocks are outside the reference).
  */
@@ -512,7 +513,8 @@ MH3_API int mh3_block_norm_bwd(const mh3_block_norm_args* args, void* stream);
  *   * a_scale[m] * b_scale[n] + bias[n]), a [M,K] and b [N,K] such matrices
  * (their products and sums take the block scales), a2 [M,R], b2 [N,R] optional
  * bf16 low-rank operands.  N, R and the strides of out, a2 and b2 multiples of
- * 8; x4 buffers contiguous, all pointers 16-byte aligned.
+ * 8; x4 buffers contiguous, all pointers 16-byte aligned.  Scales past K must be
+ * finite, as mh3_quantize_fp4 leaves them (their codes count as 0).
  */
 MH3_API uint64_t mh3_fp4_block_bytes(int64_t M, int64_t K);
 MH3_API int mh3_quantize_fp4(const void* x, int64_t x_stride, int32_t in_dtype, int64_t M, int64_t K, void* x4,

@@ -511,6 +511,15 @@ __global__ void __launch_bounds__(1024) bwd_kernel(const __grid_constant__ Param
 #pragma unroll
       for (int i = 0; i < 8; ++i) d[i] = fmaf(st.w, dn[i] - m0 - xh[i] * m1, d[i]);
     }
+    if constexpr (PT) {
+      if (!has_dh && live)  // h was not used
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < n) {
+            if (p.dscale) put1(p.dscale, p.scale.dt, row * p.C + c + i, 0.0f);
+            if (p.dshift) put1(p.dshift, p.shift.dt, row * p.C + c + i, 0.0f);
+          }
+    }
     if (live && p.dx) {
       const float k = has_y ? p.alpha : 1.0f;
 #pragma unroll
@@ -780,7 +789,7 @@ __device__ __forceinline__ void center(Vals<CH> (&v)[R], int C, float inv_c, int
       out[i].x = s[N * i] * inv_c;
       if constexpr (ONCE) {
         var[i] = fmaf(-out[i].x, out[i].x, s[N * i + 1] * inv_c);
-        far = far || out[i].x * out[i].x > 8.0f * var[i];
+        far = far || !(out[i].x * out[i].x <= 8.0f * var[i] && var[i] < INFINITY);  // or a square overflowed
       }
 #pragma unroll
       for (int q = 0; q < L::P; ++q)

@@ -182,7 +182,8 @@ def norm_modulate(
     x [B, S, C] or [T, C], bf16, f16 or f32, C <= 8192; ``norm`` "layer" or
     "rms".  scale / shift: [C], [B, C], [B, 1, C], or a row for each token
     ([B, S, C] / [T, C]); with ``cu_seqlens`` (int32 [nseq+1] on the device) also
-    [nseq, C], and rows outside every sequence give zeros.  weight / bias [C].
+    [nseq, C] (taken before [T, C] where the two are alike), and rows outside every
+    sequence give zeros.  weight / bias [C].
     Modulation and weights may be of other float types than x (kept in f32
     beside a bf16 stream); None leaves that term out.  Statistics and sums are
     f32, the result is rounded once.

@@ -912,6 +912,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
     ps = positions.stride()
     pos_b = ps[0] if len(ps) == 3 and positions.shape[0] > 1 else 0
     n = len(axes_dim)
+    if seqlen > 0x7fffffff:
+        raise ValueError("rotary: too many tokens")
     a = _lib.RotaryArgs.from_buffer_copy(_ROTARY.pack(
         batch, seqlen, shape[1], 0 if k is None else k.shape[1], shape[-1], _FLOAT_CODE[q.dtype], _POS_KIND[positions.dtype], n,
         int(interleaved), int(inverse), *axes_dim, *(0,) * (4 - n), *theta, *(0.0,) * (4 - n),
@@ -1012,20 +1014,13 @@ def block_norm_bwd(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu,
     dr, dh = (None if d is None else d.to(x.dtype) for d in (dr, dh))
     ts = (x, y, gate, scale, shift, weight, bias, y_weight)
     grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if w and t is not None else None for t, w in zip(ts, want)]
-    written = list(grads)
-    if dh is None:  # h was not used: what only h depends on has the gradient 0
-        for i in (3, 4, 5, 6):
-            if grads[i] is not None:
-                grads[i].zero_()
-                written[i] = None
     lib = _lib.load()
 
     def workspace(rows, C, groups):
         nbytes = max(16, lib.mh3_block_norm_workspace_bytes(rows, C, groups))
         return torch.empty(nbytes, dtype=torch.uint8, device=x.device)
 
-    a, keep = _norm_args(*ts, cu, max(norm, 1), y_norm, eps, alpha, per_token, None, None, stats, dr, dh, written,
-                         workspace)
+    a, keep = _norm_args(*ts, cu, max(norm, 1), y_norm, eps, alpha, per_token, None, None, stats, dr, dh, grads, workspace)
     rc = _launch(x.device, lib.mh3_block_norm_bwd, a)
     _lib.check(rc, "mh3_block_norm_bwd")
     return grads

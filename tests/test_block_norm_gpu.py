@@ -395,6 +395,17 @@ def test_streams_far_from_zero(shift, C):
     _close(h, c.h, c.eh)
 
 
+@pytest.mark.parametrize("C", [256, 251])
+def test_squares_past_the_largest_float(C):
+    """Rows near 10^20 whose squares overflow while those around their mean do not."""
+    from minimaxh3_b200.kernels.block_norm import norm_modulate
+
+    x = 1e20 * (1 + 1e-3 * _rand(101, 1, 9, C, dtype=torch.float32))
+    x[:, ::3] = _rand(102, 1, 3, C, dtype=torch.float32)
+    c = Case(x)
+    _close(norm_modulate(x), c.h, c.eh)
+
+
 def test_compiled():
     from minimaxh3_b200.kernels.block_norm import gated_residual_norm
 
