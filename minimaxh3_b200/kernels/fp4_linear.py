@@ -55,8 +55,8 @@ def quantize_fp4(x2d: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.T
     float8_e4m3fn [ceil(M/128), ceil(K/64), 32, 4, 4]: the scale of elements
     16b..16b+15 of row m at [m // 128, b // 4, m % 32, m % 128 // 32, b % 4].
     scale float32 [M, 1]: a power of two that puts the row's largest block scale
-    at the upper end of e4m3.  The value is code * block * scale; all roundings
-    are to nearest even.  A row that holds an infinity or NaN gets scale NaN.
+    at the upper end of e4m3.  Entries of blocks past M and K are 0.  The value is
+    code * block * scale; all roundings are to nearest even.  A row that holds an infinity or NaN gets scale NaN.
     """
     return _ops.quantize_fp4(x2d)
 
@@ -77,8 +77,8 @@ def fp4_linear(x: torch.Tensor, w4: torch.Tensor, w_blocks: torch.Tensor, w_scal
     """bf16 ``x W^T + bias + sum_i scale_i (x A_i^T) B_i^T`` with W [N, K] in 4 bits and x [..., K] rounded to 4 bits.
 
     (w4, w_blocks, w_scale) is ``quantize_fp4(W)``; adapters are
-    ``(A [r, K], B [N, r], scale)`` and see the unrounded x.  One to 32 rows run a
-    kernel that streams W once; more run on the tensor cores' 4-bit rate.
+    ``(A [r, K], B [N, r], scale)`` and see the unrounded x.  One or two rows run as one
+    launch, up to 16 on a kernel that streams W once, more at the tensor cores' 4-bit rate.
     """
     N, K = _ops.check_fp4(w4, w_blocks, w_scale, "fp4_linear weight")
     if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.shape[-1] != K or not x.is_floating_point():
@@ -90,7 +90,7 @@ def fp4_linear(x: torch.Tensor, w4: torch.Tensor, w_blocks: torch.Tensor, w_scal
     out = torch.ops.mh3.fp4_linear(x.reshape(-1, K), w4, w_blocks, w_scale, bias, [a for a, _, _ in adapters],
                                    [b for _, b, _ in adapters], [float(s) for _, _, s in adapters])
     if torch.is_grad_enabled():
-        asks = [t for t in (x, *(t for a, b, _ in adapters for t in (a, b))) if t.requires_grad]
+        asks = [t for t in (x, bias, *(t for a, b, _ in adapters for t in (a, b))) if t is not None and t.requires_grad]
         if asks:
             out = _NoGradient.apply(out, *asks)
     return out.reshape(*x.shape[:-1], N)

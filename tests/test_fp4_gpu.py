@@ -204,6 +204,10 @@ def test_linear_refuses_gradients():
             out.float().sum().backward()
     with torch.no_grad():
         assert not fp4_linear(x, *w).requires_grad
+    bias = _rand(60, 64).to(DEV).requires_grad_(True)
+    assert fp4_linear(x.detach(), *w, bias=bias).requires_grad
+    f = torch.compile(lambda t: fp4_linear(t, *w), backend="aot_eager")
+    assert torch.equal(f(x), fp4_linear(x, *w)) and torch.equal(f(x.detach()), fp4_linear(x, *w))
 
 
 def test_linear_types_empty_and_nan_rows():
@@ -220,7 +224,9 @@ def test_linear_types_empty_and_nan_rows():
         got = fp4_linear(bad.to(DEV), *w)
         keep = [i for i in range(M) if i != 2]
         assert bool(got[2].isnan().all()) and torch.equal(got[keep], ref[keep])
-    assert fp4_linear(torch.empty(0, 96, device=DEV), *w).shape == (0, 64)
+    A, B = _rand(52, 16, 96).to(DEV), _rand(53, 64, 16).to(DEV)
+    for rest in ((), ((A, B, 2.0),)):
+        assert fp4_linear(torch.empty(0, 96, device=DEV), *w, adapters=rest).shape == (0, 64)
 
 
 def test_linear_of_few_rows_strides_and_outputs():
