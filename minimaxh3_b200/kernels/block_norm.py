@@ -22,18 +22,12 @@ _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 _MODS = "Tensor x, Tensor? y, Tensor? gate, Tensor? scale, Tensor? shift, Tensor? weight, Tensor? bias, Tensor? y_weight, Tensor? cu"
 _CONF = "int norm, int y_norm, float eps, float alpha, bool per_token"
 _LIB = torch.library.Library("mh3", "FRAGMENT")
-_LIB.define(f"block_norm({_MODS}, {_CONF}, bool want_stats) -> (Tensor, Tensor, Tensor)")
+_LIB.define(f"block_norm({_MODS}, {_CONF}, bool want_stats) -> Tensor[]")
 _LIB.define(f"block_norm_backward(Tensor? dr, Tensor? dh, {_MODS}, Tensor stats, {_CONF}, bool[] want) -> Tensor[]")
 
 
-def _backward_cuda(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu, stats, norm, y_norm, eps, alpha, per_token, want):
-    grads = _ops.block_norm_bwd(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu, stats, norm, y_norm, eps, alpha,
-                                per_token, want)
-    return [x.new_empty(0) if g is None else g for g in grads]
-
-
 _LIB.impl("block_norm", _ops.block_norm_fwd, "CUDA")
-_LIB.impl("block_norm_backward", _backward_cuda, "CUDA")
+_LIB.impl("block_norm_backward", _ops.block_norm_bwd, "CUDA")
 
 
 @torch.library.register_fake("mh3::block_norm", lib=_LIB)
@@ -41,40 +35,38 @@ def _(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_norm, eps, a
     rows = 1
     for n in x.shape[:-1]:
         rows = rows * n
-    none = x.new_empty(0)
-    return (x.new_empty(x.shape) if y is not None else none, x.new_empty(x.shape) if norm else none.clone(),
-            x.new_empty((rows, 4), dtype=torch.float32) if want_stats else none.clone())
+    out = [x.new_empty(x.shape) for given in (y is not None, norm) if given]
+    return out + ([x.new_empty((rows, 4), dtype=torch.float32)] if want_stats else [])
 
 
 @torch.library.register_fake("mh3::block_norm_backward", lib=_LIB)
 def _(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu, stats, norm, y_norm, eps, alpha, per_token, want):
     ts = (x, y, gate, scale, shift, weight, bias, y_weight)
-    return [t.new_empty(t.shape) if w and t is not None else x.new_empty(0) for t, w in zip(ts, want)]
+    return [t.new_empty(t.shape) for t, w in zip(ts, want) if w and t is not None]
 
 
 class _BlockNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_norm, eps, alpha, per_token):
-        r, h, stats = torch.ops.mh3.block_norm(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_norm, eps, alpha,
+        *out, stats = torch.ops.mh3.block_norm(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_norm, eps, alpha,
                                                per_token, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, y, gate, scale, shift, weight, bias, y_weight, cu, stats)
         ctx.conf = (norm, y_norm, eps, alpha, per_token)
-        return r, h
+        return tuple(out)
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dr, dh):
-        x, y, gate, scale, shift, weight, bias, y_weight, cu, stats = ctx.saved_tensors
-        if y is None:
-            dr = None
-        if not ctx.conf[0]:
-            dh = None
+    def backward(ctx, *grads):
+        saved = ctx.saved_tensors
+        it = iter(grads)
+        dr = None if saved[1] is None else next(it)  # r with y, h with a norm
+        dh = next(it) if ctx.conf[0] else None
         if dr is None and dh is None:
             return (None,) * 14
-        want = [bool(n) and t is not None for n, t in zip(ctx.needs_input_grad, (x, y, gate, scale, shift, weight, bias, y_weight))]
-        grads = torch.ops.mh3.block_norm_backward(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu, stats, *ctx.conf, want)
-        return tuple(g if w else None for g, w in zip(grads, want)) + (None,) * 6
+        want = ctx.needs_input_grad[:8]  # false for what is not a tensor
+        it = iter(torch.ops.mh3.block_norm_backward(dr, dh, *saved, *ctx.conf, want))
+        return tuple(next(it) if w else None for w in want) + (None,) * 6
 
 
 def _check_stream(what, name, t, like=None):
@@ -154,7 +146,7 @@ def _run(x, y, m, weight, bias, y_weight, cu, norm, y_norm, eps, alpha, per_toke
             per_token)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:8]):
         return _BlockNormFn.apply(*args)
-    return torch.ops.mh3.block_norm(*args, False)[:2]
+    return torch.ops.mh3.block_norm(*args, False)
 
 
 def _finish_checks(what, x, eps):
@@ -197,7 +189,7 @@ def norm_modulate(
     _channels(what, x, {"weight": weight, "bias": bias})
     _finish_checks(what, x, eps)
     cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-    return _run(x, None, m, weight, bias, None, cu, _ops.NORM_KINDS[norm], 0, eps, 1.0, per_token)[1]
+    return _run(x, None, m, weight, bias, None, cu, _ops.NORM_KINDS[norm], 0, eps, 1.0, per_token)[0]
 
 
 def gated_residual_norm(
@@ -241,5 +233,5 @@ def gated_residual_norm(
     _channels(what, x, {"weight": weight, "bias": bias, "y_weight": y_weight})
     _finish_checks(what, x, eps)
     cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-    r, h = _run(x, y, m, weight, bias, y_weight, cu, _ops.NORM_KINDS[norm], _ops.NORM_KINDS[y_norm], eps, residual_scale, per_token)
-    return r, None if norm == "none" else h
+    out = _run(x, y, m, weight, bias, y_weight, cu, _ops.NORM_KINDS[norm], _ops.NORM_KINDS[y_norm], eps, residual_scale, per_token)
+    return out[0], None if norm == "none" else out[1]

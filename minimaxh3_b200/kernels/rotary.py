@@ -46,7 +46,8 @@ class _RotaryFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, gq, gk):
         (positions,) = ctx.saved_tensors
-        dq, dk = _RotaryFn.apply(gq, gk if ctx.has_k else None, positions, *ctx.rest, not ctx.inverse)
+        turn = _RotaryFn.apply if torch.is_grad_enabled() else torch.ops.mh3.rotary_axes  # with create_graph: its own gradient
+        dq, dk = turn(gq, gk if ctx.has_k else None, positions, *ctx.rest, not ctx.inverse)
         return dq, dk if ctx.has_k else None, None, None, None, None, None
 
 

@@ -935,7 +935,9 @@ _NO_MOD = (0, 0, 0, 0, 0)
 
 
 def _rows2d(t: torch.Tensor) -> torch.Tensor:
-    """[..., C] as [rows, C] with contiguous channels."""
+    """[..., C] as rows of contiguous channels a stride apart: contiguous, or [rows, C]."""
+    if t.is_contiguous():
+        return t
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
@@ -957,7 +959,7 @@ def _norm_args(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_nor
             return (0, 0)
         t = _rows2d(t)
         keep.append(t)
-        return (t.data_ptr(), t.stride(0))
+        return (t.data_ptr(), t.stride(-2) if t.shape[-2] > 1 else C)
 
     def mod(m):
         if m is None:
@@ -994,7 +996,7 @@ def _norm_args(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_nor
 
 def block_norm_fwd(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm: int, y_norm: int, eps: float, alpha: float,
                    per_token: bool, want_stats: bool):
-    """``mh3_block_norm_fwd``: (r, h, stats); r is empty without y, h with norm 0, stats when not wanted.
+    """``mh3_block_norm_fwd``: the list of r (with y), h (unless norm is 0) and stats (when wanted).
 
     gate, scale, shift: [groups, C] (any stride), or with ``per_token`` of x's shape."""
     r = torch.empty(x.shape, dtype=x.dtype, device=x.device) if y is not None else None
@@ -1004,14 +1006,14 @@ def block_norm_fwd(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm: i
                          stats)
     rc = _launch(x.device, _lib.load().mh3_block_norm_fwd, a)
     _lib.check(rc, "mh3_block_norm_fwd")
-    return tuple(x.new_empty(0) if t is None else t for t in (r, h, stats))
+    return [t for t in (r, h, stats) if t is not None]
 
 
 def block_norm_bwd(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu, stats, norm: int, y_norm: int, eps: float,
                    alpha: float, per_token: bool, want):
-    """``mh3_block_norm_bwd``: the gradients of (x, y, gate, scale, shift, weight, bias, y_weight) whose
-    entry of ``want`` is true, None for the others; dr or dh may be None."""
-    dr, dh = (None if d is None else d.to(x.dtype) for d in (dr, dh))
+    """``mh3_block_norm_bwd``: the list of the gradients of those of (x, y, gate, scale, shift, weight, bias,
+    y_weight) that are given and whose entry of ``want`` is true; dr or dh may be None."""
+    dr, dh = (d if d is None or d.dtype == x.dtype else d.to(x.dtype) for d in (dr, dh))
     ts = (x, y, gate, scale, shift, weight, bias, y_weight)
     grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if w and t is not None else None for t, w in zip(ts, want)]
     lib = _lib.load()
@@ -1023,7 +1025,7 @@ def block_norm_bwd(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu,
     a, keep = _norm_args(*ts, cu, max(norm, 1), y_norm, eps, alpha, per_token, None, None, stats, dr, dh, grads, workspace)
     rc = _launch(x.device, lib.mh3_block_norm_bwd, a)
     _lib.check(rc, "mh3_block_norm_bwd")
-    return grads
+    return [g for g in grads if g is not None]
 
 
 # ---------------------------------------------------------------------------
