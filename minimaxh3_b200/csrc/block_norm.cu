@@ -789,7 +789,8 @@ __device__ __forceinline__ void center(Vals<CH> (&v)[R], int C, float inv_c, int
       out[i].x = s[N * i] * inv_c;
       if constexpr (ONCE) {
         var[i] = fmaf(-out[i].x, out[i].x, s[N * i + 1] * inv_c);
-        far = far || !(out[i].x * out[i].x <= 8.0f * var[i] && var[i] < INFINITY);  // or a square overflowed
+        // 8 var - mean^2 negative, or an infinity or NaN because a square overflowed
+        far = far || __float_as_uint(fmaf(8.0f, var[i], -out[i].x * out[i].x)) >= 0x7f800000u;
       }
 #pragma unroll
       for (int q = 0; q < L::P; ++q)

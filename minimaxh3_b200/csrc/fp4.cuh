@@ -87,24 +87,27 @@ __device__ __forceinline__ long long block_offset(long long row, int b, int nk64
 }
 
 // One block: its scale byte and 16 codes, from its absmax and the row's exponent.
-// The quotients x / (block scale) are div_by in packed pairs, which halves their issue
-// slots; an approximate reciprocal serves: where the true quotient is a border it has
-// a few bits, the remainder is exact, and the corrected quotient lands on it; where it
-// is not, 16-bit input is at least 2^-13 of it away.  Divisor and reciprocal carry the
-// row's power of two (2^-109 to 2^126 in magnitude); a remainder below the normal
-// range is off by 2^-150 at most, which the reciprocal makes 2^-41 of a code.
-__device__ __forceinline__ uint32_t round_block(const float2 (&x)[8], uint32_t top, int e, uint2& code) {
+// The quotients x / (block scale) are x r + x r', r + r' the reciprocal to 2^-45, in
+// packed pairs: off by 2^-44 before their rounding, so a true quotient on a border of
+// two codes lands on it (it has three bits), and 16-bit input that is not on one is at
+// least 2^-11 of it away.  r and r' carry the row's power of two; rows so large that r'
+// would be subnormal are brought down first (exactly: what underflows is far below a code).
+__device__ __forceinline__ uint32_t round_block(float2 (&x)[8], uint32_t top, int e, uint2& code) {
   // e4m3 of absmax / (6 scale): the division by 6 is the only rounding before it
   const float raw = div_by(__uint_as_float(top) * pow2f(-e), 6.0f, 1.0f / 6.0f);
   const uint32_t s8 = cvt_e4m3x2_f32(0.0f, raw) & 0xffu;
   if (s8 != 0) {
-    const float s = e4m3_value(s8);
-    const float2 d2 = both(-s * pow2f(e)), r2 = both(rcp_approx(s) * pow2f(-e));  // e in [-100, 117]
+    if (e > 60) {  // of 117 at most
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = fmul2(x[i], both(pow2f(-64)));
+      e -= 64;
+    }
+    const float s = e4m3_value(s8), r = rcp_approx(s);
+    const float2 r2 = both(r * pow2f(-e)), t2 = both(fmaf(-s, r, 1.0f) * r * pow2f(-e));
     float q[16];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float2 a = fmul2(x[i], r2);
-      const float2 c = ffma2(ffma2(d2, a, x[i]), r2, a);
+      const float2 c = ffma2(x[i], r2, fmul2(x[i], t2));
       q[2 * i] = c.x;
       q[2 * i + 1] = c.y;
     }
