@@ -58,13 +58,14 @@ def _dtype_code(dt: torch.dtype) -> int:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # a tensor exists: CUDA is initialised
 
 
 def _launch(dev: torch.device, fn, *args) -> int:
     """``fn(*args, stream)`` with ``dev`` current, on its current stream.  The small calls' time is
     the host's: the device is switched only where it has to be."""
     index = dev.index
-    if _raw_stream is not None and index == torch.cuda.current_device():
+    if _raw_stream is not None and index == _current_device():
         return fn(*args, _raw_stream(index))
     with torch.cuda.device(dev):
         return fn(*args, _stream(dev))
