@@ -741,9 +741,9 @@ def quantize_fp4(x2d: torch.Tensor):
         x2d = x2d.contiguous()
     lib = _lib.load()
     dev = x2d.device
-    x4 = torch.empty((M, K // 2), dtype=torch.uint8, device=dev)
-    blocks = torch.empty(_fp4_blocks_shape(M, K), dtype=E4M3, device=dev)
-    scale = torch.empty((M, 1), dtype=torch.float32, device=dev)
+    x4 = x2d.new_empty((M, K // 2), dtype=torch.uint8)
+    blocks = x2d.new_empty(_fp4_blocks_shape(M, K), dtype=E4M3)
+    scale = x2d.new_empty((M, 1), dtype=torch.float32)
     if M:
         rc = _launch(dev, lib.mh3_quantize_fp4, x2d.data_ptr(), x2d.stride(0), _FLOAT_CODE[x2d.dtype], M, K, x4.data_ptr(),
                      blocks.data_ptr(), scale.data_ptr())
@@ -760,7 +760,7 @@ def dequantize_fp4(x4: torch.Tensor, blocks: torch.Tensor, scale: torch.Tensor,
         raise ValueError("dequantize_fp4: dtype must be bfloat16 or float32")
     _require_cuda(x4)
     lib = _lib.load()
-    out = torch.empty((M, K), dtype=dtype, device=x4.device)
+    out = x4.new_empty((M, K), dtype=dtype)
     if M:
         rc = _launch(x4.device, lib.mh3_dequantize_fp4, x4.data_ptr(), blocks.data_ptr(), scale.data_ptr(), M, K,
                      _FLOAT_CODE[dtype], out.data_ptr())
@@ -854,9 +854,9 @@ def fp4_linear(x2d: torch.Tensor, w4: torch.Tensor, w_blocks: torch.Tensor, w_sc
         if bias.dtype != torch.bfloat16 or not bias.is_contiguous():
             bias = bias.to(torch.bfloat16).contiguous()
     lib = _lib.load()
-    out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+    out = x2d.new_empty((M, N), dtype=torch.bfloat16)
     nbytes = lib.mh3_fp4_linear_workspace_bytes(M, K)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    ws = x2d.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     rc = _launch(dev, lib.mh3_fp4_linear, x2d.data_ptr(), x2d.stride(0), _FLOAT_CODE[x2d.dtype], M, N, K, w4.data_ptr(),
                  w_blocks.data_ptr(), w_scale.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), N,
                  None if ws is None else ws.data_ptr())
@@ -1000,9 +1000,9 @@ def block_norm_fwd(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm: i
     """``mh3_block_norm_fwd``: the list of r (with y), h (unless norm is 0) and stats (when wanted).
 
     gate, scale, shift: [groups, C] (any stride), or with ``per_token`` of x's shape."""
-    r = torch.empty(x.shape, dtype=x.dtype, device=x.device) if y is not None else None
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if norm else None
-    stats = torch.empty((x.numel() // x.shape[-1], 4), dtype=torch.float32, device=x.device) if want_stats else None
+    r = x.new_empty(x.shape) if y is not None else None  # (new_empty: half the time of torch.empty)
+    h = x.new_empty(x.shape) if norm else None
+    stats = x.new_empty((x.numel() // x.shape[-1], 4), dtype=torch.float32) if want_stats else None
     a, keep = _norm_args(x, y, gate, scale, shift, weight, bias, y_weight, cu, max(norm, 1), y_norm, eps, alpha, per_token, r, h,
                          stats)
     rc = _launch(x.device, _lib.load().mh3_block_norm_fwd, a)
@@ -1016,12 +1016,12 @@ def block_norm_bwd(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu,
     y_weight) that are given and whose entry of ``want`` is true; dr or dh may be None."""
     dr, dh = (d if d is None or d.dtype == x.dtype else d.to(x.dtype) for d in (dr, dh))
     ts = (x, y, gate, scale, shift, weight, bias, y_weight)
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if w and t is not None else None for t, w in zip(ts, want)]
+    grads = [t.new_empty(t.shape) if w and t is not None else None for t, w in zip(ts, want)]
     lib = _lib.load()
 
     def workspace(rows, C, groups):
         nbytes = max(16, lib.mh3_block_norm_workspace_bytes(rows, C, groups))
-        return torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        return x.new_empty(nbytes, dtype=torch.uint8)
 
     a, keep = _norm_args(*ts, cu, max(norm, 1), y_norm, eps, alpha, per_token, None, None, stats, dr, dh, grads, workspace)
     rc = _launch(x.device, lib.mh3_block_norm_bwd, a)
