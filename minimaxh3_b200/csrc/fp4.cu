@@ -10,22 +10,22 @@
 //   scale  = 2^max(-100, ceil(log2(absmax_row / 2688)))       2688 = 448 * 6
 //   block  = e4m3(absmax_16 / (6 scale)),  code = e2m1(x / (block scale))
 //
-// Both quotients are correctly rounded (Markstein's step, see quant.cu's
-// div_rn_by) and then rounded to nearest even: for bf16 and f16 input a quotient
-// lies on a border exactly when the true one does, so the bytes are those of the
-// definition.  With M in [1, 2) and absmax = M 2^E, absmax / 2688 = (M / 1.3125)
+// Both quotients are correctly rounded (the first by Markstein's step, see quant.cu's
+// div_rn_by; the second in round_block) and then rounded to nearest even, so the bytes
+// are those of the definition.  With M in [1, 2) and absmax = M 2^E, absmax / 2688 = (M / 1.3125)
 // 2^(E-11): the exponent is E - 11, one more if M > 1.3125 - integer compares.
 //
-// Bound: HBM, 2 bytes in and 0.5625 out per 16-bit element, once the instructions
-// of a block (about 110) fit beside it.  A thread owns the 16 elements of a block, so
-// the block's maximum needs no exchange.  CTAs are persistent and take four rows 32
+// Bound: instruction issue (74 % of its slots) beside HBM, 2 bytes in and 0.5625 out
+// per 16-bit element: 206 us = 5.6 TB/s at 32760 x 13824.  A thread owns the 16 elements
+// of a block, so the block's maximum needs no exchange.  CTAs are persistent and take four rows 32
 // apart at a time: their maxima share one barrier, and their block scales for 64
 // elements are the 16 neighbouring bytes of the scale layout, written as one
 // vector.  The rows stream through a two-stage ring in shared memory (cp.async),
 // read once for the maxima and once for the rounding.  A warp copies its blocks as
 // neighbouring 16-byte pieces: copied by their owners, two lanes' halves of every
-// 32-byte sector came from L2 twice (362 us against 245 at 32760 x 13824).  Rows too long for that ring, and rows that 16-byte vectors do not fit, are read
-// twice by the general kernel.
+// 32-byte sector came from L2 twice (362 us against 245 before the later steps).  Rows
+// too long for that ring, and rows that 16-byte vectors do not fit, are read twice by
+// the general kernel.  Back: HBM, 172 us = 6.7 TB/s.
 #include <algorithm>
 #include <string>
 
@@ -81,8 +81,14 @@ __global__ void __launch_bounds__(kMaxThreads) quantize_stream_kernel(const T* _
   const int nb = K / 16, nk64 = (K + 63) / 64, b = threadIdx.x;
   const int nthr = blockDim.x * blockDim.y, warps = blockDim.x >> 5, lane = threadIdx.x & 31;
   // [kStages][kQuad][nthr] blocks of W pieces; the warp's 32 blocks are copied piece
-  // by piece, lane after lane, and each lane reads its own block
+  // by piece, lane after lane, and each lane reads its own block.  Piece p lies at
+  // p ^ (p / 8 % W), so that eight lanes W pieces apart read from eight different places
+  // of the 128 bytes a cycle delivers.
   uint4* warp_at = ring + (threadIdx.y * blockDim.x + (threadIdx.x & ~31)) * W;
+  uint4* put_at = warp_at + (lane ^ ((lane >> 3) & (W - 1)));
+  const uint4* get_at[W];
+#pragma unroll
+  for (int w = 0; w < W; ++w) get_at[w] = warp_at + lane * W + (w ^ ((lane * W >> 3) & (W - 1)));
   const int piece0 = (threadIdx.x & ~31) * W + lane;  // of the row's nb W pieces
   const bool in = b < nb;
   const int quads = (int)((M + 127) / 128 * 32);  // of 32 in each block of 128 rows
@@ -99,7 +105,7 @@ __global__ void __launch_bounds__(kMaxThreads) quantize_stream_kernel(const T* _
           for (int w = 0; w < W; ++w)
             if (piece0 + 32 * w < nb * W)
               asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                               smem_u32(warp_at + (st * kQuad + i) * nthr * W + 32 * w + lane)),
+                               smem_u32(put_at + (st * kQuad + i) * nthr * W + 32 * w)),
                            "l"(reinterpret_cast<const uint4*>(src) + piece0 + 32 * w)
                            : "memory");
     }
@@ -116,7 +122,7 @@ __global__ void __launch_bounds__(kMaxThreads) quantize_stream_kernel(const T* _
     const long long row0 = first_row(q);
     auto load = [&](int i, uint4(&u)[W]) {
 #pragma unroll
-      for (int w = 0; w < W; ++w) u[w] = warp_at[(st * kQuad + i) * nthr * W + lane * W + w];
+      for (int w = 0; w < W; ++w) u[w] = get_at[w][(st * kQuad + i) * nthr * W];
     };
     uint32_t own[kQuad], top[kQuad];
 #pragma unroll

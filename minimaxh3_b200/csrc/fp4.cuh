@@ -88,9 +88,10 @@ __device__ __forceinline__ long long block_offset(long long row, int b, int nk64
 
 // One block: its scale byte and 16 codes, from its absmax and the row's exponent.
 // The quotients x / (block scale) are x r + x r', r + r' the reciprocal to 2^-45, in
-// packed pairs: off by 2^-44 before their rounding, so a true quotient on a border of
-// two codes lands on it (it has three bits), and 16-bit input that is not on one is at
-// least 2^-11 of it away.  r and r' carry the row's power of two; rows so large that r'
+// packed pairs: off by 2^-44 before their rounding, and x / s (24 bits by at most four) is
+// at least 2^-29 from the middle of two floats, so they are the correctly rounded ones.
+// (x r alone misses the borders of two codes at s = 15 / 8; three operations with the
+// remainder took 227 us where these two take 209.)  r and r' carry the row's power of two; rows so large that r'
 // would be subnormal are brought down first (exactly: what underflows is far below a code).
 __device__ __forceinline__ uint32_t round_block(float2 (&x)[8], uint32_t top, int e, uint2& code) {
   // e4m3 of absmax / (6 scale): the division by 6 is the only rounding before it
