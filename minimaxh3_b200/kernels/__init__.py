@@ -6,4 +6,6 @@ Importing ``minimaxh3_b200.kernels.attention_router`` / ``.fp8_attention`` /
 ``kernels/fp8_linear.py``; the runtime can alias this package as ``kernels``.
 ``.lora.attach_lora_registry`` is the fused form of the reference's
 ``runtime/lora.py`` wrapper of the unquantised ``nn.Linear`` layers.
+``.rotary``, ``.block_norm`` and ``.fp4_linear`` have no counterpart there: what
+a block does between its linears and attention, and the linears in 4 bits.
 """

@@ -933,20 +933,47 @@ NORM_KINDS = {"none": 0, "rms": 1, "layer": 2}
 # mh3_block_norm_args in one packing (see _ROTARY)
 _NORM = struct.Struct("@2q6i2fP" + "Pq" * 2 + "P2q2i" * 6 + "3P" + "Pq" * 2 + "9P")
 _NO_MOD = (0, 0, 0, 0, 0)
+_NO_ROWS = (0, 0)
+_NO_GRADS = (0,) * 8
 
 
-def _rows2d(t: torch.Tensor) -> torch.Tensor:
-    """[..., C] as rows of contiguous channels a stride apart: contiguous, or [rows, C]."""
-    if t.is_contiguous():
-        return t
-    if t.dim() != 2:
-        t = t.reshape(-1, t.shape[-1])
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+def _row_arg(t: torch.Tensor, C: int, keep: list):
+    """[..., C] as rows of contiguous channels: pointer and stride."""
+    if not t.is_contiguous():
+        if t.dim() != 2:
+            t = t.reshape(-1, C)
+        if t.stride(1) != 1 and C != 1:
+            t = t.contiguous()
+        keep.append(t)
+        if t.shape[0] > 1:
+            return t.data_ptr(), t.stride(0)
+    return t.data_ptr(), C
+
+
+def _mod_arg(m: torch.Tensor, C: int, S: int, per_token: bool, keep: list):
+    """gate, scale or shift: pointer, strides of groups and rows, type."""
+    s = m.stride()
+    if s[-1] != 1 and C != 1:
+        m = m.contiguous()
+        keep.append(m)
+        s = m.stride()
+    if not per_token:
+        return m.data_ptr(), s[0], 0, _FLOAT_CODE[m.dtype], 0
+    if len(s) == 3:  # element (b, s): row b S + s
+        return m.data_ptr(), s[0] - S * s[1], s[1], _FLOAT_CODE[m.dtype], 0
+    return m.data_ptr(), 0, s[0], _FLOAT_CODE[m.dtype], 0
+
+
+def _chan_arg(v: torch.Tensor, keep: list):
+    if not v.is_contiguous():
+        v = v.contiguous()
+        keep.append(v)
+    return v.data_ptr(), 0, 0, _FLOAT_CODE[v.dtype], 0
 
 
 def _norm_args(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_norm, eps, alpha, per_token, r, h, stats,
-               dr=None, dh=None, grads=(None,) * 8, workspace=None):
-    """The C arguments, and the tensors they point into.  ``workspace``: a function of (rows, channels, groups)."""
+               dr=None, dh=None, grads=None, workspace=None):
+    """The C arguments, and the tensors made for them.  ``workspace``: a function of (rows, channels, groups)."""
     shape = x.shape
     C = shape[-1]
     S = shape[1] if len(shape) == 3 else shape[0]
@@ -954,44 +981,25 @@ def _norm_args(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_nor
     if groups == 0:
         groups, group_rows = 1, 0  # an empty batch
     keep = []
-
-    def rows(t):
-        if t is None:
-            return (0, 0)
-        t = _rows2d(t)
-        keep.append(t)
-        return (t.data_ptr(), t.stride(-2) if t.shape[-2] > 1 else C)
-
-    def mod(m):
-        if m is None:
-            return _NO_MOD
-        if m.stride(-1) != 1 and C != 1:
-            m = m.contiguous()
-        keep.append(m)
-        s = m.stride()
-        if not per_token:
-            sg, sr = s[0], 0
-        elif len(s) == 3:  # element (b, s): row b S + s
-            sg, sr = s[0] - S * s[1], s[1]
-        else:
-            sg, sr = 0, s[0]
-        return (m.data_ptr(), sg, sr, _FLOAT_CODE[m.dtype], 0)
-
-    def chan(v):
-        if v is None:
-            return _NO_MOD
-        v = v.contiguous()
-        keep.append(v)
-        return (v.data_ptr(), 0, 0, _FLOAT_CODE[v.dtype], 0)
-
-    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731  (an empty tensor's is null)
     nrows = x.numel() // C
     ws = None if workspace is None else workspace(nrows, C, groups)
-    a = _lib.BlockNormArgs.from_buffer_copy(_NORM.pack(
-        nrows, group_rows, C, groups, _FLOAT_CODE[x.dtype], norm, y_norm, int(per_token), eps, alpha, ptr(cu), *rows(x), *rows(y),
-        *mod(gate), *mod(scale), *mod(shift), *chan(weight), *chan(bias), *chan(y_weight), ptr(r), ptr(h), ptr(stats),
-        *rows(dr), *rows(dh), *map(ptr, grads), ptr(ws)))
     keep.append(ws)
+    a = _lib.BlockNormArgs.from_buffer_copy(_NORM.pack(
+        nrows, group_rows, C, groups, _FLOAT_CODE[x.dtype], norm, y_norm, int(per_token), eps, alpha,
+        0 if cu is None else cu.data_ptr(),
+        *_row_arg(x, C, keep),
+        *(_NO_ROWS if y is None else _row_arg(y, C, keep)),
+        *(_NO_MOD if gate is None else _mod_arg(gate, C, S, per_token, keep)),
+        *(_NO_MOD if scale is None else _mod_arg(scale, C, S, per_token, keep)),
+        *(_NO_MOD if shift is None else _mod_arg(shift, C, S, per_token, keep)),
+        *(_NO_MOD if weight is None else _chan_arg(weight, keep)),
+        *(_NO_MOD if bias is None else _chan_arg(bias, keep)),
+        *(_NO_MOD if y_weight is None else _chan_arg(y_weight, keep)),
+        0 if r is None else r.data_ptr(), 0 if h is None else h.data_ptr(), 0 if stats is None else stats.data_ptr(),
+        *(_NO_ROWS if dr is None else _row_arg(dr, C, keep)),
+        *(_NO_ROWS if dh is None else _row_arg(dh, C, keep)),
+        *(_NO_GRADS if grads is None else [0 if g is None else g.data_ptr() for g in grads]),
+        0 if ws is None else ws.data_ptr()))  # (an empty tensor's pointer is null)
     return a, keep
 
 

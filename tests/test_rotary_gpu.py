@@ -177,6 +177,11 @@ def test_gradient_is_the_inverse_rotation(inter):
     # only one of the two gradients is asked for, and one input without a gradient
     (only,) = torch.autograd.grad(rotary_axes(q, k.detach(), pos, axes, interleaved=inter)[0], q, dq)
     assert torch.equal(only, gq)
+    # twice: the gradient is linear in dq, and its own gradient turns forward
+    d1 = dq.clone().requires_grad_(True)
+    (g1,) = torch.autograd.grad(rotary_axes(q, k, pos, axes, interleaved=inter)[0], q, d1, create_graph=True)
+    assert torch.equal(g1, gq)
+    assert torch.equal(torch.autograd.grad(g1, d1, v)[0], rotary_axes(v, None, pos, axes, interleaved=inter)[0])
     # shared key heads: the gradient of the one head is the sum over its copies
     kv = _rand(25, B, 1, S, D, dtype=torch.float32).requires_grad_(True)
     (gs,) = torch.autograd.grad(rotary_axes(kv.expand(B, H, S, D), None, pos, axes, interleaved=inter)[0], kv, dq)
