@@ -164,6 +164,14 @@ __device__ __forceinline__ void mod8(const void* p, int dt, long long at, int n,
   }
 }
 
+// Eight gradients of a modulation with a row for each row, in its type.
+template <bool VEC>
+__device__ __forceinline__ void put8(void* p, int dt, long long at, int n, const float (&v)[8]) {
+  if (dt == MH3_DTYPE_F32) store8<float, VEC>(static_cast<float*>(p) + at, n, v);
+  else if (dt == MH3_DTYPE_F16) store8<__half, VEC>(static_cast<__half*>(p) + at, n, v);
+  else store8<__nv_bfloat16, VEC>(static_cast<__nv_bfloat16*>(p) + at, n, v);
+}
+
 // A thread's eight values in shared memory, as two float4 a stride of the CTA apart.
 __device__ __forceinline__ void slot_put(float4* s, const float (&v)[8]) {
   s[threadIdx.x] = make_float4(v[0], v[1], v[2], v[3]);
@@ -370,8 +378,9 @@ __global__ void __launch_bounds__(1024) fwd_kernel(const __grid_constant__ Param
   }
 }
 
-template <typename T, bool VEC, bool PT>
-__global__ void __launch_bounds__(1024) bwd_kernel(const __grid_constant__ Params p) {
+// MAXT: 512 where the row's threads allow it (with 64 registers a thread it spills).
+template <typename T, bool VEC, bool PT, int MAXT>
+__global__ void __launch_bounds__(MAXT) bwd_kernel(const __grid_constant__ Params p) {
   extern __shared__ float4 slots[];
   __shared__ float red[2][4][32];
   float4* sA = slots;                   // w (1 + scale)  (PT: w)
@@ -425,13 +434,9 @@ __global__ void __launch_bounds__(1024) bwd_kernel(const __grid_constant__ Param
         if (p.dx) store8<T, VEC>(static_cast<T*>(p.dx) + row * p.C + c, n, d);
         if (p.dy) store8<T, VEC>(static_cast<T*>(p.dy) + row * p.C + c, n, d);
         if constexpr (PT) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i < n) {
-              if (p.dscale) put1(p.dscale, p.scale.dt, row * p.C + c + i, 0.0f);
-              if (p.dshift) put1(p.dshift, p.shift.dt, row * p.C + c + i, 0.0f);
-              if (p.dgate) put1(p.dgate, p.gate.dt, row * p.C + c + i, 0.0f);
-            }
+          if (p.dscale) put8<VEC>(p.dscale, p.scale.dt, row * p.C + c, n, d);
+          if (p.dshift) put8<VEC>(p.dshift, p.shift.dt, row * p.C + c, n, d);
+          if (p.dgate) put8<VEC>(p.dgate, p.gate.dt, row * p.C + c, n, d);
         }
       }
       continue;
@@ -472,19 +477,13 @@ __global__ void __launch_bounds__(1024) bwd_kernel(const __grid_constant__ Param
           float sc[8];
           mod8<VEC>(p.scale.p, p.scale.dt, g * p.scale.sg + row * p.scale.sr + c, n, 0.0f, sc);
           if (p.dscale) {
-            float w[8], b[8], o[8];
+            float b[8], o[8];
             mod8<VEC>(p.b.p, p.b.dt, c, n, 0.0f, b);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = dn[i];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = t[i] * fmaf(xh[i], w[i], b[i]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (i < n) put1(p.dscale, p.scale.dt, row * p.C + c + i, o[i]);
+            for (int i = 0; i < 8; ++i) o[i] = t[i] * fmaf(xh[i], dn[i], b[i]);
+            put8<VEC>(p.dscale, p.scale.dt, row * p.C + c, n, o);
           }
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i < n && p.dshift) put1(p.dshift, p.shift.dt, row * p.C + c + i, t[i]);
+          if (p.dshift) put8<VEC>(p.dshift, p.shift.dt, row * p.C + c, n, t);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float m = t[i] * (1.0f + sc[i]);
@@ -512,13 +511,11 @@ __global__ void __launch_bounds__(1024) bwd_kernel(const __grid_constant__ Param
       for (int i = 0; i < 8; ++i) d[i] = fmaf(st.w, dn[i] - m0 - xh[i] * m1, d[i]);
     }
     if constexpr (PT) {
-      if (!has_dh && live)  // h was not used
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < n) {
-            if (p.dscale) put1(p.dscale, p.scale.dt, row * p.C + c + i, 0.0f);
-            if (p.dshift) put1(p.dshift, p.shift.dt, row * p.C + c + i, 0.0f);
-          }
+      if (!has_dh && live) {  // h was not used
+        const float zero[8] = {};
+        if (p.dscale) put8<VEC>(p.dscale, p.scale.dt, row * p.C + c, n, zero);
+        if (p.dshift) put8<VEC>(p.dshift, p.shift.dt, row * p.C + c, n, zero);
+      }
     }
     if (live && p.dx) {
       const float k = has_y ? p.alpha : 1.0f;
@@ -534,9 +531,10 @@ __global__ void __launch_bounds__(1024) bwd_kernel(const __grid_constant__ Param
           slot_get(sG, wy);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            if (i < n && p.dgate) put1(p.dgate, p.gate.dt, row * p.C + c + i, d[i] * yh[i] * wy[i]);
+            t[i] = d[i] * yh[i] * wy[i];
             a3[i] = fmaf(d[i] * gv[i], yh[i], a3[i]);
           }
+          if (p.dgate) put8<VEC>(p.dgate, p.gate.dt, row * p.C + c, n, t);
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) a3[i] = fmaf(d[i], yh[i], a3[i]);
@@ -1206,10 +1204,11 @@ __global__ void __launch_bounds__(128) chan_kernel(const __grid_constant__ Param
 
 static int threads_of(int C, int ch = 8) { return ((C + ch - 1) / ch + 31) / 32 * 32; }
 
-// CTAs: one of a 5120-channel row's 640 threads per SM, narrow rows to as many
-// threads (up to 16 CTAs).  More CTAs only add partial rows of column sums.
-static int ctas_of(long long rows, int C) {
-  const int per = std::max(1, std::min(16, 640 / threads_of(C)));
+// CTAs: of the streaming kernels one of a 5120-channel row's 640 threads per SM, narrow
+// rows to as many threads (up to 16 CTAs): more only add partial rows of column sums.  The
+// general kernels have no ring, so they hide latency with all the threads that fit.
+static int ctas_of(long long rows, int C, bool general) {
+  const int per = std::max(1, std::min(16, (general ? 1024 : 640) / threads_of(C)));
   return (int)std::min<long long>(rows, (long long)kSMs * per);
 }
 
@@ -1292,7 +1291,11 @@ static cudaError_t launch_bwd(Params& p, cudaStream_t st) {
     bool done = false;
     cudaError_t e = cudaSuccess;
     if constexpr (VEC && !PT) e = p.y ? stream_bwd<T, true>(p, st, done) : stream_bwd<T, false>(p, st, done);
-    if (!done) e = start<bwd_kernel<T, VEC, PT>>(p, threads_of(p.C), (size_t)threads_of(p.C) * 32 * (p.y ? 2 : 1), st);
+    if (!done) {
+      const int nt = threads_of(p.C);
+      const size_t smem = (size_t)nt * 32 * (p.y ? 2 : 1);
+      e = nt <= 512 ? start<bwd_kernel<T, VEC, PT, 512>>(p, nt, smem, st) : start<bwd_kernel<T, VEC, PT, 1024>>(p, nt, smem, st);
+    }
     if (e != cudaSuccess) return e;
   }
   const bool chan = p.dw || p.db || p.dwy;
@@ -1351,6 +1354,8 @@ static int run(const mh3_block_norm_args* a, bool bwd, void* stream) {
   rows_fit(a->dr, a->dr_stride);
   rows_fit(a->dh, a->dh_stride);
   for (const void* q : {(const void*)a->r, (const void*)a->h, (const void*)a->dx, (const void*)a->dy}) rows_fit(q, 0);
+  if (a->per_row)
+    for (const void* q : {(const void*)a->dgate, (const void*)a->dscale, (const void*)a->dshift}) rows_fit(q, 0);
   Mod* mods[3] = {&p.gate, &p.scale, &p.shift};
   const mh3_norm_mod* given[3] = {&a->gate, &a->scale, &a->shift};
   for (int i = 0; i < 3; ++i) {
@@ -1385,12 +1390,12 @@ static int run(const mh3_block_norm_args* a, bool bwd, void* stream) {
   p.ynorm = a->y_norm;
   p.eps = a->eps;
   p.alpha = a->residual_scale;
-  p.ctas = ctas_of(a->rows, a->channels);
+  const bool pt = a->per_row != 0;
+  p.ctas = ctas_of(a->rows, a->channels, pt || !vec);
   p.part = static_cast<float*>(a->workspace);
   if (bwd) p.gsum = p.part + ((long long)p.ctas + p.G) * 3 * p.C;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (a->rows == 0 && !bwd) return MH3_OK;
-  const bool pt = a->per_row != 0;
   const cudaError_t e = a->dtype == MH3_DTYPE_BF16  ? launch<__nv_bfloat16>(p, bwd, vec, pt, st)
                         : a->dtype == MH3_DTYPE_F16 ? launch<__half>(p, bwd, vec, pt, st)
                                                     : launch<float>(p, bwd, vec, pt, st);
@@ -1404,7 +1409,7 @@ using namespace mh3;
 
 extern "C" uint64_t mh3_block_norm_workspace_bytes(int64_t rows, int32_t channels, int32_t groups) {
   if (rows < 0 || channels <= 0 || channels > bnorm::kMaxC || groups <= 0) return 0;
-  return ((uint64_t)bnorm::ctas_of(rows, channels) + 2ull * (uint64_t)groups) * 3 * (uint64_t)channels * sizeof(float);
+  return ((uint64_t)bnorm::ctas_of(rows, channels, true) + 2ull * (uint64_t)groups) * 3 * (uint64_t)channels * sizeof(float);
 }
 
 extern "C" int mh3_block_norm_fwd(const mh3_block_norm_args* a, void* stream) {

@@ -40,7 +40,8 @@ class _NoGradient(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, out, *inputs):
-        return out.view_as(out)
+        ctx.mark_dirty(out)  # out itself, no view of it: callers may add to it in place
+        return out
 
     @staticmethod
     def backward(ctx, grad):

@@ -204,6 +204,9 @@ def test_linear_refuses_gradients():
             out.float().sum().backward()
     with torch.no_grad():
         assert not fp4_linear(x, *w).requires_grad
+    y = fp4_linear(x, *w)
+    y += 1  # the result is not a view that must not be written
+    assert torch.equal(y, fp4_linear(x, *w) + 1)
     bias = _rand(60, 64).to(DEV).requires_grad_(True)
     assert fp4_linear(x.detach(), *w, bias=bias).requires_grad
     f = torch.compile(lambda t: fp4_linear(t, *w), backend="aot_eager")
