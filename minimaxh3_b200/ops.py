@@ -960,7 +960,7 @@ def _mod_arg(m: torch.Tensor, C: int, S: int, per_token: bool, keep: list):
     if not per_token:
         return m.data_ptr(), s[0], 0, _FLOAT_CODE[m.dtype], 0
     if len(s) == 3:  # element (b, s): row b S + s
-        return m.data_ptr(), s[0] - S * s[1], s[1], _FLOAT_CODE[m.dtype], 0
+        return m.data_ptr(), s[0] - S * s[1] if m.shape[0] > 1 else 0, s[1], _FLOAT_CODE[m.dtype], 0
     return m.data_ptr(), 0, s[0], _FLOAT_CODE[m.dtype], 0
 
 

@@ -234,6 +234,61 @@ def test_gradients(B, S, C, dtype, mod, norm, y_norm, per_token):
         _close(g, *want[name], name)
 
 
+@pytest.mark.parametrize("C", [64, 1928, 5120])
+@pytest.mark.parametrize("dtype,mods", [(torch.bfloat16, (torch.float32,) * 3), (torch.bfloat16, (torch.bfloat16,) * 3),
+                                        (torch.float32, (torch.float32, torch.bfloat16, torch.float32))])
+def test_modulation_by_token_of_several_groups(C, dtype, mods):
+    """Rows of one modulation beside groups of another, views of a wider tensor, and more rows than one block's."""
+    from minimaxh3_b200.kernels.block_norm import gated_residual_norm, norm_modulate
+
+    B, S = 3, 331
+    leaf = lambda t: t.requires_grad_(True)
+    x, y = leaf(_rand(110, B, S, C, dtype=dtype)), leaf(_rand(111, B, S, C, dtype=dtype, shift=0.3))
+    wide = _rand(112, B, S, 2 * C, dtype=mods[0], scale=0.3)
+    gate, scale, shift = leaf(wide[..., C:]), leaf(_rand(113, B, C, dtype=mods[1], scale=0.3)), leaf(_rand(114, B, S, C, dtype=mods[2]))
+    per = lambda t: t if t.dim() == 3 else t[:, None].expand(B, S, C)
+    c = Case(x, y, gate=per(gate), scale=per(scale), shift=shift, norm="layer", y_norm="none")
+    r, h = gated_residual_norm(x, y, gate, scale, shift)
+    _close(r, c.r, c.er)
+    _close(h, c.h, c.eh)
+    dr, dh = _rand(115, B, S, C, dtype=dtype), _rand(116, B, S, C, dtype=dtype)
+    names = ("x", "y", "gate", "scale", "shift")
+    want = c.grads(dr, dh, lambda t: t)
+    got = dict(zip(names, torch.autograd.grad((r, h), (x, y, gate, scale, shift), (dr, dh), retain_graph=True)))
+    for name in ("x", "y", "gate", "shift"):
+        _close(got[name], *want[name], name)
+    # the rows' gradients of scale are rounded to its type one by one, and their sum once more
+    terms, err = want["scale"]
+    u = torch.finfo(mods[1]).eps / 2
+    tol = (err + u * (terms.abs() + err)).sum(1) * (1 + u) + u * terms.sum(1).abs() + S * U * terms.abs().sum(1)
+    assert bool(((got["scale"].double() - terms.sum(1)).abs() <= tol).all())
+    # h unused, r unused
+    want = c.grads(dr, None, lambda t: t)
+    for name, g in zip(names, torch.autograd.grad(r, (x, y, gate, scale, shift), dr, retain_graph=True)):
+        if name in ("scale", "shift"):
+            assert bool((g == 0).all())
+        else:
+            _close(g, *want[name], name)
+    want = c.grads(None, dh, lambda t: t)
+    for name, g in zip(("x", "y", "gate", "shift"), torch.autograd.grad(h, (x, y, gate, shift), dh)):
+        _close(g, *want[name], name)
+    # the same rows packed, with rows outside every sequence
+    flat = lambda t: t.detach().reshape(B * S, C)
+    cu = torch.tensor([7, 7, 500, B * S - 20], dtype=torch.int32, device=DEV)
+    sc, sh = leaf(flat(per(scale)).to(mods[0]).clone()), leaf(flat(shift).to(mods[0]).clone())
+    xs = leaf(flat(x).clone())
+    c = Case(xs, scale=sc, shift=sh, norm="rms")
+    h = norm_modulate(xs, sc, sh, norm="rms", cu_seqlens=cu)
+    inside = slice(7, B * S - 20)
+    _close(h[inside], c.h[inside], c.eh[inside])
+    dh = flat(dh)
+    want = c.grads(None, dh, lambda t: t)
+    for name, g in zip(("x", "scale", "shift"), torch.autograd.grad(h, (xs, sc, sh), dh)):
+        _close(g[inside], want[name][0][inside], want[name][1][inside], name)
+        assert bool((g[:7] == 0).all()) and bool((g[B * S - 20:] == 0).all())
+    assert bool((h[:7] == 0).all()) and bool((h[B * S - 20:] == 0).all())
+
+
 def test_gradients_against_differences():
     """The kernel's gradients along random directions, against central differences of the 64-bit forward (step 1e-5:
     the truncation is of order 1e-10, far below f32's 1e-6 of the slope)."""
