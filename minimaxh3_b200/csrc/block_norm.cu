@@ -83,7 +83,9 @@ __device__ __forceinline__ void put1(void* p, int dt, long long i, float v) {
 }
 
 // Eight channels of a row as loaded: converted only where they are used, so a
-// row that waits its turn holds four registers of 16-bit data.
+// row that waits its turn holds four registers of 16-bit data.  VEC: side by side, from
+// channel 8 t of thread t; if not, one in blockDim.x, from channel t, so that a warp's
+// accesses are neighbours all the same.
 template <typename T>
 struct Raw {
   uint4 u[sizeof(T) == 4 ? 2 : 1];
@@ -98,7 +100,7 @@ __device__ __forceinline__ Raw<T> load8(const T* p, int n) {
   } else {
     T e[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = i < n ? p[i] : T(0.0f);
+    for (int i = 0; i < 8; ++i) e[i] = i < n ? p[i * (int)blockDim.x] : T(0.0f);
     memcpy(&r, e, sizeof(r));
   }
   return r;
@@ -141,12 +143,14 @@ __device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 8; ++i) {
       if (i < n) {
-        if constexpr (std::is_same<T, float>::value) p[i] = v[i];
-        else if constexpr (std::is_same<T, __half>::value) p[i] = __float2half_rn(v[i]);
-        else p[i] = __float2bfloat16_rn(v[i]);
+        T& to = p[i * (int)blockDim.x];
+        if constexpr (std::is_same<T, float>::value) to = v[i];
+        else if constexpr (std::is_same<T, __half>::value) to = __float2half_rn(v[i]);
+        else to = __float2bfloat16_rn(v[i]);
       }
+    }
   }
 }
 
@@ -272,8 +276,8 @@ __global__ void __launch_bounds__(1024) fwd_kernel(const __grid_constant__ Param
   float4* sA = slots;                    // w (1 + scale)        (PT: w)
   float4* sB = slots + 2 * blockDim.x;   // b (1 + scale) + shift (PT: b)
   float4* sG = slots + 4 * blockDim.x;   // gate wy              (PT: wy); only with y
-  const int c = threadIdx.x * 8;
-  const int n = max(0, min(8, p.C - c));
+  const int c = VEC ? threadIdx.x * 8 : threadIdx.x;
+  const int n = VEC ? max(0, min(8, p.C - c)) : min(8, (max(0, p.C - c) + (int)blockDim.x - 1) / (int)blockDim.x);
   const bool live = n > 0;
   const long long lo = p.rows * blockIdx.x / p.ctas, hi = p.rows * (blockIdx.x + 1) / p.ctas;
   const bool has_y = p.y != nullptr;
@@ -386,8 +390,8 @@ __global__ void __launch_bounds__(MAXT) bwd_kernel(const __grid_constant__ Param
   __shared__ float red[2][4][32];
   float4* sA = slots;                   // w (1 + scale)  (PT: w)
   float4* sG = slots + 2 * blockDim.x;  // gate wy        (PT: wy); only with y
-  const int c = threadIdx.x * 8;
-  const int n = max(0, min(8, p.C - c));
+  const int c = VEC ? threadIdx.x * 8 : threadIdx.x;
+  const int n = VEC ? max(0, min(8, p.C - c)) : min(8, (max(0, p.C - c) + (int)blockDim.x - 1) / (int)blockDim.x);
   const bool live = n > 0;
   const long long lo = p.rows * blockIdx.x / p.ctas, hi = p.rows * (blockIdx.x + 1) / p.ctas;
   const bool has_y = p.y != nullptr, has_dr = p.dr != nullptr, has_dh = p.dh != nullptr;
