@@ -1313,14 +1313,18 @@ __global__ void __launch_bounds__(MAXT) bwd_stream_kernel(const __grid_constant_
   else if (g >= 0 && g < p.G) flush(g);
 }
 
-// Column sums of group blockIdx.y..: 32 channels x 32 partials at a time.  PT: one
-// "group" holds every CTA's partial.
-constexpr int kParts = 32;
-template <bool PT>
-__global__ void __launch_bounds__(32 * kParts) group_sum_kernel(const __grid_constant__ Params p) {
-  __shared__ float sh[3][kParts][32];
-  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;
+// Column sums of group blockIdx.y..: a CTA takes 8 channels (a sector) of 32 or 128
+// partials at a time, added over a warp's four by shuffles, then over the warps, in a
+// fixed order.  128 where a group has many: 6.4 us against 13.8 for 1480 partials of 320
+// channels, but 7.6 against 5.3 for twice 222 of 1536.  PT: one "group" holds every CTA's
+// partial.
+constexpr int kCols = 8;
+template <bool PT, int PARTS>
+__global__ void __launch_bounds__(kCols * PARTS) group_sum_kernel(const __grid_constant__ Params p) {
+  constexpr int kWarps = kCols * PARTS / 32;
+  __shared__ float sh[3][kWarps][kCols];
+  const int lane = threadIdx.x & (kCols - 1), part = threadIdx.x / kCols;
+  const int c = blockIdx.x * kCols + lane;
   const int groups = PT ? 1 : p.G;
   for (int g = blockIdx.y; g < groups; g += gridDim.y) {
     int i0 = 0, i1 = p.ctas;  // the CTAs whose rows meet the group's
@@ -1340,21 +1344,25 @@ __global__ void __launch_bounds__(32 * kParts) group_sum_kernel(const __grid_con
     float s[3] = {0.0f, 0.0f, 0.0f};
     if (c < p.C) {
 #pragma unroll 4
-      for (int i = i0 + part; i < i1; i += kParts) {
+      for (int i = i0 + part; i < i1; i += PARTS) {
         const float* q = p.part + (long long)(i + (PT ? 0 : g)) * 3 * p.C + c;
 #pragma unroll
         for (int k = 0; k < 3; ++k) s[k] += q[(long long)k * p.C];
       }
     }
 #pragma unroll
-    for (int k = 0; k < 3; ++k) sh[k][part][lane] = s[k];
+    for (int k = 0; k < 3; ++k) {
+#pragma unroll
+      for (int o = kCols; o < 32; o <<= 1) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
+      if ((threadIdx.x & 31) < kCols) sh[k][threadIdx.x >> 5][lane] = s[k];
+    }
     __syncthreads();
     if (part == 0 && c < p.C) {
 #pragma unroll
       for (int k = 0; k < 3; ++k) {
         s[k] = 0.0f;
 #pragma unroll
-        for (int q = 0; q < kParts; ++q) s[k] += sh[k][q][lane];
+        for (int q = 0; q < kWarps; ++q) s[k] += sh[k][q][lane];
         p.gsum[((long long)g * 3 + k) * p.C + c] = s[k];
       }
       if (!PT) {
@@ -1525,8 +1533,9 @@ static cudaError_t launch_bwd(Params& p, cudaStream_t st) {
   }
   const bool chan = p.dw || p.db || p.dwy;
   if (chan || (!PT && (p.dscale || p.dshift || p.dgate))) {
-    const dim3 grid((unsigned)((p.C + 31) / 32), (unsigned)std::min(PT ? 1 : p.G, 65535));
-    group_sum_kernel<PT><<<grid, 32 * kParts, 0, st>>>(p);
+    const dim3 grid((unsigned)((p.C + kCols - 1) / kCols), (unsigned)std::min(PT ? 1 : p.G, 65535));
+    if (p.ctas / (PT ? 1 : p.G) > 256) group_sum_kernel<PT, 128><<<grid, kCols * 128, 0, st>>>(p);
+    else group_sum_kernel<PT, 32><<<grid, kCols * 32, 0, st>>>(p);
     if (chan) chan_kernel<PT><<<(p.C + 127) / 128, 128, 0, st>>>(p);
   }
   return cudaGetLastError();
