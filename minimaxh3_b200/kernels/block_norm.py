@@ -45,28 +45,38 @@ def _(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu, stats, norm,
     return [t.new_empty(t.shape) for t, w in zip(ts, want) if w and t is not None]
 
 
+def _forward(x, *args):
+    return (_ops.block_norm_fwd if _ops.plain(x) else torch.ops.mh3.block_norm)(x, *args)
+
+
+def _gradients(ctx, *grads):
+    saved = ctx.saved_tensors
+    it = iter(grads)
+    dr = None if saved[1] is None else next(it)  # r with y, h with a norm
+    dh = next(it) if ctx.conf[0] else None
+    if dr is None and dh is None:
+        return (None,) * 14
+    want = ctx.needs_input_grad[:8]  # false for what is not a tensor
+    backward = _ops.block_norm_bwd if _ops.plain(dh if dr is None else dr) else torch.ops.mh3.block_norm_backward
+    it = iter(backward(dr, dh, *saved, *ctx.conf, want))
+    return (*(next(it) if w else None for w in want), None, None, None, None, None, None)
+
+
+_gradients_once = once_differentiable(_gradients)
+
+
 class _BlockNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_norm, eps, alpha, per_token):
-        *out, stats = torch.ops.mh3.block_norm(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_norm, eps, alpha,
-                                               per_token, True)
+        *out, stats = _forward(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_norm, eps, alpha, per_token, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, y, gate, scale, shift, weight, bias, y_weight, cu, stats)
         ctx.conf = (norm, y_norm, eps, alpha, per_token)
         return tuple(out)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, *grads):
-        saved = ctx.saved_tensors
-        it = iter(grads)
-        dr = None if saved[1] is None else next(it)  # r with y, h with a norm
-        dh = next(it) if ctx.conf[0] else None
-        if dr is None and dh is None:
-            return (None,) * 14
-        want = ctx.needs_input_grad[:8]  # false for what is not a tensor
-        it = iter(torch.ops.mh3.block_norm_backward(dr, dh, *saved, *ctx.conf, want))
-        return tuple(next(it) if w else None for w in want) + (None,) * 6
+        return (_gradients_once if torch.is_grad_enabled() else _gradients)(ctx, *grads)
 
 
 def _check_stream(what, name, t, like=None):
@@ -146,7 +156,7 @@ def _run(x, y, m, weight, bias, y_weight, cu, norm, y_norm, eps, alpha, per_toke
             per_token)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:8]):
         return _BlockNormFn.apply(*args)
-    return torch.ops.mh3.block_norm(*args, False)
+    return _forward(*args, False)
 
 
 def _finish_checks(what, x, eps):

@@ -88,13 +88,18 @@ def fp4_linear(x: torch.Tensor, w4: torch.Tensor, w_blocks: torch.Tensor, w_scal
         raise ValueError("fp4_linear: the number of output features must be a positive multiple of 8")
     if not x.is_cuda or x.device != w4.device:
         raise ValueError("fp4_linear: x and the weight must be on one CUDA device")
-    out = torch.ops.mh3.fp4_linear(x.reshape(-1, K), w4, w_blocks, w_scale, bias, [a for a, _, _ in adapters],
-                                   [b for _, b, _ in adapters], [float(s) for _, _, s in adapters])
+    x2d = x if x.dim() == 2 else x.reshape(-1, K)
+    asks = []
     if torch.is_grad_enabled():
         asks = [t for t in (x, bias, *(t for a, b, _ in adapters for t in (a, b))) if t is not None and t.requires_grad]
+    if not asks and _ops.plain(x):
+        out = _ops.fp4_linear(x2d, w4, w_blocks, w_scale, bias, adapters)
+    else:
+        out = torch.ops.mh3.fp4_linear(x2d, w4, w_blocks, w_scale, bias, [a for a, _, _ in adapters], [b for _, b, _ in adapters],
+                                       [float(s) for _, _, s in adapters])
         if asks:
             out = _NoGradient.apply(out, *asks)
-    return out.reshape(*x.shape[:-1], N)
+    return out if x.dim() == 2 else out.reshape(*x.shape[:-1], N)
 
 
 class FP4Linear(nn.Module):

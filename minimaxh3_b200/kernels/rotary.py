@@ -30,6 +30,10 @@ def _rotary_cuda(q, k, positions, axes_dim, theta, interleaved, inverse):
 _LIB.impl("rotary_axes", _rotary_cuda, "CUDA")
 
 
+def _turn(q, *args):
+    return (_rotary_cuda if _ops.plain(q) else torch.ops.mh3.rotary_axes)(q, *args)
+
+
 @torch.library.register_fake("mh3::rotary_axes", lib=_LIB)
 def _(q, k, positions, axes_dim, theta, interleaved, inverse):
     return torch.empty_like(q), q.new_empty(0) if k is None else torch.empty_like(k)
@@ -41,12 +45,12 @@ class _RotaryFn(torch.autograd.Function):
         ctx.save_for_backward(positions)
         ctx.rest = (axes_dim, theta, interleaved)
         ctx.inverse, ctx.has_k = inverse, k is not None
-        return torch.ops.mh3.rotary_axes(q, k, positions, axes_dim, theta, interleaved, inverse)
+        return _turn(q, k, positions, axes_dim, theta, interleaved, inverse)
 
     @staticmethod
     def backward(ctx, gq, gk):
         (positions,) = ctx.saved_tensors
-        turn = _RotaryFn.apply if torch.is_grad_enabled() else torch.ops.mh3.rotary_axes  # with create_graph: its own gradient
+        turn = _RotaryFn.apply if torch.is_grad_enabled() else _turn  # with create_graph: its own gradient
         dq, dk = turn(gq, gk if ctx.has_k else None, positions, *ctx.rest, not ctx.inverse)
         return dq, dk if ctx.has_k else None, None, None, None, None, None
 
@@ -129,5 +133,5 @@ def rotary_axes(
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         oq, ok = _RotaryFn.apply(q, k, positions, axes, thetas, bool(interleaved), False)
     else:
-        oq, ok = torch.ops.mh3.rotary_axes(q, k, positions, axes, thetas, bool(interleaved), False)
+        oq, ok = _turn(q, k, positions, axes, thetas, bool(interleaved), False)
     return oq, None if k is None else ok
