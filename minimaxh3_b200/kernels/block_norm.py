@@ -95,15 +95,17 @@ def _check_cu(what, x, cu):
         raise ValueError(f"{what}: cu_seqlens needs packed x [T, C]")
 
 
-def _modulation(what, x, cu, mods):
-    """The named modulation tensors as [groups, C] each, or of x's shape each if one of them has a row for each token."""
-    C = x.shape[-1]
+def _modulation(what, x, cu, gate, scale, shift):
+    """gate, scale and shift as [groups, C] each, or of x's shape each if one of them has a row for each token."""
+    C, device = x.shape[-1], x.device
     groups = cu.numel() - 1 if cu is not None else x.shape[0] if x.dim() == 3 else 1
-    if all(m is None or (isinstance(m, torch.Tensor) and m.shape == (groups, C) and m.dtype in _TYPES and m.device == x.device)
-           for m in mods.values()):  # the common form
-        return mods, False
+    for m in (gate, scale, shift):
+        if m is not None and not (isinstance(m, torch.Tensor) and m.shape == (groups, C) and m.dtype in _TYPES and m.device == device):
+            break
+    else:  # the common form
+        return gate, scale, shift, False
     out, per_token = {}, False
-    for name, m in mods.items():
+    for name, m in (("gate", gate), ("scale", scale), ("shift", shift)):
         if m is None:
             out[name] = None
             continue
@@ -141,21 +143,19 @@ def _modulation(what, x, cu, mods):
         else:
             m = (m if m.dim() == 1 or x.dim() == 2 else m.unsqueeze(1)).expand(x.shape)
         out[name] = m
-    return out, per_token
+    return out["gate"], out["scale"], out["shift"], per_token
 
 
-def _channels(what, x, vecs):
-    for name, v in vecs.items():
-        if v is not None and (not isinstance(v, torch.Tensor) or v.dtype not in _TYPES or tuple(v.shape) != (x.shape[-1],)
-                              or v.device != x.device):
-            raise ValueError(f"{what}: {name} must be a bf16, f16 or f32 tensor [C] on x's device")
+def _channels(what, x, name, v):
+    if not isinstance(v, torch.Tensor) or v.dtype not in _TYPES or v.shape != x.shape[-1:] or v.device != x.device:
+        raise ValueError(f"{what}: {name} must be a bf16, f16 or f32 tensor [C] on x's device")
 
 
-def _run(x, y, m, weight, bias, y_weight, cu, norm, y_norm, eps, alpha, per_token):
-    args = (x, y, m.get("gate"), m["scale"], m["shift"], weight, bias, y_weight, cu, norm, y_norm, float(eps), float(alpha),
-            per_token)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:8]):
-        return _BlockNormFn.apply(*args)
+def _run(*args):
+    if torch.is_grad_enabled():
+        for t in args[:8]:
+            if t is not None and t.requires_grad:
+                return _BlockNormFn.apply(*args)
     return _forward(*args, False)
 
 
@@ -195,11 +195,14 @@ def norm_modulate(
     _check_cu(what, x, cu_seqlens)
     if norm not in ("layer", "rms"):
         raise ValueError(f"{what}: norm must be 'layer' or 'rms'")
-    m, per_token = _modulation(what, x, cu_seqlens, {"scale": scale, "shift": shift})
-    _channels(what, x, {"weight": weight, "bias": bias})
+    _, scale, shift, per_token = _modulation(what, x, cu_seqlens, None, scale, shift)
+    if weight is not None:
+        _channels(what, x, "weight", weight)
+    if bias is not None:
+        _channels(what, x, "bias", bias)
     _finish_checks(what, x, eps)
     cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-    return _run(x, None, m, weight, bias, None, cu, _ops.NORM_KINDS[norm], 0, eps, 1.0, per_token)[0]
+    return _run(x, None, None, scale, shift, weight, bias, None, cu, _ops.NORM_KINDS[norm], 0, float(eps), 1.0, per_token)[0]
 
 
 def gated_residual_norm(
@@ -235,13 +238,16 @@ def gated_residual_norm(
     _check_cu(what, x, cu_seqlens)
     if norm not in _ops.NORM_KINDS or y_norm not in _ops.NORM_KINDS:
         raise ValueError(f"{what}: norm and y_norm must be 'none', 'rms' or 'layer'")
-    if norm == "none" and any(t is not None for t in (scale, shift, weight, bias)):
+    if norm == "none" and not (scale is shift is weight is bias is None):
         raise ValueError(f"{what}: scale, shift, weight and bias need a norm")
     if y_norm == "none" and y_weight is not None:
         raise ValueError(f"{what}: y_weight needs y_norm")
-    m, per_token = _modulation(what, x, cu_seqlens, {"gate": gate, "scale": scale, "shift": shift})
-    _channels(what, x, {"weight": weight, "bias": bias, "y_weight": y_weight})
+    gate, scale, shift, per_token = _modulation(what, x, cu_seqlens, gate, scale, shift)
+    for name, v in (("weight", weight), ("bias", bias), ("y_weight", y_weight)):
+        if v is not None:
+            _channels(what, x, name, v)
     _finish_checks(what, x, eps)
     cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-    out = _run(x, y, m, weight, bias, y_weight, cu, _ops.NORM_KINDS[norm], _ops.NORM_KINDS[y_norm], eps, residual_scale, per_token)
+    out = _run(x, y, gate, scale, shift, weight, bias, y_weight, cu, _ops.NORM_KINDS[norm], _ops.NORM_KINDS[y_norm], float(eps),
+               float(residual_scale), per_token)
     return out[0], None if norm == "none" else out[1]
