@@ -9,6 +9,7 @@ differentiable (the gradient is the inverse rotation, the same kernel).
 """
 from __future__ import annotations
 
+import math
 import typing
 
 import torch
@@ -64,37 +65,45 @@ class Rotary(typing.NamedTuple):
     interleaved: bool = True
 
 
-def _plan(axes_dim: tuple, theta) -> tuple[list[int], list[float]]:
+_AXES = "rotary_axes: axes_dim is 1 to 4 even widths whose sum is positive and at most the head dim"
+
+
+def _plan(axes_dim, theta, D: int) -> tuple[list[int], list[float]]:
     """The axes' widths and thetas as lists, checked."""
-    axes = [int(d) for d in axes_dim]
-    if not 1 <= len(axes) <= 4 or any(d < 0 or d % 2 for d in axes) or not 0 < sum(axes):
-        raise ValueError("rotary_axes: axes_dim is 1 to 4 even widths whose sum is positive and at most the head dim")
-    thetas = [float(t) for t in theta] if isinstance(theta, tuple) else [float(theta)] * len(axes)
-    if len(thetas) != len(axes) or any(not 0.0 < t <= 1e300 for t in thetas):
+    axes, total = [], 0
+    for d in axes_dim:
+        d = int(d)
+        if d < 0 or d % 2:
+            raise ValueError(_AXES)
+        axes.append(d)
+        total += d
+    if not 1 <= len(axes) <= 4 or not 0 < total <= D:
+        raise ValueError(_AXES)
+    thetas = [float(theta)] * len(axes) if isinstance(theta, (int, float)) else [float(t) for t in theta]
+    if len(thetas) != len(axes) or not 0.0 < min(thetas) <= max(thetas) <= 1e300 or math.isnan(sum(thetas)):
         raise ValueError("rotary_axes: theta is one positive number, or one for each axis")
     return axes, thetas
 
 
+def _shape(name, t):
+    if not isinstance(t, torch.Tensor) or t.dim() not in (3, 4):
+        raise ValueError(f"rotary_axes: {name} must be a tensor [B, H, S, D] or packed [T, H, D]")
+    if t.dtype not in _TYPES:
+        raise ValueError(f"rotary_axes: unsupported dtype {t.dtype} (bf16, f16 or f32)")
+    return t.shape
+
+
 def _check(q, k, positions, axes_dim, theta):
-    for name, t in (("q", q), ("k", k)):
-        if t is None and name == "k":
-            continue
-        if not isinstance(t, torch.Tensor) or t.dim() not in (3, 4):
-            raise ValueError(f"rotary_axes: {name} must be a tensor [B, H, S, D] or packed [T, H, D]")
-        if t.dtype not in _TYPES:
-            raise ValueError(f"rotary_axes: unsupported dtype {t.dtype} (bf16, f16 or f32)")
-    shape, dev = q.shape, q.device
+    shape, dev = _shape("q", q), q.device
     packed = len(shape) == 3
     tokens, D = shape[0] if packed else shape[2], shape[-1]
     if k is not None:
-        ks = k.shape
+        ks = _shape("k", k)
         if len(ks) != len(shape) or k.dtype != q.dtype or k.device != dev or ks[-1] != D:
             raise ValueError("rotary_axes: q and k must agree in dimensions, dtype, device and head dim")
         if (ks[0] if packed else ks[2]) != tokens or (not packed and ks[0] != shape[0]):
             raise ValueError("rotary_axes: q and k must have the same tokens")
-    axes, thetas = _plan(tuple(axes_dim), theta if isinstance(theta, (int, float)) else tuple(theta))
-    if sum(axes) > D:
-        raise ValueError("rotary_axes: axes_dim is 1 to 4 even widths whose sum is positive and at most the head dim")
+    axes, thetas = _plan(axes_dim, theta, D)
     if D > 256:
         raise ValueError("rotary_axes: the head dim must be at most 256")
     if not isinstance(positions, torch.Tensor) or positions.dtype not in _POS_TYPES:

@@ -891,28 +891,33 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
     ``axes_dim`` and ``theta`` are sequences of one value per axis, positions
     [S, axes] / [B, S, axes] (packed: [T, axes]).  Outputs take the inputs'
     dimension order; ``out_q`` / ``out_k`` may be q / k themselves."""
-    ptrs, outs, copies = [], [], []
+    rows = []  # of Q, Q', K and K': pointer and strides of batch, heads and tokens
+    outs, copies = [], []
     for t, o in ((q, out_q), (k, out_k)):
         if t is None:
-            ptrs += [0] * 8
+            rows += [0] * 8
             outs.append(None)
             continue
-        if t.stride(-1) != 1 and t.shape[-1] != 1:
+        s = t.stride()
+        if s[-1] != 1 and t.shape[-1] != 1:
             t = t.contiguous()
+            copies.append(t)  # alive until the launch
+            s = t.stride()
         if o is None:
             o = torch.empty_like(t)
-            if o.stride(-1) != 1 and o.shape[-1] != 1:
+            so = o.stride()
+            if so[-1] != 1 and o.shape[-1] != 1:
                 o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+                so = o.stride()
         elif o.shape != t.shape or o.dtype != t.dtype or o.device != t.device or o.stride(-1) != 1:
             raise ValueError("rotary: an output must match its input, with contiguous channels")
-        s, so = t.stride(), o.stride()
+        else:
+            so = o.stride()
         if len(s) == 4:
-            ptrs += [t.data_ptr(), s[0], s[1], s[2], o.data_ptr(), so[0], so[1], so[2]]
+            rows += [t.data_ptr(), s[0], s[1], s[2], o.data_ptr(), so[0], so[1], so[2]]
         else:  # packed [T, H, D]
-            ptrs += [t.data_ptr(), 0, s[1], s[0], o.data_ptr(), 0, so[1], so[0]]
+            rows += [t.data_ptr(), 0, s[1], s[0], o.data_ptr(), 0, so[1], so[0]]
         outs.append(o)
-        if t is not q and t is not k:
-            copies.append(t)  # alive until the launch
     shape = q.shape
     if len(shape) == 3:
         batch, seqlen = 1, shape[0]
@@ -928,7 +933,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
     a = _lib.RotaryArgs.from_buffer_copy(_ROTARY.pack(
         batch, seqlen, shape[1], 0 if k is None else k.shape[1], shape[-1], _FLOAT_CODE[q.dtype], _POS_KIND[positions.dtype], n,
         int(interleaved), int(inverse), *axes_dim, *(0,) * (4 - n), *theta, *(0.0,) * (4 - n),
-        *ptrs[0:4], *ptrs[8:12], *ptrs[4:8], *ptrs[12:16], positions.data_ptr(), pos_b, ps[-2]))
+        *rows[0:4], *rows[8:12], *rows[4:8], *rows[12:16], positions.data_ptr(), pos_b, ps[-2]))
     rc = _launch(q.device, _lib.load().mh3_rotary, a)
     _lib.check(rc, "mh3_rotary")
     return outs[0], outs[1]
