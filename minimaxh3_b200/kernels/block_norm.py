@@ -55,11 +55,11 @@ def _gradients(ctx, *grads):
     dr = None if saved[1] is None else next(it)  # r with y, h with a norm
     dh = next(it) if ctx.conf[0] else None
     if dr is None and dh is None:
-        return (None,) * 14
+        return (None,) * 10
     want = ctx.needs_input_grad[:8]  # false for what is not a tensor
     backward = _ops.block_norm_bwd if _ops.plain(dh if dr is None else dr) else torch.ops.mh3.block_norm_backward
     it = iter(backward(dr, dh, *saved, *ctx.conf, want))
-    return (*(next(it) if w else None for w in want), None, None, None, None, None, None)
+    return (*[next(it) if w else None for w in want], None, None)
 
 
 _gradients_once = once_differentiable(_gradients)
@@ -67,11 +67,11 @@ _gradients_once = once_differentiable(_gradients)
 
 class _BlockNormFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_norm, eps, alpha, per_token):
-        *out, stats = _forward(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_norm, eps, alpha, per_token, True)
+    def forward(ctx, x, y, gate, scale, shift, weight, bias, y_weight, cu, conf):
+        *out, stats = _forward(x, y, gate, scale, shift, weight, bias, y_weight, cu, *conf, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, y, gate, scale, shift, weight, bias, y_weight, cu, stats)
-        ctx.conf = (norm, y_norm, eps, alpha, per_token)
+        ctx.conf = conf
         return tuple(out)
 
     @staticmethod
@@ -155,7 +155,7 @@ def _run(*args):
     if torch.is_grad_enabled():
         for t in args[:8]:
             if t is not None and t.requires_grad:
-                return _BlockNormFn.apply(*args)
+                return _BlockNormFn.apply(*args[:9], args[9:])
     return _forward(*args, False)
 
 
