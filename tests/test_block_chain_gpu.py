@@ -193,3 +193,42 @@ def test_training_step_is_captured():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(ref, cap)) and r.requires_grad
+
+
+def test_operators_seen_by_a_dispatch_mode():
+    """Under a mode that watches operators they go through the dispatcher, with the same results."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from minimaxh3_b200.kernels.block_norm import gated_residual_norm, norm_modulate
+    from minimaxh3_b200.kernels.fp4_linear import fp4_linear, quantize_fp4
+    from minimaxh3_b200.kernels.rotary import rotary_axes
+
+    class Watch(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.seen = set()
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.seen.add(func.name())
+            return func(*args, **(kwargs or {}))
+
+    g = torch.Generator().manual_seed(7)
+    rnd = lambda *s: torch.randn(*s, generator=g).to(torch.bfloat16).cuda()  # noqa: E731
+    x, y, gate, q, k = rnd(2, 33, 64), rnd(2, 33, 64), rnd(2, 64), rnd(2, 4, 33, 32), rnd(2, 2, 33, 32)
+    pos = torch.arange(33, dtype=torch.int32).view(33, 1).cuda()
+    w = quantize_fp4(rnd(48, 64))
+
+    def run():
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, y, gate, q, k)]
+        a, b, c, d, e = leaves
+        r, h = gated_residual_norm(a, b, c)
+        outs = (r, norm_modulate(h, c), *rotary_axes(d, e, pos, (32,)))
+        grads = torch.autograd.grad(outs, leaves, [torch.ones_like(o) for o in outs])
+        with torch.no_grad():
+            return [*outs, *grads, fp4_linear(x, *w)]
+
+    plain, watch = run(), Watch()
+    with watch:
+        seen = run()
+    assert all(torch.equal(a, b) for a, b in zip(plain, seen, strict=True))
+    assert {"mh3::block_norm", "mh3::rotary_axes", "mh3::fp4_linear"} <= watch.seen
