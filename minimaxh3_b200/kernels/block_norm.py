@@ -45,8 +45,8 @@ def _(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu, stats, norm,
     return [t.new_empty(t.shape) for t, w in zip(ts, want) if w and t is not None]
 
 
-def _forward(x, *args):
-    return (_ops.block_norm_fwd if _ops.plain(x) else torch.ops.mh3.block_norm)(x, *args)
+def _forward(*args):
+    return (_ops.block_norm_fwd if _ops.plain(*args[:9]) else torch.ops.mh3.block_norm)(*args)
 
 
 def _gradients(ctx, *grads):
@@ -57,7 +57,7 @@ def _gradients(ctx, *grads):
     if dr is None and dh is None:
         return (None,) * 10
     want = ctx.needs_input_grad[:8]  # false for what is not a tensor
-    backward = _ops.block_norm_bwd if _ops.plain(dh if dr is None else dr) else torch.ops.mh3.block_norm_backward
+    backward = _ops.block_norm_bwd if _ops.plain(dr, dh, *saved) else torch.ops.mh3.block_norm_backward
     it = iter(backward(dr, dh, *saved, *ctx.conf, want))
     return (*[next(it) if w else None for w in want], None, None)
 

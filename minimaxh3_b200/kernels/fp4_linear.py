@@ -92,7 +92,7 @@ def fp4_linear(x: torch.Tensor, w4: torch.Tensor, w_blocks: torch.Tensor, w_scal
     asks = []
     if torch.is_grad_enabled():
         asks = [t for t in (x, bias, *(t for a, b, _ in adapters for t in (a, b))) if t is not None and t.requires_grad]
-    if not asks and _ops.plain(x):
+    if not asks and _ops.plain(x, w4, w_blocks, w_scale, bias, *(t for a, b, _ in adapters for t in (a, b))):
         out = _ops.fp4_linear(x2d, w4, w_blocks, w_scale, bias, adapters, checked=True)
     else:
         out = torch.ops.mh3.fp4_linear(x2d, w4, w_blocks, w_scale, bias, [a for a, _, _ in adapters], [b for _, b, _ in adapters],

@@ -31,8 +31,8 @@ def _rotary_cuda(q, k, positions, axes_dim, theta, interleaved, inverse):
 _LIB.impl("rotary_axes", _rotary_cuda, "CUDA")
 
 
-def _turn(q, *args):
-    return (_rotary_cuda if _ops.plain(q) else torch.ops.mh3.rotary_axes)(q, *args)
+def _turn(q, k, positions, *args):
+    return (_rotary_cuda if _ops.plain(q, k, positions) else torch.ops.mh3.rotary_axes)(q, k, positions, *args)
 
 
 @torch.library.register_fake("mh3::rotary_axes", lib=_LIB)

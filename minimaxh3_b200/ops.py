@@ -71,14 +71,24 @@ def _launch(dev: torch.device, fn, *args) -> int:
         return fn(*args, _stream(dev))
 
 
-_modes = getattr(torch._C, "_len_torch_dispatch_stack", lambda: 1)
+# The dispatch keys that are always there; tracing, dispatch modes, vmap and the other function transforms add theirs.
+_USUAL = 0
+for _key in (torch._C.DispatchKey.BackendSelect, torch._C.DispatchKey.ADInplaceOrView):
+    _USUAL |= torch._C.DispatchKeySet(_key).raw_repr()
+_included = torch._C._dispatch_tls_local_include_set
+_PLAIN = (torch.Tensor, torch.nn.Parameter, type(None))
 
 
-def plain(t: torch.Tensor) -> bool:
-    """Whether an operator on t may skip the dispatcher, whose way into a Python kernel costs a small
-    call 5 of its 25 us: a plain tensor, and nothing traces or intercepts operators."""
-    kind = type(t)
-    return (kind is torch.Tensor or kind is torch.nn.Parameter) and not torch.compiler.is_compiling() and not _modes()
+def plain(*ts) -> bool:
+    """Whether an operator on these tensors (None where one is left out) may skip the dispatcher, whose
+    way into a Python kernel costs a small call 5 of its 25 us: plain tensors, and nothing traces,
+    transforms or intercepts operators."""
+    if torch.compiler.is_compiling() or _included().raw_repr() & ~_USUAL:
+        return False
+    for t in ts:
+        if type(t) not in _PLAIN:
+            return False
+    return True
 
 
 _FLOAT_CODE = {torch.bfloat16: _lib.MH3_DTYPE_BF16, torch.float16: _lib.MH3_DTYPE_F16, torch.float32: _lib.MH3_DTYPE_F32}

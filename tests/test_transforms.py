@@ -1,0 +1,140 @@
+"""The block operators where something traces, transforms or intercepts operators.
+
+Plain calls go to the kernels directly; under ``torch.jit.trace``, ``torch.vmap``, the function
+transforms and tensor subclasses they have to go through the dispatcher, which serves those.
+"""
+import warnings
+
+import pytest
+import torch
+
+from minimaxh3_b200 import ops
+
+DEV = "cuda"
+
+
+class _Sub(torch.Tensor):
+    pass
+
+
+def test_plain_tensors_are_plain():
+    x = torch.zeros(2, 3)
+    assert ops.plain(x) and ops.plain(x, None, torch.nn.Parameter(x)) and ops.plain()
+    with torch.no_grad():
+        assert ops.plain(x)
+    with torch.inference_mode():
+        assert ops.plain(x, torch.zeros(2))
+    with torch.autocast("cpu"):
+        assert ops.plain(x)
+    assert not ops.plain(x.as_subclass(_Sub)) and not ops.plain(x, None, x.as_subclass(_Sub))
+
+
+def test_what_traces_or_transforms_is_not_plain():
+    x = torch.zeros(2, 3)
+    seen = []
+
+    def f(t):
+        seen.append(ops.plain(x) or ops.plain(t))
+        return (t * 2).sum()
+
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        torch.jit.trace(f, (x,), check_trace=False)
+    torch.vmap(f)(x)
+    torch.func.grad(f)(x)
+    torch.func.jvp(f, (x,), (x,))
+    torch.func.functionalize(f)(x)
+    assert seen == [False] * 5
+
+
+def test_a_batched_backward_is_not_plain():
+    seen = []
+
+    class Double(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, a):
+            return a * 2
+
+        @staticmethod
+        def backward(ctx, g):
+            seen.append(ops.plain(g))
+            return g * 2
+
+    x = torch.zeros(3, requires_grad=True)
+    g, = torch.autograd.grad(Double.apply(x), x, torch.eye(3), is_grads_batched=True)
+    assert seen == [False] and torch.equal(g, 2 * torch.eye(3))
+
+
+def _rand(seed, *shape, dtype=torch.bfloat16):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype).to(DEV)
+
+
+def _pos(n):
+    return torch.arange(2 * n, dtype=torch.int32, device=DEV).view(n, 2)
+
+
+def _calls():
+    """name -> (function, inputs, other inputs)."""
+    from minimaxh3_b200.kernels.block_norm import gated_residual_norm, norm_modulate
+    from minimaxh3_b200.kernels.fp4_linear import fp4_linear, quantize_fp4
+    from minimaxh3_b200.kernels.rotary import rotary_axes
+
+    w, pos, A, B = quantize_fp4(_rand(1, 48, 64)), _pos(9), _rand(2, 8, 64), _rand(3, 48, 8)
+    two = lambda *shapes: [tuple(_rand(10 * s + i, *sh) for i, sh in enumerate(shapes)) for s in (1, 2)]  # noqa: E731
+    return {
+        "rotary": (lambda q, k: rotary_axes(q, k, pos, (16, 16)), *two((1, 4, 9, 32), (1, 2, 9, 32))),
+        "norm": (lambda x, s: norm_modulate(x, s, s), *two((2, 9, 64), (2, 64))),
+        "gated": (lambda x, y, g: gated_residual_norm(x, y, g, y_norm="rms"), *two((2, 9, 64), (2, 9, 64), (2, 64))),
+        "linear": (lambda x: fp4_linear(x, *w), *two((9, 64))),
+        "linear with an adapter": (lambda x: fp4_linear(x, *w, adapters=[(A, B, 0.5)]), *two((9, 64))),
+    }
+
+
+def _same(a, b):
+    a, b = ((t,) if isinstance(t, torch.Tensor) else t for t in (a, b))
+    assert len(a) == len(b) and all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["rotary", "norm", "gated", "linear", "linear with an adapter"])
+def test_traced_calls_compute(name):
+    f, first, second = _calls()[name]
+    with torch.no_grad(), warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        traced = torch.jit.trace(f, first, check_trace=False)
+        assert "mh3::" in str(traced.graph)
+        _same(traced(*first), f(*first))
+        _same(traced(*second), f(*second))
+
+
+@pytest.mark.gpu
+def test_vmap_turns_each_item():
+    from minimaxh3_b200.kernels.rotary import rotary_axes
+
+    q, k, pos = _rand(1, 3, 1, 4, 9, 32), _rand(2, 3, 1, 2, 9, 32), _pos(9)
+    got = torch.vmap(lambda a, b: rotary_axes(a, b, pos, (16, 16)))(q, k)
+    for i in range(3):
+        _same([t[i] for t in got], rotary_axes(q[i], k[i], pos, (16, 16)))
+    # the first tensor plain, a later one mapped
+    got = torch.vmap(lambda b: rotary_axes(q[0], b, pos, (16, 16))[1])(k)
+    _same([got[2]], [rotary_axes(q[0], k[2], pos, (16, 16))[1]])
+
+
+@pytest.mark.gpu
+def test_batched_gradients_of_the_rotation():
+    from minimaxh3_b200.kernels.rotary import rotary_axes
+
+    q, g = _rand(1, 1, 2, 5, 32, dtype=torch.float32).requires_grad_(True), _rand(2, 3, 1, 2, 5, 32, dtype=torch.float32)
+    out = rotary_axes(q, None, _pos(5), (16, 16))[0]
+    got, = torch.autograd.grad(out, q, g, is_grads_batched=True, retain_graph=True)
+    for i in range(3):
+        assert torch.equal(got[i], torch.autograd.grad(out, q, g[i], retain_graph=True)[0])
+
+
+@pytest.mark.gpu
+def test_a_transform_that_cannot_be_served_raises():
+    """An operator that returns a list has no fallback under vmap: an error, not a wrong answer."""
+    from minimaxh3_b200.kernels.block_norm import norm_modulate
+
+    with pytest.raises(RuntimeError, match="atching rule"):
+        torch.vmap(norm_modulate)(_rand(1, 3, 5, 64))
