@@ -7,8 +7,8 @@ an activation rounding plus one tcgen05 GEMM that applies the scales, the bias
 and every adapter's delta and writes bf16 once.  Weights take 0.5625 bytes each.
 
 A 4-bit matrix is three tensors ``(values, blocks, scale)``: see ``quantize_fp4``.
-Registered as ``torch.ops.mh3.fp4_linear`` with a fake implementation for
-``torch.compile``.  Inference only: asking for a gradient raises, as with ``FP8Linear``.
+The functions are registered as operators ``torch.ops.mh3.*`` of the same names with fake
+implementations for ``torch.compile``.  Inference only: asking for a gradient raises, as with ``FP8Linear``.
 """
 from __future__ import annotations
 
@@ -21,18 +21,46 @@ from .fp8_linear import convert_linears
 _LIB = torch.library.Library("mh3", "FRAGMENT")
 _LIB.define("fp4_linear(Tensor x2d, Tensor w4, Tensor w_blocks, Tensor w_scale, Tensor? bias, Tensor[] lora_a, "
             "Tensor[] lora_b, float[] lora_scale) -> Tensor")
+_LIB.define("quantize_fp4(Tensor x2d) -> (Tensor, Tensor, Tensor)")
+_LIB.define("dequantize_fp4(Tensor values, Tensor blocks, Tensor scale, ScalarType dtype) -> Tensor")
+_LIB.define("fp4_matmul(Tensor[] a, Tensor[] b, Tensor? bias) -> Tensor")
 
 
 def _fp4_linear_cuda(x2d, w4, w_blocks, w_scale, bias, lora_a, lora_b, lora_scale):
     return _ops.fp4_linear(x2d, w4, w_blocks, w_scale, bias, list(zip(lora_a, lora_b, lora_scale)))
 
 
+def _fp4_matmul_cuda(a, b, bias):
+    return _ops.fp4_gemm(a, b, bias=bias)
+
+
 _LIB.impl("fp4_linear", _fp4_linear_cuda, "CUDA")
+_LIB.impl("quantize_fp4", _ops.quantize_fp4, "CUDA")
+_LIB.impl("dequantize_fp4", _ops.dequantize_fp4, "CUDA")
+_LIB.impl("fp4_matmul", _fp4_matmul_cuda, "CUDA")
 
 
 @torch.library.register_fake("mh3::fp4_linear", lib=_LIB)
 def _(x2d, w4, w_blocks, w_scale, bias, lora_a, lora_b, lora_scale):
     return x2d.new_empty((x2d.shape[0], w4.shape[0]), dtype=torch.bfloat16)
+
+
+@torch.library.register_fake("mh3::quantize_fp4", lib=_LIB)
+def _(x2d):
+    M, K = x2d.shape
+    return (x2d.new_empty((M, K // 2), dtype=torch.uint8),
+            x2d.new_empty((-(-M // 128), -(-K // 64), 32, 4, 4), dtype=torch.float8_e4m3fn),
+            x2d.new_empty((M, 1), dtype=torch.float32))
+
+
+@torch.library.register_fake("mh3::dequantize_fp4", lib=_LIB)
+def _(values, blocks, scale, dtype):
+    return values.new_empty((values.shape[0], 2 * values.shape[1]), dtype=dtype)
+
+
+@torch.library.register_fake("mh3::fp4_matmul", lib=_LIB)
+def _(a, b, bias):
+    return a[0].new_empty((a[0].shape[0], b[0].shape[0]), dtype=torch.bfloat16)
 
 
 class _NoGradient(torch.autograd.Function):
@@ -59,18 +87,20 @@ def quantize_fp4(x2d: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.T
     at the upper end of e4m3.  Entries of blocks past M and K are 0.  The value is
     code * block * scale; all roundings are to nearest even.  A row that holds an infinity or NaN gets scale NaN.
     """
-    return _ops.quantize_fp4(x2d)
+    return (_ops.quantize_fp4 if _ops.plain(x2d) else torch.ops.mh3.quantize_fp4)(x2d)
 
 
 def dequantize_fp4(values: torch.Tensor, blocks: torch.Tensor, scale: torch.Tensor,
                    dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The [M, K] numbers that a 4-bit matrix stands for (exact in bfloat16 and float32)."""
-    return _ops.dequantize_fp4(values, blocks, scale, dtype)
+    plain = _ops.plain(values, blocks, scale)
+    return (_ops.dequantize_fp4 if plain else torch.ops.mh3.dequantize_fp4)(values, blocks, scale, dtype)
 
 
 def fp4_matmul(a, b, bias: torch.Tensor | None = None) -> torch.Tensor:
     """bf16 ``a b^T + bias`` of two 4-bit matrices ``(values, blocks, scale)``, a [M, K], b [N, K], N a multiple of 8."""
-    return _ops.fp4_gemm(tuple(a), tuple(b), bias=bias)
+    a, b = tuple(a), tuple(b)
+    return (_fp4_matmul_cuda if _ops.plain(*a, *b, bias) else torch.ops.mh3.fp4_matmul)(a, b, bias)
 
 
 def fp4_linear(x: torch.Tensor, w4: torch.Tensor, w_blocks: torch.Tensor, w_scale: torch.Tensor,

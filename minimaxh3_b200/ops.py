@@ -86,7 +86,7 @@ def plain(*ts) -> bool:
     if torch.compiler.is_compiling() or _included().raw_repr() & ~_USUAL:
         return False
     for t in ts:
-        if type(t) not in _PLAIN:
+        if type(t) not in _PLAIN and isinstance(t, torch.Tensor):
             return False
     return True
 

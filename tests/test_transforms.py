@@ -92,7 +92,7 @@ def _calls():
 
 def _same(a, b):
     a, b = ((t,) if isinstance(t, torch.Tensor) else t for t in (a, b))
-    assert len(a) == len(b) and all(torch.equal(u, v) for u, v in zip(a, b))
+    assert len(a) == len(b) and all(u.dtype == v.dtype and torch.equal(u.view(torch.uint8), v.view(torch.uint8)) for u, v in zip(a, b))
 
 
 @pytest.mark.gpu
@@ -138,3 +138,45 @@ def test_a_transform_that_cannot_be_served_raises():
 
     with pytest.raises(RuntimeError, match="atching rule"):
         torch.vmap(norm_modulate)(_rand(1, 3, 5, 64))
+
+
+def test_what_is_no_tensor_is_refused_as_before():
+    from minimaxh3_b200.kernels.fp4_linear import quantize_fp4
+
+    with pytest.raises(ValueError, match="2D"):
+        quantize_fp4([[1.0] * 32])
+
+
+def test_four_bit_conversions_are_operators():
+    """Their shapes and types without data, as a trace or a compiler asks for them."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from minimaxh3_b200.kernels.fp4_linear import dequantize_fp4, fp4_matmul, quantize_fp4
+
+    with FakeTensorMode():
+        x, w = (torch.empty(m, 96, dtype=torch.bfloat16, device=DEV) for m in (130, 16))
+        a, b = quantize_fp4(x), quantize_fp4(w)
+        assert [(tuple(t.shape), t.dtype) for t in a] == [((130, 48), torch.uint8), ((2, 2, 32, 4, 4), torch.float8_e4m3fn), ((130, 1), torch.float32)]
+        for dt in (torch.bfloat16, torch.float32):
+            v = dequantize_fp4(*a, dtype=dt)
+            assert tuple(v.shape) == (130, 96) and v.dtype == dt and v.device.type == DEV
+        out = fp4_matmul(a, b)
+        assert tuple(out.shape) == (130, 16) and out.dtype == torch.bfloat16
+
+
+@pytest.mark.gpu
+def test_traced_and_compiled_four_bit_conversions_compute():
+    from minimaxh3_b200.kernels.fp4_linear import dequantize_fp4, fp4_matmul, quantize_fp4
+
+    w = quantize_fp4(_rand(3, 16, 96))
+
+    def f(x):
+        a = quantize_fp4(x)
+        return (*a, dequantize_fp4(*a), fp4_matmul(a, w))
+
+    x, y = _rand(1, 130, 96), _rand(2, 130, 96)
+    with torch.no_grad(), warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        for g in (torch.jit.trace(f, (x,), check_trace=False), torch.compile(f, backend="aot_eager", fullgraph=True)):
+            _same(g(x), f(x))
+            _same(g(y), f(y))
