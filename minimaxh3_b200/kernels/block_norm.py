@@ -151,7 +151,8 @@ def _channels(what, x, name, v):
         raise ValueError(f"{what}: {name} must be a bf16, f16 or f32 tensor [C] on x's device")
 
 
-def _run(*args):
+def _run(what, *args):
+    _ops.refuse_forward_mode(what, *args[:8])
     if torch.is_grad_enabled():
         for t in args[:8]:
             if t is not None and t.requires_grad:
@@ -202,7 +203,8 @@ def norm_modulate(
         _channels(what, x, "bias", bias)
     _finish_checks(what, x, eps)
     cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-    return _run(x, None, None, scale, shift, weight, bias, None, cu, _ops.NORM_KINDS[norm], 0, float(eps), 1.0, per_token)[0]
+    return _run(what, x, None, None, scale, shift, weight, bias, None, cu, _ops.NORM_KINDS[norm], 0, float(eps), 1.0,
+                per_token)[0]
 
 
 def gated_residual_norm(
@@ -248,6 +250,6 @@ def gated_residual_norm(
             _channels(what, x, name, v)
     _finish_checks(what, x, eps)
     cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-    out = _run(x, y, gate, scale, shift, weight, bias, y_weight, cu, _ops.NORM_KINDS[norm], _ops.NORM_KINDS[y_norm], float(eps),
-               float(residual_scale), per_token)
+    out = _run(what, x, y, gate, scale, shift, weight, bias, y_weight, cu, _ops.NORM_KINDS[norm], _ops.NORM_KINDS[y_norm],
+               float(eps), float(residual_scale), per_token)
     return out[0], None if norm == "none" else out[1]

@@ -139,6 +139,7 @@ def rotary_axes(
     ``interleaved=False`` channels p and p + sum(axes_dim)/2.
     """
     axes, thetas = _check(q, k, positions, axes_dim, theta)
+    _ops.refuse_forward_mode("rotary_axes", q, k, positions)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         oq, ok = _RotaryFn.apply(q, k, positions, axes, thetas, bool(interleaved), False)
     else:

@@ -13,6 +13,7 @@ import functools
 import struct
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 
@@ -89,6 +90,17 @@ def plain(*ts) -> bool:
         if type(t) not in _PLAIN and isinstance(t, torch.Tensor):
             return False
     return True
+
+
+def refuse_forward_mode(what: str, *ts) -> None:
+    """Raises where a tensor carries a forward-mode derivative (or may: it is inside a function transform),
+    which an operator without a rule for it would drop without a word."""
+    if _forward_ad._current_level < 0:
+        return
+    for t in ts:
+        if isinstance(t, torch.Tensor) and (torch._C._functorch.is_functorch_wrapped_tensor(t)
+                                            or _forward_ad.unpack_dual(t).tangent is not None):
+            raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
 _FLOAT_CODE = {torch.bfloat16: _lib.MH3_DTYPE_BF16, torch.float16: _lib.MH3_DTYPE_F16, torch.float32: _lib.MH3_DTYPE_F32}

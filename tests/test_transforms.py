@@ -180,3 +180,46 @@ def test_traced_and_compiled_four_bit_conversions_compute():
         for g in (torch.jit.trace(f, (x,), check_trace=False), torch.compile(f, backend="aot_eager", fullgraph=True)):
             _same(g(x), f(x))
             _same(g(y), f(y))
+
+
+def _dual(t):
+    return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+
+
+def test_forward_mode_is_refused():
+    """A tangent, or a function transform inside which one may hide; what carries none is let through."""
+    x = torch.zeros(2, 3)
+    ops.refuse_forward_mode("f", x, None)
+    with torch.autograd.forward_ad.dual_level():
+        ops.refuse_forward_mode("f", x, None, 1.0)
+        with pytest.raises(RuntimeError, match="f has no forward-mode"):
+            ops.refuse_forward_mode("f", x, _dual(x))
+    refuse = lambda t: (ops.refuse_forward_mode("f", t), t * 2)[1]  # noqa: E731
+    torch.vmap(refuse)(x)
+    for g in (refuse, torch.vmap(refuse), torch.func.grad(lambda t: refuse(t).sum())):
+        with pytest.raises(RuntimeError, match="f has no forward-mode"):
+            torch.func.jvp(g, (x,), (x,))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["rotary", "norm", "gated", "linear", "linear with an adapter"])
+def test_forward_mode_calls_are_refused(name):
+    f, inputs, _ = _calls()[name]
+    with torch.autograd.forward_ad.dual_level():
+        _same(f(*inputs), f(*inputs))
+        for i in range(len(inputs)):
+            with pytest.raises(RuntimeError, match="has no forward-mode derivative"):
+                f(*(_dual(t) if i == j else t for j, t in enumerate(inputs)))
+
+
+@pytest.mark.gpu
+def test_forward_mode_four_bit_conversions_are_refused():
+    from minimaxh3_b200.kernels.fp4_linear import dequantize_fp4, fp4_matmul, quantize_fp4
+
+    x = _rand(1, 16, 64)
+    v, b, s = quantize_fp4(x)
+    with torch.autograd.forward_ad.dual_level():
+        for f in (lambda: quantize_fp4(_dual(x)), lambda: dequantize_fp4(v, b, _dual(s)),
+                  lambda: fp4_matmul((v, b, s), (v, b, _dual(s))), lambda: fp4_matmul((v, b, s), (v, b, s), _dual(x[:, 0].float()))):
+            with pytest.raises(RuntimeError, match="has no forward-mode derivative"):
+                f()
