@@ -4,7 +4,7 @@ The model turns Q and K by their tokens' positions between the projection and
 attention; the reference's kernels take them already turned, so this has no
 counterpart there.  ``rotary_axes`` does both tensors in one launch
 (csrc/rotary.cu), on the layouts the attention entry points take, and is
-differentiable (the gradient is the inverse rotation, the same kernel).
+differentiable in Q and K (the gradient is the inverse rotation, the same kernel).
 ``fp8_attention_varlen(..., rotary=Rotary(...))`` applies it on the way in.
 """
 from __future__ import annotations
@@ -113,6 +113,8 @@ def _check(q, k, positions, axes_dim, theta):
         raise ValueError("rotary_axes: positions must be [S, axes] or [B, S, axes] (packed: [T, axes])")
     if positions.device != dev:
         raise ValueError("rotary_axes: positions must be on q's device")
+    if positions.requires_grad and torch.is_grad_enabled():
+        raise ValueError("rotary_axes: there is no gradient of the positions (pass positions.detach())")
     if not q.is_cuda:
         raise ValueError("rotary_axes: expected CUDA tensors")
     return axes, thetas

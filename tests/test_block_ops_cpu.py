@@ -49,6 +49,15 @@ def test_rotary_refusals(args, why):
         rotary_axes(*args)
 
 
+def test_rotary_refuses_positions_that_ask_for_a_gradient():
+    q, pos = _q(1, 2, 5, 32), POS.float().requires_grad_(True)
+    for t in (q, q.clone().requires_grad_(True)):
+        with pytest.raises(ValueError, match="no gradient of the positions"):
+            rotary_axes(t, None, pos, (16, 16))
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):  # nothing is asked for
+        rotary_axes(q, None, pos, (16, 16))
+
+
 X = _q(2, 5, 16)
 
 
