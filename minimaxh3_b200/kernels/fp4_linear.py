@@ -73,7 +73,7 @@ class _NoGradient(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad):
-        raise RuntimeError("fp4_linear has no gradient: its 4-bit operands are for inference")
+        raise RuntimeError("fp4_linear has no gradient, nor have the other 4-bit operators: they are for inference")
 
 
 def quantize_fp4(x2d: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -91,19 +91,28 @@ def quantize_fp4(x2d: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.T
     return (_ops.quantize_fp4 if _ops.plain(x2d) else torch.ops.mh3.quantize_fp4)(x2d)
 
 
+def _asking(*ts):
+    """Those of ts (None where one is left out) that ask for a gradient."""
+    return [t for t in ts if t is not None and t.requires_grad] if torch.is_grad_enabled() else []
+
+
 def dequantize_fp4(values: torch.Tensor, blocks: torch.Tensor, scale: torch.Tensor,
                    dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The [M, K] numbers that a 4-bit matrix stands for (exact in bfloat16 and float32)."""
     _ops.refuse_forward_mode("dequantize_fp4", scale)
     plain = _ops.plain(values, blocks, scale)
-    return (_ops.dequantize_fp4 if plain else torch.ops.mh3.dequantize_fp4)(values, blocks, scale, dtype)
+    out = (_ops.dequantize_fp4 if plain else torch.ops.mh3.dequantize_fp4)(values, blocks, scale, dtype)
+    asks = _asking(blocks, scale)
+    return _NoGradient.apply(out, *asks) if asks else out
 
 
 def fp4_matmul(a, b, bias: torch.Tensor | None = None) -> torch.Tensor:
     """bf16 ``a b^T + bias`` of two 4-bit matrices ``(values, blocks, scale)``, a [M, K], b [N, K], N a multiple of 8."""
     a, b = tuple(a), tuple(b)
     _ops.refuse_forward_mode("fp4_matmul", a[2], b[2], bias)
-    return (_fp4_matmul_cuda if _ops.plain(*a, *b, bias) else torch.ops.mh3.fp4_matmul)(a, b, bias)
+    out = (_fp4_matmul_cuda if _ops.plain(*a, *b, bias) else torch.ops.mh3.fp4_matmul)(a, b, bias)
+    asks = _asking(*a[1:], *b[1:], bias)
+    return _NoGradient.apply(out, *asks) if asks else out
 
 
 def fp4_linear(x: torch.Tensor, w4: torch.Tensor, w_blocks: torch.Tensor, w_scale: torch.Tensor,
@@ -124,9 +133,7 @@ def fp4_linear(x: torch.Tensor, w4: torch.Tensor, w_blocks: torch.Tensor, w_scal
     x2d = x if x.dim() == 2 else x.reshape(-1, K)
     low_rank = [t for a, b, _ in adapters for t in (a, b)]
     _ops.refuse_forward_mode("fp4_linear", x, w_scale, bias, *low_rank)
-    asks = []
-    if torch.is_grad_enabled():
-        asks = [t for t in (x, bias, *low_rank) if t is not None and t.requires_grad]
+    asks = _asking(x, w_blocks, w_scale, bias, *low_rank)
     if not asks and _ops.plain(x, w4, w_blocks, w_scale, bias, *low_rank):
         out = _ops.fp4_linear(x2d, w4, w_blocks, w_scale, bias, adapters, checked=True)
     else:

@@ -333,3 +333,22 @@ def test_wait_timeout_sets_error_and_context_survives():
     again = ops.fp4_gemm(a, b, err=err)
     torch.cuda.synchronize()
     assert int(err.item()) == 0 and torch.equal(again, good)
+
+
+def test_every_tensor_that_asks_for_a_gradient_is_refused_one():
+    """Scales and biases that ask for a gradient: the values are the same, asking raises (none is cut off)."""
+    from minimaxh3_b200.kernels.fp4_linear import dequantize_fp4, fp4_linear, fp4_matmul, quantize_fp4
+
+    x, bias = _rand(80, 5, 64).to(DEV), _rand(81, 16).to(DEV)
+    a, w = quantize_fp4(x), quantize_fp4(_rand(82, 16, 64).to(DEV))
+    asks = lambda t: t.clone().requires_grad_(True)  # noqa: E731
+    for f in (lambda s: fp4_linear(x, *w[:2], s), lambda s: fp4_matmul(a, (*w[:2], s)), lambda s: fp4_matmul((w[0], w[1], s), w),
+              lambda s: dequantize_fp4(*w[:2], s)):
+        out = f(asks(w[2]))
+        assert torch.equal(out, f(w[2]))
+        with pytest.raises(RuntimeError, match="no gradient"):
+            out.sum().backward()
+        with torch.no_grad():
+            assert not f(asks(w[2])).requires_grad
+    with pytest.raises(RuntimeError, match="no gradient"):
+        fp4_matmul(a, w, asks(bias)).sum().backward()
