@@ -624,7 +624,10 @@ def _round_up(x: int, m: int) -> int:
 # Folded LoRA operands, keyed on the identity and version of the adapter tensors and of the
 # column scale: a layer's forward reuses them until an adapter or the weight scale changes
 # (runtime/lora.py swaps the ``adapters`` list, an in-place edit bumps a tensor's version).
-# Entries hold the source tensors, so a key's ids cannot be reused while it is cached.
+# Entries hold the source tensors, so a key's ids cannot be reused while it is cached, and the
+# event after the kernels that filled them, which a call on another stream waits for.  A
+# captured call folds for itself: its kernels run at the replays, and what it reads must live
+# as long as the graph.
 _LORA_CACHE: "collections.OrderedDict" = collections.OrderedDict()
 _LORA_CACHE_MAX = 1024
 
@@ -641,15 +644,27 @@ def _lora_key(adapters, scale_src):
 def _lora_operands(adapters, N: int, K: int, device, col_scale=None, scale_src=None):
     """``_fold_lora`` with a cache over calls (see ``_LORA_CACHE``); ``scale_src`` is the tensor
     ``col_scale`` was derived from (the layer's ``w_scale`` buffer), which keys the cache."""
+    device = torch.device(device)
+    cuda = device.type == "cuda"
+    if cuda:
+        with torch.cuda.device(device):
+            if torch.cuda.is_current_stream_capturing():
+                return _fold_lora(adapters, N, K, device, col_scale)
     scale_src = col_scale if scale_src is None else scale_src
     key = _lora_key(adapters, scale_src)
+    stream = torch.cuda.current_stream(device) if cuda else None
     hit = _LORA_CACHE.get(key)
     if hit is not None:
         _LORA_CACHE.move_to_end(key)
-        return hit[1], hit[2]
+        _, A_cat, B_cat, filled_on, filled = hit
+        if stream != filled_on:
+            stream.wait_event(filled)
+            A_cat.record_stream(stream)
+            B_cat.record_stream(stream)
+        return A_cat, B_cat
     A_cat, B_cat = _fold_lora(adapters, N, K, device, col_scale)
     refs = [t for A, B_, _ in adapters for t in (A, B_)] + ([scale_src] if scale_src is not None else [])
-    _LORA_CACHE[key] = (refs, A_cat, B_cat)
+    _LORA_CACHE[key] = (refs, A_cat, B_cat, stream, stream.record_event() if cuda else None)
     while len(_LORA_CACHE) > _LORA_CACHE_MAX:
         _LORA_CACHE.popitem(last=False)
     return A_cat, B_cat

@@ -208,3 +208,42 @@ def test_convert_transformer_and_forward():
     assert isinstance(t.blocks[1].to_q, FP8Linear) and not isinstance(t.blocks[1].norm_out, FP8Linear)
     y = t(_rand(4, 8, 128).to(DEV))
     assert torch.isfinite(y.float()).all()
+
+
+def test_fp8_linear_adapters_first_captured_or_on_another_stream():
+    """A layer whose first call with its adapters is captured, or runs on a side stream: the eager call after
+    it, the replays and a call on another stream all give the first eager call's bits; an adapter edited in
+    place is seen by the replays."""
+    from minimaxh3_b200.kernels.fp8_linear import FP8Linear
+
+    lin = FP8Linear.from_linear(torch.nn.Linear(256, 128).to(torch.bfloat16).to(DEV))
+    x = _rand(1, 300, 256).to(torch.bfloat16).to(DEV)
+
+    def adapters():
+        return [(_rand(2, 16, 256, scale=0.1).to(torch.bfloat16).to(DEV), _rand(3, 128, 16, scale=0.1).to(torch.bfloat16).to(DEV), 0.5)]
+
+    lin.adapters = adapters()
+    ref = lin(x)
+    lin.adapters = adapters()
+    lin(x.clone())
+    lin.adapters = adapters()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cap = lin(x)
+    assert torch.equal(lin(x), ref)  # before any replay
+    graph.replay()
+    assert torch.equal(cap, ref)
+    lin.adapters[0][1].mul_(2)
+    doubled = lin(x)
+    assert not torch.equal(doubled, ref)
+    graph.replay()
+    assert torch.equal(cap, doubled)
+    lin.adapters = adapters()
+    torch.cuda.synchronize()
+    side, outs = torch.cuda.Stream(), []
+    with torch.cuda.stream(side):
+        outs.append(lin(x))
+    outs.append(lin(x))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, ref) for o in outs)

@@ -5,6 +5,8 @@ the reference; a layer without adapters runs its own forward and inputs the
 fused GEMM cannot take (here: CPU tensors) get the reference's two-step
 ``out + sum scale (x A^T) B^T``.
 """
+import contextlib
+
 import torch
 import torch.nn as nn
 
@@ -65,3 +67,66 @@ def test_folded_lora_operands_are_cached_until_an_input_changes():
     ws.mul_(2.0)
     new_scale = ops._lora_operands([(A, Bm, 0.5)], 32, 64, "cpu", col_scale=ws.reshape(-1), scale_src=ws)
     assert new_scale[1] is not rescaled[1]
+
+
+class _Stream:
+    """What ops._lora_operands asks of a CUDA stream, without a device."""
+
+    def __init__(self):
+        self.waited = []
+
+    def record_event(self):
+        return ("after the fold on", self)
+
+    def wait_event(self, event):
+        self.waited.append(event)
+
+
+class _Folded:
+    def __init__(self):
+        self.used_on = []
+
+    def record_stream(self, stream):
+        self.used_on.append(stream)
+
+
+def _fake_device(monkeypatch):
+    """Streams, capture and the fold as fakes: (state with the current stream, adapters to fold)."""
+    from types import SimpleNamespace
+
+    from minimaxh3_b200 import ops
+
+    state = SimpleNamespace(stream=_Stream(), capturing=False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: state.stream)
+    monkeypatch.setattr(torch.cuda, "device", contextlib.nullcontext)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state.capturing)
+    monkeypatch.setattr(ops, "_fold_lora", lambda *a: (_Folded(), _Folded()))
+    monkeypatch.setattr(ops, "_LORA_CACHE", type(ops._LORA_CACHE)())
+    return state, [(torch.zeros(16, 32), torch.zeros(8, 16), 1.0)]
+
+
+def test_folded_lora_operands_on_another_stream_wait_for_the_fold(monkeypatch):
+    from minimaxh3_b200 import ops
+
+    state, adapters = _fake_device(monkeypatch)
+    first, filled = state.stream, ops._lora_operands(adapters, 8, 32, "cuda:0")
+    assert ops._lora_operands(adapters, 8, 32, "cuda:0") == filled and first.waited == []
+    state.stream = other = _Stream()
+    again = ops._lora_operands(adapters, 8, 32, "cuda:0")
+    assert again[0] is filled[0] and again[1] is filled[1]
+    assert other.waited == [("after the fold on", first)]
+    assert all(t.used_on == [other] for t in filled)  # their memory outlives the reads there
+
+
+def test_captured_lora_operands_are_neither_kept_nor_taken(monkeypatch):
+    """A capture only records its fold, and a graph must not read memory that the cache may drop."""
+    from minimaxh3_b200 import ops
+
+    state, adapters = _fake_device(monkeypatch)
+    state.capturing = True
+    captured = ops._lora_operands(adapters, 8, 32, "cuda:0")
+    state.capturing = False
+    eager = ops._lora_operands(adapters, 8, 32, "cuda:0")
+    assert eager[0] is not captured[0]
+    state.capturing = True
+    assert ops._lora_operands(adapters, 8, 32, "cuda:0")[0] is not eager[0]
