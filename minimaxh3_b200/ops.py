@@ -77,7 +77,7 @@ _USUAL = 0
 for _key in (torch._C.DispatchKey.BackendSelect, torch._C.DispatchKey.ADInplaceOrView):
     _USUAL |= torch._C.DispatchKeySet(_key).raw_repr()
 _included = torch._C._dispatch_tls_local_include_set
-_PLAIN = (torch.Tensor, torch.nn.Parameter, type(None))
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None)))
 
 
 def plain(*ts) -> bool:
@@ -86,10 +86,7 @@ def plain(*ts) -> bool:
     transforms or intercepts operators."""
     if torch.compiler.is_compiling() or _included().raw_repr() & ~_USUAL:
         return False
-    for t in ts:
-        if type(t) not in _PLAIN and isinstance(t, torch.Tensor):
-            return False
-    return True
+    return _PLAIN.issuperset(map(type, ts)) or not any(isinstance(t, torch.Tensor) and type(t) not in _PLAIN for t in ts)
 
 
 def refuse_forward_mode(what: str, *ts) -> None:
@@ -870,6 +867,31 @@ def fp4_gemm(a, b, bias=None, a2=None, b2=None, out: torch.Tensor | None = None,
     return out
 
 
+def _fp4_low_rank(adapters, w_scale: torch.Tensor, K: int):
+    """(A_cat [R, K], (scale*B)_cat / w_scale [N, R]), bf16, the adapters side by side and R padded to a
+    multiple of 16 with zeros.  Made in each call, as the weight's own operands are not: an adapter may be
+    edited where nothing can see it (through ``.data``, or by a replayed training step)."""
+    N, dev = w_scale.numel(), w_scale.device
+    inv = w_scale.reshape(N, 1)
+    As, Bs, R = [], [], 0
+    for A, B, s in adapters:
+        r = A.shape[0]
+        if A.shape != (r, K) or B.shape != (N, r):
+            raise ValueError(f"fp4_linear: an adapter is (A [r, {K}], B [{N}, r], scale)")
+        As.append(A.to(device=dev, dtype=torch.bfloat16))
+        b = B.to(dev) / inv  # in f32, and exact: w_scale is a power of two
+        Bs.append(b if s == 1 else b * float(s))
+        R += r
+    pad = -R % 16 if R else 16
+    if pad:
+        As.append(w_scale.new_zeros((pad, K), dtype=torch.bfloat16))
+        Bs.append(w_scale.new_zeros((N, pad)))
+    A_cat, B_cat = (ts[0] if len(ts) == 1 else torch.cat(ts, dim) for ts, dim in ((As, 0), (Bs, 1)))
+    if not A_cat.is_contiguous() or A_cat.data_ptr() % 16:
+        A_cat = A_cat.clone(memory_format=torch.contiguous_format)
+    return A_cat, B_cat.to(torch.bfloat16, memory_format=torch.contiguous_format)
+
+
 @nvtx("mh3.fp4_linear")
 def fp4_linear(x2d: torch.Tensor, w4: torch.Tensor, w_blocks: torch.Tensor, w_scale: torch.Tensor, bias,
                adapters, checked: bool = False) -> torch.Tensor:
@@ -886,7 +908,7 @@ def fp4_linear(x2d: torch.Tensor, w4: torch.Tensor, w_blocks: torch.Tensor, w_sc
     if adapters:
         xq = quantize_fp4(x2d)
         xb = x2d.to(torch.bfloat16).contiguous()
-        A_cat, b2 = _lora_operands(adapters, N, K, dev, col_scale=w_scale.reshape(-1), scale_src=w_scale)
+        A_cat, b2 = _fp4_low_rank(adapters, w_scale, K)
         a2 = scaled_gemm(xb, A_cat, row_scale=xq[2], row_scale_inv=True)
         return fp4_gemm(xq, (w4, w_blocks, w_scale), bias=bias, a2=a2, b2=b2)
     if not checked:

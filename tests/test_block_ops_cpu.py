@@ -251,3 +251,24 @@ def test_fp4_conversion_policy(monkeypatch):
 
 def test_ops_check_is_shared():
     assert ops.check_fp4(*_w4(16, 96)[:1], torch.zeros(1, 2, 32, 4, 4).to(torch.float8_e4m3fn), torch.ones(16), "x") == (16, 96)
+
+
+@pytest.mark.parametrize("ranks", [(16,), (8,), (0,), (32, 8), (5, 11, 200)])
+def test_low_rank_operands_of_a_four_bit_linear(ranks):
+    """The adapters side by side, in the bits of the fold that the 8-bit linear makes, anew in each call."""
+    K, N = 64, 24
+    g = torch.Generator().manual_seed(sum(ranks))
+    w_scale = torch.exp2(torch.randint(-20, 5, (N, 1), generator=g).float())
+    types = (torch.bfloat16, torch.float32, torch.float16)
+    adapters = [(torch.randn(r, K, generator=g).to(types[i]), torch.randn(N, r, generator=g).to(types[i]), 0.3 ** i) for i, r in enumerate(ranks)]
+    for _ in range(2):
+        got, want = ops._fp4_low_rank(adapters, w_scale, K), ops._fold_lora(adapters, N, K, "cpu", col_scale=w_scale.reshape(-1))
+        assert all(a.is_contiguous() and torch.equal(a, b) for a, b in zip(got, want))
+        adapters[0][1].data.mul_(2)  # no version counter sees this
+
+
+def test_low_rank_refusals():
+    w_scale = torch.ones(24, 1)
+    for A, B in (((8, 32), (24, 8)), ((8, 64), (23, 8)), ((8, 64), (24, 9)), ((8, 1), (24, 8))):
+        with pytest.raises(ValueError, match="an adapter is"):
+            ops._fp4_low_rank([(torch.zeros(A), torch.zeros(B), 1.0)], w_scale, 64)

@@ -352,3 +352,23 @@ def test_every_tensor_that_asks_for_a_gradient_is_refused_one():
             assert not f(asks(w[2])).requires_grad
     with pytest.raises(RuntimeError, match="no gradient"):
         fp4_matmul(a, w, asks(bias)).sum().backward()
+
+
+def test_an_adapter_edited_unseen_is_used():
+    """Through ``.data`` and by a replayed graph, neither of which counts a tensor's version."""
+    from minimaxh3_b200.kernels.fp4_linear import fp4_linear, quantize_fp4
+
+    x, w = _rand(90, 20, 64).to(DEV), quantize_fp4(_rand(91, 32, 64).to(DEV))
+    A, B, B2 = _rand(92, 16, 64).to(DEV), _rand(93, 32, 16).to(DEV), _rand(94, 32, 16).to(DEV)
+    first, want = fp4_linear(x, *w, adapters=[(A, B, 0.5)]), fp4_linear(x, *w, adapters=[(A, B2, 0.5)])
+    keep = B.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        B.copy_(B2)
+        cap = fp4_linear(x, *w, adapters=[(A, B, 0.5)])
+    assert torch.equal(fp4_linear(x, *w, adapters=[(A, B, 0.5)]), first)
+    graph.replay()
+    assert torch.equal(cap, want) and torch.equal(fp4_linear(x, *w, adapters=[(A, B, 0.5)]), want)
+    B.data.copy_(keep)
+    assert torch.equal(fp4_linear(x, *w, adapters=[(A, B, 0.5)]), first)
