@@ -1407,10 +1407,12 @@ static int ctas_of(long long rows, int C, bool general) {
   return (int)std::min<long long>(rows, (long long)kSMs * per);
 }
 
+constexpr size_t kSmemMax = 224 * 1024;  // beside 1 KB of static shared memory
+
 template <auto K>
 static cudaError_t start(const Params& p, int threads, size_t smem, cudaStream_t st) {
   if (smem > 40 * 1024) {  // with the static part, past the 48 KB default
-    const cudaError_t e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = allow_smem<K>(kSmemMax);
     if (e != cudaSuccess) return e;
   }
   K<<<p.ctas, threads, smem, st>>>(p);
@@ -1419,7 +1421,6 @@ static cudaError_t start(const Params& p, int threads, size_t smem, cudaStream_t
 
 // Shared memory of a streaming kernel with ``mods`` slots and ``tensors`` x R rows a
 // stage; sets p.stages to 3, or 2 where three do not fit, and 0 where two do not.
-constexpr size_t kSmemMax = 224 * 1024;
 // ``more``: bytes of a channel in a stage beside those rows.
 static size_t ring_bytes(Params& p, int threads, int ch, int mods, int rows, int es, size_t most, int more = 0) {
   const size_t fixed = (size_t)threads * ch * 4 * mods, stage = (size_t)threads * ch * (es * rows + more);

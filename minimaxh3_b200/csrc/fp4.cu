@@ -289,8 +289,7 @@ static cudaError_t launch_quantize(const void* x, long long stride, long long M,
     return cudaGetLastError();
   }
   if (smem > 40 * 1024) {  // with the static part, past the 48 KB default
-    const cudaError_t e =
-        cudaFuncSetAttribute(quantize_stream_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = allow_smem<quantize_stream_kernel<T>>(kRingMax);
     if (e != cudaSuccess) return e;
   }
   // resident CTAs of 64 registers a thread and their rings

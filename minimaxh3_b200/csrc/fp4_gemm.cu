@@ -609,7 +609,7 @@ template <typename X>
 static cudaError_t launch_fused(const SmallParams& p, cudaStream_t st) {
   const size_t smem = (size_t)p.M * (p.K / 2 + p.K / 16);
   if (smem > 32 * 1024) {  // with the static part, past the 48 KB default
-    const cudaError_t e = cudaFuncSetAttribute(small_kernel<1, X>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = allow_smem<small_kernel<1, X>>(kFusedBytes);
     if (e != cudaSuccess) return e;
   }
   small_kernel<1, X><<<(unsigned)((p.N + kRowsW - 1) / kRowsW), kWarps * 32, smem, st>>>(p);

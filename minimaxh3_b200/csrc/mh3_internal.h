@@ -9,6 +9,7 @@
 #include <stdint.h>
 #include <string.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "mh3_b200.h"
@@ -28,6 +29,23 @@ int encode_tiled(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t rank, voi
 
 // The library's device error word on the current device.
 int* device_error_word();
+
+// Lets kernel K take up to ``most`` bytes of dynamic shared memory on the current device.  The
+// limit belongs to the device's function, which all host threads share, so a call sets the most
+// that K ever takes, not its own need: a lower value between another thread's call and its
+// launch would fail that launch.
+template <auto K>
+cudaError_t allow_smem(size_t most) {
+  static std::atomic<uint64_t> set{0};  // a bit for each device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (set.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+  if (e == cudaSuccess) set.fetch_or(bit, std::memory_order_release);
+  return e;
+}
 
 // The calling thread's current CUDA context (CUcontext), or null; through
 // the runtime's driver entry point, so the library does not link libcuda.

@@ -37,6 +37,8 @@ constexpr int kMaxThreads = 384;  // of the streaming kernel
 constexpr int kMaxPairs = 128;    // head_dim <= 256
 constexpr int kMaxTokens = 16;    // tokens per CTA
 constexpr int kDepth = 4;         // tokens in the ring
+// The most a streaming kernel takes: a ring of four vectors a thread, and the angles.
+constexpr size_t kSmemMax = (size_t)kDepth * 4 * kMaxThreads * 16 + (size_t)kMaxTokens * kMaxPairs * sizeof(float2);
 
 struct Params {
   const char *q, *k;
@@ -307,6 +309,16 @@ __global__ void __launch_bounds__(kThreads) scalar_kernel(const __grid_constant_
   }
 }
 
+template <auto K>
+static cudaError_t start(const Params& p, dim3 blocks, int threads, size_t smem, cudaStream_t st) {
+  if (smem > 40 * 1024) {  // past the 48 KB default
+    const cudaError_t e = allow_smem<K>(kSmemMax);
+    if (e != cudaSuccess) return e;
+  }
+  K<<<blocks, threads, smem, st>>>(p);
+  return cudaGetLastError();
+}
+
 template <typename T>
 static cudaError_t launch(const Params& p, bool vec, bool inter, cudaStream_t st) {
   const unsigned grid = (unsigned)((p.tokens + p.tile - 1) / p.tile);
@@ -324,14 +336,13 @@ static cudaError_t launch(const Params& p, bool vec, bool inter, cudaStream_t st
   q.side = std::min((rows + m - 1) / m, kMaxThreads / units);
   const int threads = (q.side * units + 31) / 32 * 32;
   const size_t smem = (size_t)kDepth * m * (inter ? 1 : 2) * threads * 16 + (size_t)p.tile * (inter ? p.D / 2 : p.R2) * sizeof(float2);
-  auto kern = inter ? (m == 1 ? stream_kernel<T, true, 1> : m == 2 ? stream_kernel<T, true, 2> : stream_kernel<T, true, 4>)
-                    : (m == 1 ? stream_kernel<T, false, 1> : stream_kernel<T, false, 2>);
-  if (smem > 40 * 1024) {  // past the 48 KB default
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-  }
-  kern<<<dim3(grid, (unsigned)((rows + m * q.side - 1) / (m * q.side))), threads, smem, st>>>(q);
-  return cudaGetLastError();
+  const dim3 blocks(grid, (unsigned)((rows + m * q.side - 1) / (m * q.side)));
+  if (inter)
+    return m == 1   ? start<stream_kernel<T, true, 1>>(q, blocks, threads, smem, st)
+           : m == 2 ? start<stream_kernel<T, true, 2>>(q, blocks, threads, smem, st)
+                    : start<stream_kernel<T, true, 4>>(q, blocks, threads, smem, st);
+  return m == 1 ? start<stream_kernel<T, false, 1>>(q, blocks, threads, smem, st)
+                : start<stream_kernel<T, false, 2>>(q, blocks, threads, smem, st);
 }
 
 }  // namespace rotary
