@@ -37,7 +37,7 @@ def _turn(q, k, positions, *args):
 
 @torch.library.register_fake("mh3::rotary_axes", lib=_LIB)
 def _(q, k, positions, axes_dim, theta, interleaved, inverse):
-    return torch.empty_like(q), q.new_empty(0) if k is None else torch.empty_like(k)
+    return _ops.rotary_like(q), q.new_empty(0) if k is None else _ops.rotary_like(k)
 
 
 class _RotaryFn(torch.autograd.Function):

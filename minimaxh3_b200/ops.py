@@ -944,6 +944,15 @@ _POS_KIND = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 _ROTARY = struct.Struct("@10i4i4d" + "P3q" * 4 + "P2q")
 
 
+def rotary_like(t: torch.Tensor) -> torch.Tensor:
+    """An output of ``rotary`` for t: in t's dimension order if its channels are contiguous, else contiguous."""
+    if t.stride(-1) == 1 or t.shape[-1] == 1:
+        o = torch.empty_like(t)
+        if o.stride(-1) == 1 or t.shape[-1] == 1:
+            return o
+    return t.new_empty(t.shape)
+
+
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axes_dim, theta, interleaved: bool = True,
            inverse: bool = False, out_q: torch.Tensor | None = None, out_k: torch.Tensor | None = None):
     """``mh3_rotary`` on q and k, both [B,H,S,D] or both packed [T,H,D]; ``(q', k')``, k' None without k.
@@ -964,11 +973,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
             copies.append(t)  # alive until the launch
             s = t.stride()
         if o is None:
-            o = torch.empty_like(t)
+            o = rotary_like(t)
             so = o.stride()
-            if so[-1] != 1 and o.shape[-1] != 1:
-                o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-                so = o.stride()
         elif o.shape != t.shape or o.dtype != t.dtype or o.device != t.device or o.stride(-1) != 1:
             raise ValueError("rotary: an output must match its input, with contiguous channels")
         else:

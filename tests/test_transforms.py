@@ -223,3 +223,50 @@ def test_forward_mode_four_bit_conversions_are_refused():
                   lambda: fp4_matmul((v, b, s), (v, b, _dual(s))), lambda: fp4_matmul((v, b, s), (v, b, s), _dual(x[:, 0].float()))):
             with pytest.raises(RuntimeError, match="has no forward-mode derivative"):
                 f()
+
+
+LAYOUTS = {  # of q [2, 4, 9, 32]
+    "contiguous": lambda t: t(2, 4, 9, 32),
+    "tokens first": lambda t: t(2, 9, 4, 32).transpose(1, 2),
+    "of a fused projection": lambda t: t(2, 9, 12, 32)[:, :, 4:8].transpose(1, 2),
+    "channels before tokens": lambda t: t(2, 4, 32, 9).transpose(2, 3),
+    "channels first": lambda t: t(32, 9, 2, 4).permute(2, 3, 1, 0),
+    "every other channel": lambda t: t(2, 4, 9, 64)[..., ::2],
+    "every other channel, tokens first": lambda t: t(2, 9, 4, 64)[..., ::2].transpose(1, 2),
+    "a shared head": lambda t: t(2, 1, 9, 32).expand(2, 4, 9, 32),
+    "a padded row": lambda t: t(2, 4, 9, 40)[..., :32],
+    "one channel for all": lambda t: t(2, 4, 9, 1).expand(2, 4, 9, 32),
+}
+
+
+def _fake_strides(layout):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from minimaxh3_b200.kernels.rotary import rotary_axes
+
+    with FakeTensorMode():
+        q = LAYOUTS[layout](lambda *s: torch.empty(*s, dtype=torch.bfloat16, device=DEV))
+        k = LAYOUTS[layout](lambda *s: torch.empty(*s, dtype=torch.bfloat16, device=DEV))
+        return [t.stride() for t in rotary_axes(q, k, torch.empty(9, 2, dtype=torch.int32, device=DEV), (16, 16))]
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_rotary_strides_that_a_compiler_is_told(layout):
+    """Contiguous channels, and the strides of the tensor that the real call makes."""
+    t = LAYOUTS[layout](torch.empty)
+    real = torch.empty_like(t.contiguous() if t.stride(-1) != 1 else t).stride()
+    assert real[-1] == 1 and _fake_strides(layout) == [real, real]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_rotary_strides_and_values_of_a_compiled_call(layout):
+    from minimaxh3_b200.kernels.rotary import rotary_axes
+
+    q, k, pos = LAYOUTS[layout](lambda *s: _rand(1, *s)), LAYOUTS[layout](lambda *s: _rand(2, *s)), _pos(9)
+    f = lambda a, b: rotary_axes(a, b, pos, (16, 16))  # noqa: E731
+    want = f(q, k)
+    assert [t.stride() for t in want] == _fake_strides(layout)
+    got = torch.compile(f, fullgraph=True, backend="aot_eager")(q, k)
+    _same(got, want)
+    assert [t.stride() for t in got] == [t.stride() for t in want]
