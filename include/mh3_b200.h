@@ -449,8 +449,8 @@ MH3_API int mh3_rotary(const mh3_rotary_args* args, void* stream);
  * mh3_block_norm_bwd reads dr and dh (either may be null), x, y, stats and the
  * modulation, and writes every gradient whose pointer is given: dx, dy
  * [rows, channels] in dtype; dgate, dscale, dshift [groups or rows, channels]
- * and dweight, dbias, dy_weight [channels], each in its tensor's type, all
- * contiguous (null dr or dh: that output was not used, its gradient is 0).
+ * and dweight, dbias, dy_weight [channels], each in its tensor's type (or
+ * grad_f32), all contiguous (null dr or dh: that output was not used, its gradient is 0).
  * Column sums are added in a fixed order.  workspace:
  * mh3_block_norm_workspace_bytes() bytes, 16-byte aligned.
  * No reference counterpart (the model's blocks are outside the reference).
@@ -458,7 +458,8 @@ MH3_API int mh3_rotary(const mh3_rotary_args* args, void* stream);
 typedef struct mh3_norm_mod {
   const void* ptr;
   int64_t stride_group, stride_row;
-  int32_t dtype, reserved;
+  int32_t dtype;
+  int32_t grad_f32; /* of gate, scale, shift: 1 writes its gradient in f32 whatever its type, so that sums over it lose nothing */
 } mh3_norm_mod;
 
 typedef struct mh3_block_norm_args {

@@ -102,7 +102,7 @@ class RotaryArgs(ctypes.Structure):
 class NormMod(ctypes.Structure):
     """``mh3_norm_mod`` (include/mh3_b200.h)."""
 
-    _fields_ = [("ptr", c_ptr), ("stride_group", c_i64), ("stride_row", c_i64), ("dtype", c_i32), ("reserved", c_i32)]
+    _fields_ = [("ptr", c_ptr), ("stride_group", c_i64), ("stride_row", c_i64), ("dtype", c_i32), ("grad_f32", c_i32)]
 
 
 class BlockNormArgs(ctypes.Structure):

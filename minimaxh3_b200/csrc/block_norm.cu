@@ -46,7 +46,7 @@ constexpr int kSMs = 148;    // fixed: the order of the column sums depends on t
 struct Mod {
   const void* p;
   long long sg, sr;
-  int dt;
+  int dt, gdt;  // its type, and its gradient's
 };
 struct Chan {
   const void* p;  // [C]
@@ -439,9 +439,9 @@ __global__ void __launch_bounds__(MAXT) bwd_kernel(const __grid_constant__ Param
         if (p.dx) store8<T, VEC>(static_cast<T*>(p.dx) + row * p.C + c, n, d);
         if (p.dy) store8<T, VEC>(static_cast<T*>(p.dy) + row * p.C + c, n, d);
         if constexpr (PT) {
-          if (p.dscale) put8<VEC>(p.dscale, p.scale.dt, row * p.C + c, n, d);
-          if (p.dshift) put8<VEC>(p.dshift, p.shift.dt, row * p.C + c, n, d);
-          if (p.dgate) put8<VEC>(p.dgate, p.gate.dt, row * p.C + c, n, d);
+          if (p.dscale) put8<VEC>(p.dscale, p.scale.gdt, row * p.C + c, n, d);
+          if (p.dshift) put8<VEC>(p.dshift, p.shift.gdt, row * p.C + c, n, d);
+          if (p.dgate) put8<VEC>(p.dgate, p.gate.gdt, row * p.C + c, n, d);
         }
       }
       continue;
@@ -486,9 +486,9 @@ __global__ void __launch_bounds__(MAXT) bwd_kernel(const __grid_constant__ Param
             mod8<VEC>(p.b.p, p.b.dt, c, n, 0.0f, b);
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[i] = t[i] * fmaf(xh[i], dn[i], b[i]);
-            put8<VEC>(p.dscale, p.scale.dt, row * p.C + c, n, o);
+            put8<VEC>(p.dscale, p.scale.gdt, row * p.C + c, n, o);
           }
-          if (p.dshift) put8<VEC>(p.dshift, p.shift.dt, row * p.C + c, n, t);
+          if (p.dshift) put8<VEC>(p.dshift, p.shift.gdt, row * p.C + c, n, t);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float m = t[i] * (1.0f + sc[i]);
@@ -518,8 +518,8 @@ __global__ void __launch_bounds__(MAXT) bwd_kernel(const __grid_constant__ Param
     if constexpr (PT) {
       if (!has_dh && live) {  // h was not used
         const float zero[8] = {};
-        if (p.dscale) put8<VEC>(p.dscale, p.scale.dt, row * p.C + c, n, zero);
-        if (p.dshift) put8<VEC>(p.dshift, p.shift.dt, row * p.C + c, n, zero);
+        if (p.dscale) put8<VEC>(p.dscale, p.scale.gdt, row * p.C + c, n, zero);
+        if (p.dshift) put8<VEC>(p.dshift, p.shift.gdt, row * p.C + c, n, zero);
       }
     }
     if (live && p.dx) {
@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(MAXT) bwd_kernel(const __grid_constant__ Param
             t[i] = d[i] * yh[i] * wy[i];
             a3[i] = fmaf(d[i] * gv[i], yh[i], a3[i]);
           }
-          if (p.dgate) put8<VEC>(p.dgate, p.gate.dt, row * p.C + c, n, t);
+          if (p.dgate) put8<VEC>(p.dgate, p.gate.gdt, row * p.C + c, n, t);
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) a3[i] = fmaf(d[i], yh[i], a3[i]);
@@ -761,13 +761,13 @@ struct ModRing {
   static __device__ __forceinline__ const M* row_of(const Mod& m, long long g, long long row) {
     return static_cast<const M*>(m.p) + g * m.sg + row * m.sr;
   }
-  // Writes a row of M; null: nothing.
-  static __device__ __forceinline__ void store(void* p, long long row, int C, const Vals<CH>& v) {
+  // Writes a row of a gradient, of M or f32; null: nothing.
+  static __device__ __forceinline__ void store(void* p, const Mod& m, long long row, int C, const Vals<CH>& v) {
     if (p == nullptr) return;
-    M* to = static_cast<M*>(p) + row * C;
-    if constexpr (std::is_same<T, M>::value) {
-      store_row<T, CH, FIT>(to, C, v);
+    if (std::is_same<T, M>::value && (std::is_same<M, float>::value || m.gdt != MH3_DTYPE_F32)) {
+      store_row<T, CH, FIT>(static_cast<T*>(p) + row * C, C, v);
     } else {
+      float* to = static_cast<float*>(p) + row * C;
 #pragma unroll
       for (int q = 0; q < L::P; ++q)
         if (L::in(q, C))
@@ -1158,8 +1158,11 @@ __global__ void __launch_bounds__(MAXT) bwd_stream_kernel(const __grid_constant_
         for (int i = j; i < n; ++i) {
           if (p.dx) store_row<T, CH>(static_cast<T*>(p.dx) + (long long)(row + i) * p.C, p.C, z);
           if (p.dy) store_row<T, CH>(static_cast<T*>(p.dy) + (long long)(row + i) * p.C, p.C, z);
-          if (PT)
-            for (void* q : {p.dscale, p.dshift, p.dgate}) mring.store(q, row + i, p.C, z);
+          if (PT) {
+            mring.store(p.dscale, p.scale, row + i, p.C, z);
+            mring.store(p.dshift, p.shift, row + i, p.C, z);
+            mring.store(p.dgate, p.gate, row + i, p.C, z);
+          }
         }
         j = n;
         continue;
@@ -1205,13 +1208,13 @@ __global__ void __launch_bounds__(MAXT) bwd_stream_kernel(const __grid_constant_
 #pragma unroll
               for (int k = 0; k < CH / 2; ++k) xh[i].e[k] = fmul2(fadd2(xh[i].e[k], both(-rs[i].z)), both(rs[i].w));
               if (PT) {
-                mring.store(p.dshift, row + i, p.C, t);
+                mring.store(p.dshift, p.shift, row + i, p.C, t);
                 Vals<CH> u;
                 if (p.dscale) {
                   slots_get<CH>(sB, u);
 #pragma unroll
                   for (int k = 0; k < CH / 2; ++k) u.e[k] = fmul2(t.e[k], ffma2(xh[i].e[k], d[i].e[k], u.e[k]));
-                  mring.store(p.dscale, row + i, p.C, u);
+                  mring.store(p.dscale, p.scale, row + i, p.C, u);
                 }
                 if (p.scale.p) {
                   mring.get(st * NM * R + i, u);
@@ -1230,8 +1233,8 @@ __global__ void __launch_bounds__(MAXT) bwd_stream_kernel(const __grid_constant_
               s[2 * i] = s0.x + s0.y;
               s[2 * i + 1] = s1.x + s1.y;
             } else if (PT) {  // h was not used
-              mring.store(p.dscale, row + i, p.C, d[i]);
-              mring.store(p.dshift, row + i, p.C, d[i]);
+              mring.store(p.dscale, p.scale, row + i, p.C, d[i]);
+              mring.store(p.dshift, p.shift, row + i, p.C, d[i]);
             }
           }
         }
@@ -1274,7 +1277,7 @@ __global__ void __launch_bounds__(MAXT) bwd_stream_kernel(const __grid_constant_
               Vals<CH> t;
 #pragma unroll
               for (int k = 0; k < CH / 2; ++k) t.e[k] = fmul2(fmul2(d[i].e[k], yh[i].e[k]), gt.e[k]);
-              mring.store(p.dgate, row + i, p.C, t);
+              mring.store(p.dgate, p.gate, row + i, p.C, t);
               gated(i, d[i], dg);
               gated(i, gt, gi);
             }
@@ -1369,9 +1372,9 @@ __global__ void __launch_bounds__(kCols * PARTS) group_sum_kernel(const __grid_c
         const float w = p.w.p ? get1(p.w.p, p.w.dt, c) : 1.0f, b = p.b.p ? get1(p.b.p, p.b.dt, c) : 0.0f;
         const float wy = p.wy.p ? get1(p.wy.p, p.wy.dt, c) : 1.0f;
         const long long at = (long long)g * p.C + c;
-        if (p.dscale) put1(p.dscale, p.scale.dt, at, fmaf(w, s[0], b * s[1]));
-        if (p.dshift) put1(p.dshift, p.shift.dt, at, s[1]);
-        if (p.dgate) put1(p.dgate, p.gate.dt, at, wy * s[2]);
+        if (p.dscale) put1(p.dscale, p.scale.gdt, at, fmaf(w, s[0], b * s[1]));
+        if (p.dshift) put1(p.dshift, p.shift.gdt, at, s[1]);
+        if (p.dgate) put1(p.dgate, p.gate.gdt, at, wy * s[2]);
       }
     }
     __syncthreads();
@@ -1596,7 +1599,8 @@ static int run(const mh3_block_norm_args* a, bool bwd, void* stream) {
   for (int i = 0; i < 3; ++i) {
     if (given[i]->ptr && !float_type(given[i]->dtype))
       return fail(MH3_ERR_INVALID, "mh3_block_norm: modulations must be bf16, f16 or f32");
-    *mods[i] = Mod{given[i]->ptr, given[i]->stride_group, given[i]->stride_row, given[i]->dtype};
+    *mods[i] = Mod{given[i]->ptr, given[i]->stride_group, given[i]->stride_row, given[i]->dtype,
+                   given[i]->grad_f32 ? MH3_DTYPE_F32 : given[i]->dtype};
     if (given[i]->ptr) {
       const int ms = size_of(given[i]->dtype);
       vec = vec && al16(given[i]->ptr) && given[i]->stride_group * ms % 16 == 0 && given[i]->stride_row * ms % 16 == 0;

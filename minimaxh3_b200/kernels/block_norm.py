@@ -23,7 +23,8 @@ _MODS = "Tensor x, Tensor? y, Tensor? gate, Tensor? scale, Tensor? shift, Tensor
 _CONF = "int norm, int y_norm, float eps, float alpha, bool per_token"
 _LIB = torch.library.Library("mh3", "FRAGMENT")
 _LIB.define(f"block_norm({_MODS}, {_CONF}, bool want_stats) -> Tensor[]")
-_LIB.define(f"block_norm_backward(Tensor? dr, Tensor? dh, {_MODS}, Tensor stats, {_CONF}, bool[] want) -> Tensor[]")
+_LIB.define(f"block_norm_backward(Tensor? dr, Tensor? dh, {_MODS}, Tensor stats, {_CONF}, bool[] want, "
+            "int wide=0) -> Tensor[]")
 
 
 _LIB.impl("block_norm", _ops.block_norm_fwd, "CUDA")
@@ -40,26 +41,41 @@ def _(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_norm, eps, a
 
 
 @torch.library.register_fake("mh3::block_norm_backward", lib=_LIB)
-def _(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu, stats, norm, y_norm, eps, alpha, per_token, want):
+def _(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu, stats, norm, y_norm, eps, alpha, per_token, want, wide=0):
     ts = (x, y, gate, scale, shift, weight, bias, y_weight)
-    return [t.new_empty(t.shape) for t, w in zip(ts, want) if w and t is not None]
+    f32 = [False] * 2 + [bool(wide >> i & 1) for i in range(3)] + [False] * 3
+    return [t.new_empty(t.shape, dtype=torch.float32 if f else t.dtype) for t, w, f in zip(ts, want, f32) if w and t is not None]
 
 
-def _forward(*args):
-    return (_ops.block_norm_fwd if _ops.plain(*args[:9]) else torch.ops.mh3.block_norm)(*args)
+def _rows(mods, shape):
+    """gate, scale and shift with a row for each group or token."""
+    return mods if shape is None else [m if m is None or m.shape == shape else m.expand(shape) for m in mods]
 
 
 def _gradients(ctx, *grads):
     saved = ctx.saved_tensors
+    mods, shape = saved[2:5], ctx.shape
     it = iter(grads)
     dr = None if saved[1] is None else next(it)  # r with y, h with a norm
     dh = next(it) if ctx.conf[0] else None
     if dr is None and dh is None:
-        return (None,) * 10
+        return (None,) * 11
     want = ctx.needs_input_grad[:8]  # false for what is not a tensor
-    backward = _ops.block_norm_bwd if _ops.plain(dr, dh, *saved) else torch.ops.mh3.block_norm_backward
-    it = iter(backward(dr, dh, *saved, *ctx.conf, want))
-    return (*[next(it) if w else None for w in want], None, None)
+    # A modulation shared by groups or tokens: its rows' gradients come in f32 and are summed before they are rounded.
+    wide = 0
+    if shape is not None:
+        for i, m in enumerate(mods):
+            if want[2 + i] and m.shape != shape:
+                wide |= 1 << i
+    plain = ctx.plain and _ops.plain_backward(dr, dh)
+    backward = _ops.block_norm_bwd if plain else torch.ops.mh3.block_norm_backward
+    it = iter(backward(dr, dh, *saved[:2], *_rows(mods, shape), *saved[5:], *ctx.conf, want, wide))
+    out = [next(it) if w else None for w in want]
+    if wide:
+        for i, m in enumerate(mods):
+            if wide >> i & 1:
+                out[2 + i] = out[2 + i].sum_to_size(m.shape).to(m.dtype)
+    return (*out, None, None, None)
 
 
 _gradients_once = once_differentiable(_gradients)
@@ -67,11 +83,13 @@ _gradients_once = once_differentiable(_gradients)
 
 class _BlockNormFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, y, gate, scale, shift, weight, bias, y_weight, cu, conf):
-        *out, stats = _forward(x, y, gate, scale, shift, weight, bias, y_weight, cu, *conf, True)
+    def forward(ctx, x, y, gate, scale, shift, weight, bias, y_weight, cu, conf, shape):
+        ctx.plain = _ops.plain(x, y, gate, scale, shift, weight, bias, y_weight, cu)
+        forward = _ops.block_norm_fwd if ctx.plain else torch.ops.mh3.block_norm
+        *out, stats = forward(x, y, *_rows((gate, scale, shift), shape), weight, bias, y_weight, cu, *conf, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, y, gate, scale, shift, weight, bias, y_weight, cu, stats)
-        ctx.conf = conf
+        ctx.conf, ctx.shape = conf, shape
         return tuple(out)
 
     @staticmethod
@@ -96,14 +114,15 @@ def _check_cu(what, x, cu):
 
 
 def _modulation(what, x, cu, gate, scale, shift):
-    """gate, scale and shift as [groups, C] each, or of x's shape each if one of them has a row for each token."""
+    """gate, scale and shift in as many dimensions as the shape they broadcast to; that shape, [groups, C], or x's if
+    one of them has a row for each token (None: they have it); and whether it is x's."""
     C, device = x.shape[-1], x.device
     groups = cu.numel() - 1 if cu is not None else x.shape[0] if x.dim() == 3 else 1
     for m in (gate, scale, shift):
         if m is not None and not (isinstance(m, torch.Tensor) and m.shape == (groups, C) and m.dtype in _TYPES and m.device == device):
             break
     else:  # the common form
-        return gate, scale, shift, False
+        return gate, scale, shift, None, False
     out, per_token = {}, False
     for name, m in (("gate", gate), ("scale", scale), ("shift", shift)):
         if m is None:
@@ -134,16 +153,14 @@ def _modulation(what, x, cu, gate, scale, shift):
         if km is None:
             continue
         kind, m = km
-        if not per_token:
-            m = m.expand(groups, C)
-        elif kind == "token":
-            m = m.expand(x.shape)
-        elif cu is not None and m.dim() == 2 and m.shape[0] != 1:
+        if per_token and kind == "group" and cu is not None and m.dim() == 2 and m.shape[0] != 1:
             raise ValueError(f"{what}: {name} is per sequence while another modulation is per token")
-        else:
-            m = (m if m.dim() == 1 or x.dim() == 2 else m.unsqueeze(1)).expand(x.shape)
+        if m.dim() == 1:
+            m = m.unsqueeze(0)
+        if per_token and kind == "group" and x.dim() == 3:
+            m = m.unsqueeze(1)
         out[name] = m
-    return out["gate"], out["scale"], out["shift"], per_token
+    return out["gate"], out["scale"], out["shift"], tuple(x.shape) if per_token else (groups, C), per_token
 
 
 def _channels(what, x, name, v):
@@ -151,13 +168,17 @@ def _channels(what, x, name, v):
         raise ValueError(f"{what}: {name} must be a bf16, f16 or f32 tensor [C] on x's device")
 
 
-def _run(what, *args):
-    _ops.refuse_forward_mode(what, *args[:8])
+def _run(what, shape, *args):
+    if _ops.forward_ad._current_level >= 0:
+        _ops.refuse_forward_mode(what, *args[:8])
     if torch.is_grad_enabled():
         for t in args[:8]:
             if t is not None and t.requires_grad:
-                return _BlockNormFn.apply(*args[:9], args[9:])
-    return _forward(*args, False)
+                return _BlockNormFn.apply(*args[:9], args[9:], shape)
+    forward = _ops.block_norm_fwd if _ops.plain(*args[:9]) else torch.ops.mh3.block_norm
+    if shape is not None:
+        args = (*args[:2], *_rows(args[2:5], shape), *args[5:])
+    return forward(*args, False)
 
 
 def _finish_checks(what, x, eps):
@@ -196,14 +217,14 @@ def norm_modulate(
     _check_cu(what, x, cu_seqlens)
     if norm not in ("layer", "rms"):
         raise ValueError(f"{what}: norm must be 'layer' or 'rms'")
-    _, scale, shift, per_token = _modulation(what, x, cu_seqlens, None, scale, shift)
+    _, scale, shift, shape, per_token = _modulation(what, x, cu_seqlens, None, scale, shift)
     if weight is not None:
         _channels(what, x, "weight", weight)
     if bias is not None:
         _channels(what, x, "bias", bias)
     _finish_checks(what, x, eps)
     cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-    return _run(what, x, None, None, scale, shift, weight, bias, None, cu, _ops.NORM_KINDS[norm], 0, float(eps), 1.0,
+    return _run(what, shape, x, None, None, scale, shift, weight, bias, None, cu, _ops.NORM_KINDS[norm], 0, float(eps), 1.0,
                 per_token)[0]
 
 
@@ -244,12 +265,12 @@ def gated_residual_norm(
         raise ValueError(f"{what}: scale, shift, weight and bias need a norm")
     if y_norm == "none" and y_weight is not None:
         raise ValueError(f"{what}: y_weight needs y_norm")
-    gate, scale, shift, per_token = _modulation(what, x, cu_seqlens, gate, scale, shift)
+    gate, scale, shift, shape, per_token = _modulation(what, x, cu_seqlens, gate, scale, shift)
     for name, v in (("weight", weight), ("bias", bias), ("y_weight", y_weight)):
         if v is not None:
             _channels(what, x, name, v)
     _finish_checks(what, x, eps)
     cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-    out = _run(what, x, y, gate, scale, shift, weight, bias, y_weight, cu, _ops.NORM_KINDS[norm], _ops.NORM_KINDS[y_norm],
+    out = _run(what, shape, x, y, gate, scale, shift, weight, bias, y_weight, cu, _ops.NORM_KINDS[norm], _ops.NORM_KINDS[y_norm],
                float(eps), float(residual_scale), per_token)
     return out[0], None if norm == "none" else out[1]

@@ -87,7 +87,8 @@ def quantize_fp4(x2d: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.T
     at the upper end of e4m3.  Entries of blocks past M and K are 0.  The value is
     code * block * scale; all roundings are to nearest even.  A row that holds an infinity or NaN gets scale NaN.
     """
-    _ops.refuse_forward_mode("quantize_fp4", x2d)
+    if _ops.forward_ad._current_level >= 0:
+        _ops.refuse_forward_mode("quantize_fp4", x2d)
     return (_ops.quantize_fp4 if _ops.plain(x2d) else torch.ops.mh3.quantize_fp4)(x2d)
 
 
@@ -99,7 +100,8 @@ def _asking(*ts):
 def dequantize_fp4(values: torch.Tensor, blocks: torch.Tensor, scale: torch.Tensor,
                    dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The [M, K] numbers that a 4-bit matrix stands for (exact in bfloat16 and float32)."""
-    _ops.refuse_forward_mode("dequantize_fp4", scale)
+    if _ops.forward_ad._current_level >= 0:
+        _ops.refuse_forward_mode("dequantize_fp4", scale)
     plain = _ops.plain(values, blocks, scale)
     out = (_ops.dequantize_fp4 if plain else torch.ops.mh3.dequantize_fp4)(values, blocks, scale, dtype)
     asks = _asking(blocks, scale)
@@ -109,7 +111,8 @@ def dequantize_fp4(values: torch.Tensor, blocks: torch.Tensor, scale: torch.Tens
 def fp4_matmul(a, b, bias: torch.Tensor | None = None) -> torch.Tensor:
     """bf16 ``a b^T + bias`` of two 4-bit matrices ``(values, blocks, scale)``, a [M, K], b [N, K], N a multiple of 8."""
     a, b = tuple(a), tuple(b)
-    _ops.refuse_forward_mode("fp4_matmul", a[2], b[2], bias)
+    if _ops.forward_ad._current_level >= 0:
+        _ops.refuse_forward_mode("fp4_matmul", a[2], b[2], bias)
     out = (_fp4_matmul_cuda if _ops.plain(*a, *b, bias) else torch.ops.mh3.fp4_matmul)(a, b, bias)
     asks = _asking(*a[1:], *b[1:], bias)
     return _NoGradient.apply(out, *asks) if asks else out
@@ -131,8 +134,9 @@ def fp4_linear(x: torch.Tensor, w4: torch.Tensor, w_blocks: torch.Tensor, w_scal
     if not x.is_cuda or x.device != w4.device:
         raise ValueError("fp4_linear: x and the weight must be on one CUDA device")
     x2d = x if x.dim() == 2 else x.reshape(-1, K)
-    low_rank = [t for a, b, _ in adapters for t in (a, b)]
-    _ops.refuse_forward_mode("fp4_linear", x, w_scale, bias, *low_rank)
+    low_rank = [t for a, b, _ in adapters for t in (a, b)] if adapters else ()
+    if _ops.forward_ad._current_level >= 0:
+        _ops.refuse_forward_mode("fp4_linear", x, w_scale, bias, *low_rank)
     asks = _asking(x, w_blocks, w_scale, bias, *low_rank)
     if not asks and _ops.plain(x, w4, w_blocks, w_scale, bias, *low_rank):
         out = _ops.fp4_linear(x2d, w4, w_blocks, w_scale, bias, adapters, checked=True)

@@ -31,8 +31,9 @@ def _rotary_cuda(q, k, positions, axes_dim, theta, interleaved, inverse):
 _LIB.impl("rotary_axes", _rotary_cuda, "CUDA")
 
 
-def _turn(q, k, positions, *args):
-    return (_rotary_cuda if _ops.plain(q, k, positions) else torch.ops.mh3.rotary_axes)(q, k, positions, *args)
+def _turn(q, k, positions, *args):  # in or beside a backward pass
+    plain = type(positions) is torch.Tensor and _ops.plain_backward(q, k)
+    return (_rotary_cuda if plain else torch.ops.mh3.rotary_axes)(q, k, positions, *args)
 
 
 @torch.library.register_fake("mh3::rotary_axes", lib=_LIB)
@@ -141,9 +142,11 @@ def rotary_axes(
     ``interleaved=False`` channels p and p + sum(axes_dim)/2.
     """
     axes, thetas = _check(q, k, positions, axes_dim, theta)
-    _ops.refuse_forward_mode("rotary_axes", q, k, positions)
+    if _ops.forward_ad._current_level >= 0:
+        _ops.refuse_forward_mode("rotary_axes", q, k, positions)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         oq, ok = _RotaryFn.apply(q, k, positions, axes, thetas, bool(interleaved), False)
     else:
-        oq, ok = _turn(q, k, positions, axes, thetas, bool(interleaved), False)
+        turn = _rotary_cuda if _ops.plain(q, k, positions) else torch.ops.mh3.rotary_axes
+        oq, ok = turn(q, k, positions, axes, thetas, bool(interleaved), False)
     return oq, None if k is None else ok

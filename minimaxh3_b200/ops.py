@@ -13,7 +13,7 @@ import functools
 import struct
 
 import torch
-from torch.autograd import forward_ad as _forward_ad
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -72,31 +72,37 @@ def _launch(dev: torch.device, fn, *args) -> int:
         return fn(*args, _stream(dev))
 
 
-# The dispatch keys that are always there; tracing, dispatch modes, vmap and the other function transforms add theirs.
-_USUAL = 0
-for _key in (torch._C.DispatchKey.BackendSelect, torch._C.DispatchKey.ADInplaceOrView):
-    _USUAL |= torch._C.DispatchKeySet(_key).raw_repr()
-_included = torch._C._dispatch_tls_local_include_set
+_compiling = torch.compiler.is_dynamo_compiling
+_modes = torch._C._len_torch_dispatch_stack
+_transforms = torch._C._functorch.peek_interpreter_stack
+_tracing = torch._C._is_tracing
 _PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None)))
+_batched = torch._C._functorch.is_legacy_batchedtensor
 
 
 def plain(*ts) -> bool:
     """Whether an operator on these tensors (None where one is left out) may skip the dispatcher, whose
     way into a Python kernel costs a small call 5 of its 25 us: plain tensors, and nothing traces,
     transforms or intercepts operators."""
-    if torch.compiler.is_compiling() or _included().raw_repr() & ~_USUAL:
+    if _compiling() or _modes() or _transforms() is not None or _tracing():
         return False
     return _PLAIN.issuperset(map(type, ts)) or not any(isinstance(t, torch.Tensor) and type(t) not in _PLAIN for t in ts)
 
 
+def plain_backward(g, g2) -> bool:
+    """``plain`` for gradients g and g2 (None where there is one), which autograd may batch (``is_grads_batched``)."""
+    return plain(g, g2) and not (g is not None and _batched(g) or g2 is not None and _batched(g2))
+
+
 def refuse_forward_mode(what: str, *ts) -> None:
     """Raises where a tensor carries a forward-mode derivative (or may: it is inside a function transform),
-    which an operator without a rule for it would drop without a word."""
-    if _forward_ad._current_level < 0:
+    which an operator without a rule for it would drop without a word.  (Callers look at the level first too,
+    which is quicker than a call.)"""
+    if forward_ad._current_level < 0:
         return
     for t in ts:
         if isinstance(t, torch.Tensor) and (torch._C._functorch.is_functorch_wrapped_tensor(t)
-                                            or _forward_ad.unpack_dual(t).tangent is not None):
+                                            or forward_ad.unpack_dual(t).tangent is not None):
             raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
@@ -973,8 +979,11 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
             copies.append(t)  # alive until the launch
             s = t.stride()
         if o is None:
-            o = rotary_like(t)
+            o = torch.empty_like(t)  # rotary_like, in fewer calls
             so = o.stride()
+            if so[-1] != 1 and o.shape[-1] != 1:
+                o = t.new_empty(t.shape)
+                so = o.stride()
         elif o.shape != t.shape or o.dtype != t.dtype or o.device != t.device or o.stride(-1) != 1:
             raise ValueError("rotary: an output must match its input, with contiguous channels")
         else:
@@ -1031,18 +1040,18 @@ def _row_arg(t: torch.Tensor, C: int, keep: list):
     return t.data_ptr(), C
 
 
-def _mod_arg(m: torch.Tensor, C: int, S: int, per_token: bool, keep: list):
-    """gate, scale or shift: pointer, strides of groups and rows, type."""
+def _mod_arg(m: torch.Tensor, C: int, S: int, per_token: bool, wide: int, keep: list):
+    """gate, scale or shift: pointer, strides of groups and rows, type, and whether its gradient is f32."""
     s = m.stride()
     if s[-1] != 1 and C != 1:
         m = m.contiguous()
         keep.append(m)
         s = m.stride()
     if not per_token:
-        return m.data_ptr(), s[0], 0, _FLOAT_CODE[m.dtype], 0
+        return m.data_ptr(), s[0], 0, _FLOAT_CODE[m.dtype], wide
     if len(s) == 3:  # element (b, s): row b S + s
-        return m.data_ptr(), s[0] - S * s[1] if m.shape[0] > 1 else 0, s[1], _FLOAT_CODE[m.dtype], 0
-    return m.data_ptr(), 0, s[0], _FLOAT_CODE[m.dtype], 0
+        return m.data_ptr(), s[0] - S * s[1] if m.shape[0] > 1 else 0, s[1], _FLOAT_CODE[m.dtype], wide
+    return m.data_ptr(), 0, s[0], _FLOAT_CODE[m.dtype], wide
 
 
 def _chan_arg(v: torch.Tensor, keep: list):
@@ -1053,7 +1062,7 @@ def _chan_arg(v: torch.Tensor, keep: list):
 
 
 def _norm_args(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_norm, eps, alpha, per_token, r, h, stats,
-               dr=None, dh=None, grads=None, workspace=None):
+               dr=None, dh=None, grads=None, workspace=None, wide=0):
     """The C arguments, and the tensors made for them.  ``workspace``: a function of (rows, channels, groups)."""
     shape = x.shape
     C = shape[-1]
@@ -1070,9 +1079,9 @@ def _norm_args(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_nor
         0 if cu is None else cu.data_ptr(),
         *_row_arg(x, C, keep),
         *(_NO_ROWS if y is None else _row_arg(y, C, keep)),
-        *(_NO_MOD if gate is None else _mod_arg(gate, C, S, per_token, keep)),
-        *(_NO_MOD if scale is None else _mod_arg(scale, C, S, per_token, keep)),
-        *(_NO_MOD if shift is None else _mod_arg(shift, C, S, per_token, keep)),
+        *(_NO_MOD if gate is None else _mod_arg(gate, C, S, per_token, wide & 1, keep)),
+        *(_NO_MOD if scale is None else _mod_arg(scale, C, S, per_token, wide >> 1 & 1, keep)),
+        *(_NO_MOD if shift is None else _mod_arg(shift, C, S, per_token, wide >> 2 & 1, keep)),
         *(_NO_MOD if weight is None else _chan_arg(weight, keep)),
         *(_NO_MOD if bias is None else _chan_arg(bias, keep)),
         *(_NO_MOD if y_weight is None else _chan_arg(y_weight, keep)),
@@ -1100,19 +1109,25 @@ def block_norm_fwd(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm: i
 
 
 def block_norm_bwd(dr, dh, x, y, gate, scale, shift, weight, bias, y_weight, cu, stats, norm: int, y_norm: int, eps: float,
-                   alpha: float, per_token: bool, want):
+                   alpha: float, per_token: bool, want, wide: int = 0):
     """``mh3_block_norm_bwd``: the list of the gradients of those of (x, y, gate, scale, shift, weight, bias,
-    y_weight) that are given and whose entry of ``want`` is true; dr or dh may be None."""
+    y_weight) that are given and whose entry of ``want`` is true; dr or dh may be None.  ``wide``: bits 0, 1 and 2
+    ask for those of gate, scale and shift in f32."""
     dr, dh = (d if d is None or d.dtype == x.dtype else d.to(x.dtype) for d in (dr, dh))
     ts = (x, y, gate, scale, shift, weight, bias, y_weight)
     grads = [t.new_empty(t.shape) if w and t is not None else None for t, w in zip(ts, want)]
+    if wide:
+        for i in range(3):
+            if wide >> i & 1 and grads[2 + i] is not None:
+                grads[2 + i] = grads[2 + i].new_empty(grads[2 + i].shape, dtype=torch.float32)
     lib = _lib.load()
 
     def workspace(rows, C, groups):
         nbytes = max(16, lib.mh3_block_norm_workspace_bytes(rows, C, groups))
         return x.new_empty(nbytes, dtype=torch.uint8)
 
-    a, keep = _norm_args(*ts, cu, max(norm, 1), y_norm, eps, alpha, per_token, None, None, stats, dr, dh, grads, workspace)
+    a, keep = _norm_args(*ts, cu, max(norm, 1), y_norm, eps, alpha, per_token, None, None, stats, dr, dh, grads, workspace,
+                         wide)
     rc = _launch(x.device, lib.mh3_block_norm_bwd, a)
     _lib.check(rc, "mh3_block_norm_bwd")
     return [g for g in grads if g is not None]

@@ -527,3 +527,46 @@ def test_long_and_short_sequences_share_a_stage():
     want = c.grads(None, dh, lambda t: torch.zeros(n, C, dtype=t.dtype, device=DEV).index_add_(0, rep, t))
     _close(dx, *want["x"], "x")
     _close(ds, *want["scale"], "scale")
+
+
+@pytest.mark.parametrize("C", [104, 1928, 2051])
+@pytest.mark.parametrize("dtype,by_token", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float16, torch.float16),
+                                            (torch.float32, torch.float32), (torch.float32, torch.bfloat16)])
+@pytest.mark.parametrize("shared", ["token", "group", "packed"])
+def test_gradients_of_shared_modulations_are_rounded_once(C, dtype, by_token, shared):
+    """16-bit modulations that tokens or batch items share: the sum over them is in f32 (a term is off by its own F
+    and the sum by n u of their magnitudes) and rounded once - where terms cancel, rounding each would show."""
+    from minimaxh3_b200.kernels.block_norm import gated_residual_norm
+
+    B, S, low = 3, 150, torch.float16 if dtype == torch.float16 else torch.bfloat16
+    leaf = lambda t: t.requires_grad_(True)  # noqa: E731
+    lead = (B, S) if shared != "packed" else (B * S,)
+    x, y = leaf(_rand(210, *lead, C, dtype=dtype)), leaf(_rand(211, *lead, C, dtype=dtype, shift=0.3))
+    dr, dh = _rand(212, *lead, C, dtype=dtype), _rand(213, *lead, C, dtype=dtype)
+    cu = torch.tensor([0, 70, 70 + S, B * S], dtype=torch.int32, device=DEV) if shared == "packed" else None
+    gate = leaf(_rand(214, C, dtype=low))
+    scale = leaf(_rand(215, *((1, S, C) if shared == "token" else (1, C) if shared == "packed" else (C,)), dtype=low, scale=0.3))
+    shift = leaf(_rand(216, *((B, S, C) if shared == "token" else (B, C)), dtype=by_token if shared == "token" else low))
+    if shared == "token":
+        rows = lambda t: t.expand(B, S, C)  # noqa: E731
+    elif shared == "group":
+        rows = lambda t: (t if t.dim() == 1 else t[:, None]).expand(B, S, C)  # noqa: E731
+    else:
+        rep = torch.repeat_interleave(torch.arange(3, device=DEV), torch.tensor([70, S, B * S - 70 - S], device=DEV))
+        rows = lambda t: t[rep] if t.shape[:-1] == (3,) else t.expand(B * S, C)  # noqa: E731
+    c = Case(x, y, gate=gate, scale=scale, shift=shift, rows_of=rows)
+    r, h = gated_residual_norm(x, y, gate, scale, shift, cu_seqlens=cu)
+    got = torch.autograd.grad((r, h), (x, y, gate, scale, shift), (dr, dh))
+    want = c.grads(dr, dh, lambda t: t)
+    _close(got[0], *want["x"], "x")
+    _close(got[1], *want["y"], "y")
+    for name, m, g in zip(("gate", "scale", "shift"), (gate, scale, shift), got[2:]):
+        assert g.dtype == m.dtype and g.shape == m.shape
+        terms, err = want[name]
+        if shared == "packed" and m.shape[0] == 3:
+            total = lambda t: torch.zeros(3, C, dtype=t.dtype, device=DEV).index_add_(0, rep, t)  # noqa: E731
+        elif shared == "group" and m.shape[:-1] == (B,):
+            total = lambda t: t.sum(1)  # noqa: E731
+        else:
+            total = lambda t: t.sum_to_size(m.shape)  # noqa: E731
+        _close(g, total(terms), total(err + terms.abs() * B * S * U), name)

@@ -19,7 +19,7 @@ class _Sub(torch.Tensor):
 
 def test_plain_tensors_are_plain():
     x = torch.zeros(2, 3)
-    assert ops.plain(x) and ops.plain(x, None, torch.nn.Parameter(x)) and ops.plain()
+    assert ops.plain(x) and ops.plain(x, None, torch.nn.Parameter(x)) and ops.plain() and ops.plain_backward(x, None)
     with torch.no_grad():
         assert ops.plain(x)
     with torch.inference_mode():
@@ -57,7 +57,7 @@ def test_a_batched_backward_is_not_plain():
 
         @staticmethod
         def backward(ctx, g):
-            seen.append(ops.plain(g))
+            seen.append(ops.plain_backward(g, None) or ops.plain_backward(None, g) or ops.plain_backward(x, g))
             return g * 2
 
     x = torch.zeros(3, requires_grad=True)
@@ -129,6 +129,8 @@ def test_batched_gradients_of_the_rotation():
     got, = torch.autograd.grad(out, q, g, is_grads_batched=True, retain_graph=True)
     for i in range(3):
         assert torch.equal(got[i], torch.autograd.grad(out, q, g[i], retain_graph=True)[0])
+    twice, = torch.autograd.grad(out, q, g, is_grads_batched=True, create_graph=True)
+    assert torch.equal(twice, got)
 
 
 @pytest.mark.gpu
