@@ -1068,10 +1068,14 @@ def _norm_args(x, y, gate, scale, shift, weight, bias, y_weight, cu, norm, y_nor
     C = shape[-1]
     S = shape[1] if len(shape) == 3 else shape[0]
     groups, group_rows = (cu.numel() - 1, 0) if cu is not None else (shape[0], S) if len(shape) == 3 else (1, S)
+    nrows = x.numel() // C
     if groups == 0:
         groups, group_rows = 1, 0  # an empty batch
+    elif group_rows == 1 and groups > 1:
+        # Groups of one row are modulation by row: no partial column sums for each row (4 GB of
+        # workspace for 32760 rows of 5120), no modulation combined for one row alone.
+        groups, group_rows, per_token = 1, nrows, True
     keep = []
-    nrows = x.numel() // C
     ws = None if workspace is None else workspace(nrows, C, groups)
     keep.append(ws)
     a = _lib.BlockNormArgs.from_buffer_copy(_NORM.pack(

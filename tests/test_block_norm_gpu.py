@@ -570,3 +570,32 @@ def test_gradients_of_shared_modulations_are_rounded_once(C, dtype, by_token, sh
         else:
             total = lambda t: t.sum_to_size(m.shape)  # noqa: E731
         _close(g, total(terms), total(err + terms.abs() * B * S * U), name)
+
+
+@pytest.mark.parametrize("C", [64, 1928, 2051])
+@pytest.mark.parametrize("dtype,mods", [(torch.bfloat16, (torch.float32,) * 3), (torch.float32, (torch.bfloat16, torch.float32, torch.float16))])
+def test_many_batch_items_of_one_row(C, dtype, mods):
+    """[B, 1, C] with modulation [B, C]: each row has its own, and the call's memory does not grow by f32 rows for each."""
+    from minimaxh3_b200.kernels.block_norm import gated_residual_norm
+
+    B = 3001
+    leaf = lambda t: t.requires_grad_(True)  # noqa: E731
+    x, y = leaf(_rand(220, B, 1, C, dtype=dtype)), leaf(_rand(221, B, 1, C, dtype=dtype, shift=0.3))
+    kw = dict(gate=leaf(_rand(222, B, C, dtype=mods[0])), scale=leaf(_rand(223, B, C, dtype=mods[1], scale=0.3)),
+              shift=leaf(_rand(224, B, C, dtype=mods[2])), weight=leaf(_rand(225, C, dtype=torch.float32, shift=1.0)),
+              bias=leaf(_rand(226, C, dtype=torch.float32)), y_weight=leaf(_rand(227, C, dtype=dtype, shift=1.0)))
+    dr, dh = _rand(228, B, 1, C, dtype=dtype), _rand(229, B, 1, C, dtype=dtype)
+    c = Case(x, y, norm="layer", y_norm="rms", rows_of=lambda t: t[:, None], **kw)
+    r, h = gated_residual_norm(x, y, norm="layer", y_norm="rms", **kw)
+    _close(r, c.r, c.er, "r")
+    _close(h, c.h, c.eh, "h")
+    want = c.grads(dr, dh, lambda t: t.sum(1))
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    grads = torch.autograd.grad((r, h), (x, y, *kw.values()), (dr, dh))
+    made = sum(g.numel() * g.element_size() for g in grads)
+    # the gradients, and partial sums of at most 16 CTAs an SM
+    assert torch.cuda.max_memory_allocated() - before <= made + (16 * 148 + 2) * 3 * C * 4 + (1 << 20)
+    for name, g in zip(("x", "y", *kw), grads):
+        _close(g, *want[name], name)
