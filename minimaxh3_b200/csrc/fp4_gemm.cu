@@ -50,6 +50,11 @@ constexpr int kGroupM = 8;                     // 256-row blocks per raster grou
 constexpr int SF_COL = 256, SF_COLS = 48;      // scales of a stage: 4 x 4 columns of A, 4 x 8 of B
 constexpr int kSmallM = 16;
 
+// A row's scale as the factors before and after the column's, so that no product passes
+// f32's range while the result does not: the smaller of 1 and the scale first (a NaN stays in
+// the second).  Powers of two: exact.
+__device__ __forceinline__ float2 split_scale(float s) { return s <= 1.0f ? make_float2(s, 1.0f) : make_float2(1.0f, s); }
+
 struct Params {
   CUtensorMap tma_a, tma_b;    // bytes (K/2, rows), box (128, 128), 128B swizzle
   CUtensorMap tma_sa, tma_sb;  // words (128, K/64, rows/128), box (128, 4, 1)
@@ -280,7 +285,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) pair_kernel(const __grid_const
       named_barrier_sync(1, 32 * EPI_WARPS);
       const int m0 = mb * BM + (int)crank * HALF + q * 32;  // first row of this warp's boxes
       const int m = m0 + lane;
-      const float rsv = m < p.M ? __ldg(p.rs + m) : 0.0f;
+      const float2 rsv = split_scale(m < p.M ? __ldg(p.rs + m) : 0.0f);
       mbar_wait(smem_u32(&sm.acc_full), (uint32_t)tcount & 1u, g);
       tc_fence_after();
       uint32_t v[4][32];
@@ -301,10 +306,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) pair_kernel(const __grid_const
         for (int i = 0; i < 8; ++i) {
           const float4 c4 = *reinterpret_cast<const float4*>(cs + 4 * i);
           const float4 b4 = *reinterpret_cast<const float4*>(bs + 4 * i);
-          const __nv_bfloat162 h0 = __floats2bfloat162_rn(fmaf(__uint_as_float(v[c][4 * i + 0]) * rsv, c4.x, b4.x),
-                                                          fmaf(__uint_as_float(v[c][4 * i + 1]) * rsv, c4.y, b4.y));
-          const __nv_bfloat162 h1 = __floats2bfloat162_rn(fmaf(__uint_as_float(v[c][4 * i + 2]) * rsv, c4.z, b4.z),
-                                                          fmaf(__uint_as_float(v[c][4 * i + 3]) * rsv, c4.w, b4.w));
+          const __nv_bfloat162 h0 = __floats2bfloat162_rn(fmaf(__uint_as_float(v[c][4 * i + 0]) * rsv.x * c4.x, rsv.y, b4.x),
+                                                          fmaf(__uint_as_float(v[c][4 * i + 1]) * rsv.x * c4.y, rsv.y, b4.y));
+          const __nv_bfloat162 h1 = __floats2bfloat162_rn(fmaf(__uint_as_float(v[c][4 * i + 2]) * rsv.x * c4.z, rsv.y, b4.z),
+                                                          fmaf(__uint_as_float(v[c][4 * i + 3]) * rsv.x * c4.w, rsv.y, b4.w));
           packed[2 * i] = *reinterpret_cast<const uint32_t*>(&h0);
           packed[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&h1);
         }
@@ -522,7 +527,8 @@ __global__ void __launch_bounds__(kWarps * 32) small_kernel(const __grid_constan
     if constexpr (FUSED) rs = top[m] < 0x7f800000u ? fp4::pow2f(fp4::row_exponent(top[m])) : __uint_as_float(0x7fffffffu);
     else rs = p.rs[m];
     const float b = p.bias != nullptr ? __bfloat162float(p.bias[n]) : 0.0f;
-    p.out[m * p.ldo + n] = __float2bfloat16_rn(fmaf(s * rs, p.cs[n], b));
+    const float2 r2 = split_scale(rs);
+    p.out[m * p.ldo + n] = __float2bfloat16_rn(fmaf(s * r2.x * p.cs[n], r2.y, b));
   }
 }
 

@@ -372,3 +372,23 @@ def test_an_adapter_edited_unseen_is_used():
     assert torch.equal(cap, want) and torch.equal(fp4_linear(x, *w, adapters=[(A, B, 0.5)]), want)
     B.data.copy_(keep)
     assert torch.equal(fp4_linear(x, *w, adapters=[(A, B, 0.5)]), first)
+
+
+@pytest.mark.parametrize("M", [1, 3, 40, 300])
+def test_products_of_rows_at_the_ends_of_the_range(M):
+    """A power of two on x's rows or on the weight goes through to the result exactly, as long as that is in range:
+    no product of a sum with one scale alone may overflow or vanish."""
+    from minimaxh3_b200.kernels.fp4_linear import fp4_linear, quantize_fp4
+
+    K, N = 128, 64
+    x, w = _rand(100, M, K).to(DEV), _rand(101, N, K, scale=0.05).to(DEV)
+    A, B = _rand(102, 16, K, scale=0.1).to(DEV), _rand(103, N, 16, scale=0.1).to(DEV)
+    ref, low = fp4_linear(x, *quantize_fp4(w)), fp4_linear(x, *quantize_fp4(w), adapters=[(A, B, 0.5)])
+    for px, pw in ((0, 0), (118, 0), (110, -40), (-60, 70), (-80, 100), (20, 95), (100, 15)):
+        fx, fw = 2.0 ** px, 2.0 ** pw
+        want = (ref.double() * fx * fw).to(torch.bfloat16)
+        assert bool(want.isfinite().all())
+        assert torch.equal(fp4_linear(x * fx, *quantize_fp4(w * fw)), want), (px, pw)
+        if M > 2 and px + pw < 110:
+            want = (low.double() * fx * fw).to(torch.bfloat16)
+            assert torch.equal(fp4_linear(x * fx, *quantize_fp4(w * fw), adapters=[(A, B * fw, 0.5)]), want), (px, pw)
