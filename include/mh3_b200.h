@@ -508,7 +508,9 @@ MH3_API int mh3_block_norm_bwd(const mh3_block_norm_args* args, void* stream);
  * quotients; a block whose scale rounds to 0 has codes 0.  A row with an
  * infinity or NaN gets scale NaN and zeros elsewhere.  Scales past K and past M
  * in the last blocks are 0.
- * mh3_dequantize_fp4: the values, bf16 or f32 (both exact), [M, K] contiguous.
+ * mh3_dequantize_fp4: the values, bf16 or f32, [M, K] contiguous.  Both are
+ * exact, but for a row whose magnitudes come within a twentieth of f32's end:
+ * there a value may round up past it, and is infinite.
  *
  * mh3_fp4_gemm: out[m,n] = bf16((sum_k a[m,k] b[n,k] + sum_r a2[m,r] b2[n,r])
  *   * a_scale[m] * b_scale[n] + bias[n]), a [M,K] and b [N,K] such matrices

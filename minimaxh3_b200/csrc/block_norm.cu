@@ -18,8 +18,8 @@
 // It recomputes xhat and yhat from x, y and the rows' saved (mean, rstd).
 //
 // Bound: HBM (4 bytes a bf16 element for norm_modulate, 8 for the gated form;
-// backward 6 and 12).  A CTA spans a row, eight channels a thread, and walks a
-// contiguous range of rows, so the modulation is read and combined once per
+// backward 6 and 12).  A CTA spans a row, eight channels a thread (sixteen in the
+// modulated norm's forward pass), and walks a contiguous range of rows, so the modulation is read and combined once per
 // group (kept in the thread's own slots of shared memory).  The rows stream
 // through a ring of two or three stages in shared memory: each thread copies its
 // own sixteen bytes with cp.async and reads back only what it copied, so the ring
@@ -622,8 +622,7 @@ __device__ __forceinline__ void mod_piece(const void* p, int dt, long long at, f
   }
 }
 
-// f(piece index, its first channel, E values of up to three tensors) for the thread's
-// pieces inside the row; results go to slots.
+// A thread's CH values in its slots of shared memory, four to a float4, and back.
 template <int CH>
 __device__ __forceinline__ void slots_put(float4* s, const float (&v)[CH]) {
 #pragma unroll
@@ -1318,9 +1317,11 @@ __global__ void __launch_bounds__(MAXT) bwd_stream_kernel(const __grid_constant_
 
 // Column sums of group blockIdx.y..: a CTA takes 8 channels (a sector) of 32 or 128
 // partials at a time, added over a warp's four by shuffles, then over the warps, in a
-// fixed order.  128 where a group has many: 6.4 us against 13.8 for 1480 partials of 320
-// channels, but 7.6 against 5.3 for twice 222 of 1536.  PT: one "group" holds every CTA's
-// partial.
+// fixed order.  128 where a group has many.  With 128 against 32: 8.4 and 21.4 us for 2368
+// partials of 64 channels, 6.3 and 14.1 for 1480 of 320, 5.2 and 9.3 for 592 of 640, 5.6 and
+// 6.6 for 444 of 1536; at 296 it turns: 5.5 and 6.3 for twice 640 channels, 7.8 and 5.7 for
+// 2560; below, 6.9 and 5.0 for twice 222 of 1536, 10.0 and 4.9 for 148 of 5120.  PT: one
+// "group" holds every CTA's partial.
 constexpr int kCols = 8;
 template <bool PT, int PARTS>
 __global__ void __launch_bounds__(kCols * PARTS) group_sum_kernel(const __grid_constant__ Params p) {
@@ -1433,8 +1434,14 @@ static size_t ring_bytes(Params& p, int threads, int ch, int mods, int rows, int
 
 // norm_modulate: 16 channels a thread and two rows a stage, two CTAs of a
 // 5120-channel row per SM (146 us with 8 channels and four rows in one CTA, at
-// 32760 x 5120: the reductions' instructions per channel halve).  The gated form
-// holds three modulation slots and two tensors, so one CTA with 8 channels.
+// 32760 x 5120: the reductions' instructions per channel halve).  f32 rows spill 44 bytes
+// there and take as long with one CTA of twice the registers: 241 us against 244 at 5120
+// channels, 187 against 172 at 4096, 117 against 121 at 2560.  The gated form holds three
+// modulation slots and two tensors, so one CTA with 8 channels.
+//
+// ``wide`` here and below: rows of more than 5120 channels need more than 640 threads, which
+// leaves a thread 64 registers, not 102.  Narrower rows would lose by it (16384 x 5120 bf16:
+// gated 153 us against 113; backward 188 against 140, by row and gated 476 against 374).
 template <typename T>
 static cudaError_t stream_fwd(Params& p, cudaStream_t st, bool& done) {
   constexpr int R = 2;
@@ -1476,8 +1483,9 @@ static cudaError_t stream_bwd(Params& p, cudaStream_t st, bool& done) {
               : start<bwd_stream_kernel<T, void, Y, R, 640>>(p, nt, smem, st);
 }
 
-// Modulation by row, in one type (T or f32): its rows stream beside x's, one row a stage (at 32760 x 5120 bf16 with f32 modulation 313 us
-// against 599 with the general kernel, and 425 against 1176 backward with bf16 modulation).
+// Modulation by row, in one type (T or f32): its rows stream beside x's, one row a stage (at
+// 32760 x 5120 bf16 with f32 modulation 313 us against 599 with the general kernel, and 425
+// against 1176 backward with bf16 modulation).
 template <typename T, typename M, bool Y>
 static cudaError_t stream_rows(Params& p, bool bwd, cudaStream_t st, bool& done) {
   const int nt = threads_of(p.C), ctas = p.ctas;

@@ -210,7 +210,9 @@ def norm_modulate(
     sequence give zeros.  weight / bias [C].
     Modulation and weights may be of other float types than x (kept in f32
     beside a bf16 stream); None leaves that term out.  Statistics and sums are
-    f32, the result is rounded once.
+    f32, the result is rounded once; so is the gradient of a modulation that
+    tokens or batch items share (where another one has a row for each token, its
+    rows' f32 gradients take 4 bytes an element of x until they are summed).
     """
     what = "norm_modulate"
     _check_stream(what, "x", x)

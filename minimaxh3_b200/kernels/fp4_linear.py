@@ -99,7 +99,8 @@ def _asking(*ts):
 
 def dequantize_fp4(values: torch.Tensor, blocks: torch.Tensor, scale: torch.Tensor,
                    dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The [M, K] numbers that a 4-bit matrix stands for (exact in bfloat16 and float32)."""
+    """The [M, K] numbers that a 4-bit matrix stands for, exact in bfloat16 and float32 (infinite where a
+    magnitude within a twentieth of the type's end was rounded up past it)."""
     if _ops.forward_ad._current_level >= 0:
         _ops.refuse_forward_mode("dequantize_fp4", scale)
     plain = _ops.plain(values, blocks, scale)

@@ -922,7 +922,7 @@ def fp4_linear(x2d: torch.Tensor, w4: torch.Tensor, w_blocks: torch.Tensor, w_sc
             raise ValueError("fp4_linear: x is [M,K] and the weight [N,K]")
         if w4.device != dev:
             raise ValueError("fp4_linear: x and the weight must be on one device")
-    if K != 1 and x2d.stride(1) != 1:
+    if x2d.stride(1) != 1:
         x2d = x2d.contiguous()
     if bias is not None:
         if bias.numel() != N or bias.device != dev:

@@ -392,3 +392,21 @@ def test_products_of_rows_at_the_ends_of_the_range(M):
         if M > 2 and px + pw < 110:
             want = (low.double() * fx * fw).to(torch.bfloat16)
             assert torch.equal(fp4_linear(x * fx, *quantize_fp4(w * fw), adapters=[(A, B * fw, 0.5)]), want), (px, pw)
+
+
+def test_values_at_the_end_of_the_range():
+    """Within a twentieth of the largest number a block may round up past it: infinite values, as their definition
+    in 64 bits says; the product of such a row is finite where the result is."""
+    from minimaxh3_b200.kernels.fp4_linear import dequantize_fp4, fp4_linear, quantize_fp4
+
+    top = torch.finfo(torch.bfloat16).max
+    x = torch.full((2, 64), top, dtype=torch.bfloat16)
+    x[1] *= 0.95
+    ref = _values(*_ref(x))
+    assert float(ref[0, 0]) > torch.finfo(torch.float32).max > float(ref[1, 0])
+    q = quantize_fp4(x.to(DEV))
+    for dt in (torch.bfloat16, torch.float32):
+        assert torch.equal(dequantize_fp4(*q, dtype=dt).cpu(), ref.to(dt))
+    w = (torch.ones(8, 64) * 2.0 ** -20).to(torch.bfloat16)
+    want = ref @ _values(*_ref(w)).t()  # 64 equal products of few bits: exact in f32
+    assert torch.equal(fp4_linear(x.to(DEV), *quantize_fp4(w.to(DEV))).cpu(), want.to(torch.bfloat16))

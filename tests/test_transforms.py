@@ -272,3 +272,20 @@ def test_rotary_strides_and_values_of_a_compiled_call(layout):
     got = torch.compile(f, fullgraph=True, backend="aot_eager")(q, k)
     _same(got, want)
     assert [t.stride() for t in got] == [t.stride() for t in want]
+
+
+@pytest.mark.gpu
+def test_compiled_gradients_of_shared_modulations():
+    """A [C] gate beside modulation by token, and [C] scale and shift of several batch items, forward and backward."""
+    from minimaxh3_b200.kernels.block_norm import gated_residual_norm, norm_modulate
+
+    def f(x, y, gate, scale, shift):
+        r, h = gated_residual_norm(x, y, gate, scale, shift)
+        return r, norm_modulate(h, gate, gate)
+
+    leaves = [t.requires_grad_(True) for t in (_rand(1, 2, 9, 64), _rand(2, 2, 9, 64), _rand(3, 64), _rand(4, 2, 9, 64), _rand(5, 2, 64))]
+    grads = _rand(6, 2, 9, 64), _rand(7, 2, 9, 64)
+    want = f(*leaves)
+    want = (*want, *torch.autograd.grad(want, leaves, grads))
+    got = torch.compile(f, fullgraph=True, backend="aot_eager")(*leaves)
+    _same((*got, *torch.autograd.grad(got, leaves, grads)), want)
